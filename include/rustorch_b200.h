@@ -252,6 +252,84 @@ int rtb_conv2d_backward(rtb_ctx* ctx, int64_t N, int64_t Ci, int64_t H, int64_t 
                         const float* x, const float* w, const float* dy, float* dx, float* dw,
                         int accumulate, int precision, void* stream);
 
+/* ---------------------------------------------------------------- layer norm, training */
+/* rtb_layer_norm that also leaves what its backward pass reads: mean[r] and
+ * rstd[r] = 1 / sqrt(var + eps) of every row (rows floats each; d >= 1).
+ * Replaces layer_norm's saved statistics (rustorch-core/src/ops/norm.rs:
+ * 613-700); x == y (in place) is allowed. */
+int rtb_layer_norm_fwd(rtb_ctx* ctx, int64_t rows, int64_t d, const float* x, int64_t ldx,
+                       const float* norm_weight, const float* norm_bias, float eps, int act,
+                       float* y, int64_t ldy, float* mean, float* rstd, void* stream);
+/* Gradients of y = act(u * norm_weight + norm_bias), u = (x - mean) * rstd,
+ * for the incoming gradient dy [rows, d]; with dz = dy * act'(z), h = dz *
+ * norm_weight:
+ *   dx      = rstd * (h - mean(h) - u * mean(h * u))   when dx != NULL
+ *   dweight = sum over rows of dz * u                  when dweight != NULL
+ *   dbias   = sum over rows of dz                      when dbias != NULL
+ * norm_weight / norm_bias as in the forward call (NULL: 1 and 0).  accumulate
+ * != 0 adds into dx, dweight and dbias.  The sums are fp32 in an order that
+ * depends on the shape alone (the same bits on every call).  ReLU's derivative
+ * is 0 where z is 0 or NaN. */
+int rtb_layer_norm_backward(rtb_ctx* ctx, int64_t rows, int64_t d, const float* x, int64_t ldx,
+                            const float* mean, const float* rstd, const float* norm_weight,
+                            const float* norm_bias, int act, const float* dy, int64_t lddy,
+                            float* dx, int64_t lddx, float* dweight, float* dbias, int accumulate,
+                            void* stream);
+/* The same with x kept as an 8-bit checkpoint (rtb_fp8_quantize, block_rows =
+ * 1): x[r, c] = q[r, c] * 2^(scale[r, c / 128] - 127). */
+int rtb_layer_norm_backward_fp8(rtb_ctx* ctx, int64_t rows, int64_t d, const uint8_t* q,
+                                int64_t ldq, const uint8_t* scale, int64_t lds, const float* mean,
+                                const float* rstd, const float* norm_weight,
+                                const float* norm_bias, int act, const float* dy, int64_t lddy,
+                                float* dx, int64_t lddx, float* dweight, float* dbias,
+                                int accumulate, void* stream);
+
+/* ---------------------------------------------------------------- 8-bit block-scaled tensors */
+/* (Extension: the reference's tensors are f32 only.)  q [rows, cols] e4m3
+ * bytes, row stride ldq, and one scale for each block of 128 columns of one
+ * row (block_rows = 1: activations) or of 128 rows (128: weights): scale
+ * [ceil(rows / block_rows), ceil(cols / 128)], row stride lds.  The scales that
+ * rtb_fp8_quantize writes are powers of two held as e8m0 bytes: value = q *
+ * 2^(byte - 127) (255: NaN).  The byte is the smallest whose power of two holds
+ * the block's largest finite magnitude within 448 (at least 1; 127 for a block
+ * of zeros), the scaling is exact and the value is rounded once, to nearest
+ * even: at most 2^-4 relative, or half of e4m3's smallest step 2^-9 (times the
+ * scale) near zero.  An infinity or NaN becomes NaN and does not set the
+ * scale. */
+enum { RTB_SCALE_E8M0 = 0, RTB_SCALE_F32 = 1 };
+int rtb_fp8_quantize(rtb_ctx* ctx, int64_t rows, int64_t cols, const float* x, int64_t ldx,
+                     int block_rows, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds,
+                     void* stream);
+/* y = q * scale (e8m0). */
+int rtb_fp8_dequantize(rtb_ctx* ctx, int64_t rows, int64_t cols, const uint8_t* q, int64_t ldq,
+                       const uint8_t* scale, int64_t lds, int block_rows, float* y, int64_t ldy,
+                       void* stream);
+/* C[M,N] = act(deq(A) . deq(B) + bias), fp32 out, row-major C with ldc.
+ *   A: [M,K] e4m3, row-major; scale_a [ceil(M / block_rows_a), ceil(K / 128)].
+ *   transB = 1: B is [N,K] row-major (nn::Linear's weight), scale_b
+ *               [ceil(N / block_rows_b), ceil(K / 128)];
+ *            0: B is [K,N] row-major, scale_b [ceil(K / 128), ceil(N / 128)],
+ *               block_rows_b = 128.
+ *   scale_type_*: RTB_SCALE_E8M0 bytes or RTB_SCALE_F32 floats (weights scaled
+ *   elsewhere); the product of the two blocks' scales is taken in fp32.
+ *   bias: [N] or NULL.  act: any RTB_ACT_*.
+ * The products of a 128-element block are summed on the tensor cores, the
+ * blocks in fp32.  K = 0 gives act(bias) or zeros. */
+int rtb_fp8_matmul(rtb_ctx* ctx, int64_t M, int64_t N, int64_t K, const uint8_t* A, int64_t lda,
+                   const void* scale_a, int64_t ldsa, int block_rows_a, int scale_type_a,
+                   const uint8_t* B, int64_t ldb, int transB, const void* scale_b, int64_t ldsb,
+                   int block_rows_b, int scale_type_b, const float* bias, int act, float* C,
+                   int64_t ldc, void* stream);
+/* rtb_matmul_backward with A kept as an 8-bit checkpoint (rtb_fp8_quantize):
+ *   dA = dC . B^T          when dA != NULL (does not read the checkpoint)
+ *   dB = deq(A)^T . dC     when dB != NULL (does not read B)
+ * B [K,N], dC [M,N], dA [M,K], dB [K,N] fp32, row-major contiguous.  The
+ * checkpoint's values enter exactly and dC with 24 bits (RTB_PREC_TF32: 16). */
+int rtb_matmul_backward_fp8(rtb_ctx* ctx, int64_t M, int64_t N, int64_t K, const uint8_t* A,
+                            int64_t lda, const uint8_t* scale_a, int64_t ldsa, int block_rows_a,
+                            const float* B, const float* dC, float* dA, float* dB, int accumulate,
+                            int precision, void* stream);
+
 /* ---------------------------------------------------------------- small ops */
 /* ops::max_pool2d (rustorch-core/src/ops/pool.rs:115-191): -inf init, padding skipped. */
 int rtb_max_pool2d(rtb_ctx* ctx, int64_t N, int64_t C, int64_t H, int64_t W, int64_t kh,

@@ -22,6 +22,7 @@ RTB_E_NCCL = 6
 ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_TANH = 0, 1, 2, 3
 PREC_3XTF32, PREC_TF32, PREC_DEFAULT = 0, 1, -1
 LAYOUT_NCHW, LAYOUT_NHWC = 0, 1
+SCALE_E8M0, SCALE_F32 = 0, 1
 
 # Every symbol the header declares, with (restype, argtypes).
 _i = ctypes.c_int
@@ -65,6 +66,17 @@ SIGNATURES = {
                                       ctypes.c_float, _i, _p, _i64, _i, _p]),
     "rtb_layer_norm": (_i, [_p, _i64, _i64, _p, _i64, _p, _p, ctypes.c_float, _i, _p, _i64, _p]),
     "rtb_matmul_backward": (_i, [_p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i, _i, _p]),
+    "rtb_layer_norm_fwd": (_i, [_p, _i64, _i64, _p, _i64, _p, _p, _f, _i, _p, _i64, _p, _p, _p]),
+    "rtb_layer_norm_backward": (_i, [_p, _i64, _i64, _p, _i64, _p, _p, _p, _p, _i, _p, _i64, _p,
+                                     _i64, _p, _p, _i, _p]),
+    "rtb_layer_norm_backward_fp8": (_i, [_p, _i64, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p, _i,
+                                         _p, _i64, _p, _i64, _p, _p, _i, _p]),
+    "rtb_fp8_quantize": (_i, [_p, _i64, _i64, _p, _i64, _i, _p, _i64, _p, _i64, _p]),
+    "rtb_fp8_dequantize": (_i, [_p, _i64, _i64, _p, _i64, _p, _i64, _i, _p, _i64, _p]),
+    "rtb_fp8_matmul": (_i, [_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _i, _i, _p, _i64, _i, _p,
+                            _i64, _i, _i, _p, _i, _p, _i64, _p]),
+    "rtb_matmul_backward_fp8": (_i, [_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _i, _p, _p, _p, _p,
+                                     _i, _i, _p]),
     "rtb_peer_buffer_create": (_i, [_p, _p, _sz, _p]),
     "rtb_peer_buffer_local": (_i, [_p, _p]),
     "rtb_peer_buffer_destroy": (_i, [_p, _p]),

@@ -82,6 +82,30 @@ int make_tmap_2d_swz(CUtensorMap* map, const void* base, uint64_t dim0, uint64_t
   return RTB_OK;
 }
 
+int make_tmap_2d_bytes(CUtensorMap* map, const void* base, int elem_bytes, uint64_t dim0,
+                       uint64_t dim1, uint64_t row_stride_elems, uint32_t box0, uint32_t box1) {
+  EncodeTiledFn enc = get_encode_tiled();
+  if (!enc) return set_error(RTB_E_CUDA, "cuTensorMapEncodeTiled unavailable");
+  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || (row_stride_elems * elem_bytes) % 16 != 0)
+    return set_error(RTB_E_INVALID, "tensor map: base and row stride must be multiples of 16 bytes");
+  const cuuint64_t dims[2] = {dim0, dim1};
+  const cuuint64_t strides[1] = {row_stride_elems * elem_bytes};
+  const cuuint32_t box[2] = {box0, box1};
+  const cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(map, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                   2, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    char buf[160];
+    snprintf(buf, sizeof buf, "cuTensorMapEncodeTiled failed (%d): dims %llu x %llu stride %llu",
+             (int)r, (unsigned long long)dim0, (unsigned long long)dim1,
+             (unsigned long long)row_stride_elems);
+    return set_error(RTB_E_CUDA, buf);
+  }
+  return RTB_OK;
+}
+
 typedef CUresult (*EncodeIm2colFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                    const cuuint64_t*, const cuuint64_t*, const int*, const int*,
                                    cuuint32_t, cuuint32_t, const cuuint32_t*,
@@ -199,6 +223,9 @@ using namespace rtb;
 
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 static inline int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+// Largest row, column or contraction length of the 8-bit entry points: tile
+// indices and tensor-map coordinates are 32-bit.
+constexpr int64_t kMaxExtent = INT32_MAX - 512;
 
 extern "C" {
 
@@ -1009,6 +1036,236 @@ int rtb_conv2d_backward(rtb_ctx* ctx, int64_t N, int64_t Ci, int64_t H, int64_t 
     if (st) return st;
   }
   return RTB_OK;
+}
+
+// ---------------------------------------------------------------- layer norm, training
+int rtb_layer_norm_fwd(rtb_ctx* ctx, int64_t rows, int64_t d, const float* x, int64_t ldx,
+                       const float* norm_weight, const float* norm_bias, float eps, int act,
+                       float* y, int64_t ldy, float* mean, float* rstd, void* stream) {
+  RTB_CHECK_CTX(ctx);
+  int st;
+  if ((st = check_act(act))) return st;
+  if (rows < 0 || d < 0) return set_error(RTB_E_INVALID, "layer_norm_fwd: negative dimension");
+  if (rows == 0) return RTB_OK;
+  if (d == 0) return set_error(RTB_E_INVALID, "layer_norm_fwd: rows of no columns have no statistics");
+  if (!x || !y || !mean || !rstd) return set_error(RTB_E_INVALID, "layer_norm_fwd: null pointer");
+  if (ldx < d || ldy < d) return set_error(RTB_E_INVALID, "layer_norm_fwd: leading dimension below d");
+  DeviceGuard g(ctx->device);
+  return launch_layernorm_act(ctx, x, ldx, y, ldy, rows, d, norm_weight, norm_bias, eps, act,
+                              pick_stream(ctx, stream), mean, rstd);
+}
+
+static int layer_norm_backward(rtb_ctx* ctx, const char* who, NormBwdDesc& n, void* stream) {
+  int st;
+  if ((st = check_act(n.act))) return st;
+  const std::string w = std::string(who) + ": ";
+  if (n.rows < 0 || n.d < 0) return set_error(RTB_E_INVALID, w + "negative dimension");
+  if (n.d > kMaxExtent) return set_error(RTB_E_UNSUPPORTED, w + "d too large");
+  if (n.d == 0 || (!n.dx && !n.dg && !n.db)) return RTB_OK;
+  DeviceGuard g(ctx->device);
+  cudaStream_t s = pick_stream(ctx, stream);
+  if (n.rows == 0) {  // empty sums
+    if (n.accumulate) return RTB_OK;
+    cudaError_t e = cudaSuccess;
+    if (n.dg) e = cudaMemsetAsync(n.dg, 0, (size_t)n.d * 4, s);
+    if (e == cudaSuccess && n.db) e = cudaMemsetAsync(n.db, 0, (size_t)n.d * 4, s);
+    return e == cudaSuccess ? RTB_OK : cuda_status(e, "layer_norm_backward memset");
+  }
+  if ((!n.x && !(n.q && n.scale)) || !n.mean || !n.rstd || !n.dy)
+    return set_error(RTB_E_INVALID, w + "null pointer");
+  if ((n.x && n.ldx < n.d) || (n.q && (n.ldq < n.d || n.lds < (n.d + 127) / 128)) ||
+      n.lddy < n.d || (n.dx && n.lddx < n.d))
+    return set_error(RTB_E_INVALID, w + "leading dimension below the row's length");
+  return norm_backward_run(ctx, n, s);
+}
+
+int rtb_layer_norm_backward(rtb_ctx* ctx, int64_t rows, int64_t d, const float* x, int64_t ldx,
+                            const float* mean, const float* rstd, const float* norm_weight,
+                            const float* norm_bias, int act, const float* dy, int64_t lddy,
+                            float* dx, int64_t lddx, float* dweight, float* dbias, int accumulate,
+                            void* stream) {
+  RTB_CHECK_CTX(ctx);
+  NormBwdDesc n;
+  n.rows = rows; n.d = d; n.x = x; n.ldx = ldx; n.mean = mean; n.rstd = rstd;
+  n.g = norm_weight; n.b = norm_bias; n.act = act; n.dy = dy; n.lddy = lddy;
+  n.dx = dx; n.lddx = lddx; n.dg = dweight; n.db = dbias; n.accumulate = accumulate;
+  return layer_norm_backward(ctx, "layer_norm_backward", n, stream);
+}
+
+int rtb_layer_norm_backward_fp8(rtb_ctx* ctx, int64_t rows, int64_t d, const uint8_t* q,
+                                int64_t ldq, const uint8_t* scale, int64_t lds, const float* mean,
+                                const float* rstd, const float* norm_weight,
+                                const float* norm_bias, int act, const float* dy, int64_t lddy,
+                                float* dx, int64_t lddx, float* dweight, float* dbias,
+                                int accumulate, void* stream) {
+  RTB_CHECK_CTX(ctx);
+  NormBwdDesc n;
+  n.rows = rows; n.d = d; n.q = q; n.ldq = ldq; n.scale = scale; n.lds = lds; n.mean = mean;
+  n.rstd = rstd; n.g = norm_weight; n.b = norm_bias; n.act = act; n.dy = dy; n.lddy = lddy;
+  n.dx = dx; n.lddx = lddx; n.dg = dweight; n.db = dbias; n.accumulate = accumulate;
+  return layer_norm_backward(ctx, "layer_norm_backward_fp8", n, stream);
+}
+
+// ---------------------------------------------------------------- 8-bit block-scaled tensors
+static int check_blocks(const char* who, int64_t rows, int64_t cols, int block_rows) {
+  const std::string w = std::string(who) + ": ";
+  if (rows < 0 || cols < 0) return set_error(RTB_E_INVALID, w + "negative dimension");
+  if (block_rows != 1 && block_rows != 128)
+    return set_error(RTB_E_INVALID, w + "block_rows must be 1 or 128");
+  if (cols > kMaxExtent) return set_error(RTB_E_UNSUPPORTED, w + "too many columns");
+  return RTB_OK;
+}
+
+int rtb_fp8_quantize(rtb_ctx* ctx, int64_t rows, int64_t cols, const float* x, int64_t ldx,
+                     int block_rows, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds,
+                     void* stream) {
+  RTB_CHECK_CTX(ctx);
+  int st;
+  if ((st = check_blocks("fp8_quantize", rows, cols, block_rows))) return st;
+  if (rows == 0 || cols == 0) return RTB_OK;
+  if (!x || !q || !scale) return set_error(RTB_E_INVALID, "fp8_quantize: null pointer");
+  if (ldx < cols || ldq < cols || lds < (cols + 127) / 128)
+    return set_error(RTB_E_INVALID, "fp8_quantize: leading dimension below the row's length");
+  DeviceGuard g(ctx->device);
+  return launch_fp8_quantize(ctx, x, ldx, rows, cols, block_rows, q, ldq, scale, lds,
+                             pick_stream(ctx, stream));
+}
+
+int rtb_fp8_dequantize(rtb_ctx* ctx, int64_t rows, int64_t cols, const uint8_t* q, int64_t ldq,
+                       const uint8_t* scale, int64_t lds, int block_rows, float* y, int64_t ldy,
+                       void* stream) {
+  RTB_CHECK_CTX(ctx);
+  int st;
+  if ((st = check_blocks("fp8_dequantize", rows, cols, block_rows))) return st;
+  if (rows == 0 || cols == 0) return RTB_OK;
+  if (!q || !scale || !y) return set_error(RTB_E_INVALID, "fp8_dequantize: null pointer");
+  if (ldy < cols || ldq < cols || lds < (cols + 127) / 128)
+    return set_error(RTB_E_INVALID, "fp8_dequantize: leading dimension below the row's length");
+  DeviceGuard g(ctx->device);
+  return launch_fp8_dequantize(ctx, q, ldq, rows, cols, scale, lds, block_rows, y, ldy,
+                               pick_stream(ctx, stream));
+}
+
+// [rows, K] e4m3 with K contiguous, as the tensor maps want it: the caller's
+// matrix where its base and row stride are multiples of 16 bytes, else a copy.
+static int fp8_operand(rtb_ctx* ctx, const uint8_t* src, int64_t rows, int64_t K, int64_t rs,
+                       int64_t cs, const uint8_t** out, int64_t* ld, void** ws, cudaStream_t s) {
+  if (cs == 1 && aligned16(src) && rs % 16 == 0) {
+    *out = src;
+    *ld = rs;
+    return RTB_OK;
+  }
+  const int64_t Kp = round_up(K, 16);
+  int st = ws_alloc(ctx, ws, (size_t)(rows * Kp), s);
+  if (st) return st;
+  *out = static_cast<const uint8_t*>(*ws);
+  *ld = Kp;
+  return launch_pack_bytes(ctx, src, rows, K, rs, cs, static_cast<uint8_t*>(*ws), Kp, s);
+}
+
+int rtb_fp8_matmul(rtb_ctx* ctx, int64_t M, int64_t N, int64_t K, const uint8_t* A, int64_t lda,
+                   const void* scale_a, int64_t ldsa, int block_rows_a, int scale_type_a,
+                   const uint8_t* B, int64_t ldb, int transB, const void* scale_b, int64_t ldsb,
+                   int block_rows_b, int scale_type_b, const float* bias, int act, float* C,
+                   int64_t ldc, void* stream) {
+  RTB_CHECK_CTX(ctx);
+  int st;
+  if (M < 0 || N < 0 || K < 0) return set_error(RTB_E_INVALID, "fp8_matmul: negative dimension");
+  if (transB != 0 && transB != 1) return set_error(RTB_E_INVALID, "fp8_matmul: transB must be 0 or 1");
+  if ((st = check_act(act))) return st;
+  if ((block_rows_a != 1 && block_rows_a != 128) || (block_rows_b != 1 && block_rows_b != 128))
+    return set_error(RTB_E_INVALID, "fp8_matmul: block_rows must be 1 or 128");
+  if ((scale_type_a != RTB_SCALE_E8M0 && scale_type_a != RTB_SCALE_F32) ||
+      (scale_type_b != RTB_SCALE_E8M0 && scale_type_b != RTB_SCALE_F32))
+    return set_error(RTB_E_INVALID, "fp8_matmul: unknown scale type");
+  if (!transB && block_rows_b != 128)
+    return set_error(RTB_E_UNSUPPORTED, "fp8_matmul: a [K,N] B needs 128 x 128 blocks");
+  if (M > kMaxExtent || N > kMaxExtent || K > kMaxExtent)
+    return set_error(RTB_E_UNSUPPORTED, "fp8_matmul: dimension too large");
+  if (M == 0 || N == 0) return RTB_OK;
+  if (!C) return set_error(RTB_E_INVALID, "fp8_matmul: null C");
+  if (ldc < N) return set_error(RTB_E_INVALID, "fp8_matmul: ldc < N");
+  DeviceGuard g(ctx->device);
+  cudaStream_t s = pick_stream(ctx, stream);
+  if (K == 0) return launch_fill_rows(C, M, N, ldc, bias, act, s);
+  if (!A || !B || !scale_a || !scale_b) return set_error(RTB_E_INVALID, "fp8_matmul: null operand");
+  const int64_t kb = (K + 127) / 128, nb = (N + 127) / 128;
+  if (lda < K || ldb < (transB ? K : N) || ldsa < kb || ldsb < (transB ? kb : nb))
+    return set_error(RTB_E_INVALID, "fp8_matmul: leading dimension below the row's length");
+  Fp8Desc d;
+  d.M = M; d.N = N; d.K = K; d.bias = bias; d.act = act; d.C = C; d.ldc = ldc;
+  d.sa.p = scale_a;
+  d.sa.ld_row = ldsa;
+  d.sa.row_shift = block_rows_a == 1 ? 0 : 7;
+  d.sa.is_f32 = scale_type_a == RTB_SCALE_F32;
+  d.sb.p = scale_b;
+  d.sb.ld_row = transB ? ldsb : 1;
+  d.sb.ld_col = transB ? 1 : ldsb;
+  d.sb.row_shift = block_rows_b == 1 ? 0 : 7;
+  d.sb.is_f32 = scale_type_b == RTB_SCALE_F32;
+  void *wa = nullptr, *wb = nullptr;
+  st = fp8_operand(ctx, A, M, K, lda, 1, &d.A, &d.lda, &wa, s);
+  if (st == RTB_OK)
+    st = fp8_operand(ctx, B, N, K, transB ? ldb : 1, transB ? 1 : ldb, &d.B, &d.ldb, &wb, s);
+  if (st == RTB_OK) st = fp8_gemm_run(ctx, d, s);
+  ws_free(wa, s);
+  ws_free(wb, s);
+  return st;
+}
+
+int rtb_matmul_backward_fp8(rtb_ctx* ctx, int64_t M, int64_t N, int64_t K, const uint8_t* A,
+                            int64_t lda, const uint8_t* scale_a, int64_t ldsa, int block_rows_a,
+                            const float* B, const float* dC, float* dA, float* dB, int accumulate,
+                            int precision, void* stream) {
+  RTB_CHECK_CTX(ctx);
+  int split3 = 1, st;
+  if ((st = check_blocks("matmul_backward_fp8", M, K, block_rows_a))) return st;
+  if (N < 0) return set_error(RTB_E_INVALID, "negative dimension");
+  if (M > kMaxExtent / 4 || N > kMaxExtent)
+    return set_error(RTB_E_UNSUPPORTED, "matmul_backward_fp8: dimension too large");
+  if ((st = resolve_precision(ctx, precision, &split3))) return st;
+  if (dB && M > 0 && N > 0 && K > 0) {
+    if (!A || !scale_a || !dC) return set_error(RTB_E_INVALID, "matmul_backward_fp8: null operand");
+    if (lda < K || ldsa < (K + 127) / 128)
+      return set_error(RTB_E_INVALID, "matmul_backward_fp8: leading dimension below the row's length");
+  }
+  // grad_lhs does not read the checkpoint (null A: no grad_rhs in that call)
+  if (dA && (st = rtb_matmul_backward(ctx, M, N, K, nullptr, B, dC, dA, nullptr, accumulate,
+                                      precision, stream)))
+    return st;
+  if (!dB || K == 0 || N == 0) return RTB_OK;
+  DeviceGuard g(ctx->device);
+  cudaStream_t s = pick_stream(ctx, stream);
+  if (M == 0) {
+    if (accumulate) return RTB_OK;
+    cudaError_t e = cudaMemsetAsync(dB, 0, (size_t)(K * N) * 4, s);
+    return e == cudaSuccess ? RTB_OK : cuda_status(e, "matmul_backward_fp8 memset");
+  }
+  // grad_rhs = deq(A)^T . dC: the checkpoint is exact in bf16 and dC is the sum
+  // of three bf16 terms (24 bits; two in TF32 mode: 16 bits, TF32 keeps 11)
+  WgradDesc w;
+  w.rows = M;
+  w.rows_pad = round_up(M, 64);
+  w.K = K;
+  w.N = N;
+  w.ldx = round_up(K, 8);
+  w.ldy = round_up(N, 8);
+  w.pieces = split3 ? 3 : 2;
+  w.D = dB;
+  w.ldd = N;
+  w.accumulate = accumulate;
+  void *wx = nullptr, *wy = nullptr;
+  st = ws_alloc(ctx, &wx, (size_t)(w.rows_pad * w.ldx) * 2, s);
+  if (st == RTB_OK) st = ws_alloc(ctx, &wy, (size_t)(w.pieces * w.rows_pad * w.ldy) * 2, s);
+  w.X = wx;
+  w.Y = wy;
+  if (st == RTB_OK)
+    st = launch_decode_bf16(ctx, A, lda, M, K, scale_a, ldsa, block_rows_a, wx, w.ldx, w.rows_pad, s);
+  if (st == RTB_OK) st = launch_split_bf16(ctx, dC, N, M, N, wy, w.ldy, w.rows_pad, w.pieces, s);
+  if (st == RTB_OK) st = wgrad_run(ctx, w, s);
+  ws_free(wx, s);
+  ws_free(wy, s);
+  return st;
 }
 
 // ---------------------------------------------------------------- small ops

@@ -80,6 +80,11 @@ constexpr int kTmapSwizzleNone = 0, kTmapSwizzle128 = 1, kTmapSwizzle128Atom32 =
 int make_tmap_2d_swz(CUtensorMap* map, const void* base, uint64_t dim0, uint64_t dim1,
                      uint64_t row_stride_elems, uint32_t box0, uint32_t box1, int swizzle);
 
+// 2-D map of 1-byte or bf16 elements (elem_bytes 1 or 2), 128-byte swizzle:
+// base 16-byte aligned, row stride a multiple of 16 bytes.
+int make_tmap_2d_bytes(CUtensorMap* map, const void* base, int elem_bytes, uint64_t dim0,
+                       uint64_t dim1, uint64_t row_stride_elems, uint32_t box0, uint32_t box1);
+
 // 4-D im2col map over an NHWC tensor [N, H, W, Cp] for a forward conv with
 // filter R x S, stride (sh, sw), padding (ph, pw): channels_per_pixel x
 // pixels_per_column boxes, rows swizzled in 16-byte units over swizzle_bytes
@@ -213,7 +218,79 @@ int launch_unpack_weight_grad(const float* dwp, int64_t Co, int64_t Ci, int64_t 
 // matrices (X == Y allowed); g / b optional.
 int launch_layernorm_act(rtb_ctx* ctx, const float* X, int64_t ldx, float* Y, int64_t ldy,
                          int64_t M, int64_t N, const float* g, const float* b, float eps, int act,
-                         cudaStream_t s);
+                         cudaStream_t s, float* mean = nullptr, float* rstd = nullptr);
+
+// LayerNorm backward (rtb_norm_bwd.cu): x as fp32 (x != null) or as an 8-bit
+// checkpoint (q, scale); mean, rstd as the forward pass left them.  Any of dx,
+// dg, db may be null.
+struct NormBwdDesc {
+  int64_t rows = 0, d = 0;
+  const float* x = nullptr;
+  int64_t ldx = 0;
+  const uint8_t* q = nullptr;  // e4m3 [rows, d], one scale byte per 128 columns of a row
+  int64_t ldq = 0;
+  const uint8_t* scale = nullptr;
+  int64_t lds = 0;
+  const float *mean = nullptr, *rstd = nullptr;
+  const float *g = nullptr, *b = nullptr;  // null: 1 and 0
+  int act = 0;
+  const float* dy = nullptr;
+  int64_t lddy = 0;
+  float* dx = nullptr;
+  int64_t lddx = 0;
+  float *dg = nullptr, *db = nullptr;
+  int accumulate = 0;
+};
+int norm_backward_run(rtb_ctx* ctx, const NormBwdDesc& d, cudaStream_t s);
+
+// 8-bit block-scaled tensors (rtb_fp8.cu).
+int launch_fp8_quantize(rtb_ctx* ctx, const float* x, int64_t ldx, int64_t rows, int64_t cols,
+                        int block_rows, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds,
+                        cudaStream_t s);
+int launch_fp8_dequantize(rtb_ctx* ctx, const uint8_t* q, int64_t ldq, int64_t rows, int64_t cols,
+                          const uint8_t* scale, int64_t lds, int block_rows, float* y, int64_t ldy,
+                          cudaStream_t s);
+// dst[r][c] = c < cols ? src[r * rs + c * cs] : 0 for c < ldd (rs or cs is 1).
+int launch_pack_bytes(rtb_ctx* ctx, const uint8_t* src, int64_t rows, int64_t cols, int64_t rs,
+                      int64_t cs, uint8_t* dst, int64_t ldd, cudaStream_t s);
+// bf16 copy of an 8-bit tensor, and fp32 as a sum of bf16 terms ([pieces]
+// [rows_pad][ldo]); ldo % 8 == 0, zero padded.
+int launch_decode_bf16(rtb_ctx* ctx, const uint8_t* q, int64_t ldq, int64_t rows, int64_t cols,
+                       const uint8_t* scale, int64_t lds, int block_rows, void* out, int64_t ldo,
+                       int64_t rows_pad, cudaStream_t s);
+int launch_split_bf16(rtb_ctx* ctx, const float* x, int64_t ldx, int64_t rows, int64_t cols,
+                      void* out, int64_t ldo, int64_t rows_pad, int pieces, cudaStream_t s);
+
+// Block-scaled products on the tensor cores (rtb_blockgemm.cu).
+struct ScaleRef {            // scale of the 128-column block kb of row r:
+  const void* p = nullptr;   // p[(r >> row_shift) * ld_row + kb * ld_col]
+  int64_t ld_row = 0, ld_col = 1;
+  int row_shift = 0;
+  int is_f32 = 0;            // fp32 values, else e8m0 bytes
+};
+struct Fp8Desc {  // C [M, N] = act(A . B^T + bias): A [M, K], B [N, K] e4m3, K-major
+  int64_t M = 0, N = 0, K = 0;
+  const uint8_t *A = nullptr, *B = nullptr;
+  int64_t lda = 0, ldb = 0;  // 16-byte aligned bases, multiples of 16
+  ScaleRef sa, sb;
+  const float* bias = nullptr;
+  int act = 0;
+  float* C = nullptr;
+  int64_t ldc = 0;
+};
+int fp8_gemm_run(rtb_ctx* ctx, const Fp8Desc& d, cudaStream_t s);
+// D [K, N] (+)= X^T . Y over `rows`: X bf16 [rows, ldx], Y = the sum of
+// `pieces` bf16 matrices [pieces][rows_pad][ldy] (launch_split_bf16).
+struct WgradDesc {
+  int64_t rows = 0, rows_pad = 0, K = 0, N = 0;
+  const void *X = nullptr, *Y = nullptr;
+  int64_t ldx = 0, ldy = 0;
+  int pieces = 3;
+  float* D = nullptr;
+  int64_t ldd = 0;
+  int accumulate = 0;
+};
+int wgrad_run(rtb_ctx* ctx, const WgradDesc& d, cudaStream_t s);
 
 // Stream-ordered workspace.
 int ws_alloc(rtb_ctx* ctx, void** p, size_t bytes, cudaStream_t s);

@@ -12,6 +12,8 @@
 //     flight per SM;
 //   other rows: one 256-thread CTA per row, block reductions in double, the
 //     row staged in shared memory (or re-read through L2 beyond 16384).
+// Training takes the row's mean and 1 / std from the same pass (8 bytes a row
+// more, written by one thread).
 // Both grids are the resident CTAs with rows strided over them; the output is
 // written with streaming stores.
 #include <cmath>
@@ -63,7 +65,8 @@ __global__ void __launch_bounds__(256) layernorm_act_rows_kernel(const float* X,
                                                                  int64_t M, int N,
                                                                  const float* __restrict__ g,
                                                                  const float* __restrict__ b,
-                                                                 float eps, int act) {
+                                                                 float eps, int act, float* mean_out,
+                                                                 float* rstd_out) {
   constexpr int G = VEC ? E / 4 : E;  // loads per thread
   constexpr int R = 256 / T;          // rows per CTA
   constexpr int W = T / 32;           // warps per row
@@ -115,6 +118,10 @@ __global__ void __launch_bounds__(256) layernorm_act_rows_kernel(const float* X,
     }
     const double var = group_sum((double)q, red_q) / N;
     const float inv_std = (float)(1.0 / sqrt(var + (double)eps));
+    if (mean_out && t == 0) {
+      mean_out[m] = meanf;
+      rstd_out[m] = inv_std;
+    }
     float* out = Y + m * ldy;
 #pragma unroll
     for (int i = 0; i < G; ++i) {
@@ -152,7 +159,9 @@ __global__ void __launch_bounds__(kLnThreads) layernorm_act_kernel(const float* 
                                                                    int64_t M, int N,
                                                                    const float* __restrict__ g,
                                                                    const float* __restrict__ b,
-                                                                   float eps, int act) {
+                                                                   float eps, int act,
+                                                                   float* mean_out,
+                                                                   float* rstd_out) {
   extern __shared__ float4 srow4[];
   float* srow = reinterpret_cast<float*>(srow4);
   __shared__ double red[kLnThreads / 32];
@@ -199,6 +208,10 @@ __global__ void __launch_bounds__(kLnThreads) layernorm_act_kernel(const float* 
     const double var = block_sum(q, red) / N;
     const float inv_std = (float)(1.0 / sqrt(var + (double)eps));
     const float meanf = (float)mean;
+    if (mean_out && threadIdx.x == 0) {
+      mean_out[m] = meanf;
+      rstd_out[m] = inv_std;
+    }
     if (VEC) {
       const float4* g4 = reinterpret_cast<const float4*>(g);
       const float4* b4 = reinterpret_cast<const float4*>(b);
@@ -238,7 +251,8 @@ __global__ void __launch_bounds__(kLnThreads) layernorm_act_kernel(const float* 
 
 template <bool VEC, bool ON_CHIP>
 int launch_ln(const float* X, int64_t ldx, float* Y, int64_t ldy, int64_t M, int N,
-              const float* g, const float* b, float eps, int act, cudaStream_t s) {
+              const float* g, const float* b, float eps, int act, float* mean, float* rstd,
+              cudaStream_t s) {
   auto* k = layernorm_act_kernel<VEC, ON_CHIP>;
   const size_t smem = ON_CHIP ? (size_t)((N + 3) & ~3) * sizeof(float) : 0;
   int dev = 0, sms = 148;
@@ -255,14 +269,15 @@ int launch_ln(const float* X, int64_t ldx, float* Y, int64_t ldy, int64_t M, int
   const int64_t blocks = M < cap ? M : cap;
   clear_stale_cuda_error();
   cudaError_t e = launch_pdl(k, dim3((unsigned)blocks), dim3(kLnThreads), smem, s, X, ldx, Y, ldy,
-                             M, N, g, b, eps, act);
+                             M, N, g, b, eps, act, mean, rstd);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? RTB_OK : cuda_status(e, "layernorm kernel launch");
 }
 
 template <int T, int E, bool VEC>
 int launch_ln_rows(rtb_ctx* ctx, const float* X, int64_t ldx, float* Y, int64_t ldy, int64_t M,
-                   int N, const float* g, const float* b, float eps, int act, cudaStream_t s) {
+                   int N, const float* g, const float* b, float eps, int act, float* mean,
+                   float* rstd, cudaStream_t s) {
   auto* k = layernorm_act_rows_kernel<T, E, VEC>;
   int per_sm = 1;
   cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, 256, 0);
@@ -272,7 +287,7 @@ int launch_ln_rows(rtb_ctx* ctx, const float* X, int64_t ldx, float* Y, int64_t 
   const int64_t blocks = need < cap ? need : cap;
   clear_stale_cuda_error();
   cudaError_t e = launch_pdl(k, dim3((unsigned)blocks), dim3(256), 0, s, X, ldx, Y, ldy, M, N, g, b,
-                             eps, act);
+                             eps, act, mean, rstd);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? RTB_OK : cuda_status(e, "layernorm (rows) kernel launch");
 }
@@ -281,7 +296,7 @@ int launch_ln_rows(rtb_ctx* ctx, const float* X, int64_t ldx, float* Y, int64_t 
 
 int launch_layernorm_act(rtb_ctx* ctx, const float* X, int64_t ldx, float* Y, int64_t ldy,
                          int64_t M, int64_t N, const float* g, const float* b, float eps, int act,
-                         cudaStream_t s) {
+                         cudaStream_t s, float* mean, float* rstd) {
   if (M <= 0 || N <= 0) return RTB_OK;
   if (N > INT32_MAX) return set_error(RTB_E_UNSUPPORTED, "layernorm: N too large");
   auto al16 = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
@@ -290,26 +305,26 @@ int launch_layernorm_act(rtb_ctx* ctx, const float* X, int64_t ldx, float* Y, in
   const int n = (int)N;
   if (vec && N <= 16384) {  // T threads per row, up to 16 float4 per thread, in registers
     const int per = (int)((N / 4 + 31) / 32);  // float4 per lane of one warp
-    if (per <= 1) return launch_ln_rows<32, 4, true>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, s);
-    if (per <= 2) return launch_ln_rows<32, 8, true>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, s);
-    if (per <= 4) return launch_ln_rows<32, 16, true>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, s);
-    if (per <= 8) return launch_ln_rows<32, 32, true>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, s);
-    if (per <= 16) return launch_ln_rows<64, 32, true>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, s);
-    if (per <= 32) return launch_ln_rows<128, 32, true>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, s);
-    if (per <= 64) return launch_ln_rows<256, 32, true>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, s);
-    return launch_ln_rows<256, 64, true>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, s);
+    if (per <= 1) return launch_ln_rows<32, 4, true>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, mean, rstd, s);
+    if (per <= 2) return launch_ln_rows<32, 8, true>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, mean, rstd, s);
+    if (per <= 4) return launch_ln_rows<32, 16, true>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, mean, rstd, s);
+    if (per <= 8) return launch_ln_rows<32, 32, true>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, mean, rstd, s);
+    if (per <= 16) return launch_ln_rows<64, 32, true>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, mean, rstd, s);
+    if (per <= 32) return launch_ln_rows<128, 32, true>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, mean, rstd, s);
+    if (per <= 64) return launch_ln_rows<256, 32, true>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, mean, rstd, s);
+    return launch_ln_rows<256, 64, true>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, mean, rstd, s);
   }
   if (!vec && N <= 512) {  // one warp per row, scalar
     const int per = (int)((N + 31) / 32);
-    if (per <= 4) return launch_ln_rows<32, 4, false>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, s);
-    if (per <= 8) return launch_ln_rows<32, 8, false>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, s);
-    return launch_ln_rows<32, 16, false>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, s);
+    if (per <= 4) return launch_ln_rows<32, 4, false>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, mean, rstd, s);
+    if (per <= 8) return launch_ln_rows<32, 8, false>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, mean, rstd, s);
+    return launch_ln_rows<32, 16, false>(ctx, X, ldx, Y, ldy, M, n, g, b, eps, act, mean, rstd, s);
   }
   // a CTA per row: float4-aligned rows beyond 16384 columns (re-read through
   // L2), other rows staged in shared memory up to 16384 columns
-  if (vec) return launch_ln<true, false>(X, ldx, Y, ldy, M, n, g, b, eps, act, s);
-  return N <= kLnMaxOnChip ? launch_ln<false, true>(X, ldx, Y, ldy, M, n, g, b, eps, act, s)
-                           : launch_ln<false, false>(X, ldx, Y, ldy, M, n, g, b, eps, act, s);
+  if (vec) return launch_ln<true, false>(X, ldx, Y, ldy, M, n, g, b, eps, act, mean, rstd, s);
+  return N <= kLnMaxOnChip ? launch_ln<false, true>(X, ldx, Y, ldy, M, n, g, b, eps, act, mean, rstd, s)
+                           : launch_ln<false, false>(X, ldx, Y, ldy, M, n, g, b, eps, act, mean, rstd, s);
 }
 
 }  // namespace rtb

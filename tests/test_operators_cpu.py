@@ -1,0 +1,46 @@
+"""Refusals of the training and 8-bit entry points that need no GPU: a null
+context, tensors that are not on one, wrong types."""
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def rb():
+    from rustorch_b200 import build
+    build.build()
+    import rustorch_b200
+    rustorch_b200.lib()
+    return rustorch_b200
+
+
+def test_null_context(rb):
+    L = rb.lib()
+    for st in (
+            L.rtb_layer_norm_fwd(None, 2, 2, None, 2, None, None, 1e-5, 0, None, 2, None, None, None),
+            L.rtb_layer_norm_backward(None, 2, 2, None, 2, None, None, None, None, 0, None, 2, None,
+                                      2, None, None, 0, None),
+            L.rtb_layer_norm_backward_fp8(None, 2, 2, None, 2, None, 1, None, None, None, None, 0,
+                                          None, 2, None, 2, None, None, 0, None),
+            L.rtb_fp8_quantize(None, 2, 2, None, 2, 1, None, 2, None, 1, None),
+            L.rtb_fp8_dequantize(None, 2, 2, None, 2, None, 1, 1, None, 2, None),
+            L.rtb_fp8_matmul(None, 2, 2, 2, None, 2, None, 1, 1, 0, None, 2, 1, None, 1, 1, 0, None,
+                             0, None, 2, None),
+            L.rtb_matmul_backward_fp8(None, 2, 2, 2, None, 2, None, 1, 1, None, None, None, None, 0,
+                                      0, None)):
+        assert st == rb._lib.RTB_E_INVALID
+        assert "rtb_ctx" in rb._lib.last_error()
+
+
+def test_host_tensors_refused(rb):
+    x = torch.zeros((4, 128))
+    q = x.to(torch.float8_e4m3fn)
+    s = torch.full((4, 1), 127, dtype=torch.uint8).view(torch.float8_e8m0fnu)
+    m = torch.zeros(4)
+    for call in (lambda: rb.fp8_quantize(x), lambda: rb.fp8_dequantize(q, s),
+                 lambda: rb.fp8_matmul(q, s, q.t(), s.t()),
+                 lambda: rb.matmul_backward_fp8(q, s, None, x, need_a=False),
+                 lambda: rb.layer_norm_fwd(x),
+                 lambda: rb.layer_norm_backward(x, m, m, x),
+                 lambda: rb.layer_norm_backward(q, m, m, x, x_scale=s)):
+        with pytest.raises(ValueError):
+            call()
