@@ -73,12 +73,14 @@ _contexts: dict = {}
 
 
 def get_context(device: int = 0) -> Context:
-    with _ctx_lock:
-        c = _contexts.get(device)
-        if c is None:
-            c = Context(device)
-            _contexts[device] = c
-        return c
+    c = _contexts.get(device)
+    if c is None:
+        with _ctx_lock:
+            c = _contexts.get(device)
+            if c is None:
+                c = Context(device)
+                _contexts[device] = c
+    return c
 
 
 def _torch():
@@ -87,8 +89,9 @@ def _torch():
 
 
 def _stream_of(t):
-    torch = _torch()
-    return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+    # the raw handle (an int): making a torch Stream object for it costs 2 us a
+    # call, a tenth of a small operator's time
+    return _torch()._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _dev(t) -> int:
@@ -96,16 +99,14 @@ def _dev(t) -> int:
 
 
 def _check_f32_cuda(*ts):
-    torch = _torch()
+    f32 = _torch().float32
     for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda or t.dtype != torch.float32:
+        if t is not None and not (t.is_cuda and t.dtype is f32):
             raise ValueError("rustorch_b200 expects float32 CUDA tensors")
 
 
 def _ptr(t):
-    return ctypes.c_void_p(t.data_ptr()) if t is not None else None
+    return t.data_ptr() if t is not None else None
 
 
 def _operand_2d(t):
@@ -180,9 +181,7 @@ def layer_norm(x, norm_weight=None, norm_bias=None, eps: float = 1e-5, act: int 
     if x.dim() == 0:
         raise ValueError("LayerNorm: Input shape smaller than normalized shape")
     d = x.shape[-1]
-    x2 = x.reshape(-1, d) if d else x.reshape(-1, 0)
-    if x2.numel() and x2.stride(1) != 1:
-        x2 = x2.contiguous()
+    x2 = _rows_2d(x, d) if d else x.reshape(-1, 0)
     for t in (norm_weight, norm_bias):
         if t is not None and t.numel() != d:
             raise ValueError("LayerNorm: Input shape does not match normalized shape")
@@ -288,48 +287,85 @@ def conv2d_backward(x, w, grad, stride=(1, 1), padding=(0, 0), need_x: bool = Tr
 def _rows_2d(t, d):
     """t as [rows, d] with contiguous rows that do not overlap (a copy only where
     t has no such view: a transposed or an expanded tensor)."""
+    if t.is_contiguous():
+        return t if t.dim() == 2 else t.view(-1, d)
     t2 = t.reshape(-1, d) if t.dim() != 2 else t
     if (d > 1 and t2.stride(1) != 1) or (t2.shape[0] > 1 and t2.stride(0) < d):
         t2 = t2.contiguous()
     return t2
 
 
-def _same_device(*ts):
-    dev = None
-    for t in ts:
-        if t is None:
-            continue
-        if dev is not None and t.device != dev:
+def _ld(t, d):
+    """Leading dimension of _rows_2d's result (a single row's stride says nothing)."""
+    return max(t.stride(0), d)
+
+
+def _flat(t, n, message):
+    """A vector of n elements, contiguous; None stays None."""
+    if t is None:
+        return None
+    if t.numel() != n:
+        raise ValueError(message)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _same_device(first, *rest):
+    dev = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != dev:
             raise ValueError("rustorch_b200: tensors on different devices")
-        dev = t.device
+    return dev
+
+
+def _empty_like(x):
+    """float32, contiguous, of x's shape and on its device."""
+    torch = _torch()
+    if x.dtype is torch.float32 and x.is_contiguous():
+        return torch.empty_like(x)
+    return torch.empty(x.shape, dtype=torch.float32, device=x.device)
+
+
+def _result(out, need, accumulate, shape, like, who):
+    """The tensor that a gradient is written to (or added to): `out` or a new one."""
+    if not need:
+        return None
+    if out is None:
+        if accumulate:
+            raise ValueError(f"{who}: accumulate adds to given outputs")
+        return like.new_empty(shape, dtype=_torch().float32)
+    if not out.is_contiguous() or tuple(out.shape) != tuple(shape):
+        raise ValueError(f"{who}: outputs must be contiguous and of the gradient's shape")
+    return out
+
+
+_LN_SHAPE = "LayerNorm: Input shape does not match normalized shape"
 
 
 def layer_norm_fwd(x, norm_weight=None, norm_bias=None, eps: float = 1e-5, act: int = ACT_NONE,
                    out=None):
     """layer_norm that also returns what its backward pass reads: (y, mean,
     rstd), the statistics float32 of x's leading shape; out may be x."""
-    torch = _torch()
     _check_f32_cuda(x, norm_weight, norm_bias, out)
-    _same_device(x, norm_weight, norm_bias, out)
-    if x.dim() == 0 or x.shape[-1] == 0:
+    dev = _same_device(x, norm_weight, norm_bias, out)
+    d = x.shape[-1] if x.dim() else 0
+    if d == 0:
         raise ValueError("LayerNorm: Input shape smaller than normalized shape")
-    d = x.shape[-1]
-    for t in (norm_weight, norm_bias):
-        if t is not None and t.numel() != d:
-            raise ValueError("LayerNorm: Input shape does not match normalized shape")
+    w, b = _flat(norm_weight, d, _LN_SHAPE), _flat(norm_bias, d, _LN_SHAPE)
     x2 = _rows_2d(x, d)
     if out is None:
-        out = torch.empty(x.shape, dtype=torch.float32, device=x.device)
-    elif out.shape != x.shape or out.stride(-1) != 1:
-        raise ValueError("layer_norm_fwd: out must have x's shape and contiguous rows")
-    y2 = out.view(-1, d)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    rstd = torch.empty_like(mean)
-    norm_weight, norm_bias = (t.contiguous() if t is not None else None
-                              for t in (norm_weight, norm_bias))
-    call("rtb_layer_norm_fwd", get_context(_dev(x)).handle, x2.shape[0], d, _ptr(x2),
-         max(x2.stride(0), d), _ptr(norm_weight), _ptr(norm_bias), float(eps), act, _ptr(y2),
-         max(y2.stride(0), d), _ptr(mean), _ptr(rstd), _stream_of(x))
+        out = y2 = _empty_like(x)
+        ldy = d
+    else:
+        if out.shape != x.shape or (d > 1 and out.stride(-1) != 1):
+            raise ValueError("layer_norm_fwd: out must have x's shape and contiguous rows")
+        y2 = out if out.dim() == 2 else out.view(-1, d)
+        if y2.shape[0] > 1 and y2.stride(0) < d:
+            raise ValueError("layer_norm_fwd: out's rows overlap")
+        ldy = _ld(y2, d)
+    mean = x.new_empty(x.shape[:-1])
+    rstd = x.new_empty(x.shape[:-1])
+    call("rtb_layer_norm_fwd", get_context(dev).handle, x2.shape[0], d, _ptr(x2), _ld(x2, d),
+         _ptr(w), _ptr(b), eps, act, _ptr(y2), ldy, _ptr(mean), _ptr(rstd), _stream_of(x))
     return out, mean, rstd
 
 
@@ -341,75 +377,59 @@ def layer_norm_backward(x, mean, rstd, grad, norm_weight=None, norm_bias=None,
     gradient `grad`; x is the forward's input, float32 or an 8-bit checkpoint
     (fp8_quantize(x) -> x, x_scale).  With accumulate the results are added to
     out_x / out_weight / out_bias."""
-    torch = _torch()
-    saved = x.dtype == torch.float8_e4m3fn
-    _check_f32_cuda(mean, rstd, grad, norm_weight, norm_bias, out_x, out_weight, out_bias,
-                    *(() if saved else (x,)))
-    _same_device(x, mean, rstd, grad, norm_weight, norm_bias, x_scale, out_x, out_weight, out_bias)
-    if x.dim() == 0 or x.shape[-1] == 0 or grad.shape != x.shape:
+    who = "layer_norm_backward"
+    saved = x.dtype is _torch().float8_e4m3fn
+    _check_f32_cuda(mean, rstd, grad, norm_weight, norm_bias, out_x, out_weight, out_bias)
+    if not saved:
+        _check_f32_cuda(x)
+    dev = _same_device(x, mean, rstd, grad, norm_weight, norm_bias, x_scale, out_x, out_weight,
+                       out_bias)
+    d = x.shape[-1] if x.dim() else 0
+    if d == 0 or grad.shape != x.shape:
         raise ValueError("layer_norm_backward: grad must have x's shape, with a last dimension")
-    d = x.shape[-1]
     x2, g2 = _rows_2d(x, d), _rows_2d(grad, d)
     rows = x2.shape[0]
-    if mean.numel() != rows or rstd.numel() != rows:
-        raise ValueError("layer_norm_backward: one mean and rstd for each row")
-    for t in (norm_weight, norm_bias, out_weight, out_bias):
-        if t is not None and t.numel() != d:
-            raise ValueError("LayerNorm: Input shape does not match normalized shape")
+    per_row = "layer_norm_backward: one mean and rstd for each row"
+    mean, rstd = _flat(mean, rows, per_row), _flat(rstd, rows, per_row)
+    w, b = _flat(norm_weight, d, _LN_SHAPE), _flat(norm_bias, d, _LN_SHAPE)
     if saved != (x_scale is not None):
         raise ValueError("layer_norm_backward: x_scale goes with an 8-bit x, and only with one")
-
-    def result(out, need, shape):
-        if not need:
-            return None
-        if out is None:
-            if accumulate:
-                raise ValueError("layer_norm_backward: accumulate adds to given outputs")
-            return torch.empty(shape, dtype=torch.float32, device=x.device)
-        if not out.is_contiguous() or out.numel() != shape.numel():
-            raise ValueError("layer_norm_backward: outputs must be contiguous and of full size")
-        return out
-
-    dx = result(out_x, need_x, x.shape)
-    dw = result(out_weight, need_weight, torch.Size((d,)))
-    db = result(out_bias, need_bias, torch.Size((d,)))
-    mean, rstd = mean.contiguous(), rstd.contiguous()
-    norm_weight, norm_bias = (t.contiguous() if t is not None else None
-                              for t in (norm_weight, norm_bias))
-    rest = (_ptr(mean), _ptr(rstd), _ptr(norm_weight), _ptr(norm_bias), act, _ptr(g2),
-            max(g2.stride(0), d), _ptr(dx), d, _ptr(dw), _ptr(db), int(accumulate), _stream_of(x))
-    h = get_context(_dev(x)).handle
+    dx = _result(out_x, need_x, accumulate, x.shape, grad, who)
+    dw = _result(out_weight, need_weight, accumulate, (d,), grad, who)
+    db = _result(out_bias, need_bias, accumulate, (d,), grad, who)
+    rest = (_ptr(mean), _ptr(rstd), _ptr(w), _ptr(b), act, _ptr(g2), _ld(g2, d), _ptr(dx), d,
+            _ptr(dw), _ptr(db), bool(accumulate), _stream_of(x))
+    h = get_context(dev).handle
     if saved:
-        s2, block_rows, kind = _scales(x_scale, rows, d, "layer_norm_backward")
+        s2, block_rows, kind = _scales(x_scale, rows, d, who)
         if kind != _lib.SCALE_E8M0 or block_rows != 1:
             raise ValueError("layer_norm_backward: a checkpoint has a power-of-two scale for each "
                              "128 columns of a row")
-        call("rtb_layer_norm_backward_fp8", h, rows, d, _ptr(x2), max(x2.stride(0), d), _ptr(s2),
-             s2.stride(0), *rest)
+        call("rtb_layer_norm_backward_fp8", h, rows, d, _ptr(x2), _ld(x2, d), _ptr(s2),
+             _ld(s2, s2.shape[1]), *rest)
     else:
-        call("rtb_layer_norm_backward", h, rows, d, _ptr(x2), max(x2.stride(0), d), *rest)
+        call("rtb_layer_norm_backward", h, rows, d, _ptr(x2), _ld(x2, d), *rest)
     return dx, dw, db
 
 
 def _scales(scale, rows, cols, who):
     """(2-D scales with contiguous rows, block_rows, scale type) of a [rows, cols] 8-bit tensor."""
     torch = _torch()
-    if not scale.is_cuda or scale.dtype not in (torch.float8_e8m0fnu, torch.float32):
+    e8m0 = scale.dtype is torch.float8_e8m0fnu
+    if not scale.is_cuda or not (e8m0 or scale.dtype is torch.float32):
         raise ValueError(f"{who}: scales are float8_e8m0fnu or float32 CUDA tensors")
-    cb = -(-cols // 128)
-    s = scale.reshape(-1, scale.shape[-1]) if scale.dim() != 2 else scale
-    if s.shape[1] != cb or s.shape[0] not in (rows, -(-rows // 128)):
+    cb = (cols + 127) // 128
+    s = _rows_2d(scale, cb)
+    n = s.shape[0]
+    if s.shape[1] != cb or n not in (rows, (rows + 127) // 128):
         raise ValueError(f"{who}: scales must be [rows or ceil(rows / 128), ceil(cols / 128)]")
-    if (s.shape[1] != 1 and s.stride(1) != 1) or s.stride(0) < cb:
-        s = s.contiguous()
-    return (s, 1 if s.shape[0] == rows else 128,
-            _lib.SCALE_E8M0 if s.dtype == torch.float8_e8m0fnu else _lib.SCALE_F32)
+    return s, 1 if n == rows else 128, _lib.SCALE_E8M0 if e8m0 else _lib.SCALE_F32
 
 
 def _check_fp8(who, *ts):
-    torch = _torch()
+    e4m3 = _torch().float8_e4m3fn
     for t in ts:
-        if not t.is_cuda or t.dtype != torch.float8_e4m3fn:
+        if not (t.is_cuda and t.dtype is e4m3):
             raise ValueError(f"{who} expects float8_e4m3fn CUDA tensors")
 
 
@@ -420,45 +440,42 @@ def fp8_quantize(x, block_rows: int = 1):
     operand of fp8_matmul."""
     torch = _torch()
     _check_f32_cuda(x)
-    if x.dim() == 0 or (block_rows != 1 and x.dim() != 2):
-        raise ValueError("fp8_quantize: x needs a last dimension, and two for 128-row blocks")
     if block_rows not in (1, 128):
         raise ValueError("fp8_quantize: block_rows must be 1 or 128")
+    if x.dim() == 0 or (block_rows != 1 and x.dim() != 2):
+        raise ValueError("fp8_quantize: x needs a last dimension, and two for 128-row blocks")
     cols = x.shape[-1]
-    cb = -(-cols // 128)
-    rows = x.numel() // cols if cols else 0
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    lead = x.shape[:-1] if block_rows == 1 else (-(-x.shape[0] // 128),)
-    scale = torch.empty((*lead, cb), dtype=torch.float8_e8m0fnu, device=x.device)
-    if rows and cols:
+    cb = (cols + 127) // 128
+    q = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
+    lead = x.shape[:-1] if block_rows == 1 else ((x.shape[0] + 127) // 128,)
+    scale = x.new_empty((*lead, cb), dtype=torch.float8_e8m0fnu)
+    if x.numel():
         x2 = _rows_2d(x, cols)
-        call("rtb_fp8_quantize", get_context(_dev(x)).handle, rows, cols, _ptr(x2),
-             max(x2.stride(0), cols), block_rows, _ptr(q), cols, _ptr(scale), cb, _stream_of(x))
+        call("rtb_fp8_quantize", get_context(x.get_device()).handle, x2.shape[0], cols, _ptr(x2),
+             _ld(x2, cols), block_rows, _ptr(q), cols, _ptr(scale), cb, _stream_of(x))
     return q, scale
 
 
 def fp8_dequantize(q, scale, out=None):
     """The float32 values q * scale of fp8_quantize's (q, scale)."""
-    torch = _torch()
     _check_fp8("fp8_dequantize", q)
     _check_f32_cuda(out)
-    _same_device(q, scale, out)
+    dev = _same_device(q, scale, out)
     if q.dim() == 0:
         raise ValueError("fp8_dequantize: q needs a last dimension")
     cols = q.shape[-1]
-    rows = q.numel() // cols if cols else 0
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+        out = _empty_like(q)
     elif out.shape != q.shape or not out.is_contiguous():
         raise ValueError("fp8_dequantize: out must be contiguous and have q's shape")
-    if rows and cols:
+    if q.numel():
         q2 = _rows_2d(q, cols)
+        rows = q2.shape[0]
         s, block_rows, kind = _scales(scale, rows, cols, "fp8_dequantize")
         if kind != _lib.SCALE_E8M0:
             raise ValueError("fp8_dequantize: scales are float8_e8m0fnu")
-        call("rtb_fp8_dequantize", get_context(_dev(q)).handle, rows, cols, _ptr(q2),
-             max(q2.stride(0), cols), _ptr(s), s.stride(0), block_rows, _ptr(out), cols,
-             _stream_of(q))
+        call("rtb_fp8_dequantize", get_context(dev).handle, rows, cols, _ptr(q2), _ld(q2, cols),
+             _ptr(s), _ld(s, s.shape[1]), block_rows, _ptr(out), cols, _stream_of(q))
     return out
 
 
@@ -467,21 +484,20 @@ def fp8_matmul(a, a_scale, b, b_scale, bias=None, act: int = ACT_NONE, out=None)
     and b [K,N].  b is a Linear weight's transposed view (w.t(), with its
     scales' ws.t()) or a row-major matrix with 128 x 128 blocks; scales are
     float8_e8m0fnu or float32."""
-    torch = _torch()
     _check_fp8("fp8_matmul", a, b)
     _check_f32_cuda(bias, out)
-    _same_device(a, a_scale, b, b_scale, bias, out)
+    dev = _same_device(a, a_scale, b, b_scale, bias, out)
     if a.dim() != 2 or b.dim() != 2 or b_scale.dim() != 2:
         raise ValueError("Matmul only supports 2D")
     M, K = a.shape
     K2, N = b.shape
     if K != K2:
         raise ValueError("Matmul dimension mismatch")
-    if bias is not None and bias.numel() != N:
-        raise ValueError("fp8_matmul: bias must have N elements")
+    bias = _flat(bias, N, "fp8_matmul: bias must have N elements")
     if out is None:
-        out = torch.empty((M, N), dtype=torch.float32, device=a.device)
-    elif tuple(out.shape) != (M, N) or out.stride(1) != 1:
+        out = a.new_empty((M, N), dtype=_torch().float32)
+    elif tuple(out.shape) != (M, N) or (N > 1 and out.stride(1) != 1) or (
+            M > 1 and out.stride(0) < N):
         raise ValueError("fp8_matmul: out must be [M, N] with contiguous rows")
     a_ = _rows_2d(a, K)
     sa, ra, ka = _scales(a_scale, M, K, "fp8_matmul")
@@ -489,16 +505,14 @@ def fp8_matmul(a, a_scale, b, b_scale, bias=None, act: int = ACT_NONE, out=None)
         w, trans = _rows_2d(b.t(), K), 1
         sb, rb_, kb = _scales(b_scale.t(), N, K, "fp8_matmul")
     else:
-        w, trans = b, 0
+        w, trans = _rows_2d(b, N), 0
         sb, rb_, kb = _scales(b_scale, K, N, "fp8_matmul")
         if rb_ != 128 and K > 1:
             raise ValueError("fp8_matmul: a row-major b needs 128 x 128 blocks")
         rb_ = 128
-    bias = bias.contiguous() if bias is not None else None
-    call("rtb_fp8_matmul", get_context(_dev(a)).handle, M, N, K, _ptr(a_), max(a_.stride(0), K),
-         _ptr(sa), max(sa.stride(0), sa.shape[1]), ra, ka, _ptr(w), max(w.stride(0), w.shape[1]),
-         trans, _ptr(sb), max(sb.stride(0), sb.shape[1]), rb_, kb, _ptr(bias), act, _ptr(out),
-         max(out.stride(0), N), _stream_of(a))
+    call("rtb_fp8_matmul", get_context(dev).handle, M, N, K, _ptr(a_), _ld(a_, K), _ptr(sa),
+         _ld(sa, sa.shape[1]), ra, ka, _ptr(w), _ld(w, w.shape[1]), trans, _ptr(sb),
+         _ld(sb, sb.shape[1]), rb_, kb, _ptr(bias), act, _ptr(out), _ld(out, N), _stream_of(a))
     return out
 
 
@@ -508,10 +522,10 @@ def matmul_backward_fp8(a, a_scale, b, grad, need_a: bool = True, need_b: bool =
     (fp8_quantize): (grad @ b.T, deq(a).T @ grad); b (float32 [K,N]) is read for
     the first only and may be None without it.  With accumulate the results
     are added to out_a / out_b."""
-    torch = _torch()
-    _check_fp8("matmul_backward_fp8", a)
+    who = "matmul_backward_fp8"
+    _check_fp8(who, a)
     _check_f32_cuda(b, grad, out_a, out_b)
-    _same_device(a, a_scale, b, grad, out_a, out_b)
+    dev = _same_device(a, a_scale, b, grad, out_a, out_b)
     if a.dim() != 2 or grad.dim() != 2:
         raise ValueError("Matmul only supports 2D")
     M, K = a.shape
@@ -520,28 +534,18 @@ def matmul_backward_fp8(a, a_scale, b, grad, need_a: bool = True, need_b: bool =
         raise ValueError("matmul_backward_fp8: shape mismatch")
     if need_a and b is None:
         raise ValueError("matmul_backward_fp8: the gradient of a needs b")
-
-    def result(out, need, shape):
-        if not need:
-            return None
-        if out is None:
-            if accumulate:
-                raise ValueError("matmul_backward_fp8: accumulate adds to given outputs")
-            return torch.empty(shape, dtype=torch.float32, device=a.device)
-        if not out.is_contiguous() or tuple(out.shape) != shape:
-            raise ValueError("matmul_backward_fp8: outputs must be contiguous and of full size")
-        return out
-
-    da, db = result(out_a, need_a, (M, K)), result(out_b, need_b, (K, N))
-    grad = grad.contiguous()
+    da = _result(out_a, need_a, accumulate, (M, K), grad, who)
+    db = _result(out_b, need_b, accumulate, (K, N), grad, who)
+    if not grad.is_contiguous():
+        grad = grad.contiguous()
     b = b.contiguous() if b is not None and need_a else None
     a_ = _rows_2d(a, K)
-    sa, ra, kind = _scales(a_scale, M, K, "matmul_backward_fp8")
+    sa, ra, kind = _scales(a_scale, M, K, who)
     if kind != _lib.SCALE_E8M0:
         raise ValueError("matmul_backward_fp8: a checkpoint's scales are float8_e8m0fnu")
-    call("rtb_matmul_backward_fp8", get_context(_dev(a)).handle, M, N, K, _ptr(a_),
-         max(a_.stride(0), K), _ptr(sa), max(sa.stride(0), sa.shape[1]), ra, _ptr(b), _ptr(grad),
-         _ptr(da), _ptr(db), int(accumulate), precision, _stream_of(a))
+    call("rtb_matmul_backward_fp8", get_context(dev).handle, M, N, K, _ptr(a_), _ld(a_, K),
+         _ptr(sa), _ld(sa, sa.shape[1]), ra, _ptr(b), _ptr(grad), _ptr(da), _ptr(db),
+         bool(accumulate), precision, _stream_of(a))
     return da, db
 
 

@@ -146,8 +146,15 @@ def check(status: int, where: str) -> None:
         raise RtbError(status, where, last_error())
 
 
+_entry: dict = {}
+
+
 def call(name: str, *args) -> int:
     """Call an rtb_* entry point and raise RtbError on a non-zero status."""
-    st = getattr(lib(), name)(*args)
-    check(st, name)
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(lib(), name)
+    st = fn(*args)
+    if st != RTB_OK:
+        check(st, name)
     return st

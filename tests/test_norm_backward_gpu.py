@@ -260,3 +260,11 @@ def test_refusals(gpu):
             call()
     with pytest.raises(gpu.RtbError):
         gpu.layer_norm_backward(x, mean, rstd, dy, w, b, 5)
+
+
+def test_layer_norm_of_an_expanded_row(gpu):
+    """layer_norm of rows that share their memory (a stride of 0) reads them as
+    they are."""
+    row = torch.randn((1, 300), generator=torch.Generator().manual_seed(1)).cuda()
+    y = gpu.layer_norm(row.expand(50, 300))
+    assert torch.equal(y, gpu.layer_norm(row.expand(50, 300).contiguous()))
