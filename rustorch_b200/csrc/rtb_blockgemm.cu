@@ -24,12 +24,9 @@
 // Shared memory (128-byte swizzle throughout):
 //   MODE 0, K-major: row r at r * 128 B holds 128 e4m3 of the contraction.
 //   MODE 1, MN-major: boxes of 64 contraction rows x 64 bf16 (8 KB).
-#include <cuda.h>
+#include <cstdlib>
 
-#include "rtb_act.cuh"
-#include "rtb_fp8.cuh"
-#include "rtb_internal.h"
-#include "rtb_ptx.cuh"
+#include "rtb_blockgemm.cuh"
 
 namespace rtb {
 
@@ -55,37 +52,6 @@ struct Cfg {
   static_assert(kStages >= 2, "two stages");
 };
 
-struct BlockParams {
-  int64_t xrows, ycols;  // output extents along X and Y
-  int depth;             // contraction length
-  int stages_total;      // ceil(depth / kDepth)
-  int tiles_x, tiles_y;
-  float* out;            // element (x, y) at x * sx + y * sy
-  int64_t sx, sy;
-  const float* bias;     // per Y column (bias_on_x = 0) or per X row
-  int bias_on_x;
-  int act;
-  int accumulate;
-  int pieces;            // MODE 1
-  int64_t piece_rows;    // MODE 1: contraction rows between Y's pieces
-  ScaleRef scx, scy;     // MODE 0
-  int* err;
-  unsigned long long timeout_ns;
-};
-
-__device__ __forceinline__ float load_scale(const ScaleRef& s, int64_t i) {
-  return s.is_f32 ? __ldg(static_cast<const float*>(s.p) + i)
-                  : e8m0_to_float(__ldg(static_cast<const uint8_t*>(s.p) + i));
-}
-
-// Instruction descriptor, fp32 accumulate, dense.  Bits: D format [4,6) = 1;
-// A format [7,10), B format [10,13): e4m3 = 0 (kind::f8f6f4), bf16 = 1
-// (kind::f16); A MN-major [15], B MN-major [16]; N >> 3 [17,23); M >> 4 [24,29).
-constexpr uint32_t idesc(int mode, int m, int n) {
-  return (1u << 4) | (mode == 0 ? 0u : (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16)) |
-         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
-}
-
 template <int MODE>
 __device__ __forceinline__ void mma_e(uint32_t d, uint64_t a, uint64_t b, uint32_t id,
                                       uint32_t acc) {
@@ -106,16 +72,6 @@ __device__ __forceinline__ void mma_e(uint32_t d, uint64_t a, uint64_t b, uint32
         "l"(a), "l"(b), "r"(id), "r"(acc)
         : "memory");
   }
-}
-
-__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
 }
 
 // YVEC (MODE 0): a scale for every Y column (block_rows 1); otherwise the
@@ -196,7 +152,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp == 1) {
-    constexpr uint32_t id = idesc(MODE, kX, BN);
+    constexpr uint32_t id = block_idesc(MODE, kX, BN);
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
       int got = 0;
@@ -280,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = 0; c < BN; c += 16) {
         uint32_t r[16];
         tmem_ld_x16(t_lane + (uint32_t)(b * BN + c), r);
-        tmem_ld_wait();
+        tmem_wait_x16(r);
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const float t = __uint_as_float(r[j]);
@@ -341,6 +297,17 @@ int launch(const CUtensorMap& tmX, const CUtensorMap& tmY, BlockParams& p, cudaS
   return e == cudaSuccess ? RTB_OK : cuda_status(e, "block gemm launch");
 }
 
+// CTA pairs where their 256 x 256 tiles occupy most of the SMs.
+bool use_pairs(const rtb_ctx* ctx, const BlockParams& p) {
+  static const int env = [] {
+    const char* v = std::getenv("RTB_PAIR");
+    return v ? std::atoi(v) : -1;
+  }();
+  if (env >= 0) return env != 0;
+  const int64_t tiles = ((p.xrows + 255) / 256) * ((p.ycols + 255) / 256);
+  return tiles * 2 > ctx->sm_count / 2;
+}
+
 int check_extents(int64_t a, int64_t b, int64_t c) {
   if (a > INT32_MAX - 512 || b > INT32_MAX - 512 || c > INT32_MAX - 512)
     return set_error(RTB_E_UNSUPPORTED, "block gemm: dimension exceeds 2^31-513");
@@ -380,6 +347,7 @@ int fp8_gemm_run(rtb_ctx* ctx, const Fp8Desc& d, cudaStream_t s) {
   if ((st = make_tmap_2d_bytes(&tmY, Y, 1, (uint64_t)d.K, (uint64_t)p.ycols,
                                (uint64_t)(swap ? d.lda : d.ldb), 128, (uint32_t)bn)))
     return st;
+  if (!swap && use_pairs(ctx, p)) return launch_pair(ctx, 0, yvec, tmX, tmY, p, s);
   if (bn == 16) return yvec ? launch<0, 16, true>(tmX, tmY, p, s) : launch<0, 16, false>(tmX, tmY, p, s);
   if (bn == 32) return yvec ? launch<0, 32, true>(tmX, tmY, p, s) : launch<0, 32, false>(tmX, tmY, p, s);
   if (bn == 64) return yvec ? launch<0, 64, true>(tmX, tmY, p, s) : launch<0, 64, false>(tmX, tmY, p, s);
@@ -408,6 +376,7 @@ int wgrad_run(rtb_ctx* ctx, const WgradDesc& d, cudaStream_t s) {
   if ((st = make_tmap_2d_bytes(&tmY, d.Y, 2, (uint64_t)d.ldy, (uint64_t)(d.rows_pad * d.pieces),
                                (uint64_t)d.ldy, 64, 64)))
     return st;
+  if (use_pairs(ctx, p)) return launch_pair(ctx, 1, false, tmX, tmY, p, s);
   return launch<1, 128, false>(tmX, tmY, p, s);
 }
 

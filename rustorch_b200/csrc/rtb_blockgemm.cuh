@@ -1,0 +1,102 @@
+// Shared by the block-scaled product kernels (rtb_blockgemm.cu: one CTA a tile;
+// rtb_pairgemm.cu: two CTAs a tile): parameters, scales, instruction
+// descriptors, packed fp32 arithmetic.
+#pragma once
+#include <cuda.h>
+
+#include "rtb_act.cuh"
+#include "rtb_fp8.cuh"
+#include "rtb_internal.h"
+#include "rtb_ptx.cuh"
+
+namespace rtb {
+
+struct BlockParams {
+  int64_t xrows, ycols;  // output extents along X and Y
+  int depth;             // contraction length
+  int stages_total;      // ceil(depth / kDepth)
+  int tiles_x, tiles_y;
+  float* out;            // element (x, y) at x * sx + y * sy
+  int64_t sx, sy;
+  const float* bias;     // per Y column (bias_on_x = 0) or per X row
+  int bias_on_x;
+  int act;
+  int accumulate;
+  int pieces;            // MODE 1
+  int64_t piece_rows;    // MODE 1: contraction rows between Y's pieces
+  ScaleRef scx, scy;     // MODE 0
+  int c_tma;             // rows of the output leave through TMA stores
+  int* err;
+  unsigned long long timeout_ns;
+};
+
+__device__ __forceinline__ float load_scale(const ScaleRef& s, int64_t i) {
+  return s.is_f32 ? __ldg(static_cast<const float*>(s.p) + i)
+                  : e8m0_to_float(__ldg(static_cast<const uint8_t*>(s.p) + i));
+}
+
+// Instruction descriptor, fp32 accumulate, dense.  Bits: D format [4,6) = 1;
+// A format [7,10), B format [10,13): e4m3 = 0 (kind::f8f6f4), bf16 = 1
+// (kind::f16); A MN-major [15], B MN-major [16]; N >> 3 [17,23); M >> 4 [24,29).
+constexpr __host__ __device__ uint32_t block_idesc(int mode, int m, int n) {
+  return (1u << 4) | (mode == 0 ? 0u : (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16)) |
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+// Waits for the TMEM loads issued so far; the registers go through the
+// statement, so that their uses stay behind it.
+__device__ __forceinline__ void tmem_wait_x16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+}
+
+// Two fp32 values in one 64-bit register: one instruction adds or multiplies
+// both.
+__device__ __forceinline__ unsigned long long pack2(float lo, float hi) {
+  unsigned long long v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ unsigned long long pack2(uint32_t lo, uint32_t hi) {
+  unsigned long long v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+  return v;
+}
+__device__ __forceinline__ float2 unpack2(unsigned long long v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b,
+                                                   unsigned long long c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// Products on CTA pairs (rtb_pairgemm.cu); yvec as in rtb_blockgemm.cu.
+int launch_pair(rtb_ctx* ctx, int mode, bool yvec, const CUtensorMap& tmX, const CUtensorMap& tmY,
+                BlockParams& p, cudaStream_t s);
+
+}  // namespace rtb

@@ -1,0 +1,445 @@
+// The products of rtb_blockgemm.cu on CTA pairs (tcgen05 cta_group::2): a
+// persistent kernel whose two CTAs compute one 256 x 256 tile.  Each CTA loads
+// its own 128 X rows and half of the 256 Y columns, the pair's tensor cores
+// read both halves, and each CTA's TMEM holds its 128 rows x 256 columns of
+// the accumulator, twice.
+//
+// Why pairs: a stage of 128 contraction bytes takes 512 clocks of MMAs and 32
+// KB of loads per SM, 64 bytes a clock; one CTA alone needs 48 KB for a 128 x
+// 256 tile in the same time, more than L2 feeds an SM.
+//
+// Promotion: after every 128 contraction elements the epilogue warps add the
+// finished partial sum into registers (128 a thread: 8 warps, each 32 TMEM
+// lanes x 128 columns) while the MMAs fill the other half of TMEM.  In MODE 0
+// that is 32768 multiply-adds per 512 clocks of MMAs, half of the SM's fp32
+// lanes; packed f32x2 instructions halve the issue slots.
+//
+// Roles (warps of each CTA): 0 TMA producer; 1 TMEM allocation, and in the
+// pair's first CTA the MMA issue for both; 4..11 epilogue (lanes 32 (w % 4)..,
+// columns 128 ((w - 4) / 4)..).  The first warpgroup hands registers to the
+// epilogue's two (384 threads x 168 at launch = 128 x (40 + 232 + 232)): at 168
+// the accumulators spill.  Barriers: `full` and `tempty` live in the
+// first CTA (the producers' bytes and the epilogues' arrivals of both CTAs),
+// `empty` and `tfull` in each (the MMA's commits go to both).
+#include "rtb_blockgemm.cuh"
+
+namespace rtb {
+
+namespace {
+
+constexpr int kThreads = 384;
+constexpr int kTile = 256;
+constexpr int kChunk = 128 * 32 * 4;  // a staged 128 x 32 fp32 piece of the output
+constexpr int kSmemBytes = 232448;
+
+template <int MODE, bool YVEC>
+struct PairCfg {
+  static constexpr int kDepth = MODE == 0 ? 128 : 64;
+  static constexpr int kYPieces = MODE == 0 ? 1 : 3;
+  static constexpr int kStageBytes = 16384 * (1 + kYPieces);
+  // two staging chunks; the column scales take a stage's place
+  static constexpr int kStages = MODE == 0 ? (YVEC ? 5 : 6) : 3;
+  static constexpr int kPerUnit = 128 / kDepth;
+  static_assert(1024 + kStages * kStageBytes + 2 * kChunk + 1024 + (YVEC ? 2048 : 0) <= kSmemBytes,
+                "shared memory");
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// Address in CTA `rank` of the cluster of this CTA's shared address.
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+// Arrival on a barrier of the pair.  What it orders is TMEM traffic (the
+// loads have been waited for, tcgen05.fence on both sides) and no generic
+// memory, so CTA scope is enough: a cluster-scope release is a memory barrier
+// that also waits for the scale loads in flight (it took two thirds of the
+// epilogue's time), a cluster-scope acquire drops them from L1.
+__device__ __forceinline__ void arrive_pair(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// A tiled load into this CTA that completes on a barrier of the pair.
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                                 int32_t c0, int32_t c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+      : "memory");
+}
+template <int MODE>
+__device__ __forceinline__ void mma_pair_e(uint32_t d, uint64_t a, uint64_t b, uint32_t id,
+                                           uint32_t acc) {
+  if (MODE == 0) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t.reg .b32 r;\n\t"
+        "elect.sync r|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(id), "r"(acc)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t.reg .b32 r;\n\t"
+        "elect.sync r|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(id), "r"(acc)
+        : "memory");
+  }
+}
+// Arrive on both CTAs' barrier at this offset once the MMAs issued so far are
+// done.
+__device__ __forceinline__ void commit_pair_e(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t.reg .b32 r;\n\t.reg .b16 m;\n\t"
+      "mov.b16 m, 3;\n\t"
+      "elect.sync r|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], m;\n\t}" ::"r"(smem_u32(bar))
+      : "memory");
+}
+
+// Tiles in bands of 8 X tiles, so that the 74 pairs' working set is about
+// square.
+__device__ __forceinline__ void pair_tile(const BlockParams& p, int t, int& tx, int& ty) {
+  const int band = 8 * p.tiles_y;
+  const int g = t / band;
+  int h = p.tiles_x - 8 * g;
+  h = h < 8 ? h : 8;
+  const int r = t - g * band;
+  tx = 8 * g + r % h;
+  ty = r / h;
+}
+
+template <int MODE, bool YVEC>
+__global__ void __launch_bounds__(kThreads, 1)
+    pair_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmY,
+                     const __grid_constant__ CUtensorMap tmC, const BlockParams p) {
+  using C = PairCfg<MODE, YVEC>;
+  constexpr int S = C::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint8_t* staging = base + S * C::kStageBytes;  // 2 x kChunk, 1024-byte aligned
+  uint8_t* tail = staging + 2 * kChunk;
+  uint64_t* full = reinterpret_cast<uint64_t*>(tail);
+  uint64_t* empty = full + S;
+  uint64_t* tfull = empty + S;
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* sy_s = reinterpret_cast<float*>(tail + 512);  // YVEC: [2][256]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], 16);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&tmY);
+    if (p.c_tma) tma_prefetch_desc(&tmC);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers and TMEM are ready
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  const int pairs = (int)gridDim.x / 2, pair = (int)blockIdx.x / 2;
+  const int tiles = p.tiles_x * p.tiles_y;
+  const int nst = p.stages_total;
+  const int units = (nst + C::kPerUnit - 1) / C::kPerUnit;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 0 && lane == 0) {
+      const uint32_t bytes = 2u * 16384u * (uint32_t)(1 + (MODE == 0 ? 1 : p.pieces));
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        int tx, ty;
+        pair_tile(p, t, tx, ty);
+        const int x0 = tx * kTile + 128 * (int)rank, y0 = ty * kTile + 128 * (int)rank;
+        for (int i = 0; i < nst; ++i) {
+          if (!(ok = mbar_wait_bounded(&empty[s], ph ^ 1, abort_flag, p.err, DEV_TIMEOUT_EMPTY,
+                                  p.timeout_ns)))
+            break;
+          const uint32_t st = smem_u32(base + s * C::kStageBytes);
+          // the first CTA expects both CTAs' bytes; the second's may land first
+          const uint32_t bar = map_rank(smem_u32(&full[s]), 0);
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
+          if (MODE == 0) {
+            tma_load_2d_pair(st, &tmX, bar, i * 128, x0);
+            tma_load_2d_pair(st + 16384, &tmY, bar, i * 128, y0);
+          } else {
+            for (int b = 0; b < 2; ++b)
+              tma_load_2d_pair(st + 8192 * b, &tmX, bar, x0 + 64 * b, 64 * i);
+            for (int q = 0; q < p.pieces; ++q)
+              for (int b = 0; b < 2; ++b)
+                tma_load_2d_pair(st + 16384 * (1 + q) + 8192 * b, &tmY, bar, y0 + 64 * b,
+                                 (int)(q * p.piece_rows) + 64 * i);
+          }
+          if (++s == S) { s = 0; ph ^= 1; }
+        }
+      }
+    } else if (warp == 1 && rank == 0) {
+      constexpr uint32_t id = block_idesc(MODE, 256, 256);
+      auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+        int got = 0;
+        if (lane == 0) got = mbar_wait_bounded(bar, parity, abort_flag, p.err, code, p.timeout_ns);
+        return __shfl_sync(0xffffffffu, got, 0) != 0;
+      };
+      int s = 0, g = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        int i = 0;
+        for (int u = 0; u < units && ok; ++u, ++g) {
+          const int b = g & 1;
+          if (!(ok = wait(&tempty[b], ((g >> 1) & 1) ^ 1, DEV_TIMEOUT_TMEM_EMPTY))) break;
+          tc_fence_after();
+          const uint32_t d = tmem + (uint32_t)(b * 256);
+          for (int j = 0; j < C::kPerUnit && i < nst; ++j, ++i) {
+            if (!(ok = wait(&full[s], ph, DEV_TIMEOUT_FULL))) break;
+            tc_fence_after();
+            const uint32_t xa = smem_u32(base + s * C::kStageBytes), ya = xa + 16384;
+            if (MODE == 0) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                mma_pair_e<0>(d, umma_desc(xa + 32 * k, 16, 1024, kLayoutSW128),
+                              umma_desc(ya + 32 * k, 16, 1024, kLayoutSW128), id, k > 0);
+            } else {
+              for (int q = p.pieces - 1; q >= 0; --q)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  mma_pair_e<1>(d, umma_desc(xa + 2048 * k, 8192, 1024, kLayoutSW128),
+                                umma_desc(ya + 16384 * q + 2048 * k, 8192, 1024, kLayoutSW128), id,
+                                j > 0 || k > 0 || q < p.pieces - 1);
+            }
+            commit_pair_e(&empty[s]);
+            if (++s == S) { s = 0; ph ^= 1; }
+          }
+          if (!ok) break;
+          commit_pair_e(&tfull[b]);
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    const int row = 32 * (warp & 3) + lane;
+    const int half = (warp - 4) >> 2;
+    const int et = threadIdx.x - 128 - 128 * half;  // 0..127 within the half
+    const uint32_t t_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)(128 * half);
+    const uint32_t tempty0[2] = {map_rank(smem_u32(&tempty[0]), 0), map_rank(smem_u32(&tempty[1]), 0)};
+    uint8_t* stg = staging + half * kChunk;
+    int g = 0;
+    bool ok = true;
+    for (int t = pair; t < tiles; t += pairs) {
+      int tx, ty;
+      pair_tile(p, t, tx, ty);
+      const int64_t x = (int64_t)tx * kTile + 128 * rank + row;
+      const int64_t y0 = (int64_t)ty * kTile + 128 * half;
+      unsigned long long acc[64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) acc[j] = 0ull;
+      const int64_t yr = y0 + (YVEC ? et : 0);
+      const int64_t xi = MODE == 0 && x < p.xrows ? (x >> p.scx.row_shift) * p.scx.ld_row : -1;
+      const int64_t yi = MODE == 0 && yr < p.ycols ? (yr >> p.scy.row_shift) * p.scy.ld_row : -1;
+      auto scale_x = [&](int u) { return xi >= 0 ? load_scale(p.scx, xi + u * p.scx.ld_col) : 0.0f; };
+      auto scale_y = [&](int u) { return yi >= 0 ? load_scale(p.scy, yi + u * p.scy.ld_col) : 0.0f; };
+      float nx = 0.0f, ny = 0.0f;
+      if (MODE == 0) {
+        nx = scale_x(0);
+        ny = scale_y(0);
+      }
+      for (int u = 0; u < units; ++u, ++g) {
+        const int b = g & 1;
+        const float cx = nx, cy = ny;
+        if (MODE == 0 && u + 1 < units) {  // the next block's scales, a block ahead
+          nx = scale_x(u + 1);
+          ny = scale_y(u + 1);
+        }
+        float* sy = sy_s + 256 * b + 128 * half;
+        if (YVEC) {
+          sy[et] = cy;
+          named_bar_sync(1 + half, 128);
+        }
+        if (ok) {
+          int got = 0;
+          if (lane == 0)
+            got = mbar_wait_bounded(&tfull[b], (g >> 1) & 1, abort_flag, p.err, DEV_TIMEOUT_TMEM_FULL,
+                               p.timeout_ns);
+          ok = __shfl_sync(0xffffffffu, got, 0) != 0;
+        }
+        tc_fence_after();
+        const float sc = MODE == 0 ? (YVEC ? cx : cx * cy) : 1.0f;
+        const unsigned long long s2 = pack2(sc, sc);
+        const uint32_t ta = t_lane + (uint32_t)(256 * b);
+        uint32_t r[2][16];
+        tmem_ld_x16(ta, r[0]);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          tmem_wait_x16(r[c & 1]);
+          if (c < 7) tmem_ld_x16(ta + 16 * (c + 1), r[(c + 1) & 1]);
+          if (c == 7) {  // the last of this buffer is in registers
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_pair(tempty0[b]);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const unsigned long long v = pack2(r[c & 1][2 * j], r[c & 1][2 * j + 1]);
+            unsigned long long& a = acc[8 * c + j];
+            if (MODE == 1) a = add2(a, v);
+            else if (YVEC)
+              a = fma2(mul2(v, s2),
+                       *reinterpret_cast<const unsigned long long*>(sy + 16 * c + 2 * j), a);
+            else a = fma2(v, s2, a);
+          }
+        }
+      }
+      // the finished rows, 32 columns at a time
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int64_t yc = y0 + 32 * c;
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float2 f = unpack2(acc[16 * c + j]);
+          v[2 * j] = f.x;
+          v[2 * j + 1] = f.y;
+        }
+        if (p.bias) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += yc + j < p.ycols ? __ldg(p.bias + yc + j) : 0.0f;
+        }
+        float* o = p.out + x * p.sx + yc;
+        if (p.accumulate && x < p.xrows) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (yc + j < p.ycols) v[j] += o[j];
+        }
+        activate_n<32>(v, p.act);
+        if (p.c_tma) {
+          // the store before has read the chunk (its issuing thread waits)
+          if (et == 0) bulk_wait_group_read<0>();
+          named_bar_sync(1 + half, 128);
+          const uint32_t dst = smem_u32(stg) + row * 128;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            sts128(dst + ((j ^ (row & 7)) << 4),
+                   make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+          fence_proxy_async_smem();
+          named_bar_sync(1 + half, 128);
+          const int xs = tx * kTile + 128 * (int)rank;
+          if (et == 0 && yc < p.ycols && xs < p.xrows) {
+            tma_store_2d(&tmC, stg, (int)yc, xs);
+            bulk_commit_group();
+          }
+        } else if (x < p.xrows) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (yc + j < p.ycols) o[j] = v[j];
+        }
+      }
+    }
+    if (p.c_tma && et == 0) bulk_wait_group<0>();
+  }
+
+  // ------------------------------------------------------------ teardown
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    // copies in flight land before the CTA's shared memory is released
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 1000000ull) __nanosleep(1000);
+    __syncthreads();
+  }
+  cluster_sync_all();  // no commit or arrival for this CTA is under way any more
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
+                 : "memory");
+  }
+}
+
+template <int MODE, bool YVEC>
+int launch(rtb_ctx* ctx, const CUtensorMap& tmX, const CUtensorMap& tmY, BlockParams& p,
+           cudaStream_t s) {
+  using C = PairCfg<MODE, YVEC>;
+  auto* k = pair_gemm_kernel<MODE, YVEC>;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  if (e != cudaSuccess) return cuda_status(e, "pair gemm smem attribute");
+  p.tiles_x = (int)((p.xrows + kTile - 1) / kTile);
+  p.tiles_y = (int)((p.ycols + kTile - 1) / kTile);
+  p.stages_total = (p.depth + C::kDepth - 1) / C::kDepth;
+  const int64_t tiles = (int64_t)p.tiles_x * p.tiles_y;
+  if (tiles > INT32_MAX / 2) return set_error(RTB_E_UNSUPPORTED, "pair gemm: too many tiles");
+  CUtensorMap tmC = tmX;
+  p.c_tma = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 && p.sx % 4 == 0;
+  if (p.c_tma) {
+    const int st = make_tmap_2d(&tmC, p.out, (uint64_t)p.ycols, (uint64_t)p.xrows, (uint64_t)p.sx,
+                                32, 128, false);
+    if (st) return st;
+  }
+  const int64_t pairs = ctx->sm_count / 2 < tiles ? ctx->sm_count / 2 : tiles;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * pairs));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  clear_stale_cuda_error();
+  e = cudaLaunchKernelEx(&cfg, k, tmX, tmY, tmC, (const BlockParams)p);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return e == cudaSuccess ? RTB_OK : cuda_status(e, "pair gemm launch");
+}
+
+}  // namespace
+
+int launch_pair(rtb_ctx* ctx, int mode, bool yvec, const CUtensorMap& tmX, const CUtensorMap& tmY,
+                BlockParams& p, cudaStream_t s) {
+  if (mode == 1) return launch<1, false>(ctx, tmX, tmY, p, s);
+  return yvec ? launch<0, true>(ctx, tmX, tmY, p, s) : launch<0, false>(ctx, tmX, tmY, p, s);
+}
+
+}  // namespace rtb
