@@ -199,24 +199,33 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
     for (int j = 0; j < BN; ++j) acc[j] = 0.0f;
     bool ok = true;
-    // scales of the next block are loaded while this one is waited for
     const int64_t xi = MODE == 0 && x < p.xrows ? (x >> p.scx.row_shift) * p.scx.ld_row : -1;
     const int64_t yr = y0 + (YVEC ? et : 0);
     const int64_t yi = MODE == 0 && yr < p.ycols && (!YVEC || et < BN)
                            ? (yr >> p.scy.row_shift) * p.scy.ld_row : -1;
-    auto scale_x = [&](int u) { return xi >= 0 ? load_scale(p.scx, xi + u * p.scx.ld_col) : 0.0f; };
-    auto scale_y = [&](int u) { return yi >= 0 ? load_scale(p.scy, yi + u * p.scy.ld_col) : 0.0f; };
-    float nx = 0.0f, ny = 0.0f;
+    auto scale_x = [&](int u) -> uint32_t {
+      return xi >= 0 && u < units ? load_scale(p.scx, xi + u * p.scx.ld_col) : 0u;
+    };
+    auto scale_y = [&](int u) -> uint32_t {
+      return yi >= 0 && u < units ? load_scale(p.scy, yi + u * p.scy.ld_col) : 0u;
+    };
+    uint32_t rx[2] = {0, 0}, ry[2] = {0, 0};  // the scales of the next two blocks
     if (MODE == 0) {
-      nx = scale_x(0);
-      ny = scale_y(0);
+      rx[0] = scale_x(0);
+      ry[0] = scale_y(0);
+      rx[1] = scale_x(1);
+      ry[1] = scale_y(1);
     }
     for (int u = 0; u < units; ++u) {
       const int b = u & 1;
-      const float cx = nx, cy = ny;
-      if (MODE == 0 && u + 1 < units) {
-        nx = scale_x(u + 1);
-        ny = scale_y(u + 1);
+      float cx = 0.0f, cy = 0.0f;
+      if (MODE == 0) {
+        cx = scale_value(p.scx, rx[0]);
+        cy = scale_value(p.scy, ry[0]);
+        rx[0] = rx[1];
+        ry[0] = ry[1];
+        rx[1] = scale_x(u + 2);
+        ry[1] = scale_y(u + 2);
       }
       if (YVEC) {
         // two buffers: the block after next's write comes behind the next barrier

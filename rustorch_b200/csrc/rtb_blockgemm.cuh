@@ -30,9 +30,15 @@ struct BlockParams {
   unsigned long long timeout_ns;
 };
 
-__device__ __forceinline__ float load_scale(const ScaleRef& s, int64_t i) {
-  return s.is_f32 ? __ldg(static_cast<const float*>(s.p) + i)
-                  : e8m0_to_float(__ldg(static_cast<const uint8_t*>(s.p) + i));
+// A scale as it lies in memory, and its value.  They are apart so that a load
+// can be issued blocks ahead of its use: decoding at the load waits for it
+// (450 -> 311 us on 8192 x 4096 x 8192).
+__device__ __forceinline__ uint32_t load_scale(const ScaleRef& s, int64_t i) {
+  return s.is_f32 ? __ldg(static_cast<const uint32_t*>(s.p) + i)
+                  : (uint32_t)__ldg(static_cast<const uint8_t*>(s.p) + i);
+}
+__device__ __forceinline__ float scale_value(const ScaleRef& s, uint32_t raw) {
+  return s.is_f32 ? __uint_as_float(raw) : e8m0_to_float(raw);
 }
 
 // Instruction descriptor, fp32 accumulate, dense.  Bits: D format [4,6) = 1;
