@@ -70,6 +70,7 @@ int make_tmap_2d_swz(CUtensorMap* map, const void* base, uint64_t dim0, uint64_t
                    box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                    swizzle == kTmapSwizzle128Atom32 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B
                    : swizzle == kTmapSwizzle128     ? CU_TENSOR_MAP_SWIZZLE_128B
+                   : swizzle == kTmapSwizzle64      ? CU_TENSOR_MAP_SWIZZLE_64B
                                                     : CU_TENSOR_MAP_SWIZZLE_NONE,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {

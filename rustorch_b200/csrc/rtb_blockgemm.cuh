@@ -25,6 +25,10 @@ struct BlockParams {
   int pieces;            // MODE 1
   int64_t piece_rows;    // MODE 1: contraction rows between Y's pieces
   ScaleRef scx, scy;     // MODE 0
+  // MODE 0, CTA pairs: the scales as fp32, [block][row], zero past the operand
+  // (launch_scale_tables)
+  const float *tabx, *taby;
+  int64_t pitchx, pitchy;
   int c_tma;             // rows of the output leave through TMA stores
   int* err;
   unsigned long long timeout_ns;
@@ -100,6 +104,10 @@ __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigne
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+
+// Blocks in a scale table of `units` blocks: whole quads and one more, so that
+// a quad can be loaded ahead without a check.
+inline int64_t table_blocks(int64_t units) { return (units + 3) / 4 * 4 + 4; }
 
 // Products on CTA pairs (rtb_pairgemm.cu); yvec as in rtb_blockgemm.cu.
 int launch_pair(rtb_ctx* ctx, int mode, bool yvec, const CUtensorMap& tmX, const CUtensorMap& tmY,

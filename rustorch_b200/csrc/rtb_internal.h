@@ -76,7 +76,8 @@ int make_tmap_2d(CUtensorMap* map, const void* base, uint64_t dim0, uint64_t dim
                  uint64_t row_stride_elems, uint32_t box0, uint32_t box1, bool atom32);
 // Same with the shared-memory layout chosen explicitly (no swizzle allows an
 // inner box wider than 128 bytes).
-constexpr int kTmapSwizzleNone = 0, kTmapSwizzle128 = 1, kTmapSwizzle128Atom32 = 2;
+constexpr int kTmapSwizzleNone = 0, kTmapSwizzle128 = 1, kTmapSwizzle128Atom32 = 2,
+              kTmapSwizzle64 = 3;
 int make_tmap_2d_swz(CUtensorMap* map, const void* base, uint64_t dim0, uint64_t dim1,
                      uint64_t row_stride_elems, uint32_t box0, uint32_t box1, int swizzle);
 

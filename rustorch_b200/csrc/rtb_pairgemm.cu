@@ -40,9 +40,45 @@ struct PairCfg {
   // two staging chunks; the column scales take a stage's place
   static constexpr int kStages = MODE == 0 ? (YVEC ? 5 : 6) : 3;
   static constexpr int kPerUnit = 128 / kDepth;
-  static_assert(1024 + kStages * kStageBytes + 2 * kChunk + 1024 + (YVEC ? 2048 : 0) <= kSmemBytes,
+  static_assert(1024 + kStages * kStageBytes + 2 * kChunk + 512 + (YVEC ? 8192 : 0) <= kSmemBytes,
                 "shared memory");
 };
+
+// The scales of both operands as fp32 tables [block][row]: the epilogue then
+// takes a block's scales of 32 rows with one coalesced, unconditional load that
+// nothing has to decode (a conditional load of whatever type the caller has
+// waits for its value where the branches meet: 1000 clocks every time).
+// blockIdx.z picks the operand; rows [rows, pitch) and blocks [units, blocks)
+// are zero.  32 x 32 tiles through shared memory.
+struct TableSide {
+  ScaleRef s;
+  int64_t rows, pitch;
+  float* out;
+};
+__global__ void __launch_bounds__(256) scale_table_kernel(const TableSide x, const TableSide y,
+                                                          int units, int blocks) {
+  __shared__ float t[32][33];
+  griddep_wait();
+  griddep_launch_dependents();
+  const TableSide& d = blockIdx.z ? y : x;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int k0 = blockIdx.y * 32;
+  for (int64_t r0 = (int64_t)blockIdx.x * 32; r0 < d.pitch; r0 += (int64_t)gridDim.x * 32) {
+    __syncthreads();
+    for (int i = w; i < 32; i += 8) {
+      const int64_t r = r0 + i;
+      const int k = k0 + lane;
+      float v = 0.0f;
+      if (r < d.rows && k < units)
+        v = scale_value(d.s, load_scale(d.s, (r >> d.s.row_shift) * d.s.ld_row + k * d.s.ld_col));
+      t[i][lane] = v;
+    }
+    __syncthreads();
+    for (int i = w; i < 32; i += 8)
+      if (k0 + i < blocks && r0 + lane < d.pitch)
+        d.out[(int64_t)(k0 + i) * d.pitch + r0 + lane] = t[lane][i];
+  }
+}
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -138,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* tempty = tfull + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* sy_s = reinterpret_cast<float*>(tail + 512);  // YVEC: [2][256]
+  float* sy_s = reinterpret_cast<float*>(tail + 512);  // YVEC: [2][4 blocks][256]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
@@ -222,35 +258,56 @@ __global__ void __launch_bounds__(kThreads, 1)
       int s = 0, g = 0;
       uint32_t ph = 0;
       bool ok = true;
+      // Lane 0: whether the next stage's operands and the next accumulator were
+      // found ready before this stage's last MMA.  A wait costs this warp 200
+      // clocks of latency even when its barrier is complete, so the tests run
+      // behind the MMAs issued before them.
+      int next_full = 0, next_empty = 0;
       for (int t = pair; t < tiles && ok; t += pairs) {
         int i = 0;
         for (int u = 0; u < units && ok; ++u, ++g) {
           const int b = g & 1;
-          if (!(ok = wait(&tempty[b], ((g >> 1) & 1) ^ 1, DEV_TIMEOUT_TMEM_EMPTY))) break;
-          tc_fence_after();
           const uint32_t d = tmem + (uint32_t)(b * 256);
           for (int j = 0; j < C::kPerUnit && i < nst; ++j, ++i) {
-            if (!(ok = wait(&full[s], ph, DEV_TIMEOUT_FULL))) break;
+            if (!__shfl_sync(0xffffffffu, next_full, 0) &&
+                !(ok = wait(&full[s], ph, DEV_TIMEOUT_FULL)))
+              break;
+            if (j == 0 && !__shfl_sync(0xffffffffu, next_empty, 0) &&
+                !(ok = wait(&tempty[b], ((g >> 1) & 1) ^ 1, DEV_TIMEOUT_TMEM_EMPTY)))
+              break;
             tc_fence_after();
+            const int sn = s + 1 == S ? 0 : s + 1;
+            const uint32_t phn = s + 1 == S ? ph ^ 1u : ph;
+            const bool last = j + 1 == C::kPerUnit || i + 1 == nst;
             const uint32_t xa = smem_u32(base + s * C::kStageBytes), ya = xa + 16384;
             if (MODE == 0) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
+              for (int k = 0; k < 4; ++k) {
+                if (k == 2 && lane == 0) {
+                  next_full = mbar_test_wait(&full[sn], phn);
+                  next_empty = mbar_test_wait(&tempty[b ^ 1], (((g + 1) >> 1) & 1) ^ 1);
+                }
                 mma_pair_e<0>(d, umma_desc(xa + 32 * k, 16, 1024, kLayoutSW128),
                               umma_desc(ya + 32 * k, 16, 1024, kLayoutSW128), id, k > 0);
+              }
             } else {
-              for (int q = p.pieces - 1; q >= 0; --q)
+              for (int q = p.pieces - 1; q >= 0; --q) {
+                if (q == 0 && lane == 0) {
+                  next_full = mbar_test_wait(&full[sn], phn);
+                  if (last) next_empty = mbar_test_wait(&tempty[b ^ 1], (((g + 1) >> 1) & 1) ^ 1);
+                }
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                   mma_pair_e<1>(d, umma_desc(xa + 2048 * k, 8192, 1024, kLayoutSW128),
                                 umma_desc(ya + 16384 * q + 2048 * k, 8192, 1024, kLayoutSW128), id,
                                 j > 0 || k > 0 || q < p.pieces - 1);
+              }
             }
             commit_pair_e(&empty[s]);
-            if (++s == S) { s = 0; ph ^= 1; }
+            if (last) commit_pair_e(&tfull[b]);
+            s = sn;
+            ph = phn;
           }
-          if (!ok) break;
-          commit_pair_e(&tfull[b]);
         }
       }
     }
@@ -272,69 +329,82 @@ __global__ void __launch_bounds__(kThreads, 1)
       unsigned long long acc[64];
 #pragma unroll
       for (int j = 0; j < 64; ++j) acc[j] = 0ull;
-      const int64_t yr = y0 + (YVEC ? et : 0);
-      const int64_t xi = MODE == 0 && x < p.xrows ? (x >> p.scx.row_shift) * p.scx.ld_row : -1;
-      const int64_t yi = MODE == 0 && yr < p.ycols ? (yr >> p.scy.row_shift) * p.scy.ld_row : -1;
-      auto scale_x = [&](int u) -> uint32_t {
-        return xi >= 0 && u < units ? load_scale(p.scx, xi + u * p.scx.ld_col) : 0u;
-      };
-      auto scale_y = [&](int u) -> uint32_t {
-        return yi >= 0 && u < units ? load_scale(p.scy, yi + u * p.scy.ld_col) : 0u;
-      };
-      uint32_t rx[2] = {0, 0}, ry[2] = {0, 0};  // the scales of the next two blocks
+      // this thread's scales of the next four blocks, loaded four blocks ahead
+      const float* px = MODE == 0 ? p.tabx + x : nullptr;
+      const float* py = MODE == 0 ? p.taby + (YVEC ? y0 + et : 2 * ty + half) : nullptr;
+      float nx[4] = {}, ny[4] = {};
       if (MODE == 0) {
-        rx[0] = scale_x(0);
-        ry[0] = scale_y(0);
-        rx[1] = scale_x(1);
-        ry[1] = scale_y(1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          nx[i] = __ldg(px + i * p.pitchx);
+          ny[i] = __ldg(py + i * p.pitchy);
+        }
       }
-      for (int u = 0; u < units; ++u, ++g) {
-        const int b = g & 1;
-        float cx = 0.0f, cy = 0.0f;
+      for (int v = 0; v < units; v += 4) {
+        float sc[4];
+        float* sy = sy_s + 1024 * ((v >> 2) & 1) + 128 * half;
         if (MODE == 0) {
-          cx = scale_value(p.scx, rx[0]);
-          cy = scale_value(p.scy, ry[0]);
-          rx[0] = rx[1];
-          ry[0] = ry[1];
-          rx[1] = scale_x(u + 2);
-          ry[1] = scale_y(u + 2);
-        }
-        float* sy = sy_s + 256 * b + 128 * half;
-        if (YVEC) {
-          sy[et] = cy;
-          named_bar_sync(1 + half, 128);
-        }
-        if (ok) {
-          int got = 0;
-          if (lane == 0)
-            got = mbar_wait_bounded(&tfull[b], (g >> 1) & 1, abort_flag, p.err, DEV_TIMEOUT_TMEM_FULL,
-                               p.timeout_ns);
-          ok = __shfl_sync(0xffffffffu, got, 0) != 0;
-        }
-        tc_fence_after();
-        const float sc = MODE == 0 ? (YVEC ? cx : cx * cy) : 1.0f;
-        const unsigned long long s2 = pack2(sc, sc);
-        const uint32_t ta = t_lane + (uint32_t)(256 * b);
-        uint32_t r[2][16];
-        tmem_ld_x16(ta, r[0]);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          tmem_wait_x16(r[c & 1]);
-          if (c < 7) tmem_ld_x16(ta + 16 * (c + 1), r[(c + 1) & 1]);
-          if (c == 7) {  // the last of this buffer is in registers
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_pair(tempty0[b]);
+          for (int i = 0; i < 4; ++i) {
+            sc[i] = YVEC ? nx[i] : nx[i] * ny[i];
+            if (YVEC) sy[256 * i + et] = ny[i];
           }
+          px += 4 * p.pitchx;
+          py += 4 * p.pitchy;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const unsigned long long v = pack2(r[c & 1][2 * j], r[c & 1][2 * j + 1]);
-            unsigned long long& a = acc[8 * c + j];
-            if (MODE == 1) a = add2(a, v);
-            else if (YVEC)
-              a = fma2(mul2(v, s2),
-                       *reinterpret_cast<const unsigned long long*>(sy + 16 * c + 2 * j), a);
-            else a = fma2(v, s2, a);
+          for (int i = 0; i < 4; ++i) {
+            nx[i] = __ldg(px + i * p.pitchx);
+            ny[i] = __ldg(py + i * p.pitchy);
+          }
+          // two buffers: the quad after next is written behind the next barrier
+          if (YVEC) named_bar_sync(1 + half, 128);
+        }
+        const int n = units - v < 4 ? units - v : 4;
+#pragma unroll 1
+        for (int i = 0; i < n; ++i, ++g) {
+          const int b = g & 1;
+          if (ok) {
+            int got = 0;
+            if (lane == 0)
+              got = mbar_wait_bounded(&tfull[b], (g >> 1) & 1, abort_flag, p.err,
+                                                    DEV_TIMEOUT_TMEM_FULL, p.timeout_ns);
+            ok = __shfl_sync(0xffffffffu, got, 0) != 0;
+          }
+          tc_fence_after();
+          float f = 1.0f;
+          if (MODE == 0) {
+            f = sc[0];
+            sc[0] = sc[1];
+            sc[1] = sc[2];
+            sc[2] = sc[3];
+          }
+          const unsigned long long s2 = pack2(f, f);
+          const uint32_t ta = t_lane + (uint32_t)(256 * b);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {  // 64 columns at a time
+            uint32_t r[4][16];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld_x16(ta + 64 * h + 16 * c, r[c]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_wait_x16(r[c]);
+            if (h == 1) {  // the last of this buffer is in registers
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) arrive_pair(tempty0[b]);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const unsigned long long w = pack2(r[c][2 * j], r[c][2 * j + 1]);
+                unsigned long long& a = acc[32 * h + 8 * c + j];
+                if (MODE == 1) a = add2(a, w);
+                else if (YVEC)
+                  a = fma2(mul2(w, s2),
+                           *reinterpret_cast<const unsigned long long*>(sy + 256 * i + 64 * h +
+                                                                        16 * c + 2 * j), a);
+                else a = fma2(w, s2, a);
+              }
           }
         }
       }
@@ -448,8 +518,39 @@ int launch(rtb_ctx* ctx, const CUtensorMap& tmX, const CUtensorMap& tmY, BlockPa
 
 int launch_pair(rtb_ctx* ctx, int mode, bool yvec, const CUtensorMap& tmX, const CUtensorMap& tmY,
                 BlockParams& p, cudaStream_t s) {
-  if (mode == 1) return launch<1, false>(ctx, tmX, tmY, p, s);
-  return yvec ? launch<0, true>(ctx, tmX, tmY, p, s) : launch<0, false>(ctx, tmX, tmY, p, s);
+  if (mode == 0) {
+    const int64_t units = (p.depth + 127) / 128, blocks = table_blocks(units);
+    TableSide x = {p.scx, p.xrows, (p.xrows + kTile - 1) / kTile * kTile, nullptr};
+    TableSide y = {p.scy, p.ycols, (p.ycols + kTile - 1) / kTile * kTile, nullptr};
+    if (!yvec) {  // one entry for each 128 columns
+      y.s.row_shift = 0;
+      y.rows = (p.ycols + 127) / 128;
+      y.pitch /= 128;
+    }
+    float* ws = nullptr;
+    int st = ws_alloc(ctx, (void**)&ws, (size_t)((x.pitch + y.pitch) * blocks) * sizeof(float), s);
+    if (st) return st;
+    x.out = ws;
+    y.out = ws + x.pitch * blocks;
+    const int64_t longer = x.pitch > y.pitch ? x.pitch : y.pitch;
+    const int64_t gx = (longer + 31) / 32;
+    clear_stale_cuda_error();
+    cudaError_t e = launch_pdl(scale_table_kernel,
+                               dim3((unsigned)(gx < 512 ? gx : 512), (unsigned)((blocks + 31) / 32), 2),
+                               dim3(256), 0, s, (const TableSide)x, (const TableSide)y, (int)units,
+                               (int)blocks);
+    if (e == cudaSuccess) e = cudaGetLastError();
+    st = e == cudaSuccess ? RTB_OK : cuda_status(e, "scale table launch");
+    p.tabx = x.out;
+    p.taby = y.out;
+    p.pitchx = x.pitch;
+    p.pitchy = y.pitch;
+    if (st == RTB_OK)
+      st = yvec ? launch<0, true>(ctx, tmX, tmY, p, s) : launch<0, false>(ctx, tmX, tmY, p, s);
+    ws_free(ws, s);
+    return st;
+  }
+  return launch<1, false>(ctx, tmX, tmY, p, s);
 }
 
 }  // namespace rtb
