@@ -137,13 +137,237 @@ __device__ __forceinline__ void put(float* out, float v, int accumulate) {
   *out = accumulate ? *out + v : v;
 }
 
-// VEC: thread t of the group holds the float4 units t + T i (d % 4 == 0,
-// 16-byte aligned rows), else the columns t + T i.  SAVED: x from the
-// checkpoint.  Partial sums over at most E values in fp32, then shuffles and
-// the group's warps in order.
+constexpr int kRing = 8;                // most stages of the row ring
+constexpr int kRingBytes = 200 * 1024;  // shared memory of an SM for the ring
+
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+// At most n of this thread's copy groups are still under way (n < kRing).
+__device__ __forceinline__ void cp_async_wait_n(int n) {
+  switch (n) {
+    case 7: cp_async_wait<7>(); break;
+    case 6: cp_async_wait<6>(); break;
+    case 5: cp_async_wait<5>(); break;
+    case 4: cp_async_wait<4>(); break;
+    case 3: cp_async_wait<3>(); break;
+    case 2: cp_async_wait<2>(); break;
+    case 1: cp_async_wait<1>(); break;
+    default: cp_async_wait<0>(); break;
+  }
+}
+
+// Up to 8192 columns: T threads a row (a multiple of 32), E values of x and of
+// dy each; VEC: the float4 units t + T i (d % 4 == 0, 16-byte aligned rows),
+// else the columns t + T i.  SAVED: x from the checkpoint.  ACT: an activation
+// (its weight and bias are read again for every row; without one the weight
+// stays in registers).
+//
+// Each thread copies its own values of the group's next `stages` rows into
+// shared memory (cp.async), waits for its own copies alone and refills the slot
+// once it has used the values: no barrier is needed for the ring.  Eight values
+// a thread (five registers each) leave room for 1024 threads on an SM, whose
+// number, not the bytes in flight, hides the row's chain of loads, sums,
+// shuffles and one barrier; what bounds it then is HBM.
+template <int kBlock, int E, bool VEC, bool SAVED, bool ACT>
+__global__ void __launch_bounds__(kBlock, 1024 / kBlock)
+    norm_bwd_rows_kernel(const NormBwdParams p, const int T, const int stages, const float inv_d,
+                         float* dg, float* db) {
+  static_assert(!SAVED || VEC, "bytes have no asynchronous copy");
+  constexpr int G = VEC ? E / 4 : E;  // copies of x (and of dy) a thread
+  constexpr int C = E / G;            // columns of a copy
+  __shared__ float2 red[2][kBlock / 32];
+  extern __shared__ float4 ring4[];   // the ring, then reused for the CTA's sums
+  const int R = kBlock / T;           // rows a CTA works on
+  const int grp = threadIdx.x / T, t = threadIdx.x - grp * T;
+  const int units = VEC ? p.d >> 2 : p.d;
+  const bool sums = p.part || dg || db;
+  // a slot: x, then dy, both on 16-byte boundaries
+  const int xbytes = ((SAVED ? units * 4 : units * C * 4) + 15) & ~15;
+  const int row_bytes = xbytes + ((units * C * 4 + 15) & ~15);
+  const uint32_t slot0 = smem_u32(ring4) + (uint32_t)(grp * stages * row_bytes);
+  float ag[E], ab[E], gw[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    ag[i] = ab[i] = 0.0f;
+    gw[i] = 1.0f;
+  }
+  griddep_wait();
+  griddep_launch_dependents();
+  if (!ACT && p.g) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int j = C * (t + T * (i / C)) + i % C;
+      if (j < p.d) gw[i] = __ldg(p.g + j);
+    }
+  }
+  const int64_t step = (int64_t)gridDim.x * R;
+  auto fetch = [&](int64_t r, int s) {
+    if (r < p.rows) {
+      const uint32_t xs = slot0 + (uint32_t)(s * row_bytes), ys = xs + (uint32_t)xbytes;
+      const char* xr = SAVED ? reinterpret_cast<const char*>(p.q + r * p.ldq)
+                             : reinterpret_cast<const char*>(p.x + r * p.ldx);
+      const char* yr = reinterpret_cast<const char*>(p.dy + r * p.lddy);
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const int k = t + T * i;
+        if (k < units) {
+          if (VEC && !SAVED) cp_async_16_cg(xs + 16 * k, xr + 16 * k);
+          else cp_async_4(xs + 4 * k, xr + 4 * k);
+          if (VEC) cp_async_16_cg(ys + 16 * k, yr + 16 * k);
+          else cp_async_4(ys + 4 * k, yr + 4 * k);
+        }
+      }
+    }
+    cp_async_commit();  // (an empty group behind the last row)
+  };
+  int64_t r = grp < R ? (int64_t)blockIdx.x * R + grp : p.rows;
+  for (int s = 0; s < stages; ++s) fetch(r + s * step, s);
+  float mean = 0.0f, rstd = 0.0f;
+  if (r < p.rows) {
+    mean = __ldg(p.mean + r);
+    rstd = __ldg(p.rstd + r);
+  }
+  int slot = 0, phase = 0;
+  for (; r < p.rows; r += step, phase ^= 1) {
+    // the next row's statistics and this row's block scales
+    const int64_t rn = r + step < p.rows ? r + step : r;
+    const float mean_n = __ldg(p.mean + rn), rstd_n = __ldg(p.rstd + rn);
+    uint32_t sb[G];
+    if (SAVED) {
+      const uint8_t* sr = p.scale + r * p.lds;
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const int k = t + T * i;
+        sb[i] = __ldg(sr + ((k < units ? k : 0) >> 5));
+      }
+    }
+    cp_async_wait_n(stages - 1);  // this slot's copies, the oldest group, have landed
+    float u[E], h[E];             // x, then u; dy, then h
+    const uint32_t xs = slot0 + (uint32_t)(slot * row_bytes), ys = xs + (uint32_t)xbytes;
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const int k = t + T * i;
+      float4 a = make_float4(mean, mean, mean, mean), g = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k < units) {
+        if (SAVED) {
+          a = e4m3x4_to_float4(__float_as_uint(lds32(xs + 4 * k)));
+          const float s = e8m0_to_float(sb[i]);
+          a.x *= s; a.y *= s; a.z *= s; a.w *= s;
+        } else if (VEC) {
+          a = lds128(xs + 16 * k);
+        } else {
+          a.x = lds32(xs + 4 * k);
+        }
+        if (VEC) g = lds128(ys + 16 * k);
+        else g.x = lds32(ys + 4 * k);
+      }
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        u[C * i + c] = (&a.x)[c];
+        h[C * i + c] = (&g.x)[c];
+      }
+    }
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      u[i] = (u[i] - mean) * rstd;
+      float gv = gw[i];
+      if (ACT) {
+        const int j = C * (t + T * (i / C)) + i % C;
+        gv = p.g && j < p.d ? __ldg(p.g + j) : 1.0f;
+        const float bv = p.b && j < p.d ? __ldg(p.b + j) : 0.0f;
+        h[i] *= act_slope(fmaf(u[i], gv, bv), p.act);
+      }
+      ag[i] = fmaf(h[i], u[i], ag[i]);
+      ab[i] += h[i];
+      h[i] *= gv;
+      s1 += h[i];
+      s2 = fmaf(h[i], u[i], s2);
+    }
+    fetch(r + stages * step, slot);  // every value of the slot is in registers
+    if (++slot == stages) slot = 0;
+    if (p.dx) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+        s2 += __shfl_xor_sync(0xffffffffu, s2, o);
+      }
+      if (T > 32) {
+        // two buffers, so that one barrier a row is enough; every warp adds the
+        // warps' sums for itself, in the same order
+        const int nw = T >> 5, w0 = grp * nw;
+        if ((t & 31) == 0) red[phase][w0 + (t >> 5)] = make_float2(s1, s2);
+        named_bar_sync(1 + grp, T);
+        const float2 q = (t & 31) < nw ? red[phase][w0 + (t & 31)] : make_float2(0.f, 0.f);
+        s1 = q.x;
+        s2 = q.y;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+          s2 += __shfl_xor_sync(0xffffffffu, s2, o);
+        }
+      }
+      const float m1 = s1 * inv_d, m2 = s2 * inv_d;
+      float* dxr = p.dx + r * p.lddx;
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const int k = t + T * i;
+        if (k >= units) continue;
+        float4 w;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+          (&w.x)[c] = rstd * fmaf(-u[C * i + c], m2, h[C * i + c] - m1);
+        if (VEC) {
+          float4* o = reinterpret_cast<float4*>(dxr) + k;
+          if (p.accumulate) {
+            const float4 q = *o;
+            w.x += q.x; w.y += q.y; w.z += q.z; w.w += q.w;
+          }
+          __stcs(o, w);
+        } else {
+          put(dxr + k, w.x, p.accumulate);
+        }
+      }
+    }
+    mean = mean_n;
+    rstd = rstd_n;
+  }
+  cp_async_wait<0>();
+  if (!sums) return;
+  // the CTA's sums over its groups, in group order, where the ring was
+  float* acc_s = reinterpret_cast<float*>(ring4);
+  __syncthreads();
+  for (int gi = 0; gi < R; ++gi) {
+    if (grp == gi) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const int j = C * (t + T * (i / C)) + i % C;
+        if (j >= p.d) continue;
+        put(acc_s + j, ag[i], gi > 0);
+        put(acc_s + p.d + j, ab[i], gi > 0);
+      }
+    }
+    __syncthreads();
+  }
+  for (int j = threadIdx.x; j < p.d; j += kBlock) {
+    if (p.part) {
+      float* pr = p.part + (int64_t)blockIdx.x * 2 * p.d;
+      pr[j] = acc_s[j];
+      pr[p.d + j] = acc_s[p.d + j];
+    } else {
+      if (dg) put(dg + j, acc_s[j], p.accumulate);
+      if (db) put(db + j, acc_s[p.d + j], p.accumulate);
+    }
+  }
+}
+
+// Rows of 8193 to 16384 columns, and checkpoints that no 4-byte copy fits:
+// values loaded straight into registers, the sums for dg and db in registers
+// too, or in shared memory where 1024 threads leave 64 registers each.
 template <int T, int E, bool VEC, bool SAVED>
 __global__ void __launch_bounds__(T > 256 ? T : 256, T > 512 ? 1 : (T > 256 ? 1 : 2))
-    norm_bwd_rows_kernel(const NormBwdParams p, float* dg, float* db) {
+    norm_bwd_direct_kernel(const NormBwdParams p, float* dg, float* db) {
   constexpr int kBlock = T > 256 ? T : 256;
   constexpr int G = VEC ? E / 4 : E;  // loads of x (and of dy) a thread
   constexpr int C = E / G;            // columns of a load
@@ -353,11 +577,32 @@ __global__ void __launch_bounds__(kThreads) norm_bwd_reduce_kernel(const float* 
   }
 }
 
+// The sums' way out: a partial row for each CTA and the second kernel, or the
+// only CTA's own stores.
+template <typename Launch>
+int launch_with_sums(NormBwdParams& p, int grid, float* dg, float* db, cudaStream_t s,
+                     const Launch& launch) {
+  float* part = nullptr;
+  if (grid > 1 && (dg || db)) {
+    const int st = ws_alloc(nullptr, (void**)&part, (size_t)grid * 2 * p.d * sizeof(float), s);
+    if (st) return st;
+  }
+  p.part = part;
+  clear_stale_cuda_error();
+  cudaError_t e = launch();
+  if (e == cudaSuccess && part)
+    e = launch_pdl(norm_bwd_reduce_kernel, dim3((unsigned)((p.d + 31) / 32), 2), dim3(kThreads), 0,
+                   s, (const float*)part, grid, p.d, dg, db, p.accumulate);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  ws_free(part, s);
+  return e == cudaSuccess ? RTB_OK : cuda_status(e, "layer_norm_backward launch");
+}
+
 template <int T, int E, bool VEC, bool SAVED>
-int launch_rows(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStream_t s) {
+int launch_direct(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStream_t s) {
   constexpr int kBlock = T > 256 ? T : 256;
   constexpr int R = kBlock / T;
-  auto* k = norm_bwd_rows_kernel<T, E, VEC, SAVED>;
+  auto* k = norm_bwd_direct_kernel<T, E, VEC, SAVED>;
   const size_t smem = (dg || db) ? (size_t)2 * p.d * sizeof(float) : 0;
   cudaError_t e = cudaSuccess;
   if (smem > 48 * 1024) {
@@ -369,39 +614,55 @@ int launch_rows(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStream
   if (per_sm < 1) per_sm = 1;
   const int64_t need = (p.rows + R - 1) / R, cap = (int64_t)ctx->sm_count * per_sm;
   const int grid = (int)(need < cap ? need : cap);
-  if (!dg && !db) {
-    clear_stale_cuda_error();
-    e = launch_pdl(k, dim3((unsigned)grid), dim3(kBlock), 0, s, (const NormBwdParams)p,
-                   (float*)nullptr, (float*)nullptr);
-    if (e == cudaSuccess) e = cudaGetLastError();
-    return e == cudaSuccess ? RTB_OK : cuda_status(e, "layer_norm_backward launch");
-  }
-  float* part = nullptr;
-  if (grid > 1) {
-    const int st = ws_alloc(ctx, (void**)&part, (size_t)grid * 2 * p.d * sizeof(float), s);
-    if (st) return st;
-  }
-  p.part = part;
-  clear_stale_cuda_error();
-  e = launch_pdl(k, dim3((unsigned)grid), dim3(kBlock), smem, s, (const NormBwdParams)p, dg, db);
-  if (e == cudaSuccess && part)
-    e = launch_pdl(norm_bwd_reduce_kernel, dim3((unsigned)((p.d + 31) / 32), 2), dim3(kThreads), 0,
-                   s, (const float*)part, grid, p.d, dg, db, p.accumulate);
-  if (e == cudaSuccess) e = cudaGetLastError();
-  ws_free(part, s);
-  return e == cudaSuccess ? RTB_OK : cuda_status(e, "layer_norm_backward launch");
+  return launch_with_sums(p, grid, dg, db, s, [&] {
+    return launch_pdl(k, dim3((unsigned)grid), dim3(kBlock), smem, s, (const NormBwdParams)p, dg,
+                      db);
+  });
+}
+
+template <int kBlock, int E, bool VEC, bool SAVED, bool ACT>
+int launch_rows(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStream_t s) {
+  constexpr int G = VEC ? E / 4 : E;
+  constexpr int kPerSm = 1024 / kBlock;
+  auto* k = norm_bwd_rows_kernel<kBlock, E, VEC, SAVED, ACT>;
+  const int units = VEC ? p.d / 4 : p.d;
+  const int T = (units + 32 * G - 1) / (32 * G) * 32, R = kBlock / T;
+  const int row_bytes = (((SAVED ? p.d : 4 * p.d) + 15) & ~15) + ((4 * p.d + 15) & ~15);
+  int stages = kRingBytes / kPerSm / (R * row_bytes);
+  stages = stages < 1 ? 1 : (stages > kRing ? kRing : stages);
+  int smem = R * stages * row_bytes;
+  if (smem < 8 * p.d) smem = 8 * p.d;  // the CTA's sums
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return cuda_status(e, "layer_norm_backward smem attribute");
+  const int64_t need = (p.rows + R - 1) / R, cap = (int64_t)ctx->sm_count * kPerSm;
+  const int grid = (int)(need < cap ? need : cap);
+  return launch_with_sums(p, grid, dg, db, s, [&] {
+    return launch_pdl(k, dim3((unsigned)grid), dim3(kBlock), (size_t)smem, s,
+                      (const NormBwdParams)p, T, stages, 1.0f / (float)p.d, dg, db);
+  });
 }
 
 template <bool VEC, bool SAVED>
 int launch_width(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStream_t s) {
-  if (p.d <= 128) return launch_rows<32, 4, VEC, SAVED>(ctx, p, dg, db, s);
-  if (p.d <= 256) return launch_rows<32, 8, VEC, SAVED>(ctx, p, dg, db, s);
-  if (p.d <= 512) return launch_rows<32, 16, VEC, SAVED>(ctx, p, dg, db, s);
-  if (p.d <= 1024) return launch_rows<64, 16, VEC, SAVED>(ctx, p, dg, db, s);
-  if (p.d <= 2048) return launch_rows<128, 16, VEC, SAVED>(ctx, p, dg, db, s);
-  if (p.d <= 4096) return launch_rows<256, 16, VEC, SAVED>(ctx, p, dg, db, s);
-  if (p.d <= 8192) return launch_rows<512, 16, VEC, SAVED>(ctx, p, dg, db, s);
-  return launch_rows<1024, 16, VEC, SAVED>(ctx, p, dg, db, s);
+  if constexpr (VEC || !SAVED) {
+    const bool act = p.act != RTB_ACT_NONE;
+    if (p.d <= 128)
+      return act ? launch_rows<512, 4, VEC, SAVED, true>(ctx, p, dg, db, s)
+                 : launch_rows<512, 4, VEC, SAVED, false>(ctx, p, dg, db, s);
+    if (p.d <= 4096)
+      return act ? launch_rows<512, 8, VEC, SAVED, true>(ctx, p, dg, db, s)
+                 : launch_rows<512, 8, VEC, SAVED, false>(ctx, p, dg, db, s);
+    if (p.d <= 8192)
+      return act ? launch_rows<1024, 8, VEC, SAVED, true>(ctx, p, dg, db, s)
+                 : launch_rows<1024, 8, VEC, SAVED, false>(ctx, p, dg, db, s);
+  } else {
+    if (p.d <= 512) return launch_direct<32, 16, VEC, SAVED>(ctx, p, dg, db, s);
+    if (p.d <= 1024) return launch_direct<64, 16, VEC, SAVED>(ctx, p, dg, db, s);
+    if (p.d <= 2048) return launch_direct<128, 16, VEC, SAVED>(ctx, p, dg, db, s);
+    if (p.d <= 4096) return launch_direct<256, 16, VEC, SAVED>(ctx, p, dg, db, s);
+    if (p.d <= 8192) return launch_direct<512, 16, VEC, SAVED>(ctx, p, dg, db, s);
+  }
+  return launch_direct<1024, 16, VEC, SAVED>(ctx, p, dg, db, s);
 }
 
 }  // namespace
