@@ -158,22 +158,22 @@ __device__ __forceinline__ void cp_async_wait_n(int n) {
 }
 
 // Up to 8192 columns: T threads a row (a multiple of 32), E values of x and of
-// dy each; VEC: the float4 units t + T i (d % 4 == 0, 16-byte aligned rows),
-// else the columns t + T i.  SAVED: x from the checkpoint.  ACT: an activation
-// (its weight and bias are read again for every row; without one the weight
-// stays in registers).
+// dy each: lane l of the group's warp w holds the units 32 G w + l + 32 i, i <
+// G, where a unit is a float4 (VEC: d % 4 == 0, 16-byte aligned rows) or a
+// column; the distances are constants, so that a row's addresses cost little.
+// SAVED: x from the checkpoint.  ACT: an activation.
 //
-// Each thread copies its own values of the group's next `stages` rows into
+// VEC: each thread copies its own values of the group's next `stages` rows into
 // shared memory (cp.async), waits for its own copies alone and refills the slot
 // once it has used the values: no barrier is needed for the ring.  Eight values
 // a thread (five registers each) leave room for 1024 threads on an SM, whose
 // number, not the bytes in flight, hides the row's chain of loads, sums,
-// shuffles and one barrier; what bounds it then is HBM.
+// shuffles and one barrier; what bounds it then is HBM.  Other rows are loaded
+// into registers directly: copies of 4 bytes cost more than they hide.
 template <int kBlock, int E, bool VEC, bool SAVED, bool ACT>
 __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
     norm_bwd_rows_kernel(const NormBwdParams p, const int T, const int stages, const float inv_d,
                          float* dg, float* db) {
-  static_assert(!SAVED || VEC, "bytes have no asynchronous copy");
   constexpr int G = VEC ? E / 4 : E;  // copies of x (and of dy) a thread
   constexpr int C = E / G;            // columns of a copy
   __shared__ float2 red[2][kBlock / 32];
@@ -181,48 +181,50 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
   const int R = kBlock / T;           // rows a CTA works on
   const int grp = threadIdx.x / T, t = threadIdx.x - grp * T;
   const int units = VEC ? p.d >> 2 : p.d;
+  const int k0 = (t >> 5) * (32 * G) + (t & 31);  // this thread's first unit
+  const int rem = units - k0;                     // its unit i exists if 32 i < rem
   const bool sums = p.part || dg || db;
   // a slot: x, then dy, both on 16-byte boundaries
   const int xbytes = ((SAVED ? units * 4 : units * C * 4) + 15) & ~15;
   const int row_bytes = xbytes + ((units * C * 4 + 15) & ~15);
   const uint32_t slot0 = smem_u32(ring4) + (uint32_t)(grp * stages * row_bytes);
-  float ag[E], ab[E], gw[E];
+  constexpr bool kKeep = VEC && !ACT;  // the weight stays in registers
+  float ag[E], ab[E], gw[kKeep ? E : 1];
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     ag[i] = ab[i] = 0.0f;
-    gw[i] = 1.0f;
+    if (kKeep) gw[i] = 1.0f;
   }
   griddep_wait();
   griddep_launch_dependents();
-  if (!ACT && p.g) {
+  if (kKeep && p.g) {
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const int j = C * (t + T * (i / C)) + i % C;
-      if (j < p.d) gw[i] = __ldg(p.g + j);
+      if (32 * (i / C) < rem) gw[i] = __ldg(p.g + C * (k0 + 32 * (i / C)) + i % C);
     }
   }
   const int64_t step = (int64_t)gridDim.x * R;
   auto fetch = [&](int64_t r, int s) {
     if (r < p.rows) {
-      const uint32_t xs = slot0 + (uint32_t)(s * row_bytes), ys = xs + (uint32_t)xbytes;
-      const char* xr = SAVED ? reinterpret_cast<const char*>(p.q + r * p.ldq)
-                             : reinterpret_cast<const char*>(p.x + r * p.ldx);
-      const char* yr = reinterpret_cast<const char*>(p.dy + r * p.lddy);
+      const uint32_t xs = slot0 + (uint32_t)(s * row_bytes + (SAVED ? 4 : 16) * k0);
+      const uint32_t ys = slot0 + (uint32_t)(s * row_bytes + xbytes + 16 * k0);
+      const char* xr = SAVED ? reinterpret_cast<const char*>(p.q + r * p.ldq + 4 * k0)
+                             : reinterpret_cast<const char*>(p.x + r * p.ldx + 4 * k0);
+      const char* yr = reinterpret_cast<const char*>(p.dy + r * p.lddy + 4 * k0);
 #pragma unroll
       for (int i = 0; i < G; ++i) {
-        const int k = t + T * i;
-        if (k < units) {
-          if (VEC && !SAVED) cp_async_16_cg(xs + 16 * k, xr + 16 * k);
-          else cp_async_4(xs + 4 * k, xr + 4 * k);
-          if (VEC) cp_async_16_cg(ys + 16 * k, yr + 16 * k);
-          else cp_async_4(ys + 4 * k, yr + 4 * k);
+        if (32 * i < rem) {
+          if (SAVED) cp_async_4(xs + 128 * i, xr + 128 * i);
+          else cp_async_16_cg(xs + 512 * i, xr + 512 * i);
+          cp_async_16_cg(ys + 512 * i, yr + 512 * i);
         }
       }
     }
     cp_async_commit();  // (an empty group behind the last row)
   };
   int64_t r = grp < R ? (int64_t)blockIdx.x * R + grp : p.rows;
-  for (int s = 0; s < stages; ++s) fetch(r + s * step, s);
+  if (VEC)
+    for (int s = 0; s < stages; ++s) fetch(r + s * step, s);
   float mean = 0.0f, rstd = 0.0f;
   if (r < p.rows) {
     mean = __ldg(p.mean + r);
@@ -233,50 +235,67 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
     // the next row's statistics and this row's block scales
     const int64_t rn = r + step < p.rows ? r + step : r;
     const float mean_n = __ldg(p.mean + rn), rstd_n = __ldg(p.rstd + rn);
-    uint32_t sb[G];
-    if (SAVED) {
-      const uint8_t* sr = p.scale + r * p.lds;
+    uint32_t sb[VEC ? G : 1];
+    if (SAVED && VEC) {
+      const uint8_t* sr = p.scale + r * p.lds + (t >> 5) * G;  // one byte for 32 units
+#pragma unroll
+      for (int i = 0; i < G; ++i) sb[i] = 32 * i < rem ? __ldg(sr + i) : 0u;
+    }
+    float u[E], h[E];  // x, then u; dy, then h
+    if (VEC) {
+      cp_async_wait_n(stages - 1);  // this slot's copies, the oldest group, have landed
+      const uint32_t xs = slot0 + (uint32_t)(slot * row_bytes + (SAVED ? 4 : 16) * k0);
+      const uint32_t ys = slot0 + (uint32_t)(slot * row_bytes + xbytes + 16 * k0);
 #pragma unroll
       for (int i = 0; i < G; ++i) {
-        const int k = t + T * i;
-        sb[i] = __ldg(sr + ((k < units ? k : 0) >> 5));
-      }
-    }
-    cp_async_wait_n(stages - 1);  // this slot's copies, the oldest group, have landed
-    float u[E], h[E];             // x, then u; dy, then h
-    const uint32_t xs = slot0 + (uint32_t)(slot * row_bytes), ys = xs + (uint32_t)xbytes;
-#pragma unroll
-    for (int i = 0; i < G; ++i) {
-      const int k = t + T * i;
-      float4 a = make_float4(mean, mean, mean, mean), g = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (k < units) {
-        if (SAVED) {
-          a = e4m3x4_to_float4(__float_as_uint(lds32(xs + 4 * k)));
-          const float s = e8m0_to_float(sb[i]);
-          a.x *= s; a.y *= s; a.z *= s; a.w *= s;
-        } else if (VEC) {
-          a = lds128(xs + 16 * k);
-        } else {
-          a.x = lds32(xs + 4 * k);
+        float4 a = make_float4(mean, mean, mean, mean), g = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (32 * i < rem) {
+          if (SAVED) {
+            a = e4m3x4_to_float4(__float_as_uint(lds32(xs + 128 * i)));
+            const float s = e8m0_to_float(sb[i]);
+            a.x *= s; a.y *= s; a.z *= s; a.w *= s;
+          } else {
+            a = lds128(xs + 512 * i);
+          }
+          g = lds128(ys + 512 * i);
         }
-        if (VEC) g = lds128(ys + 16 * k);
-        else g.x = lds32(ys + 4 * k);
-      }
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        u[C * i + c] = (&a.x)[c];
-        h[C * i + c] = (&g.x)[c];
+        for (int c = 0; c < C; ++c) {
+          u[C * i + c] = (&a.x)[c];
+          h[C * i + c] = (&g.x)[c];
+        }
+      }
+    } else {
+      const float* yr = p.dy + r * p.lddy + k0;
+      const float* xr = p.x + r * p.ldx + k0;
+      const uint8_t* qr = p.q + r * p.ldq + k0;
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        u[i] = mean;
+        h[i] = 0.0f;
+        uint32_t code = 0, byte = 0;
+        if (32 * i < rem) {
+          if (SAVED) {
+            code = __ldcs(qr + 32 * i);
+            byte = __ldg(p.scale + r * p.lds + (k0 + 32 * i) / kFp8Block);
+          } else {
+            u[i] = __ldcs(xr + 32 * i);
+          }
+          h[i] = __ldcs(yr + 32 * i);
+        }
+        if (SAVED && 32 * i < rem) u[i] = e4m3x2_to_float2(code).x * e8m0_to_float(byte);
       }
     }
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       u[i] = (u[i] - mean) * rstd;
-      float gv = gw[i];
+      const int j = C * (k0 + 32 * (i / C)) + i % C;
+      float gv = 1.0f;
+      if (kKeep) gv = gw[i];
+      else if (p.g && 32 * (i / C) < rem) gv = __ldg(p.g + j);
       if (ACT) {
-        const int j = C * (t + T * (i / C)) + i % C;
-        gv = p.g && j < p.d ? __ldg(p.g + j) : 1.0f;
-        const float bv = p.b && j < p.d ? __ldg(p.b + j) : 0.0f;
+        const float bv = p.b && 32 * (i / C) < rem ? __ldg(p.b + j) : 0.0f;
         h[i] *= act_slope(fmaf(u[i], gv, bv), p.act);
       }
       ag[i] = fmaf(h[i], u[i], ag[i]);
@@ -285,8 +304,10 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
       s1 += h[i];
       s2 = fmaf(h[i], u[i], s2);
     }
-    fetch(r + stages * step, slot);  // every value of the slot is in registers
-    if (++slot == stages) slot = 0;
+    if (VEC) {
+      fetch(r + stages * step, slot);  // every value of the slot is in registers
+      if (++slot == stages) slot = 0;
+    }
     if (p.dx) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
@@ -309,24 +330,23 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
         }
       }
       const float m1 = s1 * inv_d, m2 = s2 * inv_d;
-      float* dxr = p.dx + r * p.lddx;
+      float* dxr = p.dx + r * p.lddx + C * k0;
 #pragma unroll
       for (int i = 0; i < G; ++i) {
-        const int k = t + T * i;
-        if (k >= units) continue;
+        if (32 * i >= rem) continue;
         float4 w;
 #pragma unroll
         for (int c = 0; c < C; ++c)
           (&w.x)[c] = rstd * fmaf(-u[C * i + c], m2, h[C * i + c] - m1);
         if (VEC) {
-          float4* o = reinterpret_cast<float4*>(dxr) + k;
+          float4* o = reinterpret_cast<float4*>(dxr) + 32 * i;
           if (p.accumulate) {
             const float4 q = *o;
             w.x += q.x; w.y += q.y; w.z += q.z; w.w += q.w;
           }
           __stcs(o, w);
         } else {
-          put(dxr + k, w.x, p.accumulate);
+          put(dxr + 32 * i, w.x, p.accumulate);
         }
       }
     }
@@ -342,8 +362,8 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
     if (grp == gi) {
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const int j = C * (t + T * (i / C)) + i % C;
-        if (j >= p.d) continue;
+        if (32 * (i / C) >= rem) continue;
+        const int j = C * (k0 + 32 * (i / C)) + i % C;
         put(acc_s + j, ag[i], gi > 0);
         put(acc_s + p.d + j, ab[i], gi > 0);
       }
@@ -362,9 +382,9 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
   }
 }
 
-// Rows of 8193 to 16384 columns, and checkpoints that no 4-byte copy fits:
-// values loaded straight into registers, the sums for dg and db in registers
-// too, or in shared memory where 1024 threads leave 64 registers each.
+// Rows of 8193 to 16384 columns: 1024 threads with 16 values each, loaded
+// straight into registers; the sums for dg and db, for which 64 registers a
+// thread leave no room, in shared memory.
 template <int T, int E, bool VEC, bool SAVED>
 __global__ void __launch_bounds__(T > 256 ? T : 256, T > 512 ? 1 : (T > 256 ? 1 : 2))
     norm_bwd_direct_kernel(const NormBwdParams p, float* dg, float* db) {
@@ -630,7 +650,7 @@ int launch_rows(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStream
   const int row_bytes = (((SAVED ? p.d : 4 * p.d) + 15) & ~15) + ((4 * p.d + 15) & ~15);
   int stages = kRingBytes / kPerSm / (R * row_bytes);
   stages = stages < 1 ? 1 : (stages > kRing ? kRing : stages);
-  int smem = R * stages * row_bytes;
+  int smem = VEC ? R * stages * row_bytes : 0;
   if (smem < 8 * p.d) smem = 8 * p.d;  // the CTA's sums
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return cuda_status(e, "layer_norm_backward smem attribute");
@@ -644,24 +664,16 @@ int launch_rows(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStream
 
 template <bool VEC, bool SAVED>
 int launch_width(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStream_t s) {
-  if constexpr (VEC || !SAVED) {
-    const bool act = p.act != RTB_ACT_NONE;
-    if (p.d <= 128)
-      return act ? launch_rows<512, 4, VEC, SAVED, true>(ctx, p, dg, db, s)
-                 : launch_rows<512, 4, VEC, SAVED, false>(ctx, p, dg, db, s);
-    if (p.d <= 4096)
-      return act ? launch_rows<512, 8, VEC, SAVED, true>(ctx, p, dg, db, s)
-                 : launch_rows<512, 8, VEC, SAVED, false>(ctx, p, dg, db, s);
-    if (p.d <= 8192)
-      return act ? launch_rows<1024, 8, VEC, SAVED, true>(ctx, p, dg, db, s)
-                 : launch_rows<1024, 8, VEC, SAVED, false>(ctx, p, dg, db, s);
-  } else {
-    if (p.d <= 512) return launch_direct<32, 16, VEC, SAVED>(ctx, p, dg, db, s);
-    if (p.d <= 1024) return launch_direct<64, 16, VEC, SAVED>(ctx, p, dg, db, s);
-    if (p.d <= 2048) return launch_direct<128, 16, VEC, SAVED>(ctx, p, dg, db, s);
-    if (p.d <= 4096) return launch_direct<256, 16, VEC, SAVED>(ctx, p, dg, db, s);
-    if (p.d <= 8192) return launch_direct<512, 16, VEC, SAVED>(ctx, p, dg, db, s);
-  }
+  const bool act = p.act != RTB_ACT_NONE;
+  if (p.d <= 128)
+    return act ? launch_rows<512, 4, VEC, SAVED, true>(ctx, p, dg, db, s)
+               : launch_rows<512, 4, VEC, SAVED, false>(ctx, p, dg, db, s);
+  if (p.d <= 4096)
+    return act ? launch_rows<512, 8, VEC, SAVED, true>(ctx, p, dg, db, s)
+               : launch_rows<512, 8, VEC, SAVED, false>(ctx, p, dg, db, s);
+  if (p.d <= 8192)
+    return act ? launch_rows<1024, 8, VEC, SAVED, true>(ctx, p, dg, db, s)
+               : launch_rows<1024, 8, VEC, SAVED, false>(ctx, p, dg, db, s);
   return launch_direct<1024, 16, VEC, SAVED>(ctx, p, dg, db, s);
 }
 
