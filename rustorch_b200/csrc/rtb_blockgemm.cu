@@ -14,12 +14,17 @@
 // with the length of the chain.
 //
 // A CTA computes a 128 x BN tile: X rows (MMA M side, TMEM lanes) by Y columns
-// (MMA N side).  Roles (warp index): 0 TMA producer, 1 TMEM allocator + MMA
-// issuer, 2..5 epilogue (TMEM lanes 32 (w % 4)..).  The accumulator is double
-// buffered in TMEM, so the promotion of one block overlaps the MMAs of the
-// next.  Every wait is bounded: after a timeout a role goes on without waiting
-// (no thread leaves early, so that barriers still meet), the output is
-// undefined and the error word tells the host.
+// (MMA N side).  Few tiles: a cluster of 2, 4 or 8 CTAs shares a tile, each a
+// part of the contraction, and adds the parts out of one another's shared
+// memory in rank order (no workspace, no counters, the same bits every time).
+// Roles (warp index): 0 TMA producer, 1 TMEM allocator + MMA issuer, 2..5
+// epilogue (TMEM lanes 32 (w % 4)..).  The accumulator is double buffered in
+// TMEM, so the promotion of one block overlaps the MMAs of the next.  The
+// finished tile goes through shared memory (the idle load ring), so that its
+// stores run along the output's rows and bias, activation and the sum of the
+// parts are one short loop.  Every wait is bounded: after a timeout a role goes
+// on without waiting (no thread leaves early, so that barriers still meet), the
+// output is undefined and the error word tells the host.
 //
 // Shared memory (128-byte swizzle throughout):
 //   MODE 0, K-major: row r at r * 128 B holds 128 e4m3 of the contraction.
@@ -35,18 +40,25 @@ namespace {
 constexpr int kX = 128;                // tile rows
 constexpr int kXBytes = 128 * 128;     // X bytes of a stage (16 KB, both modes)
 constexpr int kSmemMax = 232448;       // dynamic shared memory per CTA
-constexpr int kReserve = 4096;         // barriers, scales, alignment slack
+constexpr int kReserve = 2048;         // barriers, alignment slack
+constexpr int kScaleUnits = 32;        // blocks whose scales are staged at a time
 constexpr int kThreads = 192;
 
-template <int MODE, int BN>
+template <int MODE, int BN, bool YVEC>
 struct Cfg {
   static constexpr int kDepth = MODE == 0 ? 128 : 64;  // contraction elements of a stage
   static constexpr int kPieces = MODE == 0 ? 1 : 3;
   static constexpr int kYPiece = BN * 128;             // one Y piece of a stage (BN x 128 B)
   static constexpr int kStageBytes = kXBytes + kPieces * kYPiece;
-  static constexpr int kStagesRaw = (kSmemMax - kReserve) / kStageBytes;
+  static constexpr int kSy = YVEC ? BN : 1;            // column scales of a block
+  static constexpr int kScaleBytes = MODE == 0 ? kScaleUnits * (128 + kSy) * 4 : 0;
+  static constexpr int kStagesRaw = (kSmemMax - kReserve - kScaleBytes) / kStageBytes;
   static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;
-  static constexpr int kSmemBytes = kStages * kStageBytes + kReserve;
+  static constexpr int kSmemBytes = kStages * kStageBytes + kScaleBytes + kReserve;
+  // the finished tile: [128][BN + 4] floats, or [BN][132] where X is the
+  // output's columns
+  static_assert(kStages * kStageBytes >= 128 * (BN + 4) * 4 &&
+                    kStages * kStageBytes >= BN * 132 * 4, "the ring holds the finished tile");
   static constexpr int kPerUnit = 128 / kDepth;        // stages of a promotion unit
   static constexpr int kTmemCols = 2 * BN < 32 ? 32 : 2 * BN;
   static_assert(kStages >= 2, "two stages");
@@ -74,25 +86,61 @@ __device__ __forceinline__ void mma_e(uint32_t d, uint64_t a, uint64_t b, uint32
   }
 }
 
+// The scales of blocks u .. u + n - 1 of row r, decoded, to dst[0], dst[step],
+// ...; zero for rows past the operand.
+__device__ __forceinline__ void stage_scales(const ScaleRef& s, int64_t r, int64_t rows, int u,
+                                             int n, float* dst, int step) {
+  const bool in = r < rows;
+  const int64_t at = in ? (r >> s.row_shift) * s.ld_row + (int64_t)u * s.ld_col : 0;
+  for (int k = 0; k < n; k += 8) {
+    uint32_t raw[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      raw[i] = load_scale(s, at + (int64_t)(k + i < n ? k + i : k) * s.ld_col);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (k + i < n) dst[(k + i) * step] = in ? scale_value(s, raw[i]) : 0.0f;
+  }
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
 // YVEC (MODE 0): a scale for every Y column (block_rows 1); otherwise the
 // tile's columns lie in one 128-row block and share one.
 template <int MODE, int BN, bool YVEC>
 __global__ void __launch_bounds__(kThreads, 1)
     block_gemm_kernel(const __grid_constant__ CUtensorMap tmX,
                       const __grid_constant__ CUtensorMap tmY, const BlockParams p) {
-  using C = Cfg<MODE, BN>;
+  using C = Cfg<MODE, BN, YVEC>;
   constexpr int S = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  uint8_t* tail = base + S * C::kStageBytes;
+  float* sx = reinterpret_cast<float*>(base + S * C::kStageBytes);  // [kScaleUnits][128]
+  float* sy = sx + (MODE == 0 ? kScaleUnits * 128 : 0);             // [kScaleUnits][kSy]
+  uint8_t* tail = base + S * C::kStageBytes + C::kScaleBytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(tail);
   uint64_t* empty = full + S;
   uint64_t* tfull = empty + S;
   uint64_t* tempty = tfull + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* sy_s = reinterpret_cast<float*>(tail + 512);  // YVEC: [2][BN] column scales
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -122,17 +170,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   griddep_wait();
   griddep_launch_dependents();
 
-  const int tx = blockIdx.x % p.tiles_x, ty = blockIdx.x / p.tiles_x;
-  const int nst = p.stages_total;
-  const int units = (nst + C::kPerUnit - 1) / C::kPerUnit;
+  // the cluster's tile, and this CTA's part of the contraction
+  const int parts = p.parts, rank = (int)blockIdx.x % parts, tile = (int)blockIdx.x / parts;
+  const int tx = tile % p.tiles_x, ty = tile / p.tiles_x;
+  const int all = (p.stages_total + C::kPerUnit - 1) / C::kPerUnit;
+  const int u0 = (int)((int64_t)rank * all / parts), u1 = (int)((int64_t)(rank + 1) * all / parts);
+  const int units = u1 - u0;
+  const int i0 = u0 * C::kPerUnit;
+  const int i1 = u1 * C::kPerUnit < p.stages_total ? u1 * C::kPerUnit : p.stages_total;
 
   if (warp == 0) {
     if (lane == 0) {
       const uint32_t tx_bytes = kXBytes + (MODE == 0 ? 1 : p.pieces) * C::kYPiece;
-      for (int i = 0; i < nst; ++i) {
-        const int s = i % S;
-        if (!mbar_wait_bounded(&empty[s], ((i / S) & 1) ^ 1, abort_flag, p.err, DEV_TIMEOUT_EMPTY,
-                               p.timeout_ns))
+      for (int i = i0; i < i1; ++i) {
+        const int s = (i - i0) % S;
+        if (!mbar_wait_bounded(&empty[s], (((i - i0) / S) & 1) ^ 1, abort_flag, p.err,
+                               DEV_TIMEOUT_EMPTY, p.timeout_ns))
           break;
         uint8_t* st = base + s * C::kStageBytes;
         mbar_arrive_expect_tx(&full[s], tx_bytes);
@@ -159,14 +212,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) got = mbar_wait_bounded(bar, parity, abort_flag, p.err, code, p.timeout_ns);
       return __shfl_sync(0xffffffffu, got, 0) != 0;
     };
-    for (int u = 0, i = 0; u < units && ok; ++u) {
+    for (int u = 0, i = i0; u < units && ok; ++u) {
       const int b = u & 1;
-      if (!(ok = wait(&tempty[b], ((u >> 1) & 1) ^ 1, DEV_TIMEOUT_TMEM_EMPTY))) break;
-      tc_fence_after();
       const uint32_t d = tmem + (uint32_t)(b * BN);
-      for (int j = 0; j < C::kPerUnit && i < nst; ++j, ++i) {
-        const int s = i % S;
-        if (!(ok = wait(&full[s], (i / S) & 1, DEV_TIMEOUT_FULL))) break;
+      for (int j = 0; j < C::kPerUnit && i < i1; ++j, ++i) {
+        const int s = (i - i0) % S;
+        if (!(ok = wait(&full[s], ((i - i0) / S) & 1, DEV_TIMEOUT_FULL))) break;
+        if (j == 0 && !(ok = wait(&tempty[b], ((u >> 1) & 1) ^ 1, DEV_TIMEOUT_TMEM_EMPTY))) break;
         tc_fence_after();
         const uint32_t xa = smem_u32(base + s * C::kStageBytes), ya = xa + kXBytes;
         if (MODE == 0) {
@@ -193,43 +245,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int row = 32 * (warp & 3) + lane;
     const int et = threadIdx.x - 64;  // 0..127
     const uint32_t t_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-    const int64_t x = (int64_t)tx * kX + row;
-    const int64_t y0 = (int64_t)ty * BN;
-    float acc[BN];
+    unsigned long long acc[BN / 2];
 #pragma unroll
-    for (int j = 0; j < BN; ++j) acc[j] = 0.0f;
+    for (int j = 0; j < BN / 2; ++j) acc[j] = 0ull;
     bool ok = true;
-    const int64_t xi = MODE == 0 && x < p.xrows ? (x >> p.scx.row_shift) * p.scx.ld_row : -1;
-    const int64_t yr = y0 + (YVEC ? et : 0);
-    const int64_t yi = MODE == 0 && yr < p.ycols && (!YVEC || et < BN)
-                           ? (yr >> p.scy.row_shift) * p.scy.ld_row : -1;
-    auto scale_x = [&](int u) -> uint32_t {
-      return xi >= 0 && u < units ? load_scale(p.scx, xi + u * p.scx.ld_col) : 0u;
-    };
-    auto scale_y = [&](int u) -> uint32_t {
-      return yi >= 0 && u < units ? load_scale(p.scy, yi + u * p.scy.ld_col) : 0u;
-    };
-    uint32_t rx[2] = {0, 0}, ry[2] = {0, 0};  // the scales of the next two blocks
-    if (MODE == 0) {
-      rx[0] = scale_x(0);
-      ry[0] = scale_y(0);
-      rx[1] = scale_x(1);
-      ry[1] = scale_y(1);
-    }
     for (int u = 0; u < units; ++u) {
       const int b = u & 1;
-      float cx = 0.0f, cy = 0.0f;
-      if (MODE == 0) {
-        cx = scale_value(p.scx, rx[0]);
-        cy = scale_value(p.scy, ry[0]);
-        rx[0] = rx[1];
-        ry[0] = ry[1];
-        rx[1] = scale_x(u + 2);
-        ry[1] = scale_y(u + 2);
-      }
-      if (YVEC) {
-        // two buffers: the block after next's write comes behind the next barrier
-        if (et < BN) sy_s[b * BN + et] = cy;
+      if (MODE == 0 && u % kScaleUnits == 0) {
+        // the next blocks' scales, decoded, eight loads in flight a thread
+        const int n = units - u < kScaleUnits ? units - u : kScaleUnits;
+        named_bar_sync(1, 128);  // the blocks before are done with theirs
+        stage_scales(p.scx, (int64_t)tx * kX + et, p.xrows, u0 + u, n, sx + et, 128);
+        if (YVEC) {
+          if (et < BN)
+            stage_scales(p.scy, (int64_t)ty * BN + et, p.ycols, u0 + u, n, sy + et, C::kSy);
+        } else if (et < n) {
+          stage_scales(p.scy, (int64_t)ty * BN, p.ycols, u0 + u + et, 1, sy + et, 1);
+        }
         named_bar_sync(1, 128);
       }
       if (ok) {
@@ -240,40 +272,104 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __shfl_sync(0xffffffffu, got, 0) != 0;
       }
       tc_fence_after();
-      const float s = MODE == 0 ? (YVEC ? cx : cx * cy) : 1.0f;
+      const int us = u % kScaleUnits;
+      float f = 1.0f;
+      if (MODE == 0) f = YVEC ? sx[us * 128 + row] : sx[us * 128 + row] * sy[us];
+      const unsigned long long s2 = pack2(f, f);
 #pragma unroll
-      for (int c = 0; c < BN; c += 16) {
+      for (int c = 0; c < BN / 16; ++c) {
         uint32_t r[16];
-        tmem_ld_x16(t_lane + (uint32_t)(b * BN + c), r);
+        tmem_ld_x16(t_lane + (uint32_t)(b * BN + 16 * c), r);
         tmem_wait_x16(r);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float t = __uint_as_float(r[j]);
-          if (MODE == 1) acc[c + j] += t;
-          else if (YVEC) acc[c + j] = fmaf(t, s * sy_s[b * BN + c + j], acc[c + j]);
-          else acc[c + j] = fmaf(t, s, acc[c + j]);
+        for (int j = 0; j < 8; ++j) {
+          const unsigned long long v = pack2(r[2 * j], r[2 * j + 1]);
+          unsigned long long& a = acc[8 * c + j];
+          if (MODE == 1) a = add2(a, v);
+          else if (YVEC)
+            a = fma2(mul2(v, s2), *reinterpret_cast<const unsigned long long*>(
+                                      sy + us * C::kSy + 16 * c + 2 * j), a);
+          else a = fma2(v, s2, a);
         }
       }
       tc_fence_before();
       mbar_arrive(&tempty[b]);
     }
-    if (x < p.xrows) {
-      float* o = p.out + x * p.sx + y0 * p.sy;
-      const float bx = p.bias && p.bias_on_x ? p.bias[x] : 0.0f;
+    // The finished tile into the ring: every load has been used by an MMA that
+    // has completed.  Rows are the output's rows.
+    const uint32_t tb = smem_u32(base);
+    if (p.swap) {
 #pragma unroll
-      for (int j = 0; j < BN; ++j) {
-        if (y0 + j >= p.ycols) break;
-        float v = acc[j] + bx;
-        if (p.bias && !p.bias_on_x) v += __ldg(p.bias + y0 + j);
-        if (p.accumulate) v += o[j * p.sy];
-        o[j * p.sy] = activate(v, p.act);
+      for (int j = 0; j < BN / 2; ++j) {
+        const float2 v = unpack2(acc[j]);
+        sts32(tb + (uint32_t)((2 * j) * 132 + row) * 4, v.x);
+        sts32(tb + (uint32_t)((2 * j + 1) * 132 + row) * 4, v.y);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < BN / 4; ++j) {
+        const float2 v = unpack2(acc[2 * j]), w = unpack2(acc[2 * j + 1]);
+        sts128(tb + (uint32_t)(row * (BN + 4) + 4 * j) * 4, make_float4(v.x, v.y, w.x, w.y));
+      }
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  if (parts > 1) cluster_sync();
+  else __syncthreads();
+  tc_fence_after();
+
+  // Each CTA of the cluster adds its share of the rows over all parts, in rank
+  // order, and writes them.
+  {
+    const int trows = p.swap ? BN : kX, tcols = p.swap ? kX : BN;
+    const int pitch = tcols + 4, quads = tcols / 4, share = trows / parts;
+    const int64_t m0 = p.swap ? (int64_t)ty * BN : (int64_t)tx * kX;
+    const int64_t n0 = p.swap ? (int64_t)tx * kX : (int64_t)ty * BN;
+    const int64_t M = p.swap ? p.ycols : p.xrows, N = p.swap ? p.xrows : p.ycols;
+    const uint32_t tb = smem_u32(base);
+    for (int e = threadIdx.x; e < share * quads; e += kThreads) {
+      const int r = rank * share + e / quads, c = e % quads * 4;
+      const int64_t m = m0 + r, n = n0 + c;
+      if (m >= M || n >= N) continue;
+      const uint32_t at = tb + (uint32_t)(r * pitch + c) * 4;
+      float4 v;
+      if (parts == 1) {
+        v = lds128(at);
+      } else {
+        v = ld_cluster(map_rank(at, 0));
+        for (int q = 1; q < parts; ++q) {
+          const float4 w = ld_cluster(map_rank(at, (uint32_t)q));
+          v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+        }
+      }
+      float* o = p.out + m * p.ldo + n;
+      if (p.vec_ok && n + 4 <= N) {
+        if (p.bias) {
+          const float4 b4 = __ldg(reinterpret_cast<const float4*>(p.bias + n));
+          v.x += b4.x; v.y += b4.y; v.z += b4.z; v.w += b4.w;
+        }
+        if (p.accumulate) {
+          const float4 q = *reinterpret_cast<const float4*>(o);
+          v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+        }
+        *reinterpret_cast<float4*>(o) = activate4(v, p.act);
+      } else {
+        const float ve[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (n + j >= N) break;
+          float w = ve[j];
+          if (p.bias) w += __ldg(p.bias + n + j);
+          if (p.accumulate) w += o[j];
+          o[j] = activate(w, p.act);
+        }
       }
     }
   }
 
   // ------------------------------------------------------------ teardown
-  __syncwarp();
-  tc_fence_before();
   __syncthreads();
   if (*abort_flag) {
     // copies in flight land before the CTA's shared memory is released
@@ -281,15 +377,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (globaltimer_ns() - t0 < 1000000ull) __nanosleep(1000);
     __syncthreads();
   }
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem, C::kTmemCols);
-  }
+  if (parts > 1) cluster_sync();  // the other CTAs have read this one's part
+  if (warp == 1) tmem_dealloc(tmem, C::kTmemCols);
+}
+
+// CTAs that share a tile: as many as the SMs allow (a power of two up to 8),
+// with at least two blocks of the contraction each.
+int pick_parts(const rtb_ctx* ctx, int64_t tiles, int64_t units) {
+  int parts = 1;
+  while (parts < 8 && tiles * parts * 2 <= ctx->sm_count && units >= parts * 4) parts *= 2;
+  return parts;
 }
 
 template <int MODE, int BN, bool YVEC>
-int launch(const CUtensorMap& tmX, const CUtensorMap& tmY, BlockParams& p, cudaStream_t s) {
-  using C = Cfg<MODE, BN>;
+int launch(rtb_ctx* ctx, const CUtensorMap& tmX, const CUtensorMap& tmY, BlockParams& p,
+           cudaStream_t s) {
+  using C = Cfg<MODE, BN, YVEC>;
   auto* k = block_gemm_kernel<MODE, BN, YVEC>;
   cudaError_t e =
       cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
@@ -298,10 +401,26 @@ int launch(const CUtensorMap& tmX, const CUtensorMap& tmY, BlockParams& p, cudaS
   p.tiles_y = (int)((p.ycols + BN - 1) / BN);
   p.stages_total = (p.depth + C::kDepth - 1) / C::kDepth;
   const int64_t tiles = (int64_t)p.tiles_x * p.tiles_y;
-  if (tiles > INT32_MAX) return set_error(RTB_E_UNSUPPORTED, "block gemm: too many tiles");
+  if (tiles > INT32_MAX / 8) return set_error(RTB_E_UNSUPPORTED, "block gemm: too many tiles");
+  p.parts = pick_parts(ctx, tiles, (p.stages_total + C::kPerUnit - 1) / C::kPerUnit);
+  p.vec_ok = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 && p.ldo % 4 == 0 &&
+             (!p.bias || (reinterpret_cast<uintptr_t>(p.bias) & 15u) == 0);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * p.parts));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::kSmemBytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)p.parts;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
   clear_stale_cuda_error();
-  e = launch_pdl(k, dim3((unsigned)tiles), dim3(kThreads), C::kSmemBytes, s, tmX, tmY,
-                 (const BlockParams)p);
+  e = cudaLaunchKernelEx(&cfg, k, tmX, tmY, (const BlockParams)p);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? RTB_OK : cuda_status(e, "block gemm launch");
 }
@@ -336,10 +455,9 @@ int fp8_gemm_run(rtb_ctx* ctx, const Fp8Desc& d, cudaStream_t s) {
   p.ycols = swap ? d.M : d.N;
   p.depth = (int)d.K;
   p.out = d.C;
-  p.sx = swap ? 1 : d.ldc;
-  p.sy = swap ? d.ldc : 1;
+  p.ldo = d.ldc;
+  p.swap = swap;
   p.bias = d.bias;
-  p.bias_on_x = swap;
   p.act = d.act;
   p.scx = swap ? d.sb : d.sa;
   p.scy = swap ? d.sa : d.sb;
@@ -357,10 +475,10 @@ int fp8_gemm_run(rtb_ctx* ctx, const Fp8Desc& d, cudaStream_t s) {
                                (uint64_t)(swap ? d.lda : d.ldb), 128, (uint32_t)bn)))
     return st;
   if (!swap && use_pairs(ctx, p)) return launch_pair(ctx, 0, yvec, tmX, tmY, p, s);
-  if (bn == 16) return yvec ? launch<0, 16, true>(tmX, tmY, p, s) : launch<0, 16, false>(tmX, tmY, p, s);
-  if (bn == 32) return yvec ? launch<0, 32, true>(tmX, tmY, p, s) : launch<0, 32, false>(tmX, tmY, p, s);
-  if (bn == 64) return yvec ? launch<0, 64, true>(tmX, tmY, p, s) : launch<0, 64, false>(tmX, tmY, p, s);
-  return yvec ? launch<0, 128, true>(tmX, tmY, p, s) : launch<0, 128, false>(tmX, tmY, p, s);
+  if (bn == 16) return yvec ? launch<0, 16, true>(ctx, tmX, tmY, p, s) : launch<0, 16, false>(ctx, tmX, tmY, p, s);
+  if (bn == 32) return yvec ? launch<0, 32, true>(ctx, tmX, tmY, p, s) : launch<0, 32, false>(ctx, tmX, tmY, p, s);
+  if (bn == 64) return yvec ? launch<0, 64, true>(ctx, tmX, tmY, p, s) : launch<0, 64, false>(ctx, tmX, tmY, p, s);
+  return yvec ? launch<0, 128, true>(ctx, tmX, tmY, p, s) : launch<0, 128, false>(ctx, tmX, tmY, p, s);
 }
 
 int wgrad_run(rtb_ctx* ctx, const WgradDesc& d, cudaStream_t s) {
@@ -371,8 +489,7 @@ int wgrad_run(rtb_ctx* ctx, const WgradDesc& d, cudaStream_t s) {
   p.ycols = d.N;
   p.depth = (int)d.rows;
   p.out = d.D;
-  p.sx = d.ldd;
-  p.sy = 1;
+  p.ldo = d.ldd;
   p.accumulate = d.accumulate;
   p.pieces = d.pieces;
   p.piece_rows = d.rows_pad;
@@ -386,7 +503,7 @@ int wgrad_run(rtb_ctx* ctx, const WgradDesc& d, cudaStream_t s) {
                                (uint64_t)d.ldy, 64, 64)))
     return st;
   if (use_pairs(ctx, p)) return launch_pair(ctx, 1, false, tmX, tmY, p, s);
-  return launch<1, 128, false>(tmX, tmY, p, s);
+  return launch<1, 128, false>(ctx, tmX, tmY, p, s);
 }
 
 }  // namespace rtb

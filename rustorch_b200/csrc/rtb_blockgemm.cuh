@@ -16,10 +16,10 @@ struct BlockParams {
   int depth;             // contraction length
   int stages_total;      // ceil(depth / kDepth)
   int tiles_x, tiles_y;
-  float* out;            // element (x, y) at x * sx + y * sy
-  int64_t sx, sy;
-  const float* bias;     // per Y column (bias_on_x = 0) or per X row
-  int bias_on_x;
+  float* out;            // row-major, leading dimension ldo
+  int64_t ldo;
+  int swap;              // 0: X rows are the output's rows; 1: its columns (few rows)
+  const float* bias;     // per output column
   int act;
   int accumulate;
   int pieces;            // MODE 1
@@ -29,7 +29,9 @@ struct BlockParams {
   // (launch_scale_tables)
   const float *tabx, *taby;
   int64_t pitchx, pitchy;
-  int c_tma;             // rows of the output leave through TMA stores
+  int c_tma;             // CTA pairs: rows of the output leave through TMA stores
+  int parts;             // CTAs that share a tile (a cluster)
+  int vec_ok;            // 16-byte aligned output rows and bias
   int* err;
   unsigned long long timeout_ns;
 };

@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] += yc + j < p.ycols ? __ldg(p.bias + yc + j) : 0.0f;
         }
-        float* o = p.out + x * p.sx + yc;
+        float* o = p.out + x * p.ldo + yc;
         if (p.accumulate && x < p.xrows) {
 #pragma unroll
           for (int j = 0; j < 32; ++j)
@@ -487,9 +487,9 @@ int launch(rtb_ctx* ctx, const CUtensorMap& tmX, const CUtensorMap& tmY, BlockPa
   const int64_t tiles = (int64_t)p.tiles_x * p.tiles_y;
   if (tiles > INT32_MAX / 2) return set_error(RTB_E_UNSUPPORTED, "pair gemm: too many tiles");
   CUtensorMap tmC = tmX;
-  p.c_tma = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 && p.sx % 4 == 0;
+  p.c_tma = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 && p.ldo % 4 == 0;
   if (p.c_tma) {
-    const int st = make_tmap_2d(&tmC, p.out, (uint64_t)p.ycols, (uint64_t)p.xrows, (uint64_t)p.sx,
+    const int st = make_tmap_2d(&tmC, p.out, (uint64_t)p.ycols, (uint64_t)p.xrows, (uint64_t)p.ldo,
                                 32, 128, false);
     if (st) return st;
   }
