@@ -295,78 +295,32 @@ def _rows_2d(t, d):
     return t2
 
 
-def _ld(t, d):
-    """Leading dimension of _rows_2d's result (a single row's stride says nothing)."""
-    return max(t.stride(0), d)
+_ops_module = None
 
 
-def _flat(t, n, message):
-    """A vector of n elements, contiguous; None stays None."""
-    if t is None:
-        return None
-    if t.numel() != n:
-        raise ValueError(message)
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _same_device(first, *rest):
-    dev = first.get_device()
-    for t in rest:
-        if t is not None and t.get_device() != dev:
-            raise ValueError("rustorch_b200: tensors on different devices")
-    return dev
-
-
-def _empty_like(x):
-    """float32, contiguous, of x's shape and on its device."""
-    torch = _torch()
-    if x.dtype is torch.float32 and x.is_contiguous():
-        return torch.empty_like(x)
-    return torch.empty(x.shape, dtype=torch.float32, device=x.device)
-
-
-def _result(out, need, accumulate, shape, like, who):
-    """The tensor that a gradient is written to (or added to): `out` or a new one."""
-    if not need:
-        return None
-    if out is None:
-        if accumulate:
-            raise ValueError(f"{who}: accumulate adds to given outputs")
-        return like.new_empty(shape, dtype=_torch().float32)
-    if not out.is_contiguous() or tuple(out.shape) != tuple(shape):
-        raise ValueError(f"{who}: outputs must be contiguous and of the gradient's shape")
-    return out
-
-
-_LN_SHAPE = "LayerNorm: Input shape does not match normalized shape"
+def _load_ops():
+    """rustorch_b200._ops (csrc/python/ops_module.cpp): argument checks, outputs
+    and the C calls of the operators below.  There is no fallback: without the
+    built module they raise."""
+    global _ops_module
+    if _ops_module is None:
+        _torch()
+        lib()
+        try:
+            from . import _ops as module
+        except ImportError as e:
+            raise ImportError(f"rustorch_b200._ops cannot be loaded ({e}); build it with "
+                              "`python -m rustorch_b200.build`") from e
+        module.setup(get_context, _lib.check)
+        _ops_module = module
+    return _ops_module
 
 
 def layer_norm_fwd(x, norm_weight=None, norm_bias=None, eps: float = 1e-5, act: int = ACT_NONE,
                    out=None):
     """layer_norm that also returns what its backward pass reads: (y, mean,
     rstd), the statistics float32 of x's leading shape; out may be x."""
-    _check_f32_cuda(x, norm_weight, norm_bias, out)
-    dev = _same_device(x, norm_weight, norm_bias, out)
-    d = x.shape[-1] if x.dim() else 0
-    if d == 0:
-        raise ValueError("LayerNorm: Input shape smaller than normalized shape")
-    w, b = _flat(norm_weight, d, _LN_SHAPE), _flat(norm_bias, d, _LN_SHAPE)
-    x2 = _rows_2d(x, d)
-    if out is None:
-        out = y2 = _empty_like(x)
-        ldy = d
-    else:
-        if out.shape != x.shape or (d > 1 and out.stride(-1) != 1):
-            raise ValueError("layer_norm_fwd: out must have x's shape and contiguous rows")
-        y2 = out if out.dim() == 2 else out.view(-1, d)
-        if y2.shape[0] > 1 and y2.stride(0) < d:
-            raise ValueError("layer_norm_fwd: out's rows overlap")
-        ldy = _ld(y2, d)
-    mean = x.new_empty(x.shape[:-1])
-    rstd = x.new_empty(x.shape[:-1])
-    call("rtb_layer_norm_fwd", get_context(dev).handle, x2.shape[0], d, _ptr(x2), _ld(x2, d),
-         _ptr(w), _ptr(b), eps, act, _ptr(y2), ldy, _ptr(mean), _ptr(rstd), _stream_of(x))
-    return out, mean, rstd
+    return (_ops_module or _load_ops()).layer_norm_fwd(x, norm_weight, norm_bias, eps, act, out)
 
 
 def layer_norm_backward(x, mean, rstd, grad, norm_weight=None, norm_bias=None,
@@ -377,60 +331,9 @@ def layer_norm_backward(x, mean, rstd, grad, norm_weight=None, norm_bias=None,
     gradient `grad`; x is the forward's input, float32 or an 8-bit checkpoint
     (fp8_quantize(x) -> x, x_scale).  With accumulate the results are added to
     out_x / out_weight / out_bias."""
-    who = "layer_norm_backward"
-    saved = x.dtype is _torch().float8_e4m3fn
-    _check_f32_cuda(mean, rstd, grad, norm_weight, norm_bias, out_x, out_weight, out_bias)
-    if not saved:
-        _check_f32_cuda(x)
-    dev = _same_device(x, mean, rstd, grad, norm_weight, norm_bias, x_scale, out_x, out_weight,
-                       out_bias)
-    d = x.shape[-1] if x.dim() else 0
-    if d == 0 or grad.shape != x.shape:
-        raise ValueError("layer_norm_backward: grad must have x's shape, with a last dimension")
-    x2, g2 = _rows_2d(x, d), _rows_2d(grad, d)
-    rows = x2.shape[0]
-    per_row = "layer_norm_backward: one mean and rstd for each row"
-    mean, rstd = _flat(mean, rows, per_row), _flat(rstd, rows, per_row)
-    w, b = _flat(norm_weight, d, _LN_SHAPE), _flat(norm_bias, d, _LN_SHAPE)
-    if saved != (x_scale is not None):
-        raise ValueError("layer_norm_backward: x_scale goes with an 8-bit x, and only with one")
-    dx = _result(out_x, need_x, accumulate, x.shape, grad, who)
-    dw = _result(out_weight, need_weight, accumulate, (d,), grad, who)
-    db = _result(out_bias, need_bias, accumulate, (d,), grad, who)
-    rest = (_ptr(mean), _ptr(rstd), _ptr(w), _ptr(b), act, _ptr(g2), _ld(g2, d), _ptr(dx), d,
-            _ptr(dw), _ptr(db), bool(accumulate), _stream_of(x))
-    h = get_context(dev).handle
-    if saved:
-        s2, block_rows, kind = _scales(x_scale, rows, d, who)
-        if kind != _lib.SCALE_E8M0 or block_rows != 1:
-            raise ValueError("layer_norm_backward: a checkpoint has a power-of-two scale for each "
-                             "128 columns of a row")
-        call("rtb_layer_norm_backward_fp8", h, rows, d, _ptr(x2), _ld(x2, d), _ptr(s2),
-             _ld(s2, s2.shape[1]), *rest)
-    else:
-        call("rtb_layer_norm_backward", h, rows, d, _ptr(x2), _ld(x2, d), *rest)
-    return dx, dw, db
-
-
-def _scales(scale, rows, cols, who):
-    """(2-D scales with contiguous rows, block_rows, scale type) of a [rows, cols] 8-bit tensor."""
-    torch = _torch()
-    e8m0 = scale.dtype is torch.float8_e8m0fnu
-    if not scale.is_cuda or not (e8m0 or scale.dtype is torch.float32):
-        raise ValueError(f"{who}: scales are float8_e8m0fnu or float32 CUDA tensors")
-    cb = (cols + 127) // 128
-    s = _rows_2d(scale, cb)
-    n = s.shape[0]
-    if s.shape[1] != cb or n not in (rows, (rows + 127) // 128):
-        raise ValueError(f"{who}: scales must be [rows or ceil(rows / 128), ceil(cols / 128)]")
-    return s, 1 if n == rows else 128, _lib.SCALE_E8M0 if e8m0 else _lib.SCALE_F32
-
-
-def _check_fp8(who, *ts):
-    e4m3 = _torch().float8_e4m3fn
-    for t in ts:
-        if not (t.is_cuda and t.dtype is e4m3):
-            raise ValueError(f"{who} expects float8_e4m3fn CUDA tensors")
+    return (_ops_module or _load_ops()).layer_norm_backward(
+        x, mean, rstd, grad, norm_weight, norm_bias, act, x_scale, need_x, need_weight, need_bias,
+        out_x, out_weight, out_bias, accumulate)
 
 
 def fp8_quantize(x, block_rows: int = 1):
@@ -438,45 +341,12 @@ def fp8_quantize(x, block_rows: int = 1):
     (float8_e8m0fnu) for each 128 columns of a row (block_rows = 1) or of 128
     rows of a 2-D x (block_rows = 128).  An activation checkpoint, and an
     operand of fp8_matmul."""
-    torch = _torch()
-    _check_f32_cuda(x)
-    if block_rows not in (1, 128):
-        raise ValueError("fp8_quantize: block_rows must be 1 or 128")
-    if x.dim() == 0 or (block_rows != 1 and x.dim() != 2):
-        raise ValueError("fp8_quantize: x needs a last dimension, and two for 128-row blocks")
-    cols = x.shape[-1]
-    cb = (cols + 127) // 128
-    q = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
-    lead = x.shape[:-1] if block_rows == 1 else ((x.shape[0] + 127) // 128,)
-    scale = x.new_empty((*lead, cb), dtype=torch.float8_e8m0fnu)
-    if x.numel():
-        x2 = _rows_2d(x, cols)
-        call("rtb_fp8_quantize", get_context(x.get_device()).handle, x2.shape[0], cols, _ptr(x2),
-             _ld(x2, cols), block_rows, _ptr(q), cols, _ptr(scale), cb, _stream_of(x))
-    return q, scale
+    return (_ops_module or _load_ops()).fp8_quantize(x, block_rows)
 
 
 def fp8_dequantize(q, scale, out=None):
     """The float32 values q * scale of fp8_quantize's (q, scale)."""
-    _check_fp8("fp8_dequantize", q)
-    _check_f32_cuda(out)
-    dev = _same_device(q, scale, out)
-    if q.dim() == 0:
-        raise ValueError("fp8_dequantize: q needs a last dimension")
-    cols = q.shape[-1]
-    if out is None:
-        out = _empty_like(q)
-    elif out.shape != q.shape or not out.is_contiguous():
-        raise ValueError("fp8_dequantize: out must be contiguous and have q's shape")
-    if q.numel():
-        q2 = _rows_2d(q, cols)
-        rows = q2.shape[0]
-        s, block_rows, kind = _scales(scale, rows, cols, "fp8_dequantize")
-        if kind != _lib.SCALE_E8M0:
-            raise ValueError("fp8_dequantize: scales are float8_e8m0fnu")
-        call("rtb_fp8_dequantize", get_context(dev).handle, rows, cols, _ptr(q2), _ld(q2, cols),
-             _ptr(s), _ld(s, s.shape[1]), block_rows, _ptr(out), cols, _stream_of(q))
-    return out
+    return (_ops_module or _load_ops()).fp8_dequantize(q, scale, out)
 
 
 def fp8_matmul(a, a_scale, b, b_scale, bias=None, act: int = ACT_NONE, out=None):
@@ -484,36 +354,7 @@ def fp8_matmul(a, a_scale, b, b_scale, bias=None, act: int = ACT_NONE, out=None)
     and b [K,N].  b is a Linear weight's transposed view (w.t(), with its
     scales' ws.t()) or a row-major matrix with 128 x 128 blocks; scales are
     float8_e8m0fnu or float32."""
-    _check_fp8("fp8_matmul", a, b)
-    _check_f32_cuda(bias, out)
-    dev = _same_device(a, a_scale, b, b_scale, bias, out)
-    if a.dim() != 2 or b.dim() != 2 or b_scale.dim() != 2:
-        raise ValueError("Matmul only supports 2D")
-    M, K = a.shape
-    K2, N = b.shape
-    if K != K2:
-        raise ValueError("Matmul dimension mismatch")
-    bias = _flat(bias, N, "fp8_matmul: bias must have N elements")
-    if out is None:
-        out = a.new_empty((M, N), dtype=_torch().float32)
-    elif tuple(out.shape) != (M, N) or (N > 1 and out.stride(1) != 1) or (
-            M > 1 and out.stride(0) < N):
-        raise ValueError("fp8_matmul: out must be [M, N] with contiguous rows")
-    a_ = _rows_2d(a, K)
-    sa, ra, ka = _scales(a_scale, M, K, "fp8_matmul")
-    if b.stride(0) == 1 or b.stride(1) != 1:
-        w, trans = _rows_2d(b.t(), K), 1
-        sb, rb_, kb = _scales(b_scale.t(), N, K, "fp8_matmul")
-    else:
-        w, trans = _rows_2d(b, N), 0
-        sb, rb_, kb = _scales(b_scale, K, N, "fp8_matmul")
-        if rb_ != 128 and K > 1:
-            raise ValueError("fp8_matmul: a row-major b needs 128 x 128 blocks")
-        rb_ = 128
-    call("rtb_fp8_matmul", get_context(dev).handle, M, N, K, _ptr(a_), _ld(a_, K), _ptr(sa),
-         _ld(sa, sa.shape[1]), ra, ka, _ptr(w), _ld(w, w.shape[1]), trans, _ptr(sb),
-         _ld(sb, sb.shape[1]), rb_, kb, _ptr(bias), act, _ptr(out), _ld(out, N), _stream_of(a))
-    return out
+    return (_ops_module or _load_ops()).fp8_matmul(a, a_scale, b, b_scale, bias, act, out)
 
 
 def matmul_backward_fp8(a, a_scale, b, grad, need_a: bool = True, need_b: bool = True, out_a=None,
@@ -522,31 +363,8 @@ def matmul_backward_fp8(a, a_scale, b, grad, need_a: bool = True, need_b: bool =
     (fp8_quantize): (grad @ b.T, deq(a).T @ grad); b (float32 [K,N]) is read for
     the first only and may be None without it.  With accumulate the results
     are added to out_a / out_b."""
-    who = "matmul_backward_fp8"
-    _check_fp8(who, a)
-    _check_f32_cuda(b, grad, out_a, out_b)
-    dev = _same_device(a, a_scale, b, grad, out_a, out_b)
-    if a.dim() != 2 or grad.dim() != 2:
-        raise ValueError("Matmul only supports 2D")
-    M, K = a.shape
-    N = grad.shape[1]
-    if grad.shape[0] != M or (b is not None and tuple(b.shape) != (K, N)):
-        raise ValueError("matmul_backward_fp8: shape mismatch")
-    if need_a and b is None:
-        raise ValueError("matmul_backward_fp8: the gradient of a needs b")
-    da = _result(out_a, need_a, accumulate, (M, K), grad, who)
-    db = _result(out_b, need_b, accumulate, (K, N), grad, who)
-    if not grad.is_contiguous():
-        grad = grad.contiguous()
-    b = b.contiguous() if b is not None and need_a else None
-    a_ = _rows_2d(a, K)
-    sa, ra, kind = _scales(a_scale, M, K, who)
-    if kind != _lib.SCALE_E8M0:
-        raise ValueError("matmul_backward_fp8: a checkpoint's scales are float8_e8m0fnu")
-    call("rtb_matmul_backward_fp8", get_context(dev).handle, M, N, K, _ptr(a_), _ld(a_, K),
-         _ptr(sa), _ld(sa, sa.shape[1]), ra, _ptr(b), _ptr(grad), _ptr(da), _ptr(db),
-         bool(accumulate), precision, _stream_of(a))
-    return da, db
+    return (_ops_module or _load_ops()).matmul_backward_fp8(a, a_scale, b, grad, need_a, need_b, out_a,
+                                                       out_b, accumulate, precision)
 
 
 def max_pool2d(x, kernel=(3, 3), stride=(2, 2), padding=(1, 1), layout: int = LAYOUT_NCHW):

@@ -3,7 +3,9 @@
     python -m rustorch_b200.build [--force] [--verbose]
 
 Each csrc/*.cu and csrc/*.cpp compiles to _build/*.o in parallel, then links into
-rustorch_b200/librustorch_b200.so (NCCL is dlopen'ed at first use).  A source is
+rustorch_b200/librustorch_b200.so (NCCL is dlopen'ed at first use);
+csrc/python/ops_module.cpp (the Python calls of the training and 8-bit operators)
+compiles against torch's headers into rustorch_b200/_ops.so.  A source is
 recompiled when it or any header is newer than its object, and the library is
 relinked when any object changed.  Objects and the library are stamped with the time
 their compile started, so a file edited while a build runs is seen as newer by the
@@ -24,6 +26,8 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(ROOT, "_build")
 LIB = os.path.join(PKG, "librustorch_b200.so")
+OPS_SRC = os.path.join(CSRC, "python", "ops_module.cpp")
+OPS = os.path.join(PKG, "_ops.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O3",
                      "-I" + os.path.join(ROOT, "include"), "--expt-relaxed-constexpr"]
@@ -56,6 +60,15 @@ def _stale(src: str, newest_header: float) -> bool:
     return os.path.getmtime(obj) < max(os.path.getmtime(src), newest_header)
 
 
+def ops_stale() -> bool:
+    """The extension module is missing or older than its source or the C header."""
+    if not os.path.exists(OPS):
+        return True
+    t = os.path.getmtime(OPS)
+    return any(os.path.getmtime(p) > t for p in (OPS_SRC, os.path.join(ROOT, "include",
+                                                                       "rustorch_b200.h")))
+
+
 def needs_build() -> bool:
     """The library is missing or older than a source or header (objects are
     not needed to use a library that is up to date)."""
@@ -80,9 +93,38 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def _build_ops() -> None:
+    import sysconfig
+
+    import torch
+    t0 = time.time()
+    tdir = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    inc = [os.path.join(tdir, "include"), os.path.join(tdir, "include", "torch", "csrc", "api",
+                                                       "include"),
+           sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    tmp = OPS + ".tmp"
+    cmd = (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+           + ["-isystem" + i for i in inc] + [OPS_SRC, "-o", tmp, "-L" + PKG, "-lrustorch_b200",
+                                              "-Wl,-rpath,$ORIGIN", "-L" + os.path.join(tdir, "lib"),
+                                              "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"])
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {OPS_SRC}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, OPS)
+    os.utime(OPS, (t0, t0))
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
-    if not force and not needs_build():
-        return LIB
+    if force or needs_build():
+        _build_lib(force, verbose)
+    if force or ops_stale():
+        _build_ops()
+    return LIB
+
+
+def _build_lib(force: bool, verbose: bool) -> None:
     os.makedirs(BUILD, exist_ok=True)
     srcs = _sources()
     hdr = max(os.path.getmtime(p) for p in _headers())
@@ -100,7 +142,6 @@ def build(force: bool = False, verbose: bool = False) -> str:
     os.replace(tmp, LIB)
     stamp = max(os.path.getmtime(o) for o in objs)
     os.utime(LIB, (stamp, stamp))
-    return LIB
 
 
 if __name__ == "__main__":
