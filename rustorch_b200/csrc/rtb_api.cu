@@ -1148,20 +1148,22 @@ int rtb_fp8_dequantize(rtb_ctx* ctx, int64_t rows, int64_t cols, const uint8_t* 
 }
 
 // [rows, K] e4m3 with K contiguous, as the tensor maps want it: the caller's
-// matrix where its base and row stride are multiples of 16 bytes, else a copy.
-static int fp8_operand(rtb_ctx* ctx, const uint8_t* src, int64_t rows, int64_t K, int64_t rs,
-                       int64_t cs, const uint8_t** out, int64_t* ld, void** ws, cudaStream_t s) {
-  if (cs == 1 && aligned16(src) && rs % 16 == 0) {
-    *out = src;
-    *ld = rs;
-    return RTB_OK;
-  }
-  const int64_t Kp = round_up(K, 16);
-  int st = ws_alloc(ctx, ws, (size_t)(rows * Kp), s);
-  if (st) return st;
-  *out = static_cast<const uint8_t*>(*ws);
-  *ld = Kp;
-  return launch_pack_bytes(ctx, src, rows, K, rs, cs, static_cast<uint8_t*>(*ws), Kp, s);
+// matrix where its base and row stride are multiples of 16 bytes, else a copy
+// (src -> a place in the workspace, `need` bytes further on).
+static void fp8_operand(const uint8_t* src, int64_t rows, int64_t K, int64_t rs, int64_t cs,
+                        const uint8_t** out, int64_t* ld, PackDesc* pack, size_t* need) {
+  *out = src;
+  *ld = rs;
+  if (cs == 1 && aligned16(src) && rs % 16 == 0) return;
+  *ld = round_up(K, 16);
+  pack->src = src;
+  pack->rows = rows;
+  pack->cols = K;
+  pack->rs = rs;
+  pack->cs = cs;
+  pack->ldd = *ld;
+  *out = nullptr;
+  *need += (size_t)round_up(rows * *ld, 256);
 }
 
 int rtb_fp8_matmul(rtb_ctx* ctx, int64_t M, int64_t N, int64_t K, const uint8_t* A, int64_t lda,
@@ -1204,13 +1206,20 @@ int rtb_fp8_matmul(rtb_ctx* ctx, int64_t M, int64_t N, int64_t K, const uint8_t*
   d.sb.ld_col = transB ? 1 : ldsb;
   d.sb.row_shift = block_rows_b == 1 ? 0 : 7;
   d.sb.is_f32 = scale_type_b == RTB_SCALE_F32;
-  void *wa = nullptr, *wb = nullptr;
-  st = fp8_operand(ctx, A, M, K, lda, 1, &d.A, &d.lda, &wa, s);
-  if (st == RTB_OK)
-    st = fp8_operand(ctx, B, N, K, transB ? ldb : 1, transB ? 1 : ldb, &d.B, &d.ldb, &wb, s);
+  PackDesc pa, pb;
+  size_t need = 0;
+  void* ws = nullptr;
+  fp8_operand(A, M, K, lda, 1, &d.A, &d.lda, &pa, &need);
+  const size_t at_b = need;
+  fp8_operand(B, N, K, transB ? ldb : 1, transB ? 1 : ldb, &d.B, &d.ldb, &pb, &need);
+  if (need) {
+    if ((st = ws_alloc(ctx, &ws, need, s))) return st;
+    if (!d.A) d.A = pa.dst = static_cast<uint8_t*>(ws);
+    if (!d.B) d.B = pb.dst = static_cast<uint8_t*>(ws) + at_b;
+    st = launch_pack_bytes(ctx, pa, pb, s);
+  }
   if (st == RTB_OK) st = fp8_gemm_run(ctx, d, s);
-  ws_free(wa, s);
-  ws_free(wb, s);
+  ws_free(ws, s);
   return st;
 }
 
@@ -1255,17 +1264,17 @@ int rtb_matmul_backward_fp8(rtb_ctx* ctx, int64_t M, int64_t N, int64_t K, const
   w.D = dB;
   w.ldd = N;
   w.accumulate = accumulate;
-  void *wx = nullptr, *wy = nullptr;
-  st = ws_alloc(ctx, &wx, (size_t)(w.rows_pad * w.ldx) * 2, s);
-  if (st == RTB_OK) st = ws_alloc(ctx, &wy, (size_t)(w.pieces * w.rows_pad * w.ldy) * 2, s);
-  w.X = wx;
+  const size_t xbytes = (size_t)round_up((w.rows_pad * w.ldx) * 2, 256);
+  void* ws = nullptr;
+  st = ws_alloc(ctx, &ws, xbytes + (size_t)(w.pieces * w.rows_pad * w.ldy) * 2, s);
+  if (st) return st;
+  void* wy = static_cast<char*>(ws) + xbytes;
+  w.X = ws;
   w.Y = wy;
-  if (st == RTB_OK)
-    st = launch_decode_bf16(ctx, A, lda, M, K, scale_a, ldsa, block_rows_a, wx, w.ldx, w.rows_pad, s);
-  if (st == RTB_OK) st = launch_split_bf16(ctx, dC, N, M, N, wy, w.ldy, w.rows_pad, w.pieces, s);
+  st = launch_wgrad_operands(ctx, A, lda, scale_a, ldsa, block_rows_a, dC, M, K, N, ws, w.ldx, wy,
+                             w.ldy, w.rows_pad, w.pieces, s);
   if (st == RTB_OK) st = wgrad_run(ctx, w, s);
-  ws_free(wx, s);
-  ws_free(wy, s);
+  ws_free(ws, s);
   return st;
 }
 

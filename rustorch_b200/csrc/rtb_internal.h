@@ -251,16 +251,22 @@ int launch_fp8_quantize(rtb_ctx* ctx, const float* x, int64_t ldx, int64_t rows,
 int launch_fp8_dequantize(rtb_ctx* ctx, const uint8_t* q, int64_t ldq, int64_t rows, int64_t cols,
                           const uint8_t* scale, int64_t lds, int block_rows, float* y, int64_t ldy,
                           cudaStream_t s);
-// dst[r][c] = c < cols ? src[r * rs + c * cs] : 0 for c < ldd (rs or cs is 1).
-int launch_pack_bytes(rtb_ctx* ctx, const uint8_t* src, int64_t rows, int64_t cols, int64_t rs,
-                      int64_t cs, uint8_t* dst, int64_t ldd, cudaStream_t s);
-// bf16 copy of an 8-bit tensor, and fp32 as a sum of bf16 terms ([pieces]
-// [rows_pad][ldo]); ldo % 8 == 0, zero padded.
-int launch_decode_bf16(rtb_ctx* ctx, const uint8_t* q, int64_t ldq, int64_t rows, int64_t cols,
-                       const uint8_t* scale, int64_t lds, int block_rows, void* out, int64_t ldo,
-                       int64_t rows_pad, cudaStream_t s);
-int launch_split_bf16(rtb_ctx* ctx, const float* x, int64_t ldx, int64_t rows, int64_t cols,
-                      void* out, int64_t ldo, int64_t rows_pad, int pieces, cudaStream_t s);
+// dst[r][c] = c < cols ? src[r * rs + c * cs] : 0 for c < ldd (rs or cs is 1,
+// ldd % 16 == 0), of up to two matrices in one launch; a null dst is left out.
+struct PackDesc {
+  const uint8_t* src = nullptr;
+  int64_t rows = 0, cols = 0, rs = 0, cs = 0;
+  uint8_t* dst = nullptr;
+  int64_t ldd = 0;
+};
+int launch_pack_bytes(rtb_ctx* ctx, const PackDesc& a, const PackDesc& b, cudaStream_t s);
+// The weight gradient's operands: the checkpoint in bf16 ([rows_pad][ldx]) and
+// dC [rows, N] as a sum of bf16 terms ([pieces][rows_pad][ldy]); ldx, ldy
+// multiples of 8, zero padded.
+int launch_wgrad_operands(rtb_ctx* ctx, const uint8_t* q, int64_t ldq, const uint8_t* scale,
+                          int64_t lds, int block_rows, const float* dc, int64_t rows, int64_t K,
+                          int64_t N, void* x, int64_t ldx, void* y, int64_t ldy, int64_t rows_pad,
+                          int pieces, cudaStream_t s);
 
 // Block-scaled products on the tensor cores (rtb_blockgemm.cu).
 struct ScaleRef {            // scale of the 128-column block kb of row r:
@@ -281,7 +287,7 @@ struct Fp8Desc {  // C [M, N] = act(A . B^T + bias): A [M, K], B [N, K] e4m3, K-
 };
 int fp8_gemm_run(rtb_ctx* ctx, const Fp8Desc& d, cudaStream_t s);
 // D [K, N] (+)= X^T . Y over `rows`: X bf16 [rows, ldx], Y = the sum of
-// `pieces` bf16 matrices [pieces][rows_pad][ldy] (launch_split_bf16).
+// `pieces` bf16 matrices [pieces][rows_pad][ldy] (launch_wgrad_operands).
 struct WgradDesc {
   int64_t rows = 0, rows_pad = 0, K = 0, N = 0;
   const void *X = nullptr, *Y = nullptr;
