@@ -467,6 +467,9 @@ int fp8_gemm_run(rtb_ctx* ctx, const Fp8Desc& d, cudaStream_t s) {
   const int bn = swap ? (d.M <= 16 ? 16 : d.M <= 32 ? 32 : 64) : 128;
   const uint8_t* X = swap ? d.B : d.A;
   const uint8_t* Y = swap ? d.A : d.B;
+  const bool pairs = !swap && use_pairs(ctx, p);
+  if (pairs && !p.scx.is_f32 && !p.scy.is_f32)
+    return launch_mx(ctx, X, d.lda, Y, d.ldb, p, s);
   CUtensorMap tmX, tmY;
   if ((st = make_tmap_2d_bytes(&tmX, X, 1, (uint64_t)d.K, (uint64_t)p.xrows,
                                (uint64_t)(swap ? d.ldb : d.lda), 128, kX)))
@@ -474,7 +477,7 @@ int fp8_gemm_run(rtb_ctx* ctx, const Fp8Desc& d, cudaStream_t s) {
   if ((st = make_tmap_2d_bytes(&tmY, Y, 1, (uint64_t)d.K, (uint64_t)p.ycols,
                                (uint64_t)(swap ? d.lda : d.ldb), 128, (uint32_t)bn)))
     return st;
-  if (!swap && use_pairs(ctx, p)) return launch_pair(ctx, 0, yvec, tmX, tmY, p, s);
+  if (pairs) return launch_pair(ctx, 0, yvec, tmX, tmY, p, s);
   if (bn == 16) return yvec ? launch<0, 16, true>(ctx, tmX, tmY, p, s) : launch<0, 16, false>(ctx, tmX, tmY, p, s);
   if (bn == 32) return yvec ? launch<0, 32, true>(ctx, tmX, tmY, p, s) : launch<0, 32, false>(ctx, tmX, tmY, p, s);
   if (bn == 64) return yvec ? launch<0, 64, true>(ctx, tmX, tmY, p, s) : launch<0, 64, false>(ctx, tmX, tmY, p, s);

@@ -112,6 +112,8 @@ __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigne
 inline int64_t table_blocks(int64_t units) { return (units + 3) / 4 * 4 + 4; }
 
 // Products on CTA pairs (rtb_pairgemm.cu); yvec as in rtb_blockgemm.cu.
+int launch_mx(rtb_ctx* ctx, const uint8_t* X, int64_t ldx, const uint8_t* Y, int64_t ldy,
+              BlockParams& p, cudaStream_t s);  // e8m0 scales (rtb_mxgemm.cu)
 int launch_pair(rtb_ctx* ctx, int mode, bool yvec, const CUtensorMap& tmX, const CUtensorMap& tmY,
                 BlockParams& p, cudaStream_t s);
 
