@@ -4,9 +4,9 @@
 // block of 128 gives its scale to four of them).
 //
 // The scales enter inside the MMA, so a partial sum has to leave the tensor core
-// only for the accumulation's sake, every 512 elements (the tensor core does
-// not round each addition to nearest: the error grows with the chain) instead
-// of every 128: the epilogue's chain of barrier, TMEM loads and adds, 1150
+// only for the accumulation's sake, every 1024 elements (the tensor core does
+// not round each addition to nearest: the error grows with the chain, 9e-8
+// relative after 32 steps) instead of every 128: the epilogue's chain of barrier, TMEM loads and adds, 1150
 // clocks against 512 of MMAs in rtb_pairgemm.cu, is out of the way.
 //
 // Tile 256 x 224 or 256 x 192 (two accumulators leave columns of TMEM for the
@@ -33,7 +33,7 @@ constexpr int kStages = 6;
 constexpr int kStageBytes = 16384 + 16384 + 2048;  // X, Y (half of the tile's rows), scales
 constexpr int kChunk = 128 * 16 * 4;               // a staged 128 x 16 fp32 piece of the output
 constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 2 * kChunk + 512;
-constexpr int kPerUnit = 4;                        // blocks of 128 between promotions
+constexpr int kPerUnit = 8;                        // blocks of 128 between promotions
 constexpr uint32_t kScaleCol = 448;                // TMEM: two buffers of 4 + 8 columns
 static_assert(kSmemBytes <= 232448, "shared memory");
 
@@ -43,26 +43,35 @@ constexpr __host__ __device__ uint32_t mx_idesc(int tn) {
   return ((uint32_t)(tn >> 3) << 17) | (1u << 23) | ((uint32_t)(kTileX >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_mx_e(uint32_t d, uint64_t a, uint64_t b, uint32_t id,
-                                         uint32_t sa, uint32_t sb, uint32_t acc) {
+// One stage, issued by one elected lane: the three scale groups into TMEM (32
+// rows of 16 bytes of shared memory each -> 32 lanes x 4 columns, in every lane
+// quarter, in both CTAs), four MMAs of 32 contraction elements (32 bytes further
+// on in the operands' rows: 2 in the descriptors), the stage's release.  One
+// election for all: with one for each instruction the issue of a stage took
+// longer than its MMAs.
+__device__ __forceinline__ void mx_stage_e(uint32_t d, uint64_t a, uint64_t b, uint32_t id,
+                                           uint32_t sa, uint64_t sc, uint32_t acc, uint64_t* empty) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t.reg .b32 r;\n\t"
-      "elect.sync r|e, 0xffffffff;\n\t"
+      "{\n\t.reg .pred p, t, e;\n\t.reg .b32 r, sb, sb2;\n\t.reg .b16 m;\n\t"
+      ".reg .b64 a1, a2, a3, b1, b2, b3, c1, c2;\n\t"
       "setp.ne.b32 p, %6, 0;\n\t"
-      "@e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, "
-      "[%4], [%5], p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(id), "r"(sa), "r"(sb), "r"(acc)
-      : "memory");
-}
-// 32 rows of 16 bytes of shared memory -> 32 lanes x 4 columns of TMEM, in every
-// lane quarter, in both CTAs.
-__device__ __forceinline__ void copy_scales_e(uint32_t tmem, uint32_t smem) {
-  const uint64_t desc = umma_desc(smem, 128, 128, 0);  // unswizzled, 8-row groups 128 bytes apart
-  asm volatile(
-      "{\n\t.reg .pred e;\n\t.reg .b32 r;\n\t"
+      "setp.eq.b32 t, 0, 0;\n\t"
+      "mov.b16 m, 3;\n\t"
+      "add.u32 sb, %4, 4;\n\tadd.u32 sb2, %4, 8;\n\t"
+      "add.s64 c1, %5, 32;\n\tadd.s64 c2, %5, 64;\n\t"
+      "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
+      "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
       "elect.sync r|e, 0xffffffff;\n\t"
-      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(tmem),
-      "l"(desc)
+      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%4], %5;\n\t"
+      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [sb], c1;\n\t"
+      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [sb2], c2;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [sb], p;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a1, b1, %3, [%4], [sb], t;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a2, b2, %3, [%4], [sb], t;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a3, b3, %3, [%4], [sb], t;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%7], m;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(sa), "l"(sc), "r"(acc), "r"(smem_u32(empty))
       : "memory");
 }
 
@@ -214,37 +223,37 @@ __global__ void __launch_bounds__(kThreads, 1)
       int s = 0, g = 0, q = 0;
       uint32_t ph = 0;
       bool ok = true;
-      int next_full = 0;  // lane 0: the next stage was found ready before this stage's last MMAs
+      // Lane 0: whether the next stage's operands and the next unit's accumulator
+      // were found ready before this stage's MMAs were issued.  A wait costs this
+      // warp 200 clocks of latency even when its barrier is complete; the tests
+      // run behind the issue.
+      int next_full = 0, next_empty = 0;
       for (int t = pair; t < tiles && ok; t += pairs) {
         int i = 0;
         for (int u = 0; u < units && ok; ++u, ++g) {
           const int b = g & 1;
           const uint32_t d = tmem + (uint32_t)(b * TN);
           for (int j = 0; j < kPerUnit && i < nst; ++j, ++i, q ^= 1) {
-            if (!__shfl_sync(0xffffffffu, next_full, 0) &&
-                !(ok = wait(&full[s], ph, DEV_TIMEOUT_FULL)))
-              break;
-            next_full = 0;
-            if (j == 0 &&
+            const int ready = __shfl_sync(0xffffffffu, next_full | (next_empty << 1), 0);
+            if (!(ready & 1) && !(ok = wait(&full[s], ph, DEV_TIMEOUT_FULL))) break;
+            if (j == 0 && !(ready & 2) &&
                 !(ok = wait(&tempty[b], ((g >> 1) & 1) ^ 1, DEV_TIMEOUT_TMEM_EMPTY)))
               break;
             tc_fence_after();
             const int sn = s + 1 == S ? 0 : s + 1;
             const uint32_t phn = s + 1 == S ? ph ^ 1u : ph;
             const bool last = j + 1 == kPerUnit || i + 1 == nst;
-            const uint32_t xa = smem_u32(base + s * kStageBytes), ya = xa + 16384, sc = xa + 32768;
-            const uint32_t sa = tmem + kScaleCol + 12u * (uint32_t)q, sb = sa + 4;
-            copy_scales_e(sa, sc);
-            copy_scales_e(sb, sc + 512);
-            copy_scales_e(sb + 4, sc + 1024);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if (k == 2 && lane == 0) next_full = mbar_test_wait(&full[sn], phn);
-              mma_mx_e(d, umma_desc(xa + 32 * k, 16, 1024, kLayoutSW128),
-                       umma_desc(ya + 32 * k, 16, 1024, kLayoutSW128), mx_idesc(TN), sa, sb,
-                       j > 0 || k > 0);
+            if (lane == 0) {
+              next_full = mbar_test_wait(&full[sn], phn);
+              next_empty = last ? mbar_test_wait(&tempty[b ^ 1], (((g + 1) >> 1) & 1) ^ 1) : 0;
             }
-            commit_pair_e(&empty[s]);
+            // operands K-major in 128-byte swizzled rows; scale groups unswizzled,
+            // 8-row groups 128 bytes apart
+            const uint32_t xa = smem_u32(base + s * kStageBytes);
+            mx_stage_e(d, umma_desc(xa, 16, 1024, kLayoutSW128),
+                       umma_desc(xa + 16384, 16, 1024, kLayoutSW128), mx_idesc(TN),
+                       tmem + kScaleCol + 12u * (uint32_t)q, umma_desc(xa + 32768, 128, 128, 0), j > 0,
+                       &empty[s]);
             if (last) commit_pair_e(&tfull[b]);
             s = sn;
             ph = phn;
