@@ -329,41 +329,62 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int64_t n0 = p.swap ? (int64_t)tx * kX : (int64_t)ty * BN;
     const int64_t M = p.swap ? p.ycols : p.xrows, N = p.swap ? p.xrows : p.ycols;
     const uint32_t tb = smem_u32(base);
-    for (int e = threadIdx.x; e < share * quads; e += kThreads) {
-      const int r = rank * share + e / quads, c = e % quads * 4;
-      const int64_t m = m0 + r, n = n0 + c;
-      if (m >= M || n >= N) continue;
-      const uint32_t at = tb + (uint32_t)(r * pitch + c) * 4;
-      float4 v;
-      if (parts == 1) {
-        v = lds128(at);
-      } else {
-        v = ld_cluster(map_rank(at, 0));
-        for (int q = 1; q < parts; ++q) {
-          const float4 w = ld_cluster(map_rank(at, (uint32_t)q));
-          v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+    // four quads at a time: a load out of another CTA takes longer than the
+    // whole of the work on it
+    const int total = share * quads;
+    for (int e0 = threadIdx.x; e0 < total; e0 += 4 * kThreads) {
+      float4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = e0 + i * kThreads;
+        if (e < total) {
+          const uint32_t at =
+              tb + (uint32_t)((rank * share + e / quads) * pitch + e % quads * 4) * 4;
+          v[i] = parts == 1 ? lds128(at) : ld_cluster(map_rank(at, 0));
         }
       }
-      float* o = p.out + m * p.ldo + n;
-      if (p.vec_ok && n + 4 <= N) {
-        if (p.bias) {
-          const float4 b4 = __ldg(reinterpret_cast<const float4*>(p.bias + n));
-          v.x += b4.x; v.y += b4.y; v.z += b4.z; v.w += b4.w;
-        }
-        if (p.accumulate) {
-          const float4 q = *reinterpret_cast<const float4*>(o);
-          v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
-        }
-        *reinterpret_cast<float4*>(o) = activate4(v, p.act);
-      } else {
-        const float ve[4] = {v.x, v.y, v.z, v.w};
+      for (int q = 1; q < parts; ++q) {
+        float4 w[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (n + j >= N) break;
-          float w = ve[j];
-          if (p.bias) w += __ldg(p.bias + n + j);
-          if (p.accumulate) w += o[j];
-          o[j] = activate(w, p.act);
+        for (int i = 0; i < 4; ++i) {
+          const int e = e0 + i * kThreads;
+          if (e < total)
+            w[i] = ld_cluster(map_rank(
+                tb + (uint32_t)((rank * share + e / quads) * pitch + e % quads * 4) * 4, (uint32_t)q));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[i].x += w[i].x; v[i].y += w[i].y; v[i].z += w[i].z; v[i].w += w[i].w;
+        }
+      }
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        const int e = e0 + i * kThreads;
+        if (e >= total) break;
+        const int64_t m = m0 + rank * share + e / quads, n = n0 + e % quads * 4;
+        if (m >= M || n >= N) continue;
+        float4 x = i == 0 ? v[0] : i == 1 ? v[1] : i == 2 ? v[2] : v[3];
+        float* o = p.out + m * p.ldo + n;
+        if (p.vec_ok && n + 4 <= N) {
+          if (p.bias) {
+            const float4 b4 = __ldg(reinterpret_cast<const float4*>(p.bias + n));
+            x.x += b4.x; x.y += b4.y; x.z += b4.z; x.w += b4.w;
+          }
+          if (p.accumulate) {
+            const float4 q = *reinterpret_cast<const float4*>(o);
+            x.x += q.x; x.y += q.y; x.z += q.z; x.w += q.w;
+          }
+          *reinterpret_cast<float4*>(o) = activate4(x, p.act);
+        } else {
+          const float ve[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (n + j >= N) break;
+            float w = ve[j];
+            if (p.bias) w += __ldg(p.bias + n + j);
+            if (p.accumulate) w += o[j];
+            o[j] = activate(w, p.act);
+          }
         }
       }
     }

@@ -574,25 +574,35 @@ __global__ void __launch_bounds__(T > 256 ? T : 256, T > 512 ? 1 : (T > 256 ? 1 
 }
 
 // dg[j] (+)= sum over the CTAs' partial rows, db likewise (blockIdx.y picks
-// one): 32 columns per CTA, 8 threads a column, in a fixed order.
+// one): 8 columns per CTA (one 32-byte sector of a row), 32 threads a column
+// with 8 rows in flight each, added in a fixed order.
 __global__ void __launch_bounds__(kThreads) norm_bwd_reduce_kernel(const float* __restrict__ part,
                                                                    int ctas, int d, float* dg,
                                                                    float* db, int accumulate) {
-  __shared__ float t[8][33];
+  __shared__ float t[32][9];
   griddep_wait();
   griddep_launch_dependents();
   float* out = blockIdx.y ? db : dg;
   if (!out) return;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int j = blockIdx.x * 32 + lane;
+  const int col = threadIdx.x & 7, w = threadIdx.x >> 3;
+  const int j = blockIdx.x * 8 + col;
   float s = 0.0f;
-  if (j < d)
-    for (int c = w; c < ctas; c += 8) s += part[((int64_t)c * 2 + blockIdx.y) * d + j];
-  t[w][lane] = s;
+  if (j < d) {
+    const float* p = part + (int64_t)blockIdx.y * d + j;
+    for (int c0 = w; c0 < ctas; c0 += 256) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v[i] = c0 + 32 * i < ctas ? __ldg(p + (int64_t)(c0 + 32 * i) * 2 * d) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += v[i];
+    }
+  }
+  t[w][col] = s;
   __syncthreads();
   if (w == 0 && j < d) {
 #pragma unroll
-    for (int k = 1; k < 8; ++k) s += t[k][lane];
+    for (int k = 1; k < 32; ++k) s += t[k][col];
     out[j] = accumulate ? out[j] + s : s;
   }
 }
@@ -611,7 +621,7 @@ int launch_with_sums(NormBwdParams& p, int grid, float* dg, float* db, cudaStrea
   clear_stale_cuda_error();
   cudaError_t e = launch();
   if (e == cudaSuccess && part)
-    e = launch_pdl(norm_bwd_reduce_kernel, dim3((unsigned)((p.d + 31) / 32), 2), dim3(kThreads), 0,
+    e = launch_pdl(norm_bwd_reduce_kernel, dim3((unsigned)((p.d + 7) / 8), 2), dim3(kThreads), 0,
                    s, (const float*)part, grid, p.d, dg, db, p.accumulate);
   if (e == cudaSuccess) e = cudaGetLastError();
   ws_free(part, s);
@@ -721,7 +731,7 @@ int norm_backward_run(rtb_ctx* ctx, const NormBwdDesc& d, cudaStream_t s) {
   clear_stale_cuda_error();
   cudaError_t e = launch_pdl(norm_bwd_kernel, dim3((unsigned)grid), dim3(kThreads), 0, s, p);
   if (e == cudaSuccess && part)
-    e = launch_pdl(norm_bwd_reduce_kernel, dim3((unsigned)((d.d + 31) / 32), 2), dim3(kThreads), 0,
+    e = launch_pdl(norm_bwd_reduce_kernel, dim3((unsigned)((d.d + 7) / 8), 2), dim3(kThreads), 0,
                    s, (const float*)part, grid, (int)d.d, d.dg, d.db, d.accumulate);
   if (e == cudaSuccess) e = cudaGetLastError();
   ws_free(part, s);
