@@ -192,6 +192,64 @@ def test_product(gpu, m, n, k, ra, rb):
     check_product(gpu, a, sa, w, sw)
 
 
+# enough 256-row tiles for CTA pairs; more tiles than pairs, ragged edges, more
+# than one promotion unit (K > 1024) and less than one
+LARGE = [(1537, 2050, 400), (2600, 2100, 1200), (2310, 2000, 130)]
+
+
+@pytest.mark.parametrize("m,n,k", LARGE)
+@pytest.mark.parametrize("ra,rb", [(1, 128), (1, 1)])
+@pytest.mark.parametrize("floats", [False, True])
+def test_product_large(gpu, m, n, k, ra, rb, floats):
+    a, sa = operand(m, k, ra, 23)
+    w, sw = operand(n, k, rb, 24)
+    if floats:
+        sw = (0.01 + torch.rand(sw.shape, generator=torch.Generator().manual_seed(9))).cuda()
+    g = torch.Generator().manual_seed(10)
+    bias = torch.randn(n, generator=g).cuda()
+    big = torch.full((m + 2, n + 6), 3.0, device="cuda")
+    check_product(gpu, a, sa, w, sw, bias, 0, out=big[1:m + 1, 2:n + 2])
+    mask = torch.ones_like(big, dtype=torch.bool)
+    mask[1:m + 1, 2:n + 2] = False
+    assert bool((big[mask] == 3.0).all())
+    check_product(gpu, a, sa, w, sw, bias, 1)
+
+
+@pytest.mark.parametrize("m,n", [(5, 140), (150, 200), (2600, 2100)])
+def test_product_scale_range(gpu, m, n):
+    """Scales far from 1 that cancel, the smallest byte, and byte 255 (NaN), on
+    every path a size takes."""
+    g = torch.Generator().manual_seed(11)
+    k = 300
+    a = torch.randint(0, 120, (m, k), generator=g).to(torch.uint8).cuda().view(E4M3)
+    w = torch.randint(0, 120, (n, k), generator=g).to(torch.uint8).cuda().view(E4M3)
+    for ea, ew in ((27, 227), (227, 27), (0, 200), (127, 0)):
+        sa = torch.full((m, 3), ea, dtype=torch.uint8).cuda().view(E8M0)
+        sw = torch.full((n, 3), ew, dtype=torch.uint8).cuda().view(E8M0)
+        check_product(gpu, a, sa, w, sw)
+    sa = torch.full((m, 3), 127, dtype=torch.uint8).cuda()
+    sw = torch.full((n, 3), 127, dtype=torch.uint8).cuda()
+    sa[3, 1] = 255
+    sw[n - 2, 2] = 255
+    c = gpu.fp8_matmul(a, sa.view(E8M0), w.t(), sw.view(E8M0).t())
+    want = torch.zeros_like(c, dtype=torch.bool)
+    want[3, :] = True
+    want[:, n - 2] = True
+    assert torch.equal(torch.isnan(c), want)
+
+
+def test_product_nan_codes_large(gpu):
+    a, sa = operand(2600, 300, 1, 25)
+    w, sw = operand(2100, 300, 128, 26)
+    a.view(torch.uint8)[1300, 299] = 0x7F
+    w.view(torch.uint8)[2099, 5] = 0xFF
+    c = gpu.fp8_matmul(a, sa, w.t(), sw.t())
+    want = torch.zeros_like(c, dtype=torch.bool)
+    want[1300, :] = True
+    want[:, 2099] = True
+    assert torch.equal(torch.isnan(c), want)
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 200, 300), (40, 128, 256), (130, 300, 500), (300, 700, 384)])
 def test_product_row_major_b(gpu, m, n, k):
     """b given as [K, N] row-major with 128 x 128 blocks."""
@@ -296,6 +354,12 @@ def test_weight_gradient(gpu, m, n, k, precision):
     check_wgrad(gpu, m, n, k, precision)
 
 
+@pytest.mark.parametrize("m,n,k", [(300, 2050, 1537), (1100, 2100, 2600)])
+def test_weight_gradient_large(gpu, m, n, k):
+    check_wgrad(gpu, m, n, k, 0)
+    check_wgrad(gpu, m, n, k, 0, accumulate=True)
+
+
 def test_weight_gradient_accumulates(gpu):
     check_wgrad(gpu, 200, 150, 260, 0, accumulate=True)
     check_wgrad(gpu, 200, 150, 260, 0, block_rows=128)
@@ -390,6 +454,77 @@ def test_side_stream_and_graphs(gpu):
     for i in range(2):
         assert all(torch.equal(a, b) for a, b in zip(outs[i], want[i]))
     assert gpu.get_context(0).device_error() == 0
+
+
+def test_two_threads(gpu):
+    """Two host threads, a stream each, the same context."""
+    import threading
+    a, sa = operand(2100, 400, 1, 80)
+    w, sw = operand(1900, 400, 128, 81)
+    b, sb = operand(40, 640, 1, 82)
+    v, sv = operand(500, 640, 1, 83)
+    want = [gpu.fp8_matmul(a, sa, w.t(), sw.t()), gpu.fp8_matmul(b, sb, v.t(), sv.t())]
+    torch.cuda.synchronize()
+    got, streams = [[], []], [torch.cuda.Stream(), torch.cuda.Stream()]
+
+    def work(i, args):
+        with torch.cuda.stream(streams[i]):
+            for _ in range(20):
+                got[i].append(gpu.fp8_matmul(*args))
+
+    ts = [threading.Thread(target=work, args=(0, (a, sa, w.t(), sw.t()))),
+          threading.Thread(target=work, args=(1, (b, sb, v.t(), sv.t())))]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert len(got[i]) == 20 and all(torch.equal(c, want[i]) for c in got[i])
+
+
+# ------------------------------------------------------------------ a training step
+
+@pytest.mark.parametrize("rows,d,n", [(70, 200, 130), (512, 1024, 768)])
+def test_block_step(gpu, rows, d, n):
+    """Layer norm, save, 8-bit Linear with ReLU, and back: the weight gradient
+    out of the saved operand, the input's gradient through the weight and the
+    norm, whose own input was saved too.  Each stage against float64 on what the
+    stage before left."""
+    g = torch.Generator().manual_seed(90)
+    x = (torch.randn((rows, d), generator=g) + 0.3).cuda()
+    nw, nb = (1 + 0.1 * torch.randn(d, generator=g)).cuda(), (0.1 * torch.randn(d, generator=g)).cuda()
+    weight = (torch.randn((n, d), generator=g) * d ** -0.5).cuda()
+    bias = (0.1 * torch.randn(n, generator=g)).cuda()
+    grad = torch.randn((rows, n), generator=g).cuda()
+
+    xq, xs = gpu.fp8_quantize(x)
+    y, mean, rstd = gpu.layer_norm_fwd(x, nw, nb)
+    yq, ys = gpu.fp8_quantize(y)
+    wq, ws = gpu.fp8_quantize(weight, 128)
+    z = gpu.fp8_matmul(yq, ys, wq.t(), ws.t(), bias, gpu.ACT_RELU)
+    Y, W = values64(yq, ys), values64(wq, ws)
+    pre = Y @ W.t() + bias.double()
+    S = Y.abs() @ W.abs().t() + bias.double().abs()
+    assert bool(((z.double() - torch.relu(pre)).abs() <= S * 2.0 ** -18).all())
+    # the saved operand stands for y within half a step of e4m3
+    assert float((Y - y.double()).norm() / y.double().norm()) <= 2.0 ** -4
+
+    dz = grad * (z > 0)
+    wd = gpu.fp8_dequantize(wq, ws)
+    dy, dw = gpu.matmul_backward_fp8(yq, ys, wd.t().contiguous(), dz)
+    assert float((dw.double() - Y.t() @ dz.double()).norm() / dw.double().norm()) <= 1e-6
+    assert float((dy.double() - dz.double() @ W).norm() / dy.double().norm()) <= 1e-5
+    dx, dg, db = gpu.layer_norm_backward(xq, mean, rstd, dy, nw, nb, x_scale=xs)
+    u = (values64(xq, xs) - mean.double()[:, None]) * rstd.double()[:, None]
+    h = dy.double() * nw.double()
+    ref = rstd.double()[:, None] * (h - h.mean(1, keepdim=True) - u * (h * u).mean(1, keepdim=True))
+    for got, want in ((dx, ref), (dg, (dy.double() * u).sum(0)), (db, dy.double().sum(0))):
+        assert float((got.double() - want).norm() / want.norm()) <= 1e-6
+    # gradients through the checkpoint point where the exact ones do
+    u = (x.double() - mean.double()[:, None]) * rstd.double()[:, None]
+    ref = rstd.double()[:, None] * (h - h.mean(1, keepdim=True) - u * (h * u).mean(1, keepdim=True))
+    assert float((dx.double() - ref).norm() / ref.norm()) <= 2.0 ** -4
 
 
 # ------------------------------------------------------------------ refusals
