@@ -4,13 +4,13 @@
 // block of 128 gives its scale to four of them).
 //
 // The scales enter inside the MMA, so a partial sum has to leave the tensor core
-// only for the accumulation's sake, every 1024 elements (the tensor core does
-// not round each addition to nearest: the error grows with the chain, 9e-8
+// only for the accumulation's sake, every 1024 or 2048 elements (the tensor core
+// does not round each addition to nearest: the error grows with the chain, 9e-8
 // relative after 32 steps) instead of every 128: the epilogue's chain of barrier, TMEM loads and adds, 1150
 // clocks against 512 of MMAs in rtb_pairgemm.cu, is out of the way.
 //
 // Tile 256 x 224 or 256 x 192 (two accumulators leave columns of TMEM for the
-// scales), whichever takes less time in whole rounds of the pairs.  Roles (warps of each CTA): 0 TMA producer; 1 TMEM allocation, and
+// scales), whichever takes less time in whole rounds of the pairs.  Roles (warps of each CTA): 0, 2, 3 TMA producers; 1 TMEM allocation, and
 // in the pair's first CTA the issue for both; 4..11 epilogue (lanes 32 (w % 4)..,
 // one half of the columns).
 //
@@ -29,11 +29,11 @@ namespace {
 
 constexpr int kThreads = 384;
 constexpr int kTileX = 256;
-constexpr int kStages = 6;
+constexpr int kStages = 5;
 constexpr int kStageBytes = 16384 + 16384 + 2048;  // X, Y (half of the tile's rows), scales
 constexpr int kChunk = 128 * 16 * 4;               // a staged 128 x 16 fp32 piece of the output
-constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 2 * kChunk + 512;
-constexpr int kPerUnit = 8;                        // blocks of 128 between promotions
+constexpr int kBufs = 3;                           // staging chunks of an epilogue half
+constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 2 * kBufs * kChunk + 512 + 1024;
 constexpr uint32_t kScaleCol = 448;                // TMEM: two buffers of 4 + 8 columns
 static_assert(kSmemBytes <= 232448, "shared memory");
 
@@ -134,17 +134,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                    const __grid_constant__ CUtensorMap tmC, const BlockParams p) {
   constexpr int S = kStages;
   constexpr int kHalf = TN / 2;  // columns of an epilogue half, Y rows of a CTA
-  static_assert(TN % 32 == 0 && 2 * TN <= (int)kScaleCol, "two accumulators below the scales");
+  // two accumulators where the scales leave room for them; one is promoted half
+  // as often, since its MMAs wait for the promotion
+  constexpr int kAccBufs = 2 * TN <= (int)kScaleCol ? 2 : 1;
+  constexpr int kPerUnit = kAccBufs == 2 ? 8 : 16;  // blocks of 128 between promotions
+  static_assert(TN % 32 == 0 && TN <= 256, "tile width");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  uint8_t* staging = base + S * kStageBytes;  // 2 x kChunk, 1024-byte aligned
-  uint64_t* full = reinterpret_cast<uint64_t*>(staging + 2 * kChunk);
+  uint8_t* staging = base + S * kStageBytes;  // [2][kBufs] x kChunk, 1024-byte aligned
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + 2 * kBufs * kChunk);
   uint64_t* empty = full + S;
   uint64_t* tfull = empty + S;
   uint64_t* tempty = tfull + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* bias_s = reinterpret_cast<float*>(staging + 2 * kBufs * kChunk + 512);  // [2][128]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
@@ -189,7 +194,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (warp == 0 && lane == 0) {
+    if (warp != 1 && lane == 0) {
+      // three producers take the stages in turn: one thread's wait and issue of a
+      // stage's four loads takes about 600 clocks, longer than its MMAs
+      const int turn = warp ? warp - 1 : 0;
+      int q = 0;
       // X 128 rows, half of the Y rows and three scale groups, of both CTAs
       const uint32_t bytes = 2u * (16384u + (uint32_t)kHalf * 128u + 3u * 512u);
       int s = 0;
@@ -199,7 +208,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         int tx, ty;
         mx_tile(p, t, tx, ty);
         const int x0 = tx * kTileX + 128 * (int)rank, y0 = ty * TN + kHalf * (int)rank;
-        for (int i = 0; i < nst; ++i) {
+        for (int i = 0; i < nst; ++i, q = q == 2 ? 0 : q + 1) {
+          if (q != turn) {
+            if (++s == S) { s = 0; ph ^= 1; }
+            continue;
+          }
           if (!(ok = mbar_wait_bounded(&empty[s], ph ^ 1, abort_flag, p.err, DEV_TIMEOUT_EMPTY,
                                        p.timeout_ns)))
             break;
@@ -231,13 +244,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int t = pair; t < tiles && ok; t += pairs) {
         int i = 0;
         for (int u = 0; u < units && ok; ++u, ++g) {
-          const int b = g & 1;
+          const int b = kAccBufs == 2 ? g & 1 : 0, use = kAccBufs == 2 ? g >> 1 : g;
           const uint32_t d = tmem + (uint32_t)(b * TN);
           for (int j = 0; j < kPerUnit && i < nst; ++j, ++i, q ^= 1) {
             const int ready = __shfl_sync(0xffffffffu, next_full | (next_empty << 1), 0);
             if (!(ready & 1) && !(ok = wait(&full[s], ph, DEV_TIMEOUT_FULL))) break;
             if (j == 0 && !(ready & 2) &&
-                !(ok = wait(&tempty[b], ((g >> 1) & 1) ^ 1, DEV_TIMEOUT_TMEM_EMPTY)))
+                !(ok = wait(&tempty[b], (use & 1) ^ 1, DEV_TIMEOUT_TMEM_EMPTY)))
               break;
             tc_fence_after();
             const int sn = s + 1 == S ? 0 : s + 1;
@@ -245,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool last = j + 1 == kPerUnit || i + 1 == nst;
             if (lane == 0) {
               next_full = mbar_test_wait(&full[sn], phn);
-              next_empty = last ? mbar_test_wait(&tempty[b ^ 1], (((g + 1) >> 1) & 1) ^ 1) : 0;
+              next_empty = kAccBufs == 2 && last ? mbar_test_wait(&tempty[b ^ 1], (((g + 1) >> 1) & 1) ^ 1) : 0;
             }
             // operands K-major in 128-byte swizzled rows; scale groups unswizzled,
             // 8-row groups 128 bytes apart
@@ -268,23 +281,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int et = threadIdx.x - 128 - 128 * half;  // 0..127 within the half
     const uint32_t t_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)(kHalf * half);
     const uint32_t tempty0[2] = {map_rank(smem_u32(&tempty[0]), 0), map_rank(smem_u32(&tempty[1]), 0)};
-    uint8_t* stg = staging + half * kChunk;
-    int g = 0;
+    uint8_t* stg0 = staging + half * kBufs * kChunk;
+    int g = 0, buf = 0;
     bool ok = true;
     for (int t = pair; t < tiles; t += pairs) {
       int tx, ty;
       mx_tile(p, t, tx, ty);
       const int64_t x = (int64_t)tx * kTileX + 128 * rank + row;
       const int64_t y0 = (int64_t)ty * TN + kHalf * half;
+      if (p.bias) {
+        // the tile's bias: loaded here, its latency passes behind the MMAs; the
+        // barriers of the stores below keep its readers and writers apart
+        named_bar_sync(1 + half, 128);
+        if (et < kHalf) bias_s[128 * half + et] = y0 + et < p.ycols ? __ldg(p.bias + y0 + et) : 0.0f;
+        named_bar_sync(1 + half, 128);
+      }
       unsigned long long acc[kHalf / 2];
 #pragma unroll
       for (int j = 0; j < kHalf / 2; ++j) acc[j] = 0ull;
       for (int u = 0; u < units; ++u, ++g) {
-        const int b = g & 1;
+        const int b = kAccBufs == 2 ? g & 1 : 0, use = kAccBufs == 2 ? g >> 1 : g;
         if (ok) {
           int got = 0;
           if (lane == 0)
-            got = mbar_wait_bounded(&tfull[b], (g >> 1) & 1, abort_flag, p.err,
+            got = mbar_wait_bounded(&tfull[b], use & 1, abort_flag, p.err,
                                     DEV_TIMEOUT_TMEM_FULL, p.timeout_ns);
           ok = __shfl_sync(0xffffffffu, got, 0) != 0;
         }
@@ -316,12 +336,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (p.bias) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] += yc + j < p.ycols ? __ldg(p.bias + yc + j) : 0.0f;
+          for (int j = 0; j < 16; ++j) v[j] += bias_s[128 * half + 16 * c + j];
         }
         activate_n<16>(v, p.act);
         if (p.c_tma) {
-          // the store before has read the chunk (its issuing thread waits)
-          if (et == 0) bulk_wait_group_read<0>();
+          // this chunk's store before has read it (its issuing thread waits): with
+          // one chunk a half the waits made a tile's epilogue 6 us long
+          uint8_t* stg = stg0 + buf * kChunk;
+          if (et == 0) bulk_wait_group_read<kBufs - 1>();
           named_bar_sync(1 + half, 128);
           // 64-byte rows, 16-byte units swizzled by (row / 2) % 4
           const uint32_t dst = smem_u32(stg) + row * 64;
@@ -334,8 +356,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int xs = tx * kTileX + 128 * (int)rank;
           if (et == 0 && yc < p.ycols && xs < p.xrows) {
             tma_store_2d(&tmC, stg, (int)yc, xs);
-            bulk_commit_group();
           }
+          if (et == 0) bulk_commit_group();  // (an empty group where nothing is stored)
+          buf = buf + 1 == kBufs ? 0 : buf + 1;
         } else if (x < p.xrows) {
           float* o = p.out + x * p.ldo + yc;
 #pragma unroll
@@ -435,14 +458,18 @@ int launch(rtb_ctx* ctx, const uint8_t* X, int64_t ldx, const uint8_t* Y, int64_
 
 int launch_mx(rtb_ctx* ctx, const uint8_t* X, int64_t ldx, const uint8_t* Y, int64_t ldy,
               BlockParams& p, cudaStream_t s) {
-  // whole rounds of the pairs, a round as long as its tile is wide
-  auto cost = [&](int64_t tn) {
+  // 256 columns move fewer bytes for a product, 224 have room for a second
+  // accumulator, behind which a tile's epilogue (and the promotions) pass.  In
+  // whole rounds of the pairs, from the measured times of a round: 0.37 us a
+  // stage, and 6 or 4 us a tile (8192 x 4096 x 8192: 225 us against 261; 8192 x
+  // 8192 x 1024: 123 against 106).
+  auto cost = [&](int64_t tn, double tile_us) {
     const int64_t tiles = ((p.xrows + kTileX - 1) / kTileX) * ((p.ycols + tn - 1) / tn);
     const int64_t pairs = ctx->sm_count / 2;
-    return (tiles + pairs - 1) / pairs * tn;
+    return (double)((tiles + pairs - 1) / pairs) * (0.37 * ((p.depth + 127) / 128) + tile_us);
   };
-  return cost(192) < cost(224) ? launch<192>(ctx, X, ldx, Y, ldy, p, s)
-                               : launch<224>(ctx, X, ldx, Y, ldy, p, s);
+  return cost(224, 4.0) < 0.95 * cost(256, 6.0) ? launch<224>(ctx, X, ldx, Y, ldy, p, s)
+                                                : launch<256>(ctx, X, ldx, Y, ldy, p, s);
 }
 
 }  // namespace rtb

@@ -14,7 +14,7 @@
 // that is 32768 multiply-adds per 512 clocks of MMAs, half of the SM's fp32
 // lanes; packed f32x2 instructions halve the issue slots.
 //
-// Roles (warps of each CTA): 0 TMA producer; 1 TMEM allocation, and in the
+// Roles (warps of each CTA): 0, 2, 3 TMA producers; 1 TMEM allocation, and in the
 // pair's first CTA the MMA issue for both; 4..11 epilogue (lanes 32 (w % 4)..,
 // columns 128 ((w - 4) / 4)..).  The first warpgroup hands registers to the
 // epilogue's two (384 threads x 168 at launch = 128 x (40 + 232 + 232)): at 168
@@ -173,7 +173,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (warp == 0 && lane == 0) {
+    if (warp != 1 && lane == 0) {
+      // three producers take the stages in turn: one thread's wait and issue of a
+      // stage's loads takes about as long as its MMAs
+      const int turn = warp ? warp - 1 : 0;
+      int q = 0;
       const uint32_t bytes = 2u * 16384u * (uint32_t)(1 + (MODE == 0 ? 1 : p.pieces));
       int s = 0;
       uint32_t ph = 0;
@@ -182,7 +186,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         int tx, ty;
         pair_tile(p, t, tx, ty);
         const int x0 = tx * kTile + 128 * (int)rank, y0 = ty * kTile + 128 * (int)rank;
-        for (int i = 0; i < nst; ++i) {
+        for (int i = 0; i < nst; ++i, q = q == 2 ? 0 : q + 1) {
+          if (q != turn) {
+            if (++s == S) { s = 0; ph ^= 1; }
+            continue;
+          }
           if (!(ok = mbar_wait_bounded(&empty[s], ph ^ 1, abort_flag, p.err, DEV_TIMEOUT_EMPTY,
                                   p.timeout_ns)))
             break;
