@@ -137,33 +137,18 @@ __device__ __forceinline__ void put(float* out, float v, int accumulate) {
   *out = accumulate ? *out + v : v;
 }
 
-constexpr int kRing = 8;                // most stages of the row ring
-constexpr int kRingBytes = 200 * 1024;  // shared memory of an SM for the ring
+constexpr int kRing = 3;  // stages of the row ring: 96 KB for 512 threads of 8 values
 
 __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
-// At most n of this thread's copy groups are still under way (n < kRing).
-__device__ __forceinline__ void cp_async_wait_n(int n) {
-  switch (n) {
-    case 7: cp_async_wait<7>(); break;
-    case 6: cp_async_wait<6>(); break;
-    case 5: cp_async_wait<5>(); break;
-    case 4: cp_async_wait<4>(); break;
-    case 3: cp_async_wait<3>(); break;
-    case 2: cp_async_wait<2>(); break;
-    case 1: cp_async_wait<1>(); break;
-    default: cp_async_wait<0>(); break;
-  }
-}
-
 // Up to 8192 columns: T threads a row (a multiple of 32), E values of x and of
 // dy each: lane l of the group's warp w holds the units 32 G w + l + 32 i, i <
 // G, where a unit is a float4 (VEC: d % 4 == 0, 16-byte aligned rows) or a
 // column; the distances are constants, so that a row's addresses cost little.
 // SAVED: x from the checkpoint.  ACT: an activation.
 //
-// VEC: each thread copies its own values of the group's next `stages` rows into
+// VEC: each thread copies its own values of the group's next kRing rows into
 // shared memory (cp.async), waits for its own copies alone and refills the slot
 // once it has used the values: no barrier is needed for the ring.  Eight values
 // a thread (five registers each) leave room for 1024 threads on an SM, whose
@@ -172,11 +157,11 @@ __device__ __forceinline__ void cp_async_wait_n(int n) {
 // into registers directly: copies of 4 bytes cost more than they hide.
 template <int kBlock, int E, bool VEC, bool SAVED, bool ACT>
 __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
-    norm_bwd_rows_kernel(const NormBwdParams p, const int T, const int stages, const float inv_d,
-                         float* dg, float* db) {
+    norm_bwd_rows_kernel(const NormBwdParams p, const int T, const float inv_d, float* dg,
+                         float* db) {
   constexpr int G = VEC ? E / 4 : E;  // copies of x (and of dy) a thread
   constexpr int C = E / G;            // columns of a copy
-  __shared__ float2 red[2][kBlock / 32];
+  __shared__ float red[2][kBlock / 32][2];
   extern __shared__ float4 ring4[];   // the ring, then reused for the CTA's sums
   const int R = kBlock / T;           // rows a CTA works on
   const int grp = threadIdx.x / T, t = threadIdx.x - grp * T;
@@ -187,7 +172,7 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
   // a slot: x, then dy, both on 16-byte boundaries
   const int xbytes = ((SAVED ? units * 4 : units * C * 4) + 15) & ~15;
   const int row_bytes = xbytes + ((units * C * 4 + 15) & ~15);
-  const uint32_t slot0 = smem_u32(ring4) + (uint32_t)(grp * stages * row_bytes);
+  const uint32_t slot0 = smem_u32(ring4) + (uint32_t)(grp * kRing * row_bytes);
   constexpr bool kKeep = VEC && !ACT;  // the weight stays in registers
   float ag[E], ab[E], gw[kKeep ? E : 1];
 #pragma unroll
@@ -203,14 +188,18 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
       if (32 * (i / C) < rem) gw[i] = __ldg(p.g + C * (k0 + 32 * (i / C)) + i % C);
     }
   }
-  const int64_t step = (int64_t)gridDim.x * R;
-  auto fetch = [&](int64_t r, int s) {
-    if (r < p.rows) {
+  // rows and leading dimensions fit 32 bits (checked by the host), so that a
+  // row's address is one multiply-add
+  const int rows = (int)p.rows, step = (int)gridDim.x * R;
+  const int ldx = (int)p.ldx, ldq = (int)p.ldq, lds = (int)p.lds, lddy = (int)p.lddy,
+            lddx = (int)p.lddx;
+  auto fetch = [&](int r, int s) {
+    if (r < rows) {
       const uint32_t xs = slot0 + (uint32_t)(s * row_bytes + (SAVED ? 4 : 16) * k0);
       const uint32_t ys = slot0 + (uint32_t)(s * row_bytes + xbytes + 16 * k0);
-      const char* xr = SAVED ? reinterpret_cast<const char*>(p.q + r * p.ldq + 4 * k0)
-                             : reinterpret_cast<const char*>(p.x + r * p.ldx + 4 * k0);
-      const char* yr = reinterpret_cast<const char*>(p.dy + r * p.lddy + 4 * k0);
+      const char* xr = SAVED ? reinterpret_cast<const char*>(p.q + (int64_t)r * ldq + 4 * k0)
+                             : reinterpret_cast<const char*>(p.x + (int64_t)r * ldx + 4 * k0);
+      const char* yr = reinterpret_cast<const char*>(p.dy + (int64_t)r * lddy + 4 * k0);
 #pragma unroll
       for (int i = 0; i < G; ++i) {
         if (32 * i < rem) {
@@ -222,28 +211,28 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
     }
     cp_async_commit();  // (an empty group behind the last row)
   };
-  int64_t r = grp < R ? (int64_t)blockIdx.x * R + grp : p.rows;
+  int r = grp < R ? (int)blockIdx.x * R + grp : rows;
   if (VEC)
-    for (int s = 0; s < stages; ++s) fetch(r + s * step, s);
+    for (int s = 0; s < kRing; ++s) fetch(r + s * step, s);
   float mean = 0.0f, rstd = 0.0f;
-  if (r < p.rows) {
+  if (r < rows) {
     mean = __ldg(p.mean + r);
     rstd = __ldg(p.rstd + r);
   }
   int slot = 0, phase = 0;
-  for (; r < p.rows; r += step, phase ^= 1) {
+  for (; r < rows; r += step, phase ^= 1) {
     // the next row's statistics and this row's block scales
-    const int64_t rn = r + step < p.rows ? r + step : r;
+    const int rn = r + step < rows ? r + step : r;
     const float mean_n = __ldg(p.mean + rn), rstd_n = __ldg(p.rstd + rn);
     uint32_t sb[VEC ? G : 1];
     if (SAVED && VEC) {
-      const uint8_t* sr = p.scale + r * p.lds + (t >> 5) * G;  // one byte for 32 units
+      const uint8_t* sr = p.scale + (int64_t)r * lds + (t >> 5) * G;  // one byte for 32 units
 #pragma unroll
       for (int i = 0; i < G; ++i) sb[i] = 32 * i < rem ? __ldg(sr + i) : 0u;
     }
     float u[E], h[E];  // x, then u; dy, then h
     if (VEC) {
-      cp_async_wait_n(stages - 1);  // this slot's copies, the oldest group, have landed
+      cp_async_wait<kRing - 1>();  // this slot's copies, the oldest group, have landed
       const uint32_t xs = slot0 + (uint32_t)(slot * row_bytes + (SAVED ? 4 : 16) * k0);
       const uint32_t ys = slot0 + (uint32_t)(slot * row_bytes + xbytes + 16 * k0);
 #pragma unroll
@@ -266,9 +255,9 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
         }
       }
     } else {
-      const float* yr = p.dy + r * p.lddy + k0;
-      const float* xr = p.x + r * p.ldx + k0;
-      const uint8_t* qr = p.q + r * p.ldq + k0;
+      const float* yr = p.dy + (int64_t)r * lddy + k0;
+      const float* xr = p.x + (int64_t)r * ldx + k0;
+      const uint8_t* qr = p.q + (int64_t)r * ldq + k0;
 #pragma unroll
       for (int i = 0; i < G; ++i) {
         u[i] = mean;
@@ -277,7 +266,7 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
         if (32 * i < rem) {
           if (SAVED) {
             code = __ldcs(qr + 32 * i);
-            byte = __ldg(p.scale + r * p.lds + (k0 + 32 * i) / kFp8Block);
+            byte = __ldg(p.scale + (int64_t)r * lds + (k0 + 32 * i) / kFp8Block);
           } else {
             u[i] = __ldcs(xr + 32 * i);
           }
@@ -305,32 +294,32 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
       s2 = fmaf(h[i], u[i], s2);
     }
     if (VEC) {
-      fetch(r + stages * step, slot);  // every value of the slot is in registers
-      if (++slot == stages) slot = 0;
+      fetch(r + kRing * step, slot);  // every value of the slot is in registers
+      if (++slot == kRing) slot = 0;
     }
     if (p.dx) {
+      // Both sums at once: the half-warps exchange, then lanes 0..15 add up the
+      // first sum and lanes 16..31 the second.
+      const bool second = t & 16;
+      float v = second ? s2 : s1;
+      v += __shfl_xor_sync(0xffffffffu, second ? s1 : s2, 16);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        s1 += __shfl_xor_sync(0xffffffffu, s1, o);
-        s2 += __shfl_xor_sync(0xffffffffu, s2, o);
-      }
+      for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
       if (T > 32) {
         // two buffers, so that one barrier a row is enough; every warp adds the
         // warps' sums for itself, in the same order
-        const int nw = T >> 5, w0 = grp * nw;
-        if ((t & 31) == 0) red[phase][w0 + (t >> 5)] = make_float2(s1, s2);
+        const int nw = T >> 5, w0 = grp * nw, l = t & 15;
+        if (l == 0) red[phase][w0 + (t >> 5)][second] = v;
         named_bar_sync(1 + grp, T);
-        const float2 q = (t & 31) < nw ? red[phase][w0 + (t & 31)] : make_float2(0.f, 0.f);
-        s1 = q.x;
-        s2 = q.y;
+        v = l < nw ? red[phase][w0 + l][second] : 0.0f;
+        if (kBlock > 512 && l + 16 < nw) v += red[phase][w0 + 16 + l][second];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          s1 += __shfl_xor_sync(0xffffffffu, s1, o);
-          s2 += __shfl_xor_sync(0xffffffffu, s2, o);
-        }
+        for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
       }
+      s1 = __shfl_sync(0xffffffffu, v, 0);
+      s2 = __shfl_sync(0xffffffffu, v, 16);
       const float m1 = s1 * inv_d, m2 = s2 * inv_d;
-      float* dxr = p.dx + r * p.lddx + C * k0;
+      float* dxr = p.dx + (int64_t)r * lddx + C * k0;
 #pragma unroll
       for (int i = 0; i < G; ++i) {
         if (32 * i >= rem) continue;
@@ -658,9 +647,7 @@ int launch_rows(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStream
   const int units = VEC ? p.d / 4 : p.d;
   const int T = (units + 32 * G - 1) / (32 * G) * 32, R = kBlock / T;
   const int row_bytes = (((SAVED ? p.d : 4 * p.d) + 15) & ~15) + ((4 * p.d + 15) & ~15);
-  int stages = kRingBytes / kPerSm / (R * row_bytes);
-  stages = stages < 1 ? 1 : (stages > kRing ? kRing : stages);
-  int smem = VEC ? R * stages * row_bytes : 0;
+  int smem = VEC ? R * kRing * row_bytes : 0;
   if (smem < 8 * p.d) smem = 8 * p.d;  // the CTA's sums
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return cuda_status(e, "layer_norm_backward smem attribute");
@@ -668,7 +655,7 @@ int launch_rows(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStream
   const int grid = (int)(need < cap ? need : cap);
   return launch_with_sums(p, grid, dg, db, s, [&] {
     return launch_pdl(k, dim3((unsigned)grid), dim3(kBlock), (size_t)smem, s,
-                      (const NormBwdParams)p, T, stages, 1.0f / (float)p.d, dg, db);
+                      (const NormBwdParams)p, T, 1.0f / (float)p.d, dg, db);
   });
 }
 
@@ -709,7 +696,10 @@ int norm_backward_run(rtb_ctx* ctx, const NormBwdDesc& d, cudaStream_t s) {
   p.dx = d.dx;
   p.lddx = d.lddx;
   p.accumulate = d.accumulate;
-  if (d.d <= 16384) {
+  // (the row kernels index rows and rows' addresses with 32-bit factors)
+  constexpr int64_t kMax32 = INT32_MAX - (1 << 20);
+  if (d.d <= 16384 && d.rows <= kMax32 && d.ldx <= kMax32 && d.ldq <= kMax32 && d.lds <= kMax32 &&
+      d.lddy <= kMax32 && d.lddx <= kMax32) {
     auto al = [](const void* q, uintptr_t n) { return (reinterpret_cast<uintptr_t>(q) % n) == 0; };
     const bool vec = d.d % 4 == 0 && al(d.dy, 16) && d.lddy % 4 == 0 &&
                      (!d.dx || (al(d.dx, 16) && d.lddx % 4 == 0)) && (!d.g || al(d.g, 16)) &&
