@@ -306,10 +306,11 @@ __global__ void __launch_bounds__(kThreads) pack_bytes_kernel(const PackSide a, 
 //
 // X: the checkpoint's values in bf16: q * s has four significant bits, so the
 // conversion is exact (down to bf16's smallest subnormal, 2^-133).
-// Y: dC as a sum of `pieces` bf16 terms, each the rounding of what the ones
-// before left: 8 significant bits a term, so three hold an fp32 value exactly
-// (24 bits) as long as the last term is in bf16's range.  An infinity or NaN is
-// the first term alone, so that it meets the product as it would in fp32.
+// Y: dC as a sum of `pieces` bf16 terms: 8 significant bits each, truncated (a
+// value above bf16's largest would round to infinity) but for the last, which is
+// rounded, so three hold an fp32 value exactly (24 bits) as long as the last
+// term is in bf16's range.  An infinity or NaN is the first term alone, so that
+// it meets the product as it would in fp32.
 // Rows [rows, rows_pad) and the columns up to ldx and ldy are zero.
 struct OperandsParams {
   const uint8_t* q;
@@ -376,11 +377,14 @@ __global__ void __launch_bounds__(kThreads) wgrad_operands_kernel(const Operands
         uint32_t w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-          w[j] = *reinterpret_cast<const uint32_t*>(&t);
+          if (n + 1 < p.pieces)
+            asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(w[j]) : "f"(v[2 * j + 1]), "f"(v[2 * j]));
+          else
+            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[j]) : "f"(v[2 * j + 1]), "f"(v[2 * j]));
           // (an infinity or NaN leaves nothing for the next term)
-          v[2 * j] = finite_abs(v[2 * j]) > 0.0f ? v[2 * j] - __low2float(t) : 0.0f;
-          v[2 * j + 1] = finite_abs(v[2 * j + 1]) > 0.0f ? v[2 * j + 1] - __high2float(t) : 0.0f;
+          const float lo = __uint_as_float(w[j] << 16), hi = __uint_as_float(w[j] & 0xFFFF0000u);
+          v[2 * j] = finite_abs(v[2 * j]) > 0.0f ? v[2 * j] - lo : 0.0f;
+          v[2 * j + 1] = finite_abs(v[2 * j + 1]) > 0.0f ? v[2 * j + 1] - hi : 0.0f;
         }
         *reinterpret_cast<uint4*>(p.y + ((int64_t)n * p.rows_pad + r) * p.ldy + c) =
             make_uint4(w[0], w[1], w[2], w[3]);

@@ -8,7 +8,9 @@ contraction: the products of e4m3 codes are exact, the tensor core adds four
 steps of 32 (MODE fp8) or 8 steps of 16 for each of three terms (weight
 gradient) per 128-element block, each step within 2^-21 of the block's S
 (truncated alignment of the addends and of the sum), and every block is added
-in fp32 (2^-24 of the running sum, at most S)."""
+in fp32 (2^-24 of the running sum, at most S).  Where the tensor core applies the
+scales itself, 32 or 64 steps run before the addition, each within 2^-24 of the
+running sum, on average half of the unit's S: at most the same 2^-19."""
 import numpy as np
 import pytest
 import torch
@@ -397,6 +399,23 @@ def test_weight_gradient_empty_and_special(gpu):
     rest[7, :] = False
     rest[:, 11] = False
     assert bool(torch.isfinite(db[rest]).all())
+
+
+@pytest.mark.parametrize("precision", [0, 1])
+def test_weight_gradient_range(gpu, precision):
+    """Gradients at both ends of fp32: its largest value stays finite (bf16's is
+    smaller), small normal ones keep their bits."""
+    a = torch.full((3, 8), 0x38, dtype=torch.uint8).cuda().view(E4M3)  # 1.0
+    sa = torch.full((3, 1), 126, dtype=torch.uint8).cuda().view(E8M0)  # 1/2
+    grad = torch.zeros((3, 16), device="cuda")
+    grad[1, 0] = float(np.finfo(np.float32).max)
+    grad[1, 1] = -float(np.finfo(np.float32).max)
+    grad[2, 2] = 1.2345678e-30
+    db = gpu.matmul_backward_fp8(a, sa, None, grad, need_a=False, precision=precision)[1]
+    want = 0.5 * grad.double().sum(0)
+    # 24 bits (TF32 mode: 16); the third term of 1e-30 is a normal bf16
+    tol = 2.0 ** -22 if precision == 0 else 2.0 ** -16
+    assert bool(((db.double() - want).abs() <= tol * want.abs()).all())
 
 
 def test_expanded_gradient(gpu):
