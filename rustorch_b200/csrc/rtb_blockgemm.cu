@@ -5,8 +5,12 @@
 //                         + bias[n] ),  A and B e4m3 (kind::f8f6f4)
 //   MODE 1  D[k,n] (+)= sum_m X[m,k] Y[m,n],  X bf16, Y a sum of bf16 terms
 //                       (kind::f16): the weight gradient from a checkpoint
+//   MODE 2  as MODE 0 with e8m0 scales, applied by the tensor core
+//                       (kind::mxf8f6f4, see rtb_mxgemm.cu): a promotion every
+//                       1024 elements.  MODE 0 takes 1500 clocks a block, the
+//                       epilogue's chain of barrier, TMEM loads and adds.
 //
-// In both the MMAs of one 128-element block accumulate in TMEM and the
+// In the first two the MMAs of one 128-element block accumulate in TMEM and the
 // epilogue warps add the block's partial sum into fp32 registers on the CUDA
 // cores: MODE 0 because each block has scales of its own (one fused
 // multiply-add an element applies both), MODE 1 because the tensor core's own
@@ -17,8 +21,8 @@
 // (MMA N side).  Few tiles: a cluster of 2, 4 or 8 CTAs shares a tile, each a
 // part of the contraction, and adds the parts out of one another's shared
 // memory in rank order (no workspace, no counters, the same bits every time).
-// Roles (warp index): 0 TMA producer, 1 TMEM allocator + MMA issuer, 2..5
-// epilogue (TMEM lanes 32 (w % 4)..).  The accumulator is double buffered in
+// Roles (warp index): 0, 6, 7 TMA producers, 1 TMEM allocator + MMA issuer, 2..5
+// epilogue (TMEM lanes 32 (w % 4)..; MODE 2: they also lay out the scales).  The accumulator is double buffered in
 // TMEM, so the promotion of one block overlaps the MMAs of the next.  The
 // finished tile goes through shared memory (the idle load ring), so that its
 // stores run along the output's rows and bias, activation and the sum of the
@@ -42,16 +46,18 @@ constexpr int kXBytes = 128 * 128;     // X bytes of a stage (16 KB, both modes)
 constexpr int kSmemMax = 232448;       // dynamic shared memory per CTA
 constexpr int kReserve = 2048;         // barriers, alignment slack
 constexpr int kScaleUnits = 32;        // blocks whose scales are staged at a time
-constexpr int kThreads = 192;
+constexpr int kThreads = 256;
+constexpr int kSfUnits = 16;           // MODE 2: blocks of a scale buffer (there are two)
 
 template <int MODE, int BN, bool YVEC>
 struct Cfg {
-  static constexpr int kDepth = MODE == 0 ? 128 : 64;  // contraction elements of a stage
-  static constexpr int kPieces = MODE == 0 ? 1 : 3;
+  static constexpr int kDepth = MODE == 1 ? 64 : 128;  // contraction elements of a stage
+  static constexpr int kPieces = MODE == 1 ? 3 : 1;
   static constexpr int kYPiece = BN * 128;             // one Y piece of a stage (BN x 128 B)
   static constexpr int kStageBytes = kXBytes + kPieces * kYPiece;
   static constexpr int kSy = YVEC ? BN : 1;            // column scales of a block
-  static constexpr int kScaleBytes = MODE == 0 ? kScaleUnits * (128 + kSy) * 4 : 0;
+  static constexpr int kScaleBytes =
+      MODE == 0 ? kScaleUnits * (128 + kSy) * 4 : (MODE == 2 ? 2 * kSfUnits * 1024 : 0);
   static constexpr int kStagesRaw = (kSmemMax - kReserve - kScaleBytes) / kStageBytes;
   static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;
   static constexpr int kSmemBytes = kStages * kStageBytes + kScaleBytes + kReserve;
@@ -59,8 +65,12 @@ struct Cfg {
   // output's columns
   static_assert(kStages * kStageBytes >= 128 * (BN + 4) * 4 &&
                     kStages * kStageBytes >= BN * 132 * 4, "the ring holds the finished tile");
-  static constexpr int kPerUnit = 128 / kDepth;        // stages of a promotion unit
-  static constexpr int kTmemCols = 2 * BN < 32 ? 32 : 2 * BN;
+  static constexpr int kPerUnit = MODE == 0 ? 1 : (MODE == 1 ? 2 : 8);  // stages between promotions
+  static constexpr int kGrain = MODE == 1 ? 2 : 1;     // stages that parts are cut at
+  // MODE 2: two buffers of 4 + 4 scale columns behind the accumulators
+  static constexpr int kTmemNeed = 2 * BN + (MODE == 2 ? 16 : 0);
+  static constexpr int kTmemCols =
+      kTmemNeed <= 32 ? 32 : kTmemNeed <= 64 ? 64 : kTmemNeed <= 128 ? 128 : kTmemNeed <= 256 ? 256 : 512;
   static_assert(kStages >= 2, "two stages");
 };
 
@@ -84,6 +94,47 @@ __device__ __forceinline__ void mma_e(uint32_t d, uint64_t a, uint64_t b, uint32
         "l"(a), "l"(b), "r"(id), "r"(acc)
         : "memory");
   }
+}
+
+// MODE 2: a stage's two scale groups into TMEM, its four MMAs and its release,
+// by one elected lane (mx_stage_e in rtb_mxgemm.cu is the same for a pair).
+__device__ __forceinline__ void mx_stage1_e(uint32_t d, uint64_t a, uint64_t b, uint32_t id,
+                                            uint32_t sa, uint64_t cx, uint64_t cy, uint32_t acc,
+                                            uint64_t* empty) {
+  asm volatile(
+      "{\n\t.reg .pred p, t, e;\n\t.reg .b32 r, sb;\n\t"
+      ".reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+      "setp.ne.b32 p, %7, 0;\n\t"
+      "setp.eq.b32 t, 0, 0;\n\t"
+      "add.u32 sb, %4, 4;\n\t"
+      "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
+      "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
+      "elect.sync r|e, 0xffffffff;\n\t"
+      "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%4], %5;\n\t"
+      "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [sb], %6;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [sb], p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a1, b1, %3, [%4], [sb], t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a2, b2, %3, [%4], [sb], t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a3, b3, %3, [%4], [sb], t;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%8];\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(sa), "l"(cx), "l"(cy), "r"(acc), "r"(smem_u32(empty))
+      : "memory");
+}
+
+// MODE 2: the scale bytes of blocks u .. u + n - 1 (n <= 16) of row r as words of
+// the 512-byte groups that the tensor core takes (row l of a group: the word at
+// 16 (l % 32) + 4 (l / 32), its byte four times); 2^0 for rows past the operand.
+__device__ __forceinline__ void stage_scale_words(const ScaleRef& s, int64_t r, int64_t rows, int u,
+                                                  int n, uint8_t* group, int l) {
+  const bool in = r < rows;
+  const uint8_t* p = static_cast<const uint8_t*>(s.p) +
+                     (in ? (r >> s.row_shift) * s.ld_row + (int64_t)u * s.ld_col : 0);
+  uint32_t raw[kSfUnits];
+#pragma unroll
+  for (int k = 0; k < kSfUnits; ++k) raw[k] = in && k < n ? __ldg(p + (int64_t)k * s.ld_col) : 127u;
+#pragma unroll
+  for (int k = 0; k < kSfUnits; ++k)
+    *reinterpret_cast<uint32_t*>(group + 512 * k + 16 * (l & 31) + 4 * (l >> 5)) = raw[k] * 0x01010101u;
 }
 
 // The scales of blocks u .. u + n - 1 of row r, decoded, to dst[0], dst[step],
@@ -139,8 +190,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* empty = full + S;
   uint64_t* tfull = empty + S;
   uint64_t* tempty = tfull + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  uint64_t* sfull = tempty + 2;   // MODE 2: scale buffers
+  uint64_t* sempty = sfull + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sempty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint8_t* sf = reinterpret_cast<uint8_t*>(sx);  // MODE 2: [2][X, Y][kSfUnits][512]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -151,6 +205,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
       mbar_init(&tempty[b], 128);
+      mbar_init(&sfull[b], 128);
+      mbar_init(&sempty[b], 1);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -173,23 +229,26 @@ __global__ void __launch_bounds__(kThreads, 1)
   // the cluster's tile, and this CTA's part of the contraction
   const int parts = p.parts, rank = (int)blockIdx.x % parts, tile = (int)blockIdx.x / parts;
   const int tx = tile % p.tiles_x, ty = tile / p.tiles_x;
-  const int all = (p.stages_total + C::kPerUnit - 1) / C::kPerUnit;
-  const int u0 = (int)((int64_t)rank * all / parts), u1 = (int)((int64_t)(rank + 1) * all / parts);
-  const int units = u1 - u0;
-  const int i0 = u0 * C::kPerUnit;
-  const int i1 = u1 * C::kPerUnit < p.stages_total ? u1 * C::kPerUnit : p.stages_total;
+  const int all = (p.stages_total + C::kGrain - 1) / C::kGrain;
+  const int i0 = (int)((int64_t)rank * all / parts) * C::kGrain;
+  const int i1g = (int)((int64_t)(rank + 1) * all / parts) * C::kGrain;
+  const int i1 = i1g < p.stages_total ? i1g : p.stages_total;
+  const int nst = i1 - i0;
+  const int units = (nst + C::kPerUnit - 1) / C::kPerUnit;
 
-  if (warp == 0) {
+  if (warp == 0 || warp >= 6) {
     if (lane == 0) {
-      const uint32_t tx_bytes = kXBytes + (MODE == 0 ? 1 : p.pieces) * C::kYPiece;
-      for (int i = i0; i < i1; ++i) {
+      // three producers take the stages in turn: one thread's wait and issue
+      // takes longer than a stage's MMAs
+      const uint32_t tx_bytes = kXBytes + (MODE == 1 ? p.pieces : 1) * C::kYPiece;
+      for (int i = i0 + (warp ? warp - 5 : 0); i < i1; i += 3) {
         const int s = (i - i0) % S;
         if (!mbar_wait_bounded(&empty[s], (((i - i0) / S) & 1) ^ 1, abort_flag, p.err,
                                DEV_TIMEOUT_EMPTY, p.timeout_ns))
           break;
         uint8_t* st = base + s * C::kStageBytes;
         mbar_arrive_expect_tx(&full[s], tx_bytes);
-        if (MODE == 0) {
+        if (MODE != 1) {
           tma_load_2d(st, &tmX, &full[s], i * 128, tx * kX);
           tma_load_2d(st + kXBytes, &tmY, &full[s], i * 128, ty * BN);
         } else {
@@ -212,31 +271,48 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) got = mbar_wait_bounded(bar, parity, abort_flag, p.err, code, p.timeout_ns);
       return __shfl_sync(0xffffffffu, got, 0) != 0;
     };
-    for (int u = 0, i = i0; u < units && ok; ++u) {
+    // (lane 0) the next stage's operands were found ready before this stage's
+    // MMAs: a wait costs 200 clocks even when its barrier is complete
+    int next_full = 0;
+    for (int u = 0, i = 0; u < units && ok; ++u) {
       const int b = u & 1;
       const uint32_t d = tmem + (uint32_t)(b * BN);
-      for (int j = 0; j < C::kPerUnit && i < i1; ++j, ++i) {
-        const int s = (i - i0) % S;
-        if (!(ok = wait(&full[s], ((i - i0) / S) & 1, DEV_TIMEOUT_FULL))) break;
+      for (int j = 0; j < C::kPerUnit && i < nst; ++j, ++i) {
+        const int s = i % S;
+        if (!__shfl_sync(0xffffffffu, next_full, 0) &&
+            !(ok = wait(&full[s], (i / S) & 1, DEV_TIMEOUT_FULL)))
+          break;
         if (j == 0 && !(ok = wait(&tempty[b], ((u >> 1) & 1) ^ 1, DEV_TIMEOUT_TMEM_EMPTY))) break;
+        const int c = i / kSfUnits, k = i % kSfUnits;  // MODE 2: scale buffer c & 1, its block k
+        if (MODE == 2 && k == 0 && !(ok = wait(&sfull[c & 1], (c >> 1) & 1, DEV_TIMEOUT_LOADED)))
+          break;
         tc_fence_after();
+        if (lane == 0) next_full = mbar_test_wait(&full[(i + 1) % S], ((i + 1) / S) & 1);
         const uint32_t xa = smem_u32(base + s * C::kStageBytes), ya = xa + kXBytes;
         if (MODE == 0) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)  // 32 e4m3 (32 bytes of the swizzled row) a step
-            mma_e<0>(d, umma_desc(xa + 32 * k, 16, 1024, kLayoutSW128),
-                     umma_desc(ya + 32 * k, 16, 1024, kLayoutSW128), id, k > 0);
-        } else {
+          for (int q = 0; q < 4; ++q)  // 32 e4m3 (32 bytes of the swizzled row) a step
+            mma_e<0>(d, umma_desc(xa + 32 * q, 16, 1024, kLayoutSW128),
+                     umma_desc(ya + 32 * q, 16, 1024, kLayoutSW128), id, q > 0);
+          umma_commit_e(&empty[s]);
+        } else if (MODE == 1) {
           // the smallest terms first; 16 contraction rows (2 KB) a step, 8 KB
           // between 64-column boxes, 1 KB per 8 rows
           for (int q = p.pieces - 1; q >= 0; --q)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mma_e<1>(d, umma_desc(xa + 2048 * k, 8192, 1024, kLayoutSW128),
-                       umma_desc(ya + q * C::kYPiece + 2048 * k, 8192, 1024, kLayoutSW128), id,
-                       j > 0 || k > 0 || q < p.pieces - 1);
+            for (int r = 0; r < 4; ++r)
+              mma_e<1>(d, umma_desc(xa + 2048 * r, 8192, 1024, kLayoutSW128),
+                       umma_desc(ya + q * C::kYPiece + 2048 * r, 8192, 1024, kLayoutSW128), id,
+                       j > 0 || r > 0 || q < p.pieces - 1);
+          umma_commit_e(&empty[s]);
+        } else {
+          const uint32_t g = smem_u32(sf) + (uint32_t)((c & 1) * kSfUnits * 1024 + 512 * k);
+          mx_stage1_e(d, umma_desc(xa, 16, 1024, kLayoutSW128), umma_desc(ya, 16, 1024, kLayoutSW128),
+                      ((uint32_t)(BN >> 3) << 17) | (1u << 23) | ((uint32_t)(kX >> 4) << 24),
+                      tmem + 2 * BN + 8u * (uint32_t)(i & 1), umma_desc(g, 128, 128, 0),
+                      umma_desc(g + kSfUnits * 512, 128, 128, 0), j > 0, &empty[s]);
+          if (k == kSfUnits - 1) umma_commit_e(&sempty[c & 1]);
         }
-        umma_commit_e(&empty[s]);
       }
       if (!ok) break;
       umma_commit_e(&tfull[b]);
@@ -249,18 +325,40 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
     for (int j = 0; j < BN / 2; ++j) acc[j] = 0ull;
     bool ok = true;
+    // MODE 2: the scales of blocks kSfUnits c .. into buffer c & 1
+    auto scale_words = [&](int c) {
+      const int first = c * kSfUnits;
+      if (first >= nst) return;
+      if (c >= 2 && ok) {  // the buffer's MMAs before are done
+        int got = 0;
+        if (lane == 0)
+          got = mbar_wait_bounded(&sempty[c & 1], ((c >> 1) - 1) & 1, abort_flag, p.err,
+                                  DEV_TIMEOUT_EMPTY, p.timeout_ns);
+        ok = __shfl_sync(0xffffffffu, got, 0) != 0;
+      }
+      const int n = nst - first < kSfUnits ? nst - first : kSfUnits;
+      uint8_t* g = sf + (c & 1) * kSfUnits * 1024;
+      stage_scale_words(p.scx, (int64_t)tx * kX + et, p.xrows, i0 + first, n, g, et);
+      stage_scale_words(p.scy, (int64_t)ty * BN + et, et < BN ? p.ycols : 0, i0 + first, n,
+                        g + kSfUnits * 512, et);
+      fence_proxy_async_smem();  // the tensor core's copies read them
+      mbar_arrive(&sfull[c & 1]);
+    };
+    if (MODE == 2) scale_words(0);
     for (int u = 0; u < units; ++u) {
       const int b = u & 1;
+      // the next buffer, while this one's blocks are multiplied
+      if (MODE == 2 && u * C::kPerUnit % kSfUnits == 0) scale_words(u * C::kPerUnit / kSfUnits + 1);
       if (MODE == 0 && u % kScaleUnits == 0) {
         // the next blocks' scales, decoded, eight loads in flight a thread
         const int n = units - u < kScaleUnits ? units - u : kScaleUnits;
         named_bar_sync(1, 128);  // the blocks before are done with theirs
-        stage_scales(p.scx, (int64_t)tx * kX + et, p.xrows, u0 + u, n, sx + et, 128);
+        stage_scales(p.scx, (int64_t)tx * kX + et, p.xrows, i0 + u, n, sx + et, 128);
         if (YVEC) {
           if (et < BN)
-            stage_scales(p.scy, (int64_t)ty * BN + et, p.ycols, u0 + u, n, sy + et, C::kSy);
+            stage_scales(p.scy, (int64_t)ty * BN + et, p.ycols, i0 + u, n, sy + et, C::kSy);
         } else if (et < n) {
-          stage_scales(p.scy, (int64_t)ty * BN, p.ycols, u0 + u + et, 1, sy + et, 1);
+          stage_scales(p.scy, (int64_t)ty * BN, p.ycols, i0 + u + et, 1, sy + et, 1);
         }
         named_bar_sync(1, 128);
       }
@@ -285,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < 8; ++j) {
           const unsigned long long v = pack2(r[2 * j], r[2 * j + 1]);
           unsigned long long& a = acc[8 * c + j];
-          if (MODE == 1) a = add2(a, v);
+          if (MODE != 0) a = add2(a, v);
           else if (YVEC)
             a = fma2(mul2(v, s2), *reinterpret_cast<const unsigned long long*>(
                                       sy + us * C::kSy + 16 * c + 2 * j), a);
@@ -423,7 +521,7 @@ int launch(rtb_ctx* ctx, const CUtensorMap& tmX, const CUtensorMap& tmY, BlockPa
   p.stages_total = (p.depth + C::kDepth - 1) / C::kDepth;
   const int64_t tiles = (int64_t)p.tiles_x * p.tiles_y;
   if (tiles > INT32_MAX / 8) return set_error(RTB_E_UNSUPPORTED, "block gemm: too many tiles");
-  p.parts = pick_parts(ctx, tiles, (p.stages_total + C::kPerUnit - 1) / C::kPerUnit);
+  p.parts = pick_parts(ctx, tiles, (p.stages_total + C::kGrain - 1) / C::kGrain);
   p.vec_ok = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 && p.ldo % 4 == 0 &&
              (!p.bias || (reinterpret_cast<uintptr_t>(p.bias) & 15u) == 0);
   cudaLaunchConfig_t cfg = {};
@@ -499,6 +597,12 @@ int fp8_gemm_run(rtb_ctx* ctx, const Fp8Desc& d, cudaStream_t s) {
                                (uint64_t)(swap ? d.lda : d.ldb), 128, (uint32_t)bn)))
     return st;
   if (pairs) return launch_pair(ctx, 0, yvec, tmX, tmY, p, s);
+  if (!p.scx.is_f32 && !p.scy.is_f32) {
+    if (bn == 16) return launch<2, 16, false>(ctx, tmX, tmY, p, s);
+    if (bn == 32) return launch<2, 32, false>(ctx, tmX, tmY, p, s);
+    if (bn == 64) return launch<2, 64, false>(ctx, tmX, tmY, p, s);
+    return launch<2, 128, false>(ctx, tmX, tmY, p, s);
+  }
   if (bn == 16) return yvec ? launch<0, 16, true>(ctx, tmX, tmY, p, s) : launch<0, 16, false>(ctx, tmX, tmY, p, s);
   if (bn == 32) return yvec ? launch<0, 32, true>(ctx, tmX, tmY, p, s) : launch<0, 32, false>(ctx, tmX, tmY, p, s);
   if (bn == 64) return yvec ? launch<0, 64, true>(ctx, tmX, tmY, p, s) : launch<0, 64, false>(ctx, tmX, tmY, p, s);
