@@ -7,7 +7,11 @@ C ABI in include/rustorch_b200.h:
     ops.matmul_fused(lhs, rhs, bias, activation) rustorch-core/src/ops.rs:1543
     ops.conv2d(input, weight, stride, padding)   rustorch-core/src/ops/conv.rs:738
     nn.Linear / nn.Conv2d                        rustorch-nn/src/{linear,conv}.rs
+    layer_norm's autograd                        rustorch-core/src/ops/norm.rs:613
     jit.Graph / NodeType / Optimizer / Executor  rustorch-core/src/jit.rs
+
+Beyond the reference: 8-bit block-scaled tensors (fp8_quantize) as activation
+checkpoints and as operands of fp8_matmul.
 
 Tensors are torch CUDA float32 tensors (torch provides device memory and
 streams only; all arithmetic runs in this library's kernels).  Calls are

@@ -544,7 +544,11 @@ int launch(rtb_ctx* ctx, const CUtensorMap& tmX, const CUtensorMap& tmY, BlockPa
   return e == cudaSuccess ? RTB_OK : cuda_status(e, "block gemm launch");
 }
 
-// CTA pairs where their 256 x 256 tiles occupy most of the SMs.
+// CTA pairs where their 256 x 256 tiles occupy more than half of the SMs.
+// Measured, one CTA a tile against pairs: 512 x 4096 x 4096 (32 tiles) 23.1 us,
+// 24.9; 1024 x 2048 x 1024 (32) 13.8, 14.7; 1024 x 4096 x 4096 (64) 44.3, 26.0;
+// 2048 x 2048 x 512 (64) 23.2, 14.0; weight gradients with 32 and 64 tiles, 4096
+// rows, 72 us, 85, and 130, 92.  (RTB_PAIR=0 or 1 forces one, for measurements.)
 bool use_pairs(const rtb_ctx* ctx, const BlockParams& p) {
   static const int env = [] {
     const char* v = std::getenv("RTB_PAIR");
@@ -567,7 +571,8 @@ int fp8_gemm_run(rtb_ctx* ctx, const Fp8Desc& d, cudaStream_t s) {
   int st;
   if ((st = check_extents(d.M, d.N, d.K))) return st;
   // Few rows of A: the weight's rows fill the 128-row tile and A is the narrow
-  // side (C^T = B . A^T), so little of the tile is padding.
+  // side (C^T = B . A^T), so that at most 15 rows of 16, 31 of 64 are padding and
+  // not 64 of 128 (16 x 8192 x 8192: 19 us in a loop, 3.5 TB/s of the weight).
   const bool swap = d.M <= 64;
   BlockParams p{};
   p.xrows = swap ? d.N : d.M;

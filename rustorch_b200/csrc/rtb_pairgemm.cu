@@ -14,6 +14,11 @@
 // that is 32768 multiply-adds per 512 clocks of MMAs, half of the SM's fp32
 // lanes; packed f32x2 instructions halve the issue slots.
 //
+// Measured: MODE 0 (f32 scales) 8192 x 4096 x 8192 in 370 us, 1490 TFLOP/s, bound
+// by the epilogue's chain of barrier, TMEM loads and adds (about 1150 clocks a
+// block); MODE 1 8192 x 4096 x 4096 in 550 us beside 60 us for its operands, 1.5
+// PFLOP/s of bf16 MMAs, bound by them.
+//
 // Roles (warps of each CTA): 0, 2, 3 TMA producers; 1 TMEM allocation, and in the
 // pair's first CTA the MMA issue for both; 4..11 epilogue (lanes 32 (w % 4)..,
 // columns 128 ((w - 4) / 4)..).  The first warpgroup hands registers to the
