@@ -22,8 +22,8 @@
 // part of the contraction, and adds the parts out of one another's shared
 // memory in rank order (no workspace, no counters, the same bits every time).
 // Roles (warp index): 0, 6, 7 TMA producers, 1 TMEM allocator + MMA issuer, 2..5
-// epilogue (TMEM lanes 32 (w % 4)..; MODE 2: they also lay out the scales).  The accumulator is double buffered in
-// TMEM, so the promotion of one block overlaps the MMAs of the next.  The
+// epilogue (TMEM lanes 32 (w % 4)..; MODE 2: they also lay out the scales).  The
+// accumulator is double buffered in TMEM, so the promotion of one block overlaps the MMAs of the next.  The
 // finished tile goes through shared memory (the idle load ring), so that its
 // stores run along the output's rows and bias, activation and the sum of the
 // parts are one short loop.  Every wait is bounded: after a timeout a role goes
@@ -31,7 +31,7 @@
 // output is undefined and the error word tells the host.
 //
 // Shared memory (128-byte swizzle throughout):
-//   MODE 0, K-major: row r at r * 128 B holds 128 e4m3 of the contraction.
+//   MODE 0, 2, K-major: row r at r * 128 B holds 128 e4m3 of the contraction.
 //   MODE 1, MN-major: boxes of 64 contraction rows x 64 bf16 (8 KB).
 #include <cstdlib>
 

@@ -1,10 +1,11 @@
 // Shared by the block-scaled product kernels (rtb_blockgemm.cu: one CTA a tile;
-// rtb_pairgemm.cu: two CTAs a tile): parameters, scales, instruction
-// descriptors, packed fp32 arithmetic.
+// rtb_pairgemm.cu, rtb_mxgemm.cu: two CTAs a tile): parameters, scales, instruction
+// descriptors.
 #pragma once
 #include <cuda.h>
 
 #include "rtb_act.cuh"
+#include "rtb_f32x2.cuh"
 #include "rtb_fp8.cuh"
 #include "rtb_internal.h"
 #include "rtb_ptx.cuh"
@@ -71,40 +72,6 @@ __device__ __forceinline__ void tmem_wait_x16(uint32_t (&r)[16]) {
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
                  "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
                  "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
-}
-
-// Two fp32 values in one 64-bit register: one instruction adds or multiplies
-// both.
-__device__ __forceinline__ unsigned long long pack2(float lo, float hi) {
-  unsigned long long v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
-  return v;
-}
-__device__ __forceinline__ unsigned long long pack2(uint32_t lo, uint32_t hi) {
-  unsigned long long v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
-  return v;
-}
-__device__ __forceinline__ float2 unpack2(unsigned long long v) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-  return f;
-}
-__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b,
-                                                   unsigned long long c) {
-  unsigned long long d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
-  unsigned long long d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
-  unsigned long long d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
 }
 
 // Blocks in a scale table of `units` blocks: whole quads and one more, so that

@@ -6,13 +6,15 @@
 // The scales enter inside the MMA, so a partial sum has to leave the tensor core
 // only for the accumulation's sake, every 1024 or 2048 elements (the tensor core
 // does not round each addition to nearest: the error grows with the chain, 9e-8
-// relative after 32 steps) instead of every 128: the epilogue's chain of barrier, TMEM loads and adds, 1150
-// clocks against 512 of MMAs in rtb_pairgemm.cu, is out of the way.
+// relative after 32 steps) instead of every 128: the epilogue's chain of barrier,
+// TMEM loads and adds, 1150 clocks against 512 of MMAs in rtb_pairgemm.cu, is out
+// of the way.
 //
-// Tile 256 x 224 or 256 x 192 (two accumulators leave columns of TMEM for the
-// scales), whichever takes less time in whole rounds of the pairs.  Roles (warps of each CTA): 0, 2, 3 TMA producers; 1 TMEM allocation, and
-// in the pair's first CTA the issue for both; 4..11 epilogue (lanes 32 (w % 4)..,
-// one half of the columns).
+// Tile 256 x 256 with one accumulator or 256 x 224 with two (the scales need
+// columns of TMEM too), whichever takes less time in whole rounds of the pairs.
+// Roles (warps of each CTA): 0, 2, 3 TMA producers; 1 TMEM allocation, and in the
+// pair's first CTA the issue for both; 4..11 epilogue (lanes 32 (w % 4).., one
+// half of the columns).
 //
 // Scales: a kernel before lays them out once per call as 512-byte groups of 128
 // rows for each block (row r: the 32-bit word at 16 (r % 32) + 4 (r / 32), its

@@ -16,10 +16,11 @@
 // kernel.  No atomics: the order depends on the shape alone.  A single CTA writes
 // its sums itself.  Rows beyond 16384 columns take a CTA each and three passes.
 //
-// Measured: 8192 x 4096 80 us (5.0 TB/s of the 12 bytes an element, 77% of a copy),
-// 16384 x 2048 from a checkpoint 77 us (3.9 TB/s of 9 bytes: the instructions of
-// the row's fixed part count as much), 2048 x 16384 111 us, 8192 x 4097 140 us.
+// Measured: 8192 x 4096 75 us (5.4 TB/s of the 12 bytes an element, 82% of a copy),
+// 16384 x 2048 from a checkpoint 67 us (4.5 TB/s of 9 bytes: the instructions of
+// the row's fixed part count as much), 2048 x 16384 111 us, 8192 x 4097 129 us.
 #include "rtb_act.cuh"
+#include "rtb_f32x2.cuh"
 #include "rtb_fp8.cuh"
 #include "rtb_internal.h"
 #include "rtb_ptx.cuh"
@@ -144,6 +145,40 @@ constexpr int kRing = 3;  // stages of the row ring: 96 KB for 512 threads of 8 
 __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
+__device__ __forceinline__ uint32_t lds_u8(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void sts_u8(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared.u8 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+// A row of `bytes` bytes at any address into shared memory, at the same offset
+// from a 16-byte boundary: T threads take its 16-byte chunks (N each at most) in
+// turn.  Chunks that reach over [lo, hi), the tensor, go byte by byte.
+template <int N>
+__device__ __forceinline__ void copy_row(uint32_t dst, const void* row, int bytes, const void* lo,
+                                         const void* hi, int t, int T) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(row), a0 = a & ~uintptr_t(15);
+  const uintptr_t l = reinterpret_cast<uintptr_t>(lo), h = reinterpret_cast<uintptr_t>(hi);
+  const int chunks = ((int)(a - a0) + bytes + 15) >> 4;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int c = t + i * T;
+    if (c >= chunks) continue;
+    const uintptr_t g = a0 + 16 * c;
+    if (g >= l && g + 16 <= h) {
+      cp_async_16_cg(dst + 16 * c, reinterpret_cast<const void*>(g));
+    } else {
+#pragma unroll 1
+      for (int b = 0; b < 16; ++b)
+        if (g + b >= l && g + b < h)
+          sts_u8(dst + 16 * c + b, *reinterpret_cast<const uint8_t*>(g + b));
+    }
+  }
+}
+
 // Up to 8192 columns: T threads a row (a multiple of 32), E values of x and of
 // dy each: lane l of the group's warp w holds the units 32 G w + l + 32 i, i <
 // G, where a unit is a float4 (VEC: d % 4 == 0, 16-byte aligned rows) or a
@@ -155,84 +190,127 @@ __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
 // once it has used the values: no barrier is needed for the ring.  Eight values
 // a thread (five registers each) leave room for 1024 threads on an SM, whose
 // number, not the bytes in flight, hides the row's chain of loads, sums,
-// shuffles and one barrier; what bounds it then is HBM.  Other rows are loaded
-// into registers directly: copies of 4 bytes cost more than they hide.
-template <int kBlock, int E, bool VEC, bool SAVED, bool ACT>
+// shuffles and one barrier.  The arithmetic is packed, two values an
+// instruction; FULL: every thread has all of its units, and nothing asks (8192 x
+// 4096 78 -> 75 us, from a checkpoint 84 -> 71, 4096 x 8192 83 -> 74 by both).
+//
+// Rows off the 16-byte boundaries: the threads copy the row's aligned chunks for
+// one another, and the barrier of a row's sums also publishes the next row (from
+// a checkpoint 8192 x 4097: 349 us by direct loads, 160 here; 65536 x 301: 167,
+// 102; fp32 x 8192 x 4097, one group on an SM: 133, 129).  fp32 rows of up to 4096
+// columns are loaded into registers directly: with more groups on an SM the
+// copies cost more than they hide (65536 x 301: 63 us, 88 by copies; 1531 x 1001
+// with tanh 14.3, 16.7).
+template <int kBlock, bool VEC, bool SAVED>
+constexpr bool kRows = VEC || SAVED || kBlock > 512;  // rows through the ring
+
+template <int kBlock, int E, bool VEC, bool SAVED, bool ACT, bool FULL>
 __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
     norm_bwd_rows_kernel(const NormBwdParams p, const int T, const float inv_d, float* dg,
                          float* db) {
   constexpr int G = VEC ? E / 4 : E;  // copies of x (and of dy) a thread
   constexpr int C = E / G;            // columns of a copy
+  constexpr int P = E / 2;            // pairs of values
+  constexpr bool RING = kRows<kBlock, VEC, SAVED>, SHARED = RING && !VEC;
+  constexpr bool kAhead = SAVED && (kBlock > 512 || !VEC);  // block scales a row ahead
   __shared__ float red[2][kBlock / 32][2];
   extern __shared__ float4 ring4[];   // the ring, then reused for the CTA's sums
   const int R = kBlock / T;           // rows a CTA works on
   const int grp = threadIdx.x / T, t = threadIdx.x - grp * T;
   const int units = VEC ? p.d >> 2 : p.d;
   const int k0 = (t >> 5) * (32 * G) + (t & 31);  // this thread's first unit
-  const int rem = units - k0;                     // its unit i exists if 32 i < rem
+  const int rem = FULL ? 32 * G : units - k0;     // its unit i exists if 32 i < rem
   const bool sums = p.part || dg || db;
   // a slot: x, then dy, both on 16-byte boundaries
-  const int xbytes = ((SAVED ? units * 4 : units * C * 4) + 15) & ~15;
-  const int row_bytes = xbytes + ((units * C * 4 + 15) & ~15);
+  const int xrow = SAVED ? units * C : units * C * 4, yrow = units * C * 4;  // bytes of a row
+  const int xbytes = (xrow + (VEC ? 15 : 30)) & ~15;
+  const int row_bytes = xbytes + ((yrow + (VEC ? 15 : 30)) & ~15);
   const uint32_t slot0 = smem_u32(ring4) + (uint32_t)(grp * kRing * row_bytes);
   constexpr bool kKeep = VEC && !ACT;  // the weight stays in registers
-  float ag[E], ab[E], gw[kKeep ? E : 1];
+  unsigned long long ag[P], ab[P], gw[kKeep ? P : 1];
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    ag[i] = ab[i] = 0.0f;
-    if (kKeep) gw[i] = 1.0f;
+  for (int i = 0; i < P; ++i) {
+    ag[i] = ab[i] = 0ull;
+    if (kKeep) gw[i] = pack2(1.0f, 1.0f);
   }
+  // the pair of a column vector's values that belongs to values 2 i, 2 i + 1
+  auto columns = [&](const float* v, int i, float none) {
+    const bool in0 = 32 * (2 * i / C) < rem, in1 = 32 * ((2 * i + 1) / C) < rem;
+    return pack2(v && in0 ? __ldg(v + C * (k0 + 32 * (2 * i / C)) + 2 * i % C) : none,
+                 v && in1 ? __ldg(v + C * (k0 + 32 * ((2 * i + 1) / C)) + (2 * i + 1) % C) : none);
+  };
   griddep_wait();
   griddep_launch_dependents();
   if (kKeep && p.g) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      if (32 * (i / C) < rem) gw[i] = __ldg(p.g + C * (k0 + 32 * (i / C)) + i % C);
-    }
+    for (int i = 0; i < P; ++i) gw[i] = columns(p.g, i, 1.0f);
   }
   // rows and leading dimensions fit 32 bits (checked by the host), so that a
   // row's address is one multiply-add
   const int rows = (int)p.rows, step = (int)gridDim.x * R;
   const int ldx = (int)p.ldx, ldq = (int)p.ldq, lds = (int)p.lds, lddy = (int)p.lddy,
             lddx = (int)p.lddx;
+  auto xrow_at = [&](int r) {
+    return SAVED ? reinterpret_cast<const char*>(p.q + (int64_t)r * ldq)
+                 : reinterpret_cast<const char*>(p.x + (int64_t)r * ldx);
+  };
+  auto yrow_at = [&](int r) { return reinterpret_cast<const char*>(p.dy + (int64_t)r * lddy); };
   auto fetch = [&](int r, int s) {
     if (r < rows) {
-      const uint32_t xs = slot0 + (uint32_t)(s * row_bytes + (SAVED ? 4 : 16) * k0);
-      const uint32_t ys = slot0 + (uint32_t)(s * row_bytes + xbytes + 16 * k0);
-      const char* xr = SAVED ? reinterpret_cast<const char*>(p.q + (int64_t)r * ldq + 4 * k0)
-                             : reinterpret_cast<const char*>(p.x + (int64_t)r * ldx + 4 * k0);
-      const char* yr = reinterpret_cast<const char*>(p.dy + (int64_t)r * lddy + 4 * k0);
+      if (VEC) {
+        const uint32_t xs = slot0 + (uint32_t)(s * row_bytes + (SAVED ? 4 : 16) * k0);
+        const uint32_t ys = slot0 + (uint32_t)(s * row_bytes + xbytes + 16 * k0);
+        const char* xr = SAVED ? reinterpret_cast<const char*>(p.q + (int64_t)r * ldq + 4 * k0)
+                               : reinterpret_cast<const char*>(p.x + (int64_t)r * ldx + 4 * k0);
+        const char* yr = reinterpret_cast<const char*>(p.dy + (int64_t)r * lddy + 4 * k0);
 #pragma unroll
-      for (int i = 0; i < G; ++i) {
-        if (32 * i < rem) {
-          if (SAVED) cp_async_4(xs + 128 * i, xr + 128 * i);
-          else cp_async_16_cg(xs + 512 * i, xr + 512 * i);
-          cp_async_16_cg(ys + 512 * i, yr + 512 * i);
+        for (int i = 0; i < G; ++i) {
+          if (32 * i < rem) {
+            if (SAVED) cp_async_4(xs + 128 * i, xr + 128 * i);
+            else cp_async_16_cg(xs + 512 * i, xr + 512 * i);
+            cp_async_16_cg(ys + 512 * i, yr + 512 * i);
+          }
         }
+      } else {
+        const uint32_t xs = slot0 + (uint32_t)(s * row_bytes), ys = xs + (uint32_t)xbytes;
+        const char *xr = xrow_at(r), *yr = yrow_at(r);
+        copy_row<SAVED ? 1 : E / 4 + 1>(xs, xr, xrow, xrow_at(0), xrow_at(rows - 1) + xrow, t, T);
+        copy_row<E / 4 + 1>(ys, yr, yrow, yrow_at(0), yrow_at(rows - 1) + yrow, t, T);
       }
     }
     cp_async_commit();  // (an empty group behind the last row)
   };
   int r = grp < R ? (int)blockIdx.x * R + grp : rows;
-  if (VEC)
+  if (RING)
     for (int s = 0; s < kRing; ++s) fetch(r + s * step, s);
+  // a thread's block scales of a row
+  constexpr int NS = !SAVED ? 1 : VEC ? G : G / 4;
+  auto scales = [&](int r, uint32_t (&sb)[NS]) {
+    const uint8_t* sr = p.scale + (int64_t)r * lds + (t >> 5) * NS;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) sb[i] = SAVED && (VEC ? 32 : 128) * i < rem ? __ldg(sr + i) : 0u;
+  };
   float mean = 0.0f, rstd = 0.0f;
+  uint32_t sb[NS] = {};
   if (r < rows) {
     mean = __ldg(p.mean + r);
     rstd = __ldg(p.rstd + r);
+    if (kAhead) scales(r, sb);
+    if (SHARED) {
+      cp_async_wait<kRing - 1>();
+      if (T > 32) named_bar_sync(1 + grp, T);
+      else __syncwarp();
+    }
   }
   int slot = 0, phase = 0;
   for (; r < rows; r += step, phase ^= 1) {
-    // the next row's statistics and this row's block scales
+    // the next row's statistics and block scales
     const int rn = r + step < rows ? r + step : r;
     const float mean_n = __ldg(p.mean + rn), rstd_n = __ldg(p.rstd + rn);
-    uint32_t sb[VEC ? G : 1];
-    if (SAVED && VEC) {
-      const uint8_t* sr = p.scale + (int64_t)r * lds + (t >> 5) * G;  // one byte for 32 units
-#pragma unroll
-      for (int i = 0; i < G; ++i) sb[i] = 32 * i < rem ? __ldg(sr + i) : 0u;
-    }
-    float u[E], h[E];  // x, then u; dy, then h
+    uint32_t sb_n[NS] = {};
+    if (kAhead) scales(rn, sb_n);
+    else if (SAVED) scales(r, sb);
+    unsigned long long u[P], h[P];  // x, then u; dy, then h
     if (VEC) {
       cp_async_wait<kRing - 1>();  // this slot's copies, the oldest group, have landed
       const uint32_t xs = slot0 + (uint32_t)(slot * row_bytes + (SAVED ? 4 : 16) * k0);
@@ -241,65 +319,70 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
       for (int i = 0; i < G; ++i) {
         float4 a = make_float4(mean, mean, mean, mean), g = make_float4(0.f, 0.f, 0.f, 0.f);
         if (32 * i < rem) {
-          if (SAVED) {
-            a = e4m3x4_to_float4(__float_as_uint(lds32(xs + 128 * i)));
-            const float s = e8m0_to_float(sb[i]);
-            a.x *= s; a.y *= s; a.z *= s; a.w *= s;
-          } else {
-            a = lds128(xs + 512 * i);
-          }
+          if (SAVED) a = e4m3x4_to_float4(__float_as_uint(lds32(xs + 128 * i)));
+          else a = lds128(xs + 512 * i);
           g = lds128(ys + 512 * i);
         }
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-          u[C * i + c] = (&a.x)[c];
-          h[C * i + c] = (&g.x)[c];
+        u[2 * i] = pack2(a.x, a.y);
+        u[2 * i + 1] = pack2(a.z, a.w);
+        if (SAVED && 32 * i < rem) {
+          const float s = e8m0_to_float(sb[i]);
+          u[2 * i] = mul2(u[2 * i], pack2(s, s));
+          u[2 * i + 1] = mul2(u[2 * i + 1], pack2(s, s));
         }
+        h[2 * i] = pack2(g.x, g.y);
+        h[2 * i + 1] = pack2(g.z, g.w);
       }
     } else {
-      const float* yr = p.dy + (int64_t)r * lddy + k0;
       const float* xr = p.x + (int64_t)r * ldx + k0;
-      const uint8_t* qr = p.q + (int64_t)r * ldq + k0;
+      const float* yr = p.dy + (int64_t)r * lddy + k0;
+      uint32_t xs = 0, ys = 0;
+      if (SHARED) {
+        xs = slot0 + (uint32_t)(slot * row_bytes) + (SAVED ? 1 : 4) * k0;
+        ys = slot0 + (uint32_t)(slot * row_bytes + xbytes) + 4 * k0;
+        xs += (uint32_t)(reinterpret_cast<uintptr_t>(xrow_at(r)) & 15u);
+        ys += (uint32_t)(reinterpret_cast<uintptr_t>(yrow_at(r)) & 15u);
+      }
+      float a[E], g[E];
 #pragma unroll
       for (int i = 0; i < G; ++i) {
-        u[i] = mean;
-        h[i] = 0.0f;
-        uint32_t code = 0, byte = 0;
+        a[i] = mean;
+        g[i] = 0.0f;
         if (32 * i < rem) {
-          if (SAVED) {
-            code = __ldcs(qr + 32 * i);
-            byte = __ldg(p.scale + (int64_t)r * lds + (k0 + 32 * i) / kFp8Block);
-          } else {
-            u[i] = __ldcs(xr + 32 * i);
-          }
-          h[i] = __ldcs(yr + 32 * i);
+          if (SAVED) a[i] = e4m3x2_to_float2(lds_u8(xs + 32 * i)).x * e8m0_to_float(sb[i / 4 % NS]);
+          else a[i] = SHARED ? lds32(xs + 128 * i) : __ldcs(xr + 32 * i);
+          g[i] = SHARED ? lds32(ys + 128 * i) : __ldcs(yr + 32 * i);
         }
-        if (SAVED && 32 * i < rem) u[i] = e4m3x2_to_float2(code).x * e8m0_to_float(byte);
       }
-    }
-    float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      u[i] = (u[i] - mean) * rstd;
-      const int j = C * (k0 + 32 * (i / C)) + i % C;
-      float gv = 1.0f;
-      if (kKeep) gv = gw[i];
-      else if (p.g && 32 * (i / C) < rem) gv = __ldg(p.g + j);
-      if (ACT) {
-        const float bv = p.b && 32 * (i / C) < rem ? __ldg(p.b + j) : 0.0f;
-        h[i] *= act_slope(fmaf(u[i], gv, bv), p.act);
+      for (int i = 0; i < P; ++i) {
+        u[i] = pack2(a[2 * i], a[2 * i + 1]);
+        h[i] = pack2(g[2 * i], g[2 * i + 1]);
       }
-      ag[i] = fmaf(h[i], u[i], ag[i]);
-      ab[i] += h[i];
-      h[i] *= gv;
-      s1 += h[i];
-      s2 = fmaf(h[i], u[i], s2);
     }
-    if (VEC) {
-      fetch(r + kRing * step, slot);  // every value of the slot is in registers
+    unsigned long long t1 = 0ull, t2 = 0ull;
+    const unsigned long long rs = pack2(rstd, rstd), nm = pack2(-mean, -mean);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      u[i] = mul2(add2(u[i], nm), rs);
+      const unsigned long long gv = kKeep ? gw[kKeep ? i : 0] : columns(p.g, i, 1.0f);
+      if (ACT) {
+        const float2 z = unpack2(fma2(u[i], gv, columns(p.b, i, 0.0f)));
+        h[i] = mul2(h[i], pack2(act_slope(z.x, p.act), act_slope(z.y, p.act)));
+      }
+      ag[i] = fma2(h[i], u[i], ag[i]);
+      ab[i] = add2(ab[i], h[i]);
+      h[i] = mul2(h[i], gv);
+      t1 = add2(t1, h[i]);
+      t2 = fma2(h[i], u[i], t2);
+    }
+    float s1 = unpack2(t1).x + unpack2(t1).y, s2 = unpack2(t2).x + unpack2(t2).y;
+    auto refill = [&] {
+      fetch(r + kRing * step, slot);
       if (++slot == kRing) slot = 0;
-    }
-    if (p.dx) {
+    };
+    if (VEC) refill();  // every value of the slot is in registers
+    if (p.dx || SHARED) {
       // Both sums at once: the half-warps exchange, then lanes 0..15 add up the
       // first sum and lanes 16..31 the second.
       const bool second = t & 16;
@@ -307,6 +390,7 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
       v += __shfl_xor_sync(0xffffffffu, second ? s1 : s2, 16);
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (SHARED) cp_async_wait<kRing - 2>();  // this thread's copies of the next row
       if (T > 32) {
         // two buffers, so that one barrier a row is enough; every warp adds the
         // warps' sums for itself, in the same order
@@ -317,32 +401,46 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
         if (kBlock > 512 && l + 16 < nw) v += red[phase][w0 + 16 + l][second];
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      } else if (SHARED) {
+        __syncwarp();
       }
+      if (SHARED) refill();  // every thread of the group has used the slot
       s1 = __shfl_sync(0xffffffffu, v, 0);
       s2 = __shfl_sync(0xffffffffu, v, 16);
-      const float m1 = s1 * inv_d, m2 = s2 * inv_d;
+      const unsigned long long m1 = pack2(-s1 * inv_d, -s1 * inv_d), m2 = pack2(-s2 * inv_d, -s2 * inv_d);
       float* dxr = p.dx + (int64_t)r * lddx + C * k0;
 #pragma unroll
-      for (int i = 0; i < G; ++i) {
-        if (32 * i >= rem) continue;
-        float4 w;
+      for (int i = 0; i < P; ++i) u[i] = mul2(rs, fma2(u[i], m2, add2(h[i], m1)));
+      if (SHARED && !p.dx) {
+        // (only the sums were asked for)
+      } else if (VEC) {
+        float4* o = reinterpret_cast<float4*>(dxr);
+        if (p.accumulate) {
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-          (&w.x)[c] = rstd * fmaf(-u[C * i + c], m2, h[C * i + c] - m1);
-        if (VEC) {
-          float4* o = reinterpret_cast<float4*>(dxr) + 32 * i;
-          if (p.accumulate) {
-            const float4 q = *o;
-            w.x += q.x; w.y += q.y; w.z += q.z; w.w += q.w;
+          for (int i = 0; i < G; ++i) {
+            if (32 * i >= rem) continue;
+            const float4 q = o[32 * i];
+            u[2 * i] = add2(pack2(q.x, q.y), u[2 * i]);
+            u[2 * i + 1] = add2(pack2(q.z, q.w), u[2 * i + 1]);
           }
-          __stcs(o, w);
-        } else {
-          put(dxr + 32 * i, w.x, p.accumulate);
+        }
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+          const float2 a = unpack2(u[2 * i]), b = unpack2(u[2 * i + 1]);
+          if (32 * i < rem) __stcs(o + 32 * i, make_float4(a.x, a.y, b.x, b.y));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+          const float2 a = unpack2(u[i / 2]);
+          if (32 * i < rem) put(dxr + 32 * i, i % 2 ? a.y : a.x, p.accumulate);
         }
       }
     }
     mean = mean_n;
     rstd = rstd_n;
+#pragma unroll
+    for (int i = 0; i < (kAhead ? NS : 0); ++i) sb[i] = sb_n[i];
   }
   cp_async_wait<0>();
   if (!sums) return;
@@ -355,8 +453,9 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
       for (int i = 0; i < E; ++i) {
         if (32 * (i / C) >= rem) continue;
         const int j = C * (k0 + 32 * (i / C)) + i % C;
-        put(acc_s + j, ag[i], gi > 0);
-        put(acc_s + p.d + j, ab[i], gi > 0);
+        const float2 a = unpack2(ag[i / 2]), b = unpack2(ab[i / 2]);
+        put(acc_s + j, i % 2 ? a.y : a.x, gi > 0);
+        put(acc_s + p.d + j, i % 2 ? b.y : b.x, gi > 0);
       }
     }
     __syncthreads();
@@ -373,40 +472,36 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
   }
 }
 
-// Rows of 8193 to 16384 columns: 1024 threads with 16 values each, loaded
+// Rows of 8193 to 16384 columns: a CTA of 1024 threads with 16 values each, loaded
 // straight into registers; the sums for dg and db, for which 64 registers a
 // thread leave no room, in shared memory.
-template <int T, int E, bool VEC, bool SAVED>
-__global__ void __launch_bounds__(T > 256 ? T : 256, T > 512 ? 1 : (T > 256 ? 1 : 2))
+constexpr int kWide = 1024;
+
+template <bool VEC, bool SAVED>
+__global__ void __launch_bounds__(kWide, 1)
     norm_bwd_direct_kernel(const NormBwdParams p, float* dg, float* db) {
-  constexpr int kBlock = T > 256 ? T : 256;
-  constexpr int G = VEC ? E / 4 : E;  // loads of x (and of dy) a thread
-  constexpr int C = E / G;            // columns of a load
-  constexpr int R = kBlock / T;       // rows a CTA works on
-  constexpr int W = T / 32;
-  constexpr bool kAccSmem = T == 1024;
-  __shared__ float red[2][R][W][2];
-  extern __shared__ float acc_s[];  // [2][d]: the CTA's sums (kAccSmem: running)
+  constexpr int E = 16, G = VEC ? E / 4 : E;  // values, loads of x (and of dy) a thread
+  constexpr int C = E / G;                    // columns of a load
+  constexpr int W = kWide / 32;
+  __shared__ float red[2][W][2];
+  extern __shared__ float acc_s[];  // [2][d]: the CTA's running sums
   griddep_wait();
   griddep_launch_dependents();
-  const int t = threadIdx.x % T, grp = threadIdx.x / T;
+  const int t = threadIdx.x;
   const int units = VEC ? p.d >> 2 : p.d;
   const bool sums = p.part || dg || db;
-  float ag[kAccSmem ? 1 : E], ab[kAccSmem ? 1 : E];
-#pragma unroll
-  for (int i = 0; i < (kAccSmem ? 1 : E); ++i) ag[i] = ab[i] = 0.0f;
-  if (kAccSmem && sums) {
-    for (int j = threadIdx.x; j < 2 * p.d; j += kBlock) acc_s[j] = 0.0f;
+  if (sums) {
+    for (int j = t; j < 2 * p.d; j += kWide) acc_s[j] = 0.0f;
     __syncthreads();
   }
   int phase = 0;
-  for (int64_t r = (int64_t)blockIdx.x * R + grp; r < p.rows; r += (int64_t)gridDim.x * R, phase ^= 1) {
+  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x, phase ^= 1) {
     float u[E], h[E];  // x, then u; dy, then h
     const float mean = __ldg(p.mean + r), rstd = __ldg(p.rstd + r);
     const float* dyr = p.dy + r * p.lddy;
 #pragma unroll
     for (int i = 0; i < G; ++i) {
-      const int k = t + T * i;
+      const int k = t + kWide * i;
       const bool in = k < units;
       if (VEC) {
         float4 a = make_float4(mean, mean, mean, mean), g = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -440,7 +535,7 @@ __global__ void __launch_bounds__(T > 256 ? T : 256, T > 512 ? 1 : (T > 256 ? 1 
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int i = 0; i < G; ++i) {
-      const int k = t + T * i;
+      const int k = t + kWide * i;
       float gv[C], bv[C];
 #pragma unroll
       for (int c = 0; c < C; ++c) {
@@ -457,8 +552,9 @@ __global__ void __launch_bounds__(T > 256 ? T : 256, T > 512 ? 1 : (T > 256 ? 1 
           if (p.b && p.act != RTB_ACT_NONE) bv[0] = __ldg(p.b + k);
         }
       }
+      const bool add = sums && k < units;
       float4 sg, sb;
-      if (kAccSmem && sums && k < units && VEC) {
+      if (add && VEC) {
         sg = reinterpret_cast<const float4*>(acc_s)[k];
         sb = reinterpret_cast<const float4*>(acc_s + p.d)[k];
       }
@@ -468,23 +564,18 @@ __global__ void __launch_bounds__(T > 256 ? T : 256, T > 512 ? 1 : (T > 256 ? 1 
         u[e] = (u[e] - mean) * rstd;
         float dz = h[e];
         if (p.act != RTB_ACT_NONE) dz *= act_slope(fmaf(u[e], gv[c], bv[c]), p.act);
-        if (!kAccSmem) {
-          ag[e] = fmaf(dz, u[e], ag[e]);
-          ab[e] += dz;
-        } else if (sums && k < units) {
-          if (VEC) {
-            (&sg.x)[c] = fmaf(dz, u[e], (&sg.x)[c]);
-            (&sb.x)[c] += dz;
-          } else {
-            acc_s[k] = fmaf(dz, u[e], acc_s[k]);
-            acc_s[p.d + k] += dz;
-          }
+        if (add && VEC) {
+          (&sg.x)[c] = fmaf(dz, u[e], (&sg.x)[c]);
+          (&sb.x)[c] += dz;
+        } else if (add) {
+          acc_s[k] = fmaf(dz, u[e], acc_s[k]);
+          acc_s[p.d + k] += dz;
         }
         h[e] = dz * gv[c];
         s1 += h[e];
         s2 = fmaf(h[e], u[e], s2);
       }
-      if (kAccSmem && sums && k < units && VEC) {
+      if (add && VEC) {
         reinterpret_cast<float4*>(acc_s)[k] = sg;
         reinterpret_cast<float4*>(acc_s + p.d)[k] = sb;
       }
@@ -495,25 +586,23 @@ __global__ void __launch_bounds__(T > 256 ? T : 256, T > 512 ? 1 : (T > 256 ? 1 
       s1 += __shfl_xor_sync(0xffffffffu, s1, o);
       s2 += __shfl_xor_sync(0xffffffffu, s2, o);
     }
-    if (W > 1) {
-      // two buffers, so that one barrier a row is enough
-      if ((t & 31) == 0) {
-        red[phase][grp][t >> 5][0] = s1;
-        red[phase][grp][t >> 5][1] = s2;
-      }
-      named_bar_sync(1 + grp, T);
-      s1 = s2 = 0.0f;
+    // two buffers, so that one barrier a row is enough
+    if ((t & 31) == 0) {
+      red[phase][t >> 5][0] = s1;
+      red[phase][t >> 5][1] = s2;
+    }
+    __syncthreads();
+    s1 = s2 = 0.0f;
 #pragma unroll
-      for (int k = 0; k < W; ++k) {
-        s1 += red[phase][grp][k][0];
-        s2 += red[phase][grp][k][1];
-      }
+    for (int k = 0; k < W; ++k) {
+      s1 += red[phase][k][0];
+      s2 += red[phase][k][1];
     }
     const float m1 = s1 / p.d, m2 = s2 / p.d;
     float* dxr = p.dx + r * p.lddx;
 #pragma unroll
     for (int i = 0; i < G; ++i) {
-      const int k = t + T * i;
+      const int k = t + kWide * i;
       if (k >= units) continue;
       float v[C];
 #pragma unroll
@@ -532,27 +621,8 @@ __global__ void __launch_bounds__(T > 256 ? T : 256, T > 512 ? 1 : (T > 256 ? 1 
     }
   }
   if (!sums) return;
-  // the CTA's sums over its groups, in group order
-  if (!kAccSmem) {
-    for (int gi = 0; gi < R; ++gi) {
-      if (grp == gi) {
-#pragma unroll
-        for (int i = 0; i < G; ++i) {
-          const int k = t + T * i;
-          if (k >= units) continue;
-#pragma unroll
-          for (int c = 0; c < C; ++c) {
-            put(acc_s + C * k + c, ag[C * i + c], gi > 0);
-            put(acc_s + p.d + C * k + c, ab[C * i + c], gi > 0);
-          }
-        }
-      }
-      __syncthreads();
-    }
-  } else {
-    __syncthreads();
-  }
-  for (int j = threadIdx.x; j < p.d; j += kBlock) {
+  __syncthreads();
+  for (int j = t; j < p.d; j += kWide) {
     if (p.part) {
       float* pr = p.part + (int64_t)blockIdx.x * 2 * p.d;
       pr[j] = acc_s[j];
@@ -619,37 +689,29 @@ int launch_with_sums(NormBwdParams& p, int grid, float* dg, float* db, cudaStrea
   return e == cudaSuccess ? RTB_OK : cuda_status(e, "layer_norm_backward launch");
 }
 
-template <int T, int E, bool VEC, bool SAVED>
+template <bool VEC, bool SAVED>
 int launch_direct(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStream_t s) {
-  constexpr int kBlock = T > 256 ? T : 256;
-  constexpr int R = kBlock / T;
-  auto* k = norm_bwd_direct_kernel<T, E, VEC, SAVED>;
+  auto* k = norm_bwd_direct_kernel<VEC, SAVED>;
   const size_t smem = (dg || db) ? (size_t)2 * p.d * sizeof(float) : 0;
-  cudaError_t e = cudaSuccess;
-  if (smem > 48 * 1024) {
-    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return cuda_status(e, "layer_norm_backward smem attribute");
-  }
-  int per_sm = 1;
-  cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, kBlock, smem);
-  if (per_sm < 1) per_sm = 1;
-  const int64_t need = (p.rows + R - 1) / R, cap = (int64_t)ctx->sm_count * per_sm;
-  const int grid = (int)(need < cap ? need : cap);
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       2 * 16384 * (int)sizeof(float));
+  if (e != cudaSuccess) return cuda_status(e, "layer_norm_backward smem attribute");
+  const int grid = (int)(p.rows < ctx->sm_count ? p.rows : ctx->sm_count);
   return launch_with_sums(p, grid, dg, db, s, [&] {
-    return launch_pdl(k, dim3((unsigned)grid), dim3(kBlock), smem, s, (const NormBwdParams)p, dg,
-                      db);
+    return launch_pdl(k, dim3((unsigned)grid), dim3(kWide), smem, s, (const NormBwdParams)p, dg, db);
   });
 }
 
-template <int kBlock, int E, bool VEC, bool SAVED, bool ACT>
-int launch_rows(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStream_t s) {
+template <int kBlock, int E, bool VEC, bool SAVED, bool ACT, bool FULL>
+int launch_rows_as(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStream_t s) {
   constexpr int G = VEC ? E / 4 : E;
   constexpr int kPerSm = 1024 / kBlock;
-  auto* k = norm_bwd_rows_kernel<kBlock, E, VEC, SAVED, ACT>;
+  auto* k = norm_bwd_rows_kernel<kBlock, E, VEC, SAVED, ACT, FULL>;
   const int units = VEC ? p.d / 4 : p.d;
   const int T = (units + 32 * G - 1) / (32 * G) * 32, R = kBlock / T;
-  const int row_bytes = (((SAVED ? p.d : 4 * p.d) + 15) & ~15) + ((4 * p.d + 15) & ~15);
-  int smem = VEC ? R * kRing * row_bytes : 0;
+  constexpr int kPad = VEC ? 15 : 30;
+  const int row_bytes = (((SAVED ? p.d : 4 * p.d) + kPad) & ~15) + ((4 * p.d + kPad) & ~15);
+  int smem = kRows<kBlock, VEC, SAVED> ? R * kRing * row_bytes : 0;
   if (smem < 8 * p.d) smem = 8 * p.d;  // the CTA's sums
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return cuda_status(e, "layer_norm_backward smem attribute");
@@ -659,6 +721,13 @@ int launch_rows(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStream
     return launch_pdl(k, dim3((unsigned)grid), dim3(kBlock), (size_t)smem, s,
                       (const NormBwdParams)p, T, 1.0f / (float)p.d, dg, db);
   });
+}
+
+template <int kBlock, int E, bool VEC, bool SAVED, bool ACT>
+int launch_rows(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStream_t s) {
+  if (VEC && p.d % (32 * E) == 0)
+    return launch_rows_as<kBlock, E, VEC, SAVED, ACT, VEC>(ctx, p, dg, db, s);
+  return launch_rows_as<kBlock, E, VEC, SAVED, ACT, false>(ctx, p, dg, db, s);
 }
 
 template <bool VEC, bool SAVED>
@@ -673,7 +742,7 @@ int launch_width(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStrea
   if (p.d <= 8192)
     return act ? launch_rows<1024, 8, VEC, SAVED, true>(ctx, p, dg, db, s)
                : launch_rows<1024, 8, VEC, SAVED, false>(ctx, p, dg, db, s);
-  return launch_direct<1024, 16, VEC, SAVED>(ctx, p, dg, db, s);
+  return launch_direct<VEC, SAVED>(ctx, p, dg, db, s);
 }
 
 }  // namespace

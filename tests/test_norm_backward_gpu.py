@@ -268,3 +268,31 @@ def test_layer_norm_of_an_expanded_row(gpu):
     row = torch.randn((1, 300), generator=torch.Generator().manual_seed(1)).cuda()
     y = gpu.layer_norm(row.expand(50, 300))
     assert torch.equal(y, gpu.layer_norm(row.expand(50, 300).contiguous()))
+
+
+# rows that begin at any byte, several of them to each group of threads
+@pytest.mark.parametrize("rows,d,offset,pad", [(9500, 301, 1, 0), (1300, 1000, 7, 3), (700, 4097, 0, 0),
+                                               (460, 6001, 15, 5), (1, 129, 3, 1), (40000, 77, 13, 1),
+                                               (2, 8191, 9, 2)])
+@pytest.mark.parametrize("act", [0, 2])
+@pytest.mark.parametrize("saved", [False, True])
+def test_rows_at_any_byte(gpu, rows, d, offset, pad, act, saved):
+    x, w, b, dy = make(rows, d, 11)
+    _, mean, rstd = gpu.layer_norm_fwd(x, w, b, EPS, act)
+
+    def moved(t):
+        """t with a row stride of d + pad, from element `offset` of its storage;
+        NaN around the rows."""
+        wide = torch.full((offset + rows * (d + pad),), float("nan"), device="cuda").to(t.dtype)
+        view = wide.as_strided((rows, d), (d + pad, 1), offset)
+        view.copy_(t)
+        return view
+
+    scale = None
+    if saved:
+        q, scale = gpu.fp8_quantize(x)
+        x, source = gpu.fp8_dequantize(q, scale), moved(q)
+    else:
+        source = moved(x)
+    want, bound = reference(x, mean, rstd, w, b, dy, act)
+    check(gpu.layer_norm_backward(source, mean, rstd, moved(dy), w, b, act, x_scale=scale), want, bound)
