@@ -33,6 +33,7 @@
 // Shared memory (128-byte swizzle throughout):
 //   MODE 0, 2, K-major: row r at r * 128 B holds 128 e4m3 of the contraction.
 //   MODE 1, MN-major: boxes of 64 contraction rows x 64 bf16 (8 KB).
+#include <atomic>
 #include <cstdlib>
 
 #include "rtb_blockgemm.cuh"
@@ -44,10 +45,10 @@ namespace {
 constexpr int kX = 128;                // tile rows
 constexpr int kXBytes = 128 * 128;     // X bytes of a stage (16 KB, both modes)
 constexpr int kSmemMax = 232448;       // dynamic shared memory per CTA
+constexpr int kSmemHalf = 115712;      // of two CTAs on an SM
 constexpr int kReserve = 2048;         // barriers, alignment slack
 constexpr int kScaleUnits = 32;        // blocks whose scales are staged at a time
 constexpr int kThreads = 256;
-constexpr int kSfUnits = 16;           // MODE 2: blocks of a scale buffer (there are two)
 
 template <int MODE, int BN, bool YVEC>
 struct Cfg {
@@ -55,10 +56,15 @@ struct Cfg {
   static constexpr int kPieces = MODE == 1 ? 3 : 1;
   static constexpr int kYPiece = BN * 128;             // one Y piece of a stage (BN x 128 B)
   static constexpr int kStageBytes = kXBytes + kPieces * kYPiece;
+  // Narrow tiles, two CTAs on an SM: one's loads pass behind the other's start and
+  // end (a token row by 8192 x 8192: 19.9 us with one CTA of eight stages, 18.8).
+  static constexpr int kPerSm = MODE == 2 && BN <= 32 ? 2 : 1;
+  static constexpr int kSf = kPerSm == 2 ? 8 : 16;     // MODE 2: blocks of a scale buffer, of two
+  static constexpr int kBudget = kPerSm == 2 ? kSmemHalf : kSmemMax;
   static constexpr int kSy = YVEC ? BN : 1;            // column scales of a block
   static constexpr int kScaleBytes =
-      MODE == 0 ? kScaleUnits * (128 + kSy) * 4 : (MODE == 2 ? 2 * kSfUnits * 1024 : 0);
-  static constexpr int kStagesRaw = (kSmemMax - kReserve - kScaleBytes) / kStageBytes;
+      MODE == 0 ? kScaleUnits * (128 + kSy) * 4 : (MODE == 2 ? 2 * kSf * 1024 : 0);
+  static constexpr int kStagesRaw = (kBudget - kReserve - kScaleBytes) / kStageBytes;
   static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;
   static constexpr int kSmemBytes = kStages * kStageBytes + kScaleBytes + kReserve;
   // the finished tile: [128][BN + 4] floats, or [BN][132] where X is the
@@ -121,19 +127,23 @@ __device__ __forceinline__ void mx_stage1_e(uint32_t d, uint64_t a, uint64_t b, 
       : "memory");
 }
 
-// MODE 2: the scale bytes of blocks u .. u + n - 1 (n <= 16) of row r as words of
-// the 512-byte groups that the tensor core takes (row l of a group: the word at
-// 16 (l % 32) + 4 (l / 32), its byte four times); 2^0 for rows past the operand.
-__device__ __forceinline__ void stage_scale_words(const ScaleRef& s, int64_t r, int64_t rows, int u,
-                                                  int n, uint8_t* group, int l) {
+// MODE 2: the scale bytes of blocks u .. u + n - 1 (n <= N) of row r; 2^0 for rows
+// past the operand.
+template <int N>
+__device__ __forceinline__ void load_scale_bytes(const ScaleRef& s, int64_t r, int64_t rows, int u,
+                                                 int n, uint32_t (&raw)[N]) {
   const bool in = r < rows;
   const uint8_t* p = static_cast<const uint8_t*>(s.p) +
                      (in ? (r >> s.row_shift) * s.ld_row + (int64_t)u * s.ld_col : 0);
-  uint32_t raw[kSfUnits];
 #pragma unroll
-  for (int k = 0; k < kSfUnits; ++k) raw[k] = in && k < n ? __ldg(p + (int64_t)k * s.ld_col) : 127u;
+  for (int k = 0; k < N; ++k) raw[k] = in && k < n ? __ldg(p + (int64_t)k * s.ld_col) : 127u;
+}
+// ... as words of the 512-byte groups that the tensor core takes (row l of a group:
+// the word at 16 (l % 32) + 4 (l / 32), its byte four times).
+template <int N>
+__device__ __forceinline__ void store_scale_words(const uint32_t (&raw)[N], uint8_t* group, int l) {
 #pragma unroll
-  for (int k = 0; k < kSfUnits; ++k)
+  for (int k = 0; k < N; ++k)
     *reinterpret_cast<uint32_t*>(group + 512 * k + 16 * (l & 31) + 4 * (l >> 5)) = raw[k] * 0x01010101u;
 }
 
@@ -158,6 +168,12 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
                    : "memory");
 }
+// Without an order of memory: behind reads whose values have been used, when the
+// stores since need not be seen (a release would wait for them).
+__device__ __forceinline__ void cluster_sync_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" :::
+                   "memory");
+}
 __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
   uint32_t r;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
@@ -175,7 +191,7 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
 // YVEC (MODE 0): a scale for every Y column (block_rows 1); otherwise the
 // tile's columns lie in one 128-row block and share one.
 template <int MODE, int BN, bool YVEC>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, Cfg<MODE, BN, YVEC>::kPerSm)
     block_gemm_kernel(const __grid_constant__ CUtensorMap tmX,
                       const __grid_constant__ CUtensorMap tmY, const BlockParams p) {
   using C = Cfg<MODE, BN, YVEC>;
@@ -194,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* sempty = sfull + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sempty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  uint8_t* sf = reinterpret_cast<uint8_t*>(sx);  // MODE 2: [2][X, Y][kSfUnits][512]
+  uint8_t* sf = reinterpret_cast<uint8_t*>(sx);  // MODE 2: [2][X, Y][kSf][512]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -283,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             !(ok = wait(&full[s], (i / S) & 1, DEV_TIMEOUT_FULL)))
           break;
         if (j == 0 && !(ok = wait(&tempty[b], ((u >> 1) & 1) ^ 1, DEV_TIMEOUT_TMEM_EMPTY))) break;
-        const int c = i / kSfUnits, k = i % kSfUnits;  // MODE 2: scale buffer c & 1, its block k
+        const int c = i / C::kSf, k = i % C::kSf;  // MODE 2: scale buffer c & 1, its block k
         if (MODE == 2 && k == 0 && !(ok = wait(&sfull[c & 1], (c >> 1) & 1, DEV_TIMEOUT_LOADED)))
           break;
         tc_fence_after();
@@ -306,12 +322,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                        j > 0 || r > 0 || q < p.pieces - 1);
           umma_commit_e(&empty[s]);
         } else {
-          const uint32_t g = smem_u32(sf) + (uint32_t)((c & 1) * kSfUnits * 1024 + 512 * k);
+          const uint32_t g = smem_u32(sf) + (uint32_t)((c & 1) * C::kSf * 1024 + 512 * k);
           mx_stage1_e(d, umma_desc(xa, 16, 1024, kLayoutSW128), umma_desc(ya, 16, 1024, kLayoutSW128),
                       ((uint32_t)(BN >> 3) << 17) | (1u << 23) | ((uint32_t)(kX >> 4) << 24),
                       tmem + 2 * BN + 8u * (uint32_t)(i & 1), umma_desc(g, 128, 128, 0),
-                      umma_desc(g + kSfUnits * 512, 128, 128, 0), j > 0, &empty[s]);
-          if (k == kSfUnits - 1) umma_commit_e(&sempty[c & 1]);
+                      umma_desc(g + C::kSf * 512, 128, 128, 0), j > 0, &empty[s]);
+          if (k == C::kSf - 1) umma_commit_e(&sempty[c & 1]);
         }
       }
       if (!ok) break;
@@ -325,9 +341,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
     for (int j = 0; j < BN / 2; ++j) acc[j] = 0ull;
     bool ok = true;
-    // MODE 2: the scales of blocks kSfUnits c .. into buffer c & 1
+    // MODE 2: the scales of blocks kSf c .. into buffer c & 1
     auto scale_words = [&](int c) {
-      const int first = c * kSfUnits;
+      const int first = c * C::kSf;
       if (first >= nst) return;
       if (c >= 2 && ok) {  // the buffer's MMAs before are done
         int got = 0;
@@ -336,11 +352,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                                   DEV_TIMEOUT_EMPTY, p.timeout_ns);
         ok = __shfl_sync(0xffffffffu, got, 0) != 0;
       }
-      const int n = nst - first < kSfUnits ? nst - first : kSfUnits;
-      uint8_t* g = sf + (c & 1) * kSfUnits * 1024;
-      stage_scale_words(p.scx, (int64_t)tx * kX + et, p.xrows, i0 + first, n, g, et);
-      stage_scale_words(p.scy, (int64_t)ty * BN + et, et < BN ? p.ycols : 0, i0 + first, n,
-                        g + kSfUnits * 512, et);
+      const int n = nst - first < C::kSf ? nst - first : C::kSf;
+      uint8_t* g = sf + (c & 1) * C::kSf * 1024;
+      // (both operands' loads before the first store: one latency, not two)
+      uint32_t rx[C::kSf], ry[C::kSf];
+      load_scale_bytes(p.scx, (int64_t)tx * kX + et, p.xrows, i0 + first, n, rx);
+      load_scale_bytes(p.scy, (int64_t)ty * BN + et, et < BN ? p.ycols : 0, i0 + first, n, ry);
+      store_scale_words(rx, g, et);
+      store_scale_words(ry, g + C::kSf * 512, et);
       fence_proxy_async_smem();  // the tensor core's copies read them
       mbar_arrive(&sfull[c & 1]);
     };
@@ -348,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int u = 0; u < units; ++u) {
       const int b = u & 1;
       // the next buffer, while this one's blocks are multiplied
-      if (MODE == 2 && u * C::kPerUnit % kSfUnits == 0) scale_words(u * C::kPerUnit / kSfUnits + 1);
+      if (MODE == 2 && u * C::kPerUnit % C::kSf == 0) scale_words(u * C::kPerUnit / C::kSf + 1);
       if (MODE == 0 && u % kScaleUnits == 0) {
         // the next blocks' scales, decoded, eight loads in flight a thread
         const int n = units - u < kScaleUnits ? units - u : kScaleUnits;
@@ -496,15 +515,49 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (globaltimer_ns() - t0 < 1000000ull) __nanosleep(1000);
     __syncthreads();
   }
-  if (parts > 1) cluster_sync();  // the other CTAs have read this one's part
+  if (parts > 1) cluster_sync_relaxed();  // the other CTAs have read this one's part
   if (warp == 1) tmem_dealloc(tmem, C::kTmemCols);
 }
 
-// CTAs that share a tile: as many as the SMs allow (a power of two up to 8),
-// with at least two blocks of the contraction each.
+// Clusters of `parts` CTAs that the GPU holds at once (a cluster lies in one GPC, so
+// that there are fewer than SMs / parts).  The shared memory limit of k is set.
+template <int MODE, int BN, bool YVEC>
+int max_clusters(int parts) {
+  static std::atomic<int> known[4];  // by log2 of parts; 0: not asked yet
+  std::atomic<int>& slot = known[parts == 1 ? 0 : parts == 2 ? 1 : parts == 4 ? 2 : 3];
+  int n = slot.load(std::memory_order_relaxed);
+  if (n) return n;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)parts);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Cfg<MODE, BN, YVEC>::kSmemBytes;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)parts;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, block_gemm_kernel<MODE, BN, YVEC>, &cfg) != cudaSuccess || n < 1)
+    n = 1;
+  slot.store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// CTAs that share a tile: a power of two up to 8 with at least two blocks of the
+// contraction each, such that all clusters run at once (16 tiles of 8 CTAs, one on
+// an SM, take a second round for the last one: 128 x 2048 x 4096 22.8 us, 12.4 with
+// four; 512 x 512 x 4096 23.0, 12.4).  With two CTAs on an SM (the query counts one)
+// and eight blocks for each a few clusters may follow: a token row by 4096 x
+// 4096 10.7 us with eight, 10.0 with four; 32 x 4096 x 14336 18.6, 20.8.
+template <int MODE, int BN, bool YVEC>
 int pick_parts(const rtb_ctx* ctx, int64_t tiles, int64_t units) {
+  constexpr int kPerSm = Cfg<MODE, BN, YVEC>::kPerSm;
   int parts = 1;
-  while (parts < 8 && tiles * parts * 2 <= ctx->sm_count && units >= parts * 4) parts *= 2;
+  while (parts < 8 && units >= parts * 4 && tiles * parts * 2 <= kPerSm * ctx->sm_count &&
+         (tiles <= (int64_t)kPerSm * max_clusters<MODE, BN, YVEC>(parts * 2) ||
+          (kPerSm == 2 && units >= parts * 16)))
+    parts *= 2;
   return parts;
 }
 
@@ -521,7 +574,7 @@ int launch(rtb_ctx* ctx, const CUtensorMap& tmX, const CUtensorMap& tmY, BlockPa
   p.stages_total = (p.depth + C::kDepth - 1) / C::kDepth;
   const int64_t tiles = (int64_t)p.tiles_x * p.tiles_y;
   if (tiles > INT32_MAX / 8) return set_error(RTB_E_UNSUPPORTED, "block gemm: too many tiles");
-  p.parts = pick_parts(ctx, tiles, (p.stages_total + C::kGrain - 1) / C::kGrain);
+  p.parts = pick_parts<MODE, BN, YVEC>(ctx, tiles, (p.stages_total + C::kGrain - 1) / C::kGrain);
   p.vec_ok = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 && p.ldo % 4 == 0 &&
              (!p.bias || (reinterpret_cast<uintptr_t>(p.bias) & 15u) == 0);
   cudaLaunchConfig_t cfg = {};
@@ -572,7 +625,7 @@ int fp8_gemm_run(rtb_ctx* ctx, const Fp8Desc& d, cudaStream_t s) {
   if ((st = check_extents(d.M, d.N, d.K))) return st;
   // Few rows of A: the weight's rows fill the 128-row tile and A is the narrow
   // side (C^T = B . A^T), so that at most 15 rows of 16, 31 of 64 are padding and
-  // not 64 of 128 (16 x 8192 x 8192: 19 us in a loop, 3.5 TB/s of the weight).
+  // not 64 of 128 (16 x 8192 x 8192: 19.3 us in a loop, 3.5 TB/s of the weight).
   const bool swap = d.M <= 64;
   BlockParams p{};
   p.xrows = swap ? d.N : d.M;
