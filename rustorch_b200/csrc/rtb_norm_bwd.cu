@@ -635,18 +635,20 @@ __global__ void __launch_bounds__(kWide, 1)
 }
 
 // dg[j] (+)= sum over the CTAs' partial rows, db likewise (blockIdx.y picks
-// one): 8 columns per CTA (one 32-byte sector of a row), 32 threads a column
-// with 8 rows in flight each, added in a fixed order.
-__global__ void __launch_bounds__(kThreads) norm_bwd_reduce_kernel(const float* __restrict__ part,
+// one): 32 columns per CTA, 32 threads a column with 8 rows in flight each, added
+// in a fixed order.
+constexpr int kReduceThreads = 1024;
+
+__global__ void __launch_bounds__(kReduceThreads) norm_bwd_reduce_kernel(const float* __restrict__ part,
                                                                    int ctas, int d, float* dg,
                                                                    float* db, int accumulate) {
-  __shared__ float t[32][9];
+  __shared__ float t[32][33];
   griddep_wait();
   griddep_launch_dependents();
   float* out = blockIdx.y ? db : dg;
   if (!out) return;
-  const int col = threadIdx.x & 7, w = threadIdx.x >> 3;
-  const int j = blockIdx.x * 8 + col;
+  const int col = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int j = blockIdx.x * 32 + col;
   float s = 0.0f;
   if (j < d) {
     const float* p = part + (int64_t)blockIdx.y * d + j;
@@ -682,7 +684,7 @@ int launch_with_sums(NormBwdParams& p, int grid, float* dg, float* db, cudaStrea
   clear_stale_cuda_error();
   cudaError_t e = launch();
   if (e == cudaSuccess && part)
-    e = launch_pdl(norm_bwd_reduce_kernel, dim3((unsigned)((p.d + 7) / 8), 2), dim3(kThreads), 0,
+    e = launch_pdl(norm_bwd_reduce_kernel, dim3((unsigned)((p.d + 31) / 32), 2), dim3(kReduceThreads), 0,
                    s, (const float*)part, grid, p.d, dg, db, p.accumulate);
   if (e == cudaSuccess) e = cudaGetLastError();
   ws_free(part, s);
@@ -792,7 +794,7 @@ int norm_backward_run(rtb_ctx* ctx, const NormBwdDesc& d, cudaStream_t s) {
   clear_stale_cuda_error();
   cudaError_t e = launch_pdl(norm_bwd_kernel, dim3((unsigned)grid), dim3(kThreads), 0, s, p);
   if (e == cudaSuccess && part)
-    e = launch_pdl(norm_bwd_reduce_kernel, dim3((unsigned)((d.d + 7) / 8), 2), dim3(kThreads), 0,
+    e = launch_pdl(norm_bwd_reduce_kernel, dim3((unsigned)((d.d + 31) / 32), 2), dim3(kReduceThreads), 0,
                    s, (const float*)part, grid, (int)d.d, d.dg, d.db, d.accumulate);
   if (e == cudaSuccess) e = cudaGetLastError();
   ws_free(part, s);
