@@ -217,6 +217,25 @@ def test_product_large(gpu, m, n, k, ra, rb, floats):
     check_product(gpu, a, sa, w, sw, bias, 1)
 
 
+# long contractions: more blocks for a CTA than its scale buffers hold, one CTA a
+# tile and every size of cluster, a tile more or fewer than run at once
+LONG = [(3, 20000, 4224), (20, 19000, 5000), (64, 20000, 6400), (7, 2048, 16500), (30, 1000, 9000),
+        (1, 1920, 4100), (128, 2048, 9000), (64, 8300, 8192), (16, 8300, 8192)]
+
+
+@pytest.mark.parametrize("m,n,k", LONG)
+@pytest.mark.parametrize("rb", [128, 1])
+def test_product_long(gpu, m, n, k, rb):
+    a, sa = operand(m, k, 1, 17)
+    w, sw = operand(1280, k, rb, 18)
+
+    def cycled(t, rows):  # the operand's rows over and over
+        at = torch.arange(rows, device="cuda") % t.shape[0]
+        return t.view(torch.uint8)[at].view(t.dtype)
+
+    check_product(gpu, a, sa, cycled(w, n), cycled(sw, -(-n // rb)))
+
+
 @pytest.mark.parametrize("m,n", [(5, 140), (150, 200), (2600, 2100)])
 def test_product_scale_range(gpu, m, n):
     """Scales far from 1 that cancel, the smallest byte, and byte 255 (NaN), on
