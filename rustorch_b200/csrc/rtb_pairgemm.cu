@@ -289,6 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tempty0[2] = {map_rank(smem_u32(&tempty[0]), 0), map_rank(smem_u32(&tempty[1]), 0)};
     uint8_t* stg = staging + half * kChunk;
     int g = 0;
+    int quad = 0;  // quads of blocks so far, over all tiles: the buffer of a quad's column scales
     bool ok = true;
     for (int t = pair; t < tiles; t += pairs) {
       int tx, ty;
@@ -309,9 +310,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           ny[i] = __ldg(py + i * p.pitchy);
         }
       }
-      for (int v = 0; v < units; v += 4) {
+      for (int v = 0; v < units; v += 4, ++quad) {
         float sc[4];
-        float* sy = sy_s + 1024 * ((v >> 2) & 1) + 128 * half;
+        float* sy = sy_s + 1024 * (quad & 1) + 128 * half;
         if (MODE == 0) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -325,7 +326,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             nx[i] = __ldg(px + i * p.pitchx);
             ny[i] = __ldg(py + i * p.pitchy);
           }
-          // two buffers: the quad after next is written behind the next barrier
+          // Two buffers, taken in turn across tiles too: a buffer is written again
+          // two quads later, behind the barrier of the quad between, which every
+          // reader of this one has passed.  (The stores of a finished tile need
+          // have no barrier.)
           if (YVEC) named_bar_sync(1 + half, 128);
         }
         const int n = units - v < 4 ? units - v : 4;

@@ -217,6 +217,23 @@ def test_product_large(gpu, m, n, k, ra, rb, floats):
     check_product(gpu, a, sa, w, sw, bias, 1)
 
 
+@pytest.mark.parametrize("k", [130, 400, 640, 1100])
+def test_product_scales_of_consecutive_tiles(gpu, k):
+    """More tiles than CTA pairs, a float scale for every column and rows of the
+    output that are stored directly: the column scales of a tile's last blocks
+    and of the next tile's first ones lie side by side in shared memory.  An odd
+    and an even number of four-block groups; the same bits on every call."""
+    m, n = 2600, 2101
+    g = torch.Generator().manual_seed(27)
+    a, sa = operand(m, k, 1, 28)
+    w, _ = operand(n, k, 1, 29)
+    # scales apart by far more than the bound from column to column and block to block
+    sw = torch.pow(2.0, 8 * torch.rand((n, -(-k // 128)), generator=g) - 4).cuda()
+    first = check_product(gpu, a, sa, w, sw)
+    for _ in range(60):
+        assert torch.equal(gpu.fp8_matmul(a, sa, w.t(), sw.t()), first)
+
+
 # long contractions: more blocks for a CTA than its scale buffers hold, one CTA a
 # tile and every size of cluster, a tile more or fewer than run at once
 LONG = [(3, 20000, 4224), (20, 19000, 5000), (64, 20000, 6400), (7, 2048, 16500), (30, 1000, 9000),
