@@ -93,6 +93,7 @@ __global__ void __launch_bounds__(kThreads) norm_bwd_kernel(const NormBwdParams 
   griddep_wait();
   griddep_launch_dependents();
   float* pg = p.part ? p.part + (int64_t)blockIdx.x * 2 * p.d : nullptr;
+  float* pb = pg ? pg + p.d : nullptr;  // (an index p.d + j would pass 32 bits)
   bool first = true;
   for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x, first = false) {
     const float mean = p.mean[r], rstd = p.rstd[r];
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(kThreads) norm_bwd_kernel(const NormBwdParams 
       s2 = fmaf(h, u, s2);
       if (pg) {
         pg[j] = first ? dz * u : fmaf(dz, u, pg[j]);
-        pg[p.d + j] = first ? dz : pg[p.d + j] + dz;
+        pb[j] = first ? dz : pb[j] + dz;
       }
     }
     if (!p.dx) continue;

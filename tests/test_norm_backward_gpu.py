@@ -296,3 +296,17 @@ def test_rows_at_any_byte(gpu, rows, d, offset, pad, act, saved):
         source = moved(x)
     want, bound = reference(x, mean, rstd, w, b, dy, act)
     check(gpu.layer_norm_backward(source, mean, rstd, moved(dy), w, b, act, x_scale=scale), want, bound)
+
+
+def test_a_row_of_more_than_2_30_columns(gpu):
+    """One row whose two partial sums lie 2^30 floats and more apart: with mean 0
+    and rstd 1, u = x, so that the sums are x * x and x, to the bit."""
+    d = 2 ** 30 + 64
+    x = torch.empty((1, d), device="cuda")
+    x.view(-1, 64)[:] = torch.arange(1, 65, device="cuda").float()
+    x[0, ::1009] = -3.25
+    zero, one = torch.zeros(1, device="cuda"), torch.ones(1, device="cuda")
+    _, dw, db = gpu.layer_norm_backward(x, zero, one, x, need_x=False)
+    assert torch.equal(db, x[0])
+    del db
+    assert torch.equal(dw, (x * x)[0])
