@@ -254,7 +254,8 @@ int rtb_conv2d_backward(rtb_ctx* ctx, int64_t N, int64_t Ci, int64_t H, int64_t 
 
 /* ---------------------------------------------------------------- layer norm, training */
 /* rtb_layer_norm that also leaves what its backward pass reads: mean[r] and
- * rstd[r] = 1 / sqrt(var + eps) of every row (rows floats each; d >= 1).
+ * rstd[r] = 1 / sqrt(var + eps) of every row (rows floats each; d >= 1, and at
+ * most 2^31 - 513 where d, ldx, ldy or a pointer is off the 16-byte boundaries).
  * Replaces layer_norm's saved statistics (rustorch-core/src/ops/norm.rs:
  * 613-700); x == y (in place) is allowed. */
 int rtb_layer_norm_fwd(rtb_ctx* ctx, int64_t rows, int64_t d, const float* x, int64_t ldx,

@@ -302,6 +302,10 @@ int launch_layernorm_act(rtb_ctx* ctx, const float* X, int64_t ldx, float* Y, in
   auto al16 = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
   const bool vec = N % 4 == 0 && ldx % 4 == 0 && ldy % 4 == 0 && al16(X) && al16(Y) &&
                    (!g || al16(g)) && (!b || al16(b));
+  // (the scalar passes step an int column by kLnThreads, past the last one too;
+  // an unsigned one takes 8 registers more and two resident CTAs an SM)
+  if (!vec && N > INT32_MAX - 2 * kLnThreads)
+    return set_error(RTB_E_UNSUPPORTED, "layernorm: N too large for rows off the 16-byte boundaries");
   const int n = (int)N;
   if (vec && N <= 16384) {  // T threads per row, up to 16 float4 per thread, in registers
     const int per = (int)((N / 4 + 31) / 32);  // float4 per lane of one warp

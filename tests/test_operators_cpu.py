@@ -1,5 +1,7 @@
 """Refusals of the training and 8-bit entry points that need no GPU: a null
 context, tensors that are not on one, wrong types."""
+import ctypes
+
 import pytest
 import torch
 
@@ -44,3 +46,19 @@ def test_host_tensors_refused(rb):
                  lambda: rb.layer_norm_backward(q, m, m, x, x_scale=s)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_rows_beyond_the_index_range_refused(rb):
+    """Rows of almost 2^31 columns off the 16-byte boundaries are refused before
+    anything is launched (no device is touched: the context is a block of zeros)."""
+    if torch.cuda.is_available():
+        pytest.skip("checked where nothing can be launched")
+    L = rb.lib()
+    ctx = ctypes.create_string_buffer(4096)
+    p = ctypes.c_void_p(1 << 20)
+    for d in (2 ** 31 - 1, 2 ** 31 - 256):
+        ld = d | 1
+        st = L.rtb_layer_norm_fwd(ctx, 1, d, p, ld, None, None, 1e-5, 0, p, ld, p, p, None)
+        assert st == rb._lib.RTB_E_UNSUPPORTED, rb._lib.last_error()
+        st = L.rtb_layer_norm(ctx, 1, d, p, ld, None, None, 1e-5, 0, p, ld, None)
+        assert st == rb._lib.RTB_E_UNSUPPORTED, rb._lib.last_error()
