@@ -716,7 +716,15 @@ int launch_rows_as(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStr
   const int row_bytes = (((SAVED ? p.d : 4 * p.d) + kPad) & ~15) + ((4 * p.d + kPad) & ~15);
   int smem = kRows<kBlock, VEC, SAVED> ? R * kRing * row_bytes : 0;
   if (smem < 8 * p.d) smem = 8 * p.d;  // the CTA's sums
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  // The limit belongs to the kernel and not to the launch, and another thread may
+  // be between its own two: so it is one number, that of the widest launch.  Groups
+  // of T threads hold at most E values a thread, R d <= kBlock E, and R is at most
+  // kBlock / 32.
+  constexpr int kRingMax = kRing * (kBlock * E * (SAVED ? 5 : 8) + kBlock / 32 * 2 * kPad);
+  constexpr int kSumsMax = 8 * kBlock * E;
+  constexpr int kMost = kRows<kBlock, VEC, SAVED> && kRingMax > kSumsMax ? kRingMax : kSumsMax;
+  static_assert(kMost + 1024 <= 232448, "shared memory");
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
   if (e != cudaSuccess) return cuda_status(e, "layer_norm_backward smem attribute");
   const int64_t need = (p.rows + R - 1) / R, cap = (int64_t)ctx->sm_count * kPerSm;
   const int grid = (int)(need < cap ? need : cap);

@@ -310,3 +310,48 @@ def test_a_row_of_more_than_2_30_columns(gpu):
     assert torch.equal(db, x[0])
     del db
     assert torch.equal(dw, (x * x)[0])
+
+
+# widths of one kernel that need unlike amounts of shared memory
+@pytest.mark.parametrize("widths", [(768, 4096), (2304, 1024), (1001, 4001)])
+@pytest.mark.parametrize("saved", [False, True])
+def test_two_threads_with_unlike_widths(gpu, widths, saved):
+    _two_threads(gpu, [_backward_of(gpu, d, saved) for d in widths])
+
+
+def _backward_of(gpu, d, saved):
+    x, w, b, dy = make(6, d, 12)
+    _, mean, rstd = gpu.layer_norm_fwd(x, w, b, EPS)
+    scale = None
+    if saved:
+        x, scale = gpu.fp8_quantize(x)
+    return lambda: gpu.layer_norm_backward(x, mean, rstd, dy, w, b, x_scale=scale)
+
+
+def _two_threads(gpu, calls):
+    """Both calls over and over, each in a thread and on a stream of its own."""
+    import threading
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+    streams = [torch.cuda.Stream() for _ in calls]
+    start = threading.Barrier(len(calls))
+
+    def work(i):
+        try:
+            start.wait()
+            with torch.cuda.stream(streams[i]):
+                for _ in range(1500):
+                    got[i] = calls[i]()
+        except Exception as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(calls))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
