@@ -258,8 +258,9 @@ int launch_ln(const float* X, int64_t ldx, float* Y, int64_t ldy, int64_t M, int
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (smem > 48 * 1024) {  // the widest launch's limit: it is the kernel's, of all threads
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         kLnMaxOnChip * (int)sizeof(float));
     if (e != cudaSuccess) return cuda_status(e, "layernorm smem attribute");
   }
   int per_sm = 1;

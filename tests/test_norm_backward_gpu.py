@@ -319,6 +319,15 @@ def test_two_threads_with_unlike_widths(gpu, widths, saved):
     _two_threads(gpu, [_backward_of(gpu, d, saved) for d in widths])
 
 
+def test_two_threads_forward(gpu):
+    # (rows off the 16-byte boundaries, staged in shared memory)
+    def forward(d):
+        x, w, b, _ = make(4, d, 13)
+        return lambda: gpu.layer_norm_fwd(x, w, b, EPS)
+
+    _two_threads(gpu, [forward(12301), forward(16383)])
+
+
 def _backward_of(gpu, d, saved):
     x, w, b, dy = make(6, d, 12)
     _, mean, rstd = gpu.layer_norm_fwd(x, w, b, EPS)
