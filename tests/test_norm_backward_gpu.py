@@ -364,3 +364,33 @@ def _two_threads(gpu, calls):
     assert not errors, errors
     for a, b in zip(got, want):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("d", [100, 1000, 1001, 5000, 5001, 9000, 9001, 20000])
+@pytest.mark.parametrize("act", [2, 3])
+@pytest.mark.parametrize("saved", [False, True])
+def test_slopes_of_saturated_activations(gpu, d, act, saved):
+    """One row with u = 0, so that z is the bias and dbias = dy act'(z): the slope
+    keeps its relative accuracy where the activation is next to its limits.  In
+    units of 2^-24, for e / (1 + e)^2: the exponential 4 (2 ulp; the slope moves by
+    at most as much), 1 + e rounded and its reciprocal (1 ulp) 3, twice, two
+    products 2, the product with dy 1; z stays where e is a normal number."""
+    most = 80.0 if act == 2 else 40.0
+    g = torch.Generator().manual_seed(15)
+    z = most * (2 * torch.rand(d, generator=g) - 1)
+    z[:6] = torch.tensor([0.0, -0.0, most, -most, 1e-6, 12.0])
+    dy = (0.5 + torch.rand((1, d), generator=g)).cuda()
+    x, z, one = torch.zeros((1, d), device="cuda"), z.cuda(), torch.ones(1, device="cuda")
+    scale = None
+    if saved:
+        x, scale = gpu.fp8_quantize(x)
+    db = gpu.layer_norm_backward(x, torch.zeros_like(one), one, dy, None, z, act, x_scale=scale)[2]
+    z = z.double()
+    slope = torch.sigmoid(z) * torch.sigmoid(-z) if act == 2 else torch.cosh(z) ** -2
+    want = dy[0].double() * slope
+    assert bool(((db.double() - want).abs() <= 13 * U * want).all())
+    # and at the ends of the range, where the slope is 0
+    ends = torch.tensor([3e38, -3e38, float("inf"), -float("inf")] * 25, device="cuda")
+    x = torch.zeros((1, 100), device="cuda")
+    db = gpu.layer_norm_backward(x, torch.zeros_like(one), one, torch.ones_like(x), None, ends, act)[2]
+    assert bool((db == 0).all())
