@@ -394,3 +394,29 @@ def test_slopes_of_saturated_activations(gpu, d, act, saved):
     x = torch.zeros((1, 100), device="cuda")
     db = gpu.layer_norm_backward(x, torch.zeros_like(one), one, torch.ones_like(x), None, ends, act)[2]
     assert bool((db == 0).all())
+
+
+# many rows for each group of threads, CTA and partial row, on every path
+@pytest.mark.parametrize("rows,d", [(40000, 64), (40000, 77), (9500, 301), (9000, 256), (2600, 1000),
+                                    (2600, 1001), (4099, 4096), (1999, 4097), (1500, 6000), (1500, 6001),
+                                    (1203, 8192), (999, 9000), (999, 9001), (2411, 16500)])
+@pytest.mark.parametrize("saved", [False, True])
+def test_sums_over_rows_exactly(gpu, rows, d, saved):
+    """With mean 0, rstd 1 and small whole numbers every sum is a whole number
+    below 2^24, exact in any order: a row that is lost, or added twice, shows."""
+    g = torch.Generator(device="cuda").manual_seed(16)
+    x = torch.randint(1, 5, (rows, d), device="cuda", generator=g).float()
+    x *= 1 - 2 * torch.randint(0, 2, (rows, d), device="cuda", generator=g)
+    dy = torch.randint(1, 4, (rows, d), device="cuda", generator=g).float()
+    mean, rstd = torch.zeros(rows, device="cuda"), torch.ones(rows, device="cuda")
+    dw, db = (dy.double() * x.double()).sum(0), dy.double().sum(0)
+    scale = None
+    if saved:
+        x, scale = gpu.fp8_quantize(x)
+    _, gw, gb = gpu.layer_norm_backward(x, mean, rstd, dy, x_scale=scale, need_x=False)
+    assert torch.equal(gw.double(), dw) and torch.equal(gb.double(), db)
+    start = torch.arange(d, device="cuda").float()
+    gw, gb = start.clone(), -start
+    gpu.layer_norm_backward(x, mean, rstd, dy, x_scale=scale, out_x=torch.zeros_like(dy), out_weight=gw,
+                            out_bias=gb, accumulate=True)
+    assert torch.equal(gw.double(), dw + start.double()) and torch.equal(gb.double(), db - start.double())
