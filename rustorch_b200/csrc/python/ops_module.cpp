@@ -200,12 +200,20 @@ void* stream_of(const Tensor& t) {
   return c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
 }
 
-// The C call without the interpreter lock.
+// The C call without the interpreter lock, which is held again where the call
+// throws (a tensor's data pointer does where the tensor has none).
+struct Unlocked {
+  PyThreadState* state = PyEval_SaveThread();
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
 template <typename F>
 void call(const char* where, const F& f) {
   int st;
-  Py_BEGIN_ALLOW_THREADS st = f();
-  Py_END_ALLOW_THREADS check(st, where);
+  {
+    Unlocked u;
+    st = f();
+  }
+  check(st, where);
 }
 
 const char* const kShape = "LayerNorm: Input shape does not match normalized shape";
