@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <climits>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -80,8 +81,10 @@ bool flag(PyObject* o) {
   return v != 0;
 }
 int integer(PyObject* o) {
-  const long v = PyLong_AsLong(o);
+  int over = 0;
+  const long v = PyLong_AsLongAndOverflow(o, &over);
   if (v == -1 && PyErr_Occurred()) throw PyFailure();
+  if (over || v < INT_MIN || v > INT_MAX) refuse("rustorch_b200: whole number out of range");
   return (int)v;
 }
 double real(PyObject* o) {

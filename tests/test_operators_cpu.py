@@ -62,3 +62,18 @@ def test_rows_beyond_the_index_range_refused(rb):
         assert st == rb._lib.RTB_E_UNSUPPORTED, rb._lib.last_error()
         st = L.rtb_layer_norm(ctx, 1, d, p, ld, None, None, 1e-5, 0, p, ld, None)
         assert st == rb._lib.RTB_E_UNSUPPORTED, rb._lib.last_error()
+
+
+@pytest.mark.parametrize("value", [2 ** 32, 2 ** 32 + 1, -2 ** 32 + 3, 2 ** 80])
+def test_whole_numbers_out_of_range_refused(rb, value):
+    """No argument is taken modulo 2^32 (block_rows 2^32 + 1 as 1, act 2^32 as 0)."""
+    x = torch.zeros((4, 128))
+    q = x.to(torch.float8_e4m3fn)
+    s = torch.full((4, 1), 127, dtype=torch.uint8).view(torch.float8_e8m0fnu)
+    m = torch.zeros(4)
+    for call in (lambda: rb.fp8_quantize(x, value), lambda: rb.layer_norm_fwd(x, act=value),
+                 lambda: rb.layer_norm_backward(x, m, m, x, act=value),
+                 lambda: rb.fp8_matmul(q, s, q.t(), s.t(), act=value),
+                 lambda: rb.matmul_backward_fp8(q, s, None, x, need_a=False, precision=value)):
+        with pytest.raises(ValueError, match="out of range"):
+            call()
