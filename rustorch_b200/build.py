@@ -6,7 +6,7 @@ Each csrc/*.cu and csrc/*.cpp compiles to _build/*.o in parallel, then links int
 rustorch_b200/librustorch_b200.so (NCCL is dlopen'ed at first use);
 csrc/python/ops_module.cpp (the Python calls of the training and 8-bit operators)
 compiles against torch's headers into rustorch_b200/_ops.so.  A source is
-recompiled when it or any header is newer than its object, and the library is
+recompiled when it, any header or this file is newer than its object, and the library is
 relinked when any object changed.  Objects and the library are stamped with the time
 their compile started, so a file edited while a build runs is seen as newer by the
 next build.
@@ -127,7 +127,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
 def _build_lib(force: bool, verbose: bool) -> None:
     os.makedirs(BUILD, exist_ok=True)
     srcs = _sources()
-    hdr = max(os.path.getmtime(p) for p in _headers())
+    hdr = max(os.path.getmtime(p) for p in _headers() + [__file__])  # (the flags are here)
     todo = [s for s in srcs if force or verbose or _stale(s, hdr)]
     if todo:
         with cf.ThreadPoolExecutor(max_workers=min(8, len(todo))) as ex:
