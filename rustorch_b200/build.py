@@ -5,20 +5,24 @@
 Each csrc/*.cu and csrc/*.cpp compiles to _build/*.o in parallel, then links into
 rustorch_b200/librustorch_b200.so (NCCL is dlopen'ed at first use);
 csrc/python/ops_module.cpp (the Python calls of the training and 8-bit operators)
-compiles against torch's headers into rustorch_b200/_ops.so.  A source is
-recompiled when it, any header or this file is newer than its object, and the library is
-relinked when any object changed.  Objects and the library are stamped with the time
-their compile started, so a file edited while a build runs is seen as newer by the
-next build.
+compiles against torch's headers into rustorch_b200/_ops.so, and again when torch
+or Python is another one (without torch only the library is built).  A source is
+recompiled when it, any header or this file is newer than its object, and the
+library is relinked when any object changed.  Objects and the library are stamped
+with the time their compile started, so a file edited while a build runs is seen as
+newer by the next build.
 """
 from __future__ import annotations
 
 import concurrent.futures as cf
 import glob
+import importlib.util
 import os
+import runpy
 import shutil
 import subprocess
 import sys
+import sysconfig
 import time
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -28,6 +32,7 @@ BUILD = os.path.join(ROOT, "_build")
 LIB = os.path.join(PKG, "librustorch_b200.so")
 OPS_SRC = os.path.join(CSRC, "python", "ops_module.cpp")
 OPS = os.path.join(PKG, "_ops.so")
+OPS_STAMP = os.path.join(PKG, "_ops.torch")  # the torch and Python that OPS was built for
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O3",
                      "-I" + os.path.join(ROOT, "include"), "--expt-relaxed-constexpr"]
@@ -60,10 +65,24 @@ def _stale(src: str, newest_header: float) -> bool:
     return os.path.getmtime(obj) < max(os.path.getmtime(src), newest_header)
 
 
+def _torch_tag():
+    """The torch and Python that a module built now fits; None without torch.
+    (torch is not imported: that takes seconds.)"""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.origin:
+        return None
+    version = runpy.run_path(os.path.join(os.path.dirname(spec.origin), "version.py"))["__version__"]
+    return f"torch {version} {sysconfig.get_config_var('SOABI')}"
+
+
 def ops_stale() -> bool:
-    """The extension module is missing or older than its source or the C header."""
-    if not os.path.exists(OPS):
+    """The extension module is missing, older than its source or the C header, or
+    made for another torch or Python."""
+    if not (os.path.exists(OPS) and os.path.exists(OPS_STAMP)):
         return True
+    with open(OPS_STAMP) as f:
+        if f.read() != _torch_tag():
+            return True
     t = os.path.getmtime(OPS)
     return any(os.path.getmtime(p) > t for p in (OPS_SRC, os.path.join(ROOT, "include",
                                                                        "rustorch_b200.h")))
@@ -94,8 +113,6 @@ def _compile(src: str, verbose: bool) -> str:
 
 
 def _build_ops() -> None:
-    import sysconfig
-
     import torch
     t0 = time.time()
     tdir = os.path.dirname(torch.__file__)
@@ -114,12 +131,16 @@ def _build_ops() -> None:
         raise RuntimeError(f"g++ failed for {OPS_SRC}:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, OPS)
     os.utime(OPS, (t0, t0))
+    with open(OPS_STAMP, "w") as f:
+        f.write(_torch_tag())
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
     if force or needs_build():
         _build_lib(force, verbose)
-    if force or ops_stale():
+    if _torch_tag() is None:
+        sys.stderr.write("torch is not installed: the Python operators (_ops) are not built\n")
+    elif force or ops_stale():
         _build_ops()
     return LIB
 
