@@ -33,10 +33,10 @@
 // Shared memory (128-byte swizzle throughout):
 //   MODE 0, 2, K-major: row r at r * 128 B holds 128 e4m3 of the contraction.
 //   MODE 1, MN-major: boxes of 64 contraction rows x 64 bf16 (8 KB).
-#include <atomic>
 #include <cstdlib>
 
 #include "rtb_blockgemm.cuh"
+#include "rtb_per_device.h"
 
 namespace rtb {
 
@@ -522,26 +522,26 @@ __global__ void __launch_bounds__(kThreads, Cfg<MODE, BN, YVEC>::kPerSm)
 // Clusters of `parts` CTAs that the GPU holds at once (a cluster lies in one GPC, so
 // that there are fewer than SMs / parts).  The shared memory limit of k is set.
 template <int MODE, int BN, bool YVEC>
-int max_clusters(int parts) {
-  static std::atomic<int> known[4];  // by log2 of parts; 0: not asked yet
-  std::atomic<int>& slot = known[parts == 1 ? 0 : parts == 2 ? 1 : parts == 4 ? 2 : 3];
-  int n = slot.load(std::memory_order_relaxed);
-  if (n) return n;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)parts);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Cfg<MODE, BN, YVEC>::kSmemBytes;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)parts;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaOccupancyMaxActiveClusters(&n, block_gemm_kernel<MODE, BN, YVEC>, &cfg) != cudaSuccess || n < 1)
-    n = 1;
-  slot.store(n, std::memory_order_relaxed);
-  return n;
+int max_clusters(const rtb_ctx* ctx, int parts) {
+  static PerDevice<4> known;  // by log2 of parts
+  const int n = known.get(ctx->device, parts == 1 ? 0 : parts == 2 ? 1 : parts == 4 ? 2 : 3, [&] {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)parts);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Cfg<MODE, BN, YVEC>::kSmemBytes;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)parts;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int most = 0;
+    const cudaError_t e =
+        cudaOccupancyMaxActiveClusters(&most, block_gemm_kernel<MODE, BN, YVEC>, &cfg);
+    return e == cudaSuccess ? most : 0;
+  });
+  return n < 1 ? 1 : n;
 }
 
 // CTAs that share a tile: a power of two up to 8 with at least two blocks of the
@@ -555,7 +555,7 @@ int pick_parts(const rtb_ctx* ctx, int64_t tiles, int64_t units) {
   constexpr int kPerSm = Cfg<MODE, BN, YVEC>::kPerSm;
   int parts = 1;
   while (parts < 8 && units >= parts * 4 && tiles * parts * 2 <= kPerSm * ctx->sm_count &&
-         (tiles <= (int64_t)kPerSm * max_clusters<MODE, BN, YVEC>(parts * 2) ||
+         (tiles <= (int64_t)kPerSm * max_clusters<MODE, BN, YVEC>(ctx, parts * 2) ||
           (kPerSm == 2 && units >= parts * 16)))
     parts *= 2;
   return parts;

@@ -1,6 +1,8 @@
 """Refusals of the training and 8-bit entry points that need no GPU: a null
 context, tensors that are not on one, wrong types."""
 import ctypes
+import os
+import subprocess
 
 import pytest
 import torch
@@ -77,3 +79,13 @@ def test_whole_numbers_out_of_range_refused(rb, value):
                  lambda: rb.matmul_backward_fp8(q, s, None, x, need_a=False, precision=value)):
         with pytest.raises(ValueError, match="out of range"):
             call()
+
+
+def test_answers_kept_for_each_device(tmp_path):
+    """The cache of what a device holds at once (tests/cpp/test_per_device.cpp)."""
+    src = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "test_per_device.cpp")
+    exe = str(tmp_path / "per_device")
+    r = subprocess.run(["g++", "-std=c++17", "-O1", src, "-o", exe], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and r.stdout == "fine\n", r.stdout
