@@ -33,8 +33,6 @@
 // Shared memory (128-byte swizzle throughout):
 //   MODE 0, 2, K-major: row r at r * 128 B holds 128 e4m3 of the contraction.
 //   MODE 1, MN-major: boxes of 64 contraction rows x 64 bf16 (8 KB).
-#include <cstdlib>
-
 #include "rtb_blockgemm.cuh"
 #include "rtb_per_device.h"
 
@@ -601,13 +599,8 @@ int launch(rtb_ctx* ctx, const CUtensorMap& tmX, const CUtensorMap& tmY, BlockPa
 // Measured, one CTA a tile against pairs: 512 x 4096 x 4096 (32 tiles) 23.1 us,
 // 24.9; 1024 x 2048 x 1024 (32) 13.8, 14.7; 1024 x 4096 x 4096 (64) 44.3, 26.0;
 // 2048 x 2048 x 512 (64) 23.2, 14.0; weight gradients with 32 and 64 tiles, 4096
-// rows, 72 us, 85, and 130, 92.  (RTB_PAIR=0 or 1 forces one, for measurements.)
+// rows, 72 us, 85, and 130, 92.
 bool use_pairs(const rtb_ctx* ctx, const BlockParams& p) {
-  static const int env = [] {
-    const char* v = std::getenv("RTB_PAIR");
-    return v ? std::atoi(v) : -1;
-  }();
-  if (env >= 0) return env != 0;
   const int64_t tiles = ((p.xrows + 255) / 256) * ((p.ycols + 255) / 256);
   return tiles * 2 > ctx->sm_count / 2;
 }

@@ -89,3 +89,13 @@ def test_answers_kept_for_each_device(tmp_path):
     assert r.returncode == 0, r.stderr
     r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0 and r.stdout == "fine\n", r.stdout
+
+
+def test_no_hidden_switches():
+    """The kernels of these operators are chosen by the call's sizes and types and by
+    nothing in the environment."""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "rustorch_b200", "csrc")
+    for name in ("rtb_blockgemm.cu", "rtb_pairgemm.cu", "rtb_mxgemm.cu", "rtb_fp8.cu", "rtb_norm.cu",
+                 "rtb_norm_bwd.cu", os.path.join("python", "ops_module.cpp")):
+        with open(os.path.join(csrc, name)) as f:
+            assert "getenv" not in f.read(), name
