@@ -160,7 +160,7 @@ int make_tmap_im2col(CUtensorMap* map, const void* x, int N, int H, int W, int C
 
 // ---------------------------------------------------------------- workspace
 int ws_alloc(rtb_ctx* ctx, void** p, size_t bytes, cudaStream_t s) {
-  (void)ctx;
+  if (!ctx) return set_error(RTB_E_INVALID, "workspace without a context");
   cudaError_t e = cudaMallocAsync(p, bytes ? bytes : 16, s);
   if (e != cudaSuccess) return cuda_status(e, "workspace cudaMallocAsync");
   return RTB_OK;

@@ -683,11 +683,11 @@ __global__ void __launch_bounds__(kReduceThreads) norm_bwd_reduce_kernel(const f
 // The sums' way out: a partial row for each CTA and the second kernel, or the
 // only CTA's own stores.
 template <typename Launch>
-int launch_with_sums(NormBwdParams& p, int grid, float* dg, float* db, cudaStream_t s,
-                     const Launch& launch) {
+int launch_with_sums(rtb_ctx* ctx, NormBwdParams& p, int grid, float* dg, float* db,
+                     cudaStream_t s, const Launch& launch) {
   float* part = nullptr;
   if (grid > 1 && (dg || db)) {
-    const int st = ws_alloc(nullptr, (void**)&part, (size_t)grid * 2 * p.d * sizeof(float), s);
+    const int st = ws_alloc(ctx, (void**)&part, (size_t)grid * 2 * p.d * sizeof(float), s);
     if (st) return st;
   }
   p.part = part;
@@ -709,7 +709,7 @@ int launch_direct(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStre
                                        2 * 16384 * (int)sizeof(float));
   if (e != cudaSuccess) return cuda_status(e, "layer_norm_backward smem attribute");
   const int grid = (int)(p.rows < ctx->sm_count ? p.rows : ctx->sm_count);
-  return launch_with_sums(p, grid, dg, db, s, [&] {
+  return launch_with_sums(ctx, p, grid, dg, db, s, [&] {
     return launch_pdl(k, dim3((unsigned)grid), dim3(kWide), smem, s, (const NormBwdParams)p, dg, db);
   });
 }
@@ -737,7 +737,7 @@ int launch_rows_as(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStr
   if (e != cudaSuccess) return cuda_status(e, "layer_norm_backward smem attribute");
   const int64_t need = (p.rows + R - 1) / R, cap = (int64_t)ctx->sm_count * kPerSm;
   const int grid = (int)(need < cap ? need : cap);
-  return launch_with_sums(p, grid, dg, db, s, [&] {
+  return launch_with_sums(ctx, p, grid, dg, db, s, [&] {
     return launch_pdl(k, dim3((unsigned)grid), dim3(kBlock), (size_t)smem, s,
                       (const NormBwdParams)p, T, 1.0f / (float)p.d, dg, db);
   });
