@@ -312,10 +312,18 @@ int rtb_fp8_dequantize(rtb_ctx* ctx, int64_t rows, int64_t cols, const uint8_t* 
  *            0: B is [K,N] row-major, scale_b [ceil(K / 128), ceil(N / 128)],
  *               block_rows_b = 128.
  *   scale_type_*: RTB_SCALE_E8M0 bytes or RTB_SCALE_F32 floats (weights scaled
- *   elsewhere); the product of the two blocks' scales is taken in fp32.
+ *   elsewhere), one of each or twice the same.
  *   bias: [N] or NULL.  act: any RTB_ACT_*.
- * The products of a 128-element block are summed on the tensor cores, the
- * blocks in fp32.  K = 0 gives act(bias) or zeros. */
+ * Accuracy, relative to S = sum over k of |deq(A) deq(B)|: the products of codes
+ * are exact and are summed in the tensor core's accumulator, 32 at a time, where
+ * an addition truncates (at most 2^-21 of the sum so far).  Twice e8m0: the
+ * tensor core applies the scales, and the sum is added up in fp32 after every
+ * 1024 elements, 2048 for products of many tiles; measured at most 6.2e-8 S on
+ * normal operands and 1.2e-5 S on positive ones with a long tail.  With a float
+ * scale: after every 128 elements, where the two scales are applied in fp32 (as
+ * their product, or one behind the other); 3.3e-8 S and 2.0e-6 S.  Scales whose
+ * product leaves fp32's range are outside of this.  K = 0 gives act(bias) or
+ * zeros. */
 int rtb_fp8_matmul(rtb_ctx* ctx, int64_t M, int64_t N, int64_t K, const uint8_t* A, int64_t lda,
                    const void* scale_a, int64_t ldsa, int block_rows_a, int scale_type_a,
                    const uint8_t* B, int64_t ldb, int transB, const void* scale_b, int64_t ldsb,
@@ -324,8 +332,14 @@ int rtb_fp8_matmul(rtb_ctx* ctx, int64_t M, int64_t N, int64_t K, const uint8_t*
 /* rtb_matmul_backward with A kept as an 8-bit checkpoint (rtb_fp8_quantize):
  *   dA = dC . B^T          when dA != NULL (does not read the checkpoint)
  *   dB = deq(A)^T . dC     when dB != NULL (does not read B)
- * B [K,N], dC [M,N], dA [M,K], dB [K,N] fp32, row-major contiguous.  The
- * checkpoint's values enter exactly and dC with 24 bits (RTB_PREC_TF32: 16). */
+ * B [K,N], dC [M,N], dA [M,K], dB [K,N] fp32, row-major contiguous.  For dB the
+ * checkpoint's values enter as bf16: exactly under scales of 2^-124 and more (below,
+ * bf16's smallest step, 2^-133, rounds the last bits of the smallest).  dC enters
+ * as the sum of three bf16 terms: all of its 24 bits from 2^-110 on, fewer below, where the third term leaves bf16's range (RTB_PREC_TF32: two
+ * terms, 16 bits).  The tensor core's sums (see rtb_fp8_matmul) are added up in fp32
+ * after every 128 rows: of sum |deq(A) dC| they were off by at most 5.5e-8 on
+ * normal operands, 2.6e-6 on positive ones with a long tail.  Workspace while the
+ * call runs: 2 M K + 6 M N bytes (two terms: 4 M N), both operands in bf16. */
 int rtb_matmul_backward_fp8(rtb_ctx* ctx, int64_t M, int64_t N, int64_t K, const uint8_t* A,
                             int64_t lda, const uint8_t* scale_a, int64_t ldsa, int block_rows_a,
                             const float* B, const float* dC, float* dA, float* dB, int accumulate,

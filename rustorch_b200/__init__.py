@@ -357,7 +357,7 @@ def fp8_matmul(a, a_scale, b, b_scale, bias=None, act: int = ACT_NONE, out=None)
     """C = act(deq(a) @ deq(b) + bias), float32, for block-scaled 8-bit a [M,K]
     and b [K,N].  b is a Linear weight's transposed view (w.t(), with its
     scales' ws.t()) or a row-major matrix with 128 x 128 blocks; scales are
-    float8_e8m0fnu or float32."""
+    float8_e8m0fnu or float32.  (How exact: rtb_fp8_matmul in the C header.)"""
     return (_ops_module or _load_ops()).fp8_matmul(a, a_scale, b, b_scale, bias, act, out)
 
 
@@ -366,7 +366,8 @@ def matmul_backward_fp8(a, a_scale, b, grad, need_a: bool = True, need_b: bool =
     """matmul_backward of c = a @ b with a [M,K] kept as an 8-bit checkpoint
     (fp8_quantize): (grad @ b.T, deq(a).T @ grad); b (float32 [K,N]) is read for
     the first only and may be None without it.  With accumulate the results
-    are added to out_a / out_b."""
+    are added to out_a / out_b.  The second takes a workspace of 2 M K + 6 M N
+    bytes while it runs."""
     return (_ops_module or _load_ops()).matmul_backward_fp8(a, a_scale, b, grad, need_a, need_b, out_a,
                                                        out_b, accumulate, precision)
 

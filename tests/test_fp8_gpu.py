@@ -253,6 +253,30 @@ def test_product_long(gpu, m, n, k, rb):
     check_product(gpu, a, sa, cycled(w, n), cycled(sw, -(-n // rb)))
 
 
+# every kernel, with as long a chain in the tensor core's accumulator as it makes
+@pytest.mark.parametrize("m,n,k", [(1, 2048, 16384), (16, 2048, 16384), (64, 20000, 8192), (300, 2048, 8192),
+                                   (2048, 8192, 1024), (2600, 2100, 16384), (8192, 4096, 4096)])
+@pytest.mark.parametrize("floats", [False, True])
+def test_product_of_one_sign(gpu, m, n, k, floats):
+    """Positive operands with a long tail: nothing cancels, and every addition of the
+    accumulator truncates the same way.  A step of 32 products is off by at most
+    2^-21 of the running sum; float scales promote it every 4 steps, e8m0 scales
+    every 64 at most."""
+    g = torch.Generator(device="cuda").manual_seed(33)
+
+    def heavy(rows, block_rows):
+        return gpu.fp8_quantize(torch.exp(3 * torch.randn((rows, k), device="cuda", generator=g)), block_rows)
+
+    a, sa = heavy(m, 1)
+    w, sw = heavy(n, 128)
+    z = values64(a, sa) @ values64(w, sw).t()
+    if floats:
+        sw = torch.pow(2.0, sw.view(torch.uint8).float() - 127)
+    c = gpu.fp8_matmul(a, sa, w.t(), sw.t())
+    steps = 4 if floats else 64
+    assert bool(((c.double() - z).abs() <= z * (steps * 2.0 ** -21 + (k / 128 + 2) * 2.0 ** -24)).all())
+
+
 @pytest.mark.parametrize("m,n", [(5, 140), (150, 200), (2600, 2100)])
 def test_product_scale_range(gpu, m, n):
     """Scales far from 1 that cancel, the smallest byte, and byte 255 (NaN), on
