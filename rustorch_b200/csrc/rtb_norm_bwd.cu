@@ -13,12 +13,14 @@
 // registers (in shared memory for rows beyond 8192 columns, where 1024 threads
 // leave 64 registers each), added up over a CTA's groups in group order, left in
 // a row of a [CTA][2][d] workspace, and the CTAs' rows are added by a second
-// kernel.  No atomics: the order depends on the shape alone.  A single CTA writes
+// kernel.  No atomics: the order depends on the sizes, the alignment (which kernel)
+// and the device (how many CTAs) alone.  A single CTA writes
 // its sums itself.  Rows beyond 16384 columns take a CTA each and three passes.
 //
 // Measured: 8192 x 4096 75 us (5.4 TB/s of the 12 bytes an element, 82% of a copy),
 // 16384 x 2048 from a checkpoint 67 us (4.5 TB/s of 9 bytes: the instructions of
-// the row's fixed part count as much), 2048 x 16384 111 us, 8192 x 4097 129 us.
+// the row's fixed part count as much), 2048 x 16384 108 us, 8192 x 4097 130 us;
+// 8192 x 4096 with sigmoid 99 us, with tanh 101.
 #include "rtb_act.cuh"
 #include "rtb_f32x2.cuh"
 #include "rtb_fp8.cuh"
@@ -50,14 +52,16 @@ struct NormBwdParams {
   int accumulate;
 };
 
-// e / (1 + e)^2 of two values in [0, 1].  The reciprocal is the instruction's own
-// (1 ulp; with correctly rounded ones 8192 x 4096 takes 112 us for sigmoid and not 99).
+// e / (1 + e)^2 of two values in [0, 1], as e / (1 + e (2 + e)), which rounds less.
+// The reciprocal is the instruction's own (1 ulp; with correctly rounded quotients
+// 8192 x 4096 takes 112 us for sigmoid and not 99).
 __device__ __forceinline__ unsigned long long bell2(float e0, float e1) {
-  float q0, q1;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q0) : "f"(1.0f + e0));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q1) : "f"(1.0f + e1));
-  const unsigned long long q = pack2(q0, q1);
-  return mul2(mul2(pack2(e0, e1), q), q);
+  const unsigned long long e = pack2(e0, e1);
+  const float2 d = unpack2(fma2(e, add2(e, pack2(2.0f, 2.0f)), pack2(1.0f, 1.0f)));
+  float r0, r1;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(d.y));
+  return mul2(e, pack2(r0, r1));
 }
 // act'(z) as a function of z, of two values; ReLU's derivative is 0 at 0 and for
 // NaN, as its forward maps both to 0.  With e = exp(-|z|) sigmoid's is e / (1 +
@@ -209,8 +213,8 @@ __device__ __forceinline__ void copy_row(uint32_t dst, const void* row, int byte
 // a checkpoint 8192 x 4097: 349 us by direct loads, 160 here; 65536 x 301: 167,
 // 102; fp32 x 8192 x 4097, one group on an SM: 133, 129).  fp32 rows of up to 4096
 // columns are loaded into registers directly: with more groups on an SM the
-// copies cost more than they hide (65536 x 301: 63 us, 88 by copies; 1531 x 1001
-// with tanh 14.3, 16.7).
+// copies cost more than they hide (65536 x 301: 62 us, 87 by copies; 1531 x 1001
+// with tanh 13.2, 15.6).
 template <int kBlock, bool VEC, bool SAVED>
 constexpr bool kRows = VEC || SAVED || kBlock > 512;  // rows through the ring
 
