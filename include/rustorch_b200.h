@@ -269,7 +269,8 @@ int rtb_layer_norm_fwd(rtb_ctx* ctx, int64_t rows, int64_t d, const float* x, in
  *   dbias   = sum over rows of dz                      when dbias != NULL
  * norm_weight / norm_bias as in the forward call (NULL: 1 and 0).  accumulate
  * != 0 adds into dx, dweight and dbias.  The sums are fp32 in an order that
- * depends on the shape alone (the same bits on every call).  ReLU's derivative
+ * depends on the sizes, the alignment and the device alone (the same bits on
+ * every such call).  ReLU's derivative
  * is 0 where z is 0 or NaN. */
 int rtb_layer_norm_backward(rtb_ctx* ctx, int64_t rows, int64_t d, const float* x, int64_t ldx,
                             const float* mean, const float* rstd, const float* norm_weight,

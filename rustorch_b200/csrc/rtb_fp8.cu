@@ -2,7 +2,8 @@
 //   save:    s = 2^ceil(log2(max|x| / 448)) over the block, q = e4m3(x / s)
 //   restore: x' = q * s
 // Both stream their operands once (5 bytes a value): HBM-bound, 16384 x 4096
-// saved and restored in 133 us (5.0 TB/s, 77% of a copy).
+// saved and restored in 132 us (5.1 TB/s, 78% of a copy); saved alone 77 us, in 128 x
+// 128 blocks 100 us (3.4 TB/s), a CTA a block.
 #include <cuda_bf16.h>
 
 #include "rtb_fp8.cuh"

@@ -14,10 +14,14 @@
 // that is 32768 multiply-adds per 512 clocks of MMAs, half of the SM's fp32
 // lanes; packed f32x2 instructions halve the issue slots.
 //
-// Measured: MODE 0 (f32 scales) 8192 x 4096 x 8192 in 370 us, 1490 TFLOP/s, bound
-// by the epilogue's chain of barrier, TMEM loads and adds (about 1150 clocks a
-// block); MODE 1 8192 x 4096 x 4096 in 550 us beside 60 us for its operands, 1.5
-// PFLOP/s of bf16 MMAs, bound by them.
+// Measured: MODE 0 (f32 scales, one for each 128 columns) 8192 x 4096 x 8192 in 381
+// us alone, 392 in a loop, 1400 TFLOP/s, bound by the epilogue's chain of barrier,
+// TMEM loads and adds (about 1150 clocks a block); with a scale for each column 547,
+// its epilogue multiplies twice.  MODE 1 8192 x 4096 x 4096 in 633 us alone, 707 to
+// 733 in a loop (the power cap), 60 of them for its operands: 1.1 to 1.4 PFLOP/s of
+// bf16 MMAs, bound by them.  Outputs that TMA cannot store (ldc off a multiple of 4)
+// leave by scalar stores: 8192 x 4097 x 8192 777 us against 547, MODE 1 8192 x 4097
+// x 4096 849 against 707.
 //
 // Roles (warps of each CTA): 0, 2, 3 TMA producers; 1 TMEM allocation, and in the
 // pair's first CTA the MMA issue for both; 4..11 epilogue (lanes 32 (w % 4)..,
