@@ -464,7 +464,11 @@ int launch(rtb_ctx* ctx, const CUtensorMap& tmX, const CUtensorMap& tmY, BlockPa
   const int64_t tiles = (int64_t)p.tiles_x * p.tiles_y;
   if (tiles > INT32_MAX / 2) return set_error(RTB_E_UNSUPPORTED, "pair gemm: too many tiles");
   CUtensorMap tmC = tmX;
-  p.c_tma = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 && p.ldo % 4 == 0;
+  // (A TMA store clips a box at the tensor's columns in units of 16 bytes: up to three
+  // floats behind a row whose length is no multiple of 4 would be overwritten.  A test
+  // for each chunk, as in rtb_mxgemm.cu, makes the epilogue with column scales spill:
+  // 8192 x 4096 x 8192 547 -> 596 us.)
+  p.c_tma = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 && p.ldo % 4 == 0 && p.ycols % 4 == 0;
   if (p.c_tma) {
     const int st = make_tmap_2d(&tmC, p.out, (uint64_t)p.ycols, (uint64_t)p.xrows, (uint64_t)p.ldo,
                                 32, 128, false);

@@ -234,6 +234,26 @@ def test_product_scales_of_consecutive_tiles(gpu, k):
         assert torch.equal(gpu.fp8_matmul(a, sa, w.t(), sw.t()), first)
 
 
+# rows of the output with a pitch of whole 16 bytes, their length not
+@pytest.mark.parametrize("m,n,pad", [(5000, 1018, 2), (5000, 1017, 3), (5000, 1019, 1), (5000, 1018, 6),
+                                     (5000, 1016, 4), (2600, 2051, 1), (9500, 1, 3), (9500, 5, 11),
+                                     (300, 601, 3), (40, 1001, 3)])
+@pytest.mark.parametrize("floats", [False, True])
+def test_product_leaves_the_row_padding(gpu, m, n, pad, floats):
+    """What lies behind a row of the output stays as it was, behind the last row too."""
+    k = 200
+    a, sa = operand(m, k, 1, 34)
+    w, sw = operand(n, k, 1, 35)
+    if floats:
+        sw = torch.pow(2.0, sw.view(torch.uint8).float() - 127)
+    big = torch.full((m * (n + pad) + 64,), 7.0, device="cuda")
+    out = big.as_strided((m, n), (n + pad, 1), 0)
+    check_product(gpu, a, sa, w, sw, torch.ones(n, device="cuda"), 0, out=out)
+    rest = torch.ones_like(big, dtype=torch.bool)
+    rest.as_strided((m, n), (n + pad, 1), 0)[:] = False
+    assert bool((big[rest] == 7.0).all())
+
+
 # long contractions: more blocks for a CTA than its scale buffers hold, one CTA a
 # tile and every size of cluster, a tile more or fewer than run at once
 LONG = [(3, 20000, 4224), (20, 19000, 5000), (64, 20000, 6400), (7, 2048, 16500), (30, 1000, 9000),
