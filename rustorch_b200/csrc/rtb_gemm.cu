@@ -270,6 +270,11 @@ int gemm_run(rtb_ctx* ctx, const GemmDesc& d, cudaStream_t stream) {
         RTB_OK)
       p.c_tma = 1;
   }
+  // A TMA store clips a box at the tensor's columns in units of 16 bytes: up to
+  // three floats behind a row whose length is no multiple of 4 would be
+  // overwritten.  There the 32-column chunks that lie in the row as a whole are
+  // stored by TMA, the last one directly.
+  p.tma_n = !p.c_tma ? 0 : d.N % 4 == 0 ? INT32_MAX : (int)(d.N / 32 * 32);
   p.x = d.x;
   p.H = d.H;
   p.W = d.W;

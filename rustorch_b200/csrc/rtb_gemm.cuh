@@ -75,7 +75,8 @@ struct GemmParams {
   int hw;                // Ho*Wo for out_mode 1
   const float* row_bias; // out_mode 1: [M] bias per row (C^T of a skinny GEMM), or null
   int vec_ok;            // 16-byte aligned C/residual/bias with ldc, ldr % 4 == 0
-  int c_tma;             // out_mode 0 with a TMA-storable C (tmC valid)
+  int c_tma;             // out_mode 0 with a TMA-storable C (tmC valid):
+  int tma_n;             // chunks that begin before this column leave by TMA
   int vec4_nchw;         // out_mode 1: C and residual 16-byte aligned
   // implicit-GEMM conv (A gathered from NHWC input with Cp channels, Cp % 4 == 0)
   const float* x;
@@ -774,7 +775,7 @@ __global__ void __launch_bounds__(GemmRoles<SPLIT, A_MODE == 1>::kThreads, 1)
     auto emit = [&](int tm, int tn, int c, int m, const uint32_t (&r)[32]) {
       const int n0 = tn * BN + c;
       const uint32_t sb = smem_u32(sBias) + 4 * c;
-      if (p.c_tma) {
+      if (n0 < p.tma_n) {
         uint8_t* stg = sOut + (chunk % Cfg::kOutBufs) * kOutChunkBytes;
         epilogue_stage_rowmajor(p, smem_u32(stg), row, n0, m, r, sb);
         fence_proxy_async_smem();

@@ -587,3 +587,28 @@ def test_skinny_transposed_strided_output(gpu, orc, pad, act):
     ref = {0: pre, 2: 1.0 / (1.0 + np.exp(-pre)), 3: np.tanh(pre)}[act]
     assert orc.rel_frob(got[:, :n], ref) <= TOL[0]
     assert np.all(got[:, n:] == 7.0)
+
+
+@pytest.mark.parametrize("m,n,pad", [(300, 1018, 2), (300, 1017, 3), (300, 1019, 1), (129, 70, 6),
+                                     (1, 2050, 2), (9, 61, 3), (100, 2051, 1), (2000, 2050, 2),
+                                     (300, 1016, 4)])
+@pytest.mark.parametrize("k", [40, 2048])
+@pytest.mark.parametrize("precision", [0, 1])
+def test_row_padding_of_the_output_is_left(gpu, m, n, pad, k, precision):
+    """Rows of the output at a pitch of whole 16 bytes whose length is not: what lies
+    behind them, behind the last one too, stays as it was."""
+    import torch
+    g = torch.Generator().manual_seed(1)
+    a, b = torch.randn((m, k), generator=g).cuda(), torch.randn((k, n), generator=g).cuda()
+    bias = torch.randn(n, generator=g).cuda()
+    big = torch.full((m * (n + pad) + 64,), 7.0, device="cuda")
+    out = big.as_strided((m, n), (n + pad, 1), 0)
+    gpu.sgemm(a, b, bias, precision=precision, out=out)
+    ref = a.double() @ b.double() + bias.double()
+    size = a.double().abs() @ b.double().abs() + bias.double().abs()
+    # TF32 operands keep 11 bits (an error of 2^-10 for truncation, twice)
+    tol = 2.0 ** -18 if precision == 0 else 2.0 ** -9
+    assert bool(((out.double() - ref).abs() <= tol * size).all())
+    rest = torch.ones_like(big, dtype=torch.bool)
+    rest.as_strided((m, n), (n + pad, 1), 0)[:] = False
+    assert bool((big[rest] == 7.0).all())
