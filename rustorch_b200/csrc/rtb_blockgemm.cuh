@@ -31,7 +31,6 @@ struct BlockParams {
   const float *tabx, *taby;
   int64_t pitchx, pitchy;
   int c_tma;             // CTA pairs: rows of the output leave through TMA stores
-  int tma_cols;          // rtb_mxgemm.cu: chunks that begin before this column do
   int parts;             // CTAs that share a tile (a cluster)
   int vec_ok;            // 16-byte aligned output rows and bias
   int* err;

@@ -25,9 +25,9 @@
 // for their loads and fences.)
 //
 // Measured: 8192 x 4096 x 8192 in 212 us alone, 262 to 273 in a loop (the power cap),
-// 2.1 PFLOP/s; 8192 x 8192 x 1024 in 108.  Outputs that TMA cannot store (ldc off a
-// multiple of 4) leave by scalar stores, 32 rows an instruction: 8192 x 4097 x 8192
-// 429 us.
+// 2.1 PFLOP/s; 8192 x 8192 x 1024 in 97 and 105.  Outputs that TMA cannot store (N or
+// ldc off a multiple of 4) leave by scalar stores, 32 rows an instruction: 8192 x 4097
+// x 8192 429 us.
 #include "rtb_pair.cuh"
 
 namespace rtb {
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < 16; ++j) v[j] += bias_s[128 * half + 16 * c + j];
         }
         activate_n<16>(v, p.act);
-        if ((int)yc < p.tma_cols) {
+        if (p.c_tma) {
           // this chunk's store before has read it (its issuing thread waits): with
           // one chunk a half the waits made a tile's epilogue 6 us long
           uint8_t* stg = stg0 + buf * kChunk;
@@ -415,11 +415,11 @@ int launch(rtb_ctx* ctx, const uint8_t* X, int64_t ldx, const uint8_t* Y, int64_
                                TN / 2)))
     return st;
   CUtensorMap tmC = tmX;
-  p.c_tma = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 && p.ldo % 4 == 0;
-  // A TMA store clips a box at the tensor's columns in units of 16 bytes: up to three
-  // floats behind a row whose length is no multiple of 4 would be overwritten.  There
-  // the chunks that lie in the row as a whole are stored by TMA, the last directly.
-  p.tma_cols = !p.c_tma ? 0 : p.ycols % 4 == 0 ? INT32_MAX : (int)(p.ycols / 16 * 16);
+  // (A TMA store clips a box at the tensor's columns in units of 16 bytes: up to three
+  // floats behind a row whose length is no multiple of 4 would be overwritten.  A test
+  // for each chunk, so that only a row's last one is stored directly, costs the others
+  // 2 us of 97 on 8192 x 8192 x 1024.)
+  p.c_tma = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 && p.ldo % 4 == 0 && p.ycols % 4 == 0;
   if (p.c_tma && (st = make_tmap_2d_swz(&tmC, p.out, (uint64_t)p.ycols, (uint64_t)p.xrows,
                                         (uint64_t)p.ldo, 16, 128, kTmapSwizzle64)))
     return st;

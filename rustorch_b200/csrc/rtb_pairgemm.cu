@@ -19,7 +19,7 @@
 // TMEM loads and adds (about 1150 clocks a block); with a scale for each column 547,
 // its epilogue multiplies twice.  MODE 1 8192 x 4096 x 4096 in 633 us alone, 707 to
 // 733 in a loop (the power cap), 60 of them for its operands: 1.1 to 1.4 PFLOP/s of
-// bf16 MMAs, bound by them.  Outputs that TMA cannot store (ldc off a multiple of 4)
+// bf16 MMAs, bound by them.  Outputs that TMA cannot store (N or ldc off a multiple of 4)
 // leave by scalar stores: 8192 x 4097 x 8192 777 us against 547, MODE 1 8192 x 4097
 // x 4096 849 against 707.
 //
@@ -466,8 +466,8 @@ int launch(rtb_ctx* ctx, const CUtensorMap& tmX, const CUtensorMap& tmY, BlockPa
   CUtensorMap tmC = tmX;
   // (A TMA store clips a box at the tensor's columns in units of 16 bytes: up to three
   // floats behind a row whose length is no multiple of 4 would be overwritten.  A test
-  // for each chunk, as in rtb_mxgemm.cu, makes the epilogue with column scales spill:
-  // 8192 x 4096 x 8192 547 -> 596 us.)
+  // for each chunk makes the epilogue with column scales spill: 8192 x 4096 x 8192 547
+  // -> 596 us.)
   p.c_tma = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 && p.ldo % 4 == 0 && p.ycols % 4 == 0;
   if (p.c_tma) {
     const int st = make_tmap_2d(&tmC, p.out, (uint64_t)p.ycols, (uint64_t)p.xrows, (uint64_t)p.ldo,
