@@ -286,6 +286,44 @@ int rtb_layer_norm_backward_fp8(rtb_ctx* ctx, int64_t rows, int64_t d, const uin
                                 float* dx, int64_t lddx, float* dweight, float* dbias,
                                 int accumulate, void* stream);
 
+/* ---------------------------------------------------------------- root-mean-square norm */
+/* (Extension: the reference has layer norm only.)  For every row,
+ *   h = x + residual,  rstd = 1 / sqrt(mean(h^2) + eps),  y = h * rstd * norm_weight
+ * residual NULL: h = x; norm_weight [d] or NULL (1).  sum (NULL: not wanted)
+ * receives h, the residual stream behind this addition; rstd (rows floats, NULL:
+ * not wanted) is what the backward pass reads, together with h.  y and sum may each
+ * be x or residual (in place, with the same leading dimension), but not the same
+ * place.  d >= 1.  h is rounded to fp32 once and enters the sum of squares and y as
+ * rounded. */
+int rtb_rms_norm_fwd(rtb_ctx* ctx, int64_t rows, int64_t d, const float* x, int64_t ldx,
+                     const float* residual, int64_t ldr, const float* norm_weight, float eps,
+                     float* sum, int64_t ldsum, float* y, int64_t ldy, float* rstd, void* stream);
+/* The same with y as 8-bit blocks of 128 columns (q [rows, d] e4m3, scale [rows,
+ * ceil(d / 128)] e8m0: what rtb_fp8_quantize with block_rows = 1 makes of y), the
+ * left operand of rtb_fp8_matmul. */
+int rtb_rms_norm_fp8(rtb_ctx* ctx, int64_t rows, int64_t d, const float* x, int64_t ldx,
+                     const float* residual, int64_t ldr, const float* norm_weight, float eps,
+                     float* sum, int64_t ldsum, uint8_t* q, int64_t ldq, uint8_t* scale,
+                     int64_t lds, float* rstd, void* stream);
+/* Gradients for the incoming gradient dy [rows, d] of y and, where it is not NULL,
+ * dsum [rows, d] of h (the residual stream's); x is the forward pass's h.  With u =
+ * x * rstd and g = dy * norm_weight:
+ *   dx      = rstd * (g - u * mean(g * u)) + dsum     when dx != NULL
+ *   dweight = sum over rows of dy * u                 when dweight != NULL
+ * dx is the gradient of both the forward pass's x and its residual; it may be dy's or
+ * dsum's place.  accumulate != 0 adds into dx and dweight.  The sums are fp32 in an
+ * order that depends on the sizes, the alignment and the device alone. */
+int rtb_rms_norm_backward(rtb_ctx* ctx, int64_t rows, int64_t d, const float* x, int64_t ldx,
+                          const float* rstd, const float* norm_weight, const float* dy,
+                          int64_t lddy, const float* dsum, int64_t ldds, float* dx, int64_t lddx,
+                          float* dweight, int accumulate, void* stream);
+/* The same with x kept as an 8-bit checkpoint (rtb_fp8_quantize, block_rows = 1). */
+int rtb_rms_norm_backward_fp8(rtb_ctx* ctx, int64_t rows, int64_t d, const uint8_t* q,
+                              int64_t ldq, const uint8_t* scale, int64_t lds, const float* rstd,
+                              const float* norm_weight, const float* dy, int64_t lddy,
+                              const float* dsum, int64_t ldds, float* dx, int64_t lddx,
+                              float* dweight, int accumulate, void* stream);
+
 /* ---------------------------------------------------------------- 8-bit block-scaled tensors */
 /* (Extension: the reference's tensors are f32 only.)  q [rows, cols] e4m3
  * bytes, row stride ldq, and one scale for each block of 128 columns of one
@@ -345,6 +383,36 @@ int rtb_matmul_backward_fp8(rtb_ctx* ctx, int64_t M, int64_t N, int64_t K, const
                             int64_t lda, const uint8_t* scale_a, int64_t ldsa, int block_rows_a,
                             const float* B, const float* dC, float* dA, float* dB, int accumulate,
                             int precision, void* stream);
+
+/* ---------------------------------------------------------------- 4-bit block-scaled tensors */
+/* (Extension.)  q [rows, ceil(cols / 2)] bytes of two e2m1 codes, the even column in
+ * the low half (row stride ldq, bytes), and one scale for each block of 32 columns of
+ * a row: scale [rows, ceil(cols / 32)] e8m0 bytes, row stride lds: value = code *
+ * 2^(byte - 127) with the codes 0, 1/2, 1, 3/2, 2, 3, 4, 6 and a sign.  The byte that
+ * rtb_fp4_quantize writes is the smallest whose power of two holds the block's largest
+ * magnitude within 6 (at least 1; 127 for a block of zeros): nothing saturates, the
+ * scaling is exact and a value is rounded once, to nearest even: by at most 1 where
+ * the scaled magnitude is over 4, 1/2 over 2, 1/4 below.  A block that holds an
+ * infinity or NaN has the byte 255 (all of its values are NaN) and codes 0.  The half
+ * byte behind an odd last column is 0.
+ * transX = 0: x is [rows, cols] with ldx >= cols; 1: x lies as its transpose [cols,
+ * rows] with ldx >= rows (the blocks run down its columns), as the products of a
+ * backward pass take a gradient, an activation or a weight. */
+int rtb_fp4_quantize(rtb_ctx* ctx, int64_t rows, int64_t cols, const float* x, int64_t ldx,
+                     int transX, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds,
+                     void* stream);
+/* y = q * scale. */
+int rtb_fp4_dequantize(rtb_ctx* ctx, int64_t rows, int64_t cols, const uint8_t* q, int64_t ldq,
+                       const uint8_t* scale, int64_t lds, float* y, int64_t ldy, void* stream);
+/* C[M,N] = act(deq(A) . deq(B)^T + bias), fp32 out, row-major C with ldc.  A [M,K] and
+ * B [N,K] (nn::Linear's weight) as rtb_fp4_quantize writes them, K elements to a row
+ * (even: two lie in a byte; a quantised row of odd length counts its zero), lda and ldb
+ * in bytes; scale_a [M, ceil(K / 32)], scale_b [N, ceil(K / 32)].  bias [N] or NULL;
+ * act: any RTB_ACT_*.  K = 0 gives act(bias) or zeros. */
+int rtb_fp4_matmul(rtb_ctx* ctx, int64_t M, int64_t N, int64_t K, const uint8_t* A, int64_t lda,
+                   const uint8_t* scale_a, int64_t ldsa, const uint8_t* B, int64_t ldb,
+                   const uint8_t* scale_b, int64_t ldsb, const float* bias, int act, float* C,
+                   int64_t ldc, void* stream);
 
 /* ---------------------------------------------------------------- small ops */
 /* ops::max_pool2d (rustorch-core/src/ops/pool.rs:115-191): -inf init, padding skipped. */

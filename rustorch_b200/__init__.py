@@ -11,7 +11,8 @@ C ABI in include/rustorch_b200.h:
     jit.Graph / NodeType / Optimizer / Executor  rustorch-core/src/jit.rs
 
 Beyond the reference: 8-bit block-scaled tensors (fp8_quantize) as activation
-checkpoints and as operands of fp8_matmul.
+checkpoints and as operands of fp8_matmul, the root-mean-square norm, and 4-bit
+block-scaled tensors (fp4_quantize) as operands of fp4_matmul.
 
 Tensors are torch CUDA float32 tensors (torch provides device memory and
 streams only; all arithmetic runs in this library's kernels).  Calls are
@@ -30,7 +31,8 @@ __all__ = ["Context", "get_context", "sgemm", "sgemm_batched", "matmul_bias_norm
            "layer_norm",
            "conv2d_fwd", "matmul_backward",
            "conv2d_backward", "layer_norm_fwd", "layer_norm_backward", "fp8_quantize",
-           "fp8_dequantize", "fp8_matmul", "matmul_backward_fp8", "max_pool2d",
+           "fp8_dequantize", "fp8_matmul", "matmul_backward_fp8", "rms_norm_fwd", "rms_norm_fp8",
+           "rms_norm_backward", "fp4_quantize", "fp4_dequantize", "fp4_matmul", "max_pool2d",
            "global_avg_pool", "add", "relu", "fill_normal", "fill_uniform", "RtbError",
            "ACT_NONE", "ACT_RELU", "ACT_SIGMOID", "ACT_TANH", "PREC_3XTF32", "PREC_TF32",
            "PREC_DEFAULT", "LAYOUT_NCHW", "LAYOUT_NHWC", "lib"]
@@ -370,6 +372,60 @@ def matmul_backward_fp8(a, a_scale, b, grad, need_a: bool = True, need_b: bool =
     bytes while it runs."""
     return (_ops_module or _load_ops()).matmul_backward_fp8(a, a_scale, b, grad, need_a, need_b, out_a,
                                                        out_b, accumulate, precision)
+
+
+def rms_norm_fwd(x, norm_weight=None, eps: float = 1e-5, residual=None, out=None, out_sum=None):
+    """(y, sum, rstd): the root-mean-square norm over the last dimension of sum =
+    x + residual (x itself without one), y = sum * rstd * norm_weight, with rstd =
+    1 / sqrt(mean(sum^2) + eps) of every row (float32 of x's leading shape).  sum and
+    rstd are what rms_norm_backward reads.  out and out_sum may each be x or residual
+    (the residual stream is updated in place); without a residual sum is x (copied
+    where out_sum is given, and gone where out is x)."""
+    return (_ops_module or _load_ops()).rms_norm_fwd(x, norm_weight, eps, residual, out, out_sum)
+
+
+def rms_norm_fp8(x, norm_weight=None, eps: float = 1e-5, residual=None, out_sum=None):
+    """(q, scale, sum, rstd): rms_norm_fwd with its y as fp8_quantize(y) holds it
+    (float8_e4m3fn values, a power-of-two scale for each 128 columns), fp8_matmul's
+    left operand, in one pass."""
+    return (_ops_module or _load_ops()).rms_norm_fp8(x, norm_weight, eps, residual, out_sum)
+
+
+def rms_norm_backward(x, rstd, grad, norm_weight=None, grad_sum=None, x_scale=None,
+                      need_x: bool = True, need_weight: bool = True, out_x=None, out_weight=None,
+                      accumulate: bool = False):
+    """Gradients (dx, dweight) of rms_norm_fwd for the incoming gradient `grad` of y
+    and `grad_sum` of sum (the residual stream's; None: 0).  x is the forward's sum,
+    float32 or an 8-bit checkpoint (fp8_quantize(sum) -> x, x_scale); dx is the
+    gradient of both the forward's x and its residual, and out_x may be grad or
+    grad_sum.  With accumulate the results are added to out_x / out_weight."""
+    return (_ops_module or _load_ops()).rms_norm_backward(
+        x, rstd, grad, norm_weight, grad_sum, x_scale, need_x, need_weight, out_x, out_weight,
+        accumulate)
+
+
+def fp4_quantize(x):
+    """(q, scale): x [..., cols] as 4-bit e2m1 codes (float4_e2m1fn_x2 [...,
+    ceil(cols / 2)], two to a byte) with one power-of-two scale (float8_e8m0fnu) for
+    each 32 columns of a row.  The transposed view x.t() of a row-major matrix is read
+    as it lies.  An operand of fp4_matmul."""
+    return (_ops_module or _load_ops()).fp4_quantize(x)
+
+
+def fp4_dequantize(q, scale, cols=None, out=None):
+    """The float32 values of fp4_quantize's (q, scale); `cols` of them in a row (two
+    for each byte if not given)."""
+    return (_ops_module or _load_ops()).fp4_dequantize(q, scale, -1 if cols is None else cols, out)
+
+
+def fp4_matmul(a, a_scale, b, b_scale, bias=None, act: int = ACT_NONE, out=None):
+    """C = act(deq(a) @ deq(b) + bias), float32, for 4-bit block-scaled a (the values
+    [M,K], held as [M, K/2] bytes) and b, a Linear weight's transposed view (w.t(), with
+    its scales' ws.t()) of w = fp4_quantize(weight [N,K]).  A backward pass runs through
+    the same call: with dy = fp4_quantize(grad) and wt = fp4_quantize(weight.t()) the
+    input's gradient is fp4_matmul(*dy, wt.t(), ...), and with fp4_quantize(grad.t()) and
+    fp4_quantize(x.t()) the weight's."""
+    return (_ops_module or _load_ops()).fp4_matmul(a, a_scale, b, b_scale, bias, act, out)
 
 
 def max_pool2d(x, kernel=(3, 3), stride=(2, 2), padding=(1, 1), layout: int = LAYOUT_NCHW):

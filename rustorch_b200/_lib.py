@@ -77,6 +77,17 @@ SIGNATURES = {
                             _i64, _i, _i, _p, _i, _p, _i64, _p]),
     "rtb_matmul_backward_fp8": (_i, [_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _i, _p, _p, _p, _p,
                                      _i, _i, _p]),
+    "rtb_rms_norm_fwd": (_i, [_p, _i64, _i64, _p, _i64, _p, _i64, _p, _f, _p, _i64, _p, _i64, _p, _p]),
+    "rtb_rms_norm_fp8": (_i, [_p, _i64, _i64, _p, _i64, _p, _i64, _p, _f, _p, _i64, _p, _i64, _p,
+                              _i64, _p, _p]),
+    "rtb_rms_norm_backward": (_i, [_p, _i64, _i64, _p, _i64, _p, _p, _p, _i64, _p, _i64, _p, _i64,
+                                   _p, _i, _p]),
+    "rtb_rms_norm_backward_fp8": (_i, [_p, _i64, _i64, _p, _i64, _p, _i64, _p, _p, _p, _i64, _p,
+                                       _i64, _p, _i64, _p, _i, _p]),
+    "rtb_fp4_quantize": (_i, [_p, _i64, _i64, _p, _i64, _i, _p, _i64, _p, _i64, _p]),
+    "rtb_fp4_dequantize": (_i, [_p, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p]),
+    "rtb_fp4_matmul": (_i, [_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i,
+                            _p, _i64, _p]),
     "rtb_peer_buffer_create": (_i, [_p, _p, _sz, _p]),
     "rtb_peer_buffer_local": (_i, [_p, _p]),
     "rtb_peer_buffer_destroy": (_i, [_p, _p]),

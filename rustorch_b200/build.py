@@ -4,7 +4,7 @@
 
 Each csrc/*.cu and csrc/*.cpp compiles to _build/*.o in parallel, then links into
 rustorch_b200/librustorch_b200.so (NCCL is dlopen'ed at first use);
-csrc/python/ops_module.cpp (the Python calls of the training and 8-bit operators)
+csrc/python/ops_module.cpp (the Python calls of the training, 8-bit and 4-bit operators)
 compiles against torch's headers into rustorch_b200/_ops.so, and again when torch
 or Python is another one (without torch only the library is built).  A source is
 recompiled when it, any header or this file is newer than its object, and the

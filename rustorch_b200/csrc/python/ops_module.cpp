@@ -1,4 +1,4 @@
-// rustorch_b200._ops: the Python calls of the training and 8-bit operators.
+// rustorch_b200._ops: the Python calls of the training, 8-bit and 4-bit operators.
 //
 // These operators' smallest calls take less time on the GPU than an interpreted
 // wrapper takes to check their arguments, allocate their outputs and convert a
@@ -407,6 +407,246 @@ PyObject* fp8_matmul(PyObject* const* a) {
   return THPVariable_Wrap(y);
 }
 
+// A caller's output of x's shape as rows; a fresh one where none is given.
+struct Out {
+  Tensor t;
+  int64_t ld = 0;
+};
+Out output(const Tensor* out, const Tensor& x, int64_t d, const char* who, const char* name) {
+  Out o;
+  o.ld = d;
+  if (!out) {
+    o.t = empty_f32(x, x.sizes());
+    return o;
+  }
+  if (out->sizes() != x.sizes() || (d > 1 && out->stride(-1) != 1))
+    refuse(std::string(who) + ": " + name + " must have x's shape and contiguous rows");
+  o.t = *out;
+  if (!out->is_contiguous()) {
+    const Tensor o2 = out->dim() == 2 ? *out : out->view({-1, d});
+    if (o2.size(0) > 1 && o2.stride(0) < d) refuse(std::string(who) + ": " + name + "'s rows overlap");
+    o.ld = o2.stride(0) > d ? o2.stride(0) : d;
+  }
+  return o;
+}
+
+const char* const kRmsShape = "RMSNorm: Input shape does not match normalized shape";
+
+// rms_norm_fwd and rms_norm_fp8
+PyObject* rms_norm(const char* who, bool fp8, PyObject* ax, PyObject* aw, PyObject* aeps, PyObject* ar,
+                   PyObject* aout, PyObject* asum) {
+  const Tensor& x = tensor(ax, "x");
+  const Tensor* w = optional(aw, "norm_weight");
+  const float eps = (float)real(aeps);
+  const Tensor *res = optional(ar, "residual"), *out = optional(aout, "out"),
+               *out_sum = optional(asum, "out_sum");
+  for (const Tensor* t : {&x, w, res, out, out_sum}) need_f32(t);
+  same_device(x, {w, res, out, out_sum});
+  const int64_t d = x.dim() ? x.size(-1) : 0;
+  if (d == 0) refuse("RMSNorm: Input shape smaller than normalized shape");
+  if (res && res->sizes() != x.sizes()) refuse(std::string(who) + ": residual must have x's shape");
+  const Vec wv = vec(w, d, kRmsShape);
+  const Rows xr = rows_of(x, d);
+  Rows rr;
+  if (res) rr = rows_of(*res, d);
+  const bool store = res || out_sum;  // without a residual the sum is x
+  Out sum, y;
+  if (store) sum = output(out_sum, x, d, who, "out_sum");
+  Tensor q, scale;
+  const int64_t cb = (d + 127) / 128;
+  if (fp8) {
+    q = at::empty(x.sizes(), x.options().dtype(ScalarType::Float8_e4m3fn));
+    c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = cb;
+    scale = at::empty(shape, x.options().dtype(ScalarType::Float8_e8m0fnu));
+  } else {
+    y = output(out, x, d, who, "out");
+  }
+  Tensor rstd = empty_f32(x, x.sizes().slice(0, x.dim() - 1));
+  rtb_ctx* ctx = context(x.device().index());
+  void* s = stream_of(x);
+  call(fp8 ? "rtb_rms_norm_fp8" : "rtb_rms_norm_fwd", [&] {
+    const float* px = (const float*)xr.p();
+    const float* pr = res ? (const float*)rr.p() : nullptr;
+    float* ps = store ? sum.t.data_ptr<float>() : nullptr;
+    float* prstd = rstd.data_ptr<float>();
+    if (fp8)
+      return rtb_rms_norm_fp8(ctx, xr.rows, d, px, xr.ld, pr, rr.ld, wv.p, eps, ps, sum.ld,
+                              (uint8_t*)q.data_ptr(), d, (uint8_t*)scale.data_ptr(), cb, prstd, s);
+    return rtb_rms_norm_fwd(ctx, xr.rows, d, px, xr.ld, pr, rr.ld, wv.p, eps, ps, sum.ld,
+                            y.t.data_ptr<float>(), y.ld, prstd, s);
+  });
+  PyObject* total = THPVariable_Wrap(store ? sum.t : x);
+  if (fp8) return pack({THPVariable_Wrap(q), THPVariable_Wrap(scale), total, THPVariable_Wrap(rstd)});
+  return pack({THPVariable_Wrap(y.t), total, THPVariable_Wrap(rstd)});
+}
+PyObject* rms_norm_fwd(PyObject* const* a) {
+  return rms_norm("rms_norm_fwd", false, a[0], a[1], a[2], a[3], a[4], a[5]);
+}
+PyObject* rms_norm_fp8(PyObject* const* a) {
+  return rms_norm("rms_norm_fp8", true, a[0], a[1], a[2], a[3], Py_None, a[4]);
+}
+
+PyObject* rms_norm_backward(PyObject* const* a) {
+  const char* who = "rms_norm_backward";
+  const Tensor& x = tensor(a[0], "x");
+  const Tensor &rstd = tensor(a[1], "rstd"), &grad = tensor(a[2], "grad");
+  const Tensor *w = optional(a[3], "norm_weight"), *gs = optional(a[4], "grad_sum"),
+               *xs = optional(a[5], "x_scale");
+  const bool need_x = flag(a[6]), need_w = flag(a[7]);
+  const Tensor *ox = optional(a[8], "out_x"), *ow = optional(a[9], "out_weight");
+  const bool accumulate = flag(a[10]);
+  const bool saved = x.scalar_type() == ScalarType::Float8_e4m3fn;
+  for (const Tensor* t : {&rstd, &grad, w, gs, ox, ow}) need_f32(t);
+  if (saved) need_fp8(x, who);
+  else need_f32(&x);
+  same_device(x, {&rstd, &grad, w, gs, xs, ox, ow});
+  const int64_t d = x.dim() ? x.size(-1) : 0;
+  if (d == 0 || grad.sizes() != x.sizes() || (gs && gs->sizes() != x.sizes()))
+    refuse("rms_norm_backward: grad and grad_sum must have x's shape, with a last dimension");
+  const Rows xr = rows_of(x, d), gr = rows_of(grad, d);
+  Rows sr;
+  if (gs) sr = rows_of(*gs, d);
+  const Vec rv = vec(&rstd, xr.rows, "rms_norm_backward: one rstd for each row");
+  const Vec wv = vec(w, d, kRmsShape);
+  if (saved != (xs != nullptr))
+    refuse("rms_norm_backward: x_scale goes with an 8-bit x, and only with one");
+  auto dx = result(ox, need_x, accumulate, x.sizes(), grad, who);
+  auto dw = result(ow, need_w, accumulate, {d}, grad, who);
+  Scales sc;
+  if (saved) {
+    sc = scales(*xs, xr.rows, d, who);
+    if (sc.type != RTB_SCALE_E8M0 || sc.block_rows != 1)
+      refuse("rms_norm_backward: a checkpoint has a power-of-two scale for each 128 columns of a row");
+  }
+  rtb_ctx* ctx = context(x.device().index());
+  void* s = stream_of(x);
+  float *px = ptr(dx), *pw = ptr(dw);
+  call(saved ? "rtb_rms_norm_backward_fp8" : "rtb_rms_norm_backward", [&] {
+    const float* pg = (const float*)gr.p();
+    const float* ps = gs ? (const float*)sr.p() : nullptr;
+    if (saved)
+      return rtb_rms_norm_backward_fp8(ctx, xr.rows, d, (const uint8_t*)xr.p(), xr.ld,
+                                       (const uint8_t*)sc.hold.data_ptr(), sc.ld, rv.p, wv.p, pg,
+                                       gr.ld, ps, sr.ld, px, d, pw, accumulate, s);
+    return rtb_rms_norm_backward(ctx, xr.rows, d, (const float*)xr.p(), xr.ld, rv.p, wv.p, pg, gr.ld,
+                                 ps, sr.ld, px, d, pw, accumulate, s);
+  });
+  return pack({wrap(dx), wrap(dw)});
+}
+
+// A 4-bit tensor's bytes as rows (its last dimension counts them).
+Rows codes(const Tensor& t, const char* who) {
+  if (!(t.is_cuda() && t.scalar_type() == ScalarType::Float4_e2m1fn_x2))
+    refuse(std::string(who) + " expects float4_e2m1fn_x2 CUDA tensors");
+  if (t.dim() == 0) refuse(std::string(who) + ": a 4-bit tensor needs a last dimension");
+  return rows_of(t.view(ScalarType::Byte), t.size(-1));
+}
+// The rows that a tensor's leading dimensions count (a last dimension of 0 has some too).
+int64_t leading(const Tensor& t) {
+  int64_t n = 1;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) n *= t.size(i);
+  return n;
+}
+Rows scales4(const Tensor& s, int64_t rows, int64_t cols, const char* who) {
+  if (!(s.is_cuda() && s.scalar_type() == ScalarType::Float8_e8m0fnu))
+    refuse(std::string(who) + ": scales are float8_e8m0fnu CUDA tensors");
+  const int64_t cb = (cols + 31) / 32;
+  if (s.dim() < 1 || s.size(-1) != cb || leading(s) != rows)
+    refuse(std::string(who) + ": scales must be [rows, ceil(cols / 32)]");
+  return rows_of(s.view(ScalarType::Byte), cb);
+}
+
+PyObject* fp4_quantize(PyObject* const* a) {
+  const Tensor& x = tensor(a[0], "x");
+  need_f32(&x);
+  if (x.dim() == 0) refuse("fp4_quantize: x needs a last dimension");
+  const int64_t cols = x.size(-1), half = (cols + 1) / 2, cb = (cols + 31) / 32;
+  c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = half;
+  Tensor q = at::empty(shape, x.options().dtype(ScalarType::Float4_e2m1fn_x2));
+  shape.back() = cb;
+  Tensor scale = at::empty(shape, x.options().dtype(ScalarType::Float8_e8m0fnu));
+  if (x.numel()) {
+    // the transposed view of a row-major matrix stays where it is
+    const bool trans = x.dim() == 2 && !x.is_contiguous() && x.stride(0) == 1 && x.stride(1) >= x.size(0);
+    Rows xr;
+    if (trans) {
+      xr.hold = x;
+      xr.rows = x.size(0);
+      xr.ld = x.stride(1);
+    } else {
+      xr = rows_of(x, cols);
+    }
+    rtb_ctx* ctx = context(x.device().index());
+    void* s = stream_of(x);
+    call("rtb_fp4_quantize", [&] {
+      return rtb_fp4_quantize(ctx, xr.rows, cols, (const float*)xr.p(), xr.ld, trans,
+                              (uint8_t*)q.data_ptr(), half, (uint8_t*)scale.data_ptr(), cb, s);
+    });
+  }
+  return pack({THPVariable_Wrap(q), THPVariable_Wrap(scale)});
+}
+
+PyObject* fp4_dequantize(PyObject* const* a) {
+  const char* who = "fp4_dequantize";
+  const Tensor &q = tensor(a[0], "q"), &scale = tensor(a[1], "scale");
+  int64_t cols = integer(a[2]);
+  const Tensor* out = optional(a[3], "out");
+  need_f32(out);
+  same_device(q, {&scale, out});
+  const Rows qr = codes(q, who);
+  if (cols == -1) cols = 2 * q.size(-1);
+  if (cols < 0 || (cols + 1) / 2 != q.size(-1))
+    refuse("fp4_dequantize: q holds two columns in each byte of its last dimension");
+  const Rows sr = scales4(scale, leading(q), cols, who);
+  c10::SmallVector<int64_t, 6> shape(q.sizes().begin(), q.sizes().end());
+  shape.back() = cols;
+  if (out && (out->sizes() != at::IntArrayRef(shape) || !out->is_contiguous()))
+    refuse("fp4_dequantize: out must be contiguous, with q's leading shape and its columns");
+  Tensor y = out ? *out : empty_f32(q, shape);
+  if (y.numel()) {
+    rtb_ctx* ctx = context(q.device().index());
+    void* s = stream_of(q);
+    call("rtb_fp4_dequantize", [&] {
+      return rtb_fp4_dequantize(ctx, qr.rows, cols, (const uint8_t*)qr.p(), qr.ld,
+                                (const uint8_t*)sr.p(), sr.ld, y.data_ptr<float>(), cols, s);
+    });
+  }
+  return THPVariable_Wrap(y);
+}
+
+PyObject* fp4_matmul(PyObject* const* a) {
+  const char* who = "fp4_matmul";
+  const Tensor &A = tensor(a[0], "a"), &As = tensor(a[1], "a_scale"), &B = tensor(a[2], "b"),
+               &Bs = tensor(a[3], "b_scale");
+  const Tensor* bias = optional(a[4], "bias");
+  const int act = integer(a[5]);
+  const Tensor* out = optional(a[6], "out");
+  need_f32(bias);
+  need_f32(out);
+  same_device(A, {&As, &B, &Bs, bias, out});
+  if (A.dim() != 2 || B.dim() != 2 || Bs.dim() != 2) refuse("Matmul only supports 2D");
+  const int64_t M = A.size(0), K = 2 * A.size(1), N = B.size(1);
+  if (2 * B.size(0) != K) refuse("Matmul dimension mismatch");
+  const Rows ar = codes(A, who), br = codes(B.t(), who);
+  const Rows sa = scales4(As, M, K, who), sb = scales4(Bs.t(), N, K, who);
+  const Vec bv = vec(bias, N, "fp4_matmul: bias must have N elements");
+  if (out && (out->dim() != 2 || out->size(0) != M || out->size(1) != N ||
+              (N > 1 && out->stride(1) != 1) || (M > 1 && out->stride(0) < N)))
+    refuse("fp4_matmul: out must be [M, N] with contiguous rows");
+  Tensor y = out ? *out : empty_f32(A, {M, N});
+  const int64_t ldc = out && out->stride(0) > N ? out->stride(0) : N;
+  rtb_ctx* ctx = context(A.device().index());
+  void* s = stream_of(A);
+  call("rtb_fp4_matmul", [&] {
+    return rtb_fp4_matmul(ctx, M, N, K, (const uint8_t*)ar.p(), ar.ld, (const uint8_t*)sa.p(), sa.ld,
+                          (const uint8_t*)br.p(), br.ld, (const uint8_t*)sb.p(), sb.ld, bv.p, act,
+                          y.data_ptr<float>(), ldc, s);
+  });
+  return THPVariable_Wrap(y);
+}
+
 PyObject* matmul_backward_fp8(PyObject* const* a) {
   const char* who = "matmul_backward_fp8";
   const Tensor &A = tensor(a[0], "a"), &As = tensor(a[1], "a_scale");
@@ -480,6 +720,12 @@ PyMethodDef methods[] = {
     ENTRY(fp8_dequantize, 3),
     ENTRY(fp8_matmul, 7),
     ENTRY(matmul_backward_fp8, 10),
+    ENTRY(rms_norm_fwd, 6),
+    ENTRY(rms_norm_fp8, 5),
+    ENTRY(rms_norm_backward, 11),
+    ENTRY(fp4_quantize, 1),
+    ENTRY(fp4_dequantize, 4),
+    ENTRY(fp4_matmul, 7),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ops", nullptr, -1, methods,

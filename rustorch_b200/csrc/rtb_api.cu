@@ -1107,6 +1107,90 @@ int rtb_layer_norm_backward_fp8(rtb_ctx* ctx, int64_t rows, int64_t d, const uin
   return layer_norm_backward(ctx, "layer_norm_backward_fp8", n, stream);
 }
 
+// ---------------------------------------------------------------- root-mean-square norm
+static int rms_norm(rtb_ctx* ctx, const char* who, const RmsDesc& d, void* stream) {
+  const std::string w = std::string(who) + ": ";
+  if (d.rows < 0 || d.d < 0) return set_error(RTB_E_INVALID, w + "negative dimension");
+  if (d.rows == 0) return RTB_OK;
+  if (d.d == 0) return set_error(RTB_E_INVALID, w + "rows of no columns have no statistics");
+  if (d.d > kMaxExtent) return set_error(RTB_E_UNSUPPORTED, w + "d too large");
+  if (!d.x || !(d.y || (d.q && d.scale))) return set_error(RTB_E_INVALID, w + "null pointer");
+  if (d.ldx < d.d || (d.residual && d.ldr < d.d) || (d.sum && d.ldsum < d.d) ||
+      (d.y ? d.ldy < d.d : d.ldq < d.d || d.lds < (d.d + 127) / 128))
+    return set_error(RTB_E_INVALID, w + "leading dimension below the row's length");
+  if (d.sum && d.sum == d.y) return set_error(RTB_E_INVALID, w + "one place for two outputs");
+  DeviceGuard g(ctx->device);
+  return rms_norm_run(ctx, d, pick_stream(ctx, stream));
+}
+
+int rtb_rms_norm_fwd(rtb_ctx* ctx, int64_t rows, int64_t d, const float* x, int64_t ldx,
+                     const float* residual, int64_t ldr, const float* norm_weight, float eps,
+                     float* sum, int64_t ldsum, float* y, int64_t ldy, float* rstd, void* stream) {
+  RTB_CHECK_CTX(ctx);
+  RmsDesc n;
+  n.rows = rows; n.d = d; n.x = x; n.ldx = ldx; n.residual = residual; n.ldr = ldr;
+  n.w = norm_weight; n.eps = eps; n.sum = sum; n.ldsum = ldsum; n.y = y; n.ldy = ldy;
+  n.rstd = rstd;
+  return rms_norm(ctx, "rms_norm_fwd", n, stream);
+}
+
+int rtb_rms_norm_fp8(rtb_ctx* ctx, int64_t rows, int64_t d, const float* x, int64_t ldx,
+                     const float* residual, int64_t ldr, const float* norm_weight, float eps,
+                     float* sum, int64_t ldsum, uint8_t* q, int64_t ldq, uint8_t* scale,
+                     int64_t lds, float* rstd, void* stream) {
+  RTB_CHECK_CTX(ctx);
+  RmsDesc n;
+  n.rows = rows; n.d = d; n.x = x; n.ldx = ldx; n.residual = residual; n.ldr = ldr;
+  n.w = norm_weight; n.eps = eps; n.sum = sum; n.ldsum = ldsum; n.q = q; n.ldq = ldq;
+  n.scale = scale; n.lds = lds; n.rstd = rstd;
+  return rms_norm(ctx, "rms_norm_fp8", n, stream);
+}
+
+static int rms_norm_backward(rtb_ctx* ctx, const char* who, const NormBwdDesc& n, void* stream) {
+  const std::string w = std::string(who) + ": ";
+  if (n.rows < 0 || n.d < 0) return set_error(RTB_E_INVALID, w + "negative dimension");
+  if (n.d > kMaxExtent) return set_error(RTB_E_UNSUPPORTED, w + "d too large");
+  if (n.d == 0 || (!n.dx && !n.dg)) return RTB_OK;
+  DeviceGuard g(ctx->device);
+  cudaStream_t s = pick_stream(ctx, stream);
+  if (n.rows == 0) {  // empty sums
+    if (n.accumulate || !n.dg) return RTB_OK;
+    const cudaError_t e = cudaMemsetAsync(n.dg, 0, (size_t)n.d * 4, s);
+    return e == cudaSuccess ? RTB_OK : cuda_status(e, "rms_norm_backward memset");
+  }
+  if ((!n.x && !(n.q && n.scale)) || !n.rstd || !n.dy)
+    return set_error(RTB_E_INVALID, w + "null pointer");
+  if ((n.x && n.ldx < n.d) || (n.q && (n.ldq < n.d || n.lds < (n.d + 127) / 128)) ||
+      n.lddy < n.d || (n.dsum && n.ldds < n.d) || (n.dx && n.lddx < n.d))
+    return set_error(RTB_E_INVALID, w + "leading dimension below the row's length");
+  return norm_backward_run(ctx, n, s);
+}
+
+int rtb_rms_norm_backward(rtb_ctx* ctx, int64_t rows, int64_t d, const float* x, int64_t ldx,
+                          const float* rstd, const float* norm_weight, const float* dy,
+                          int64_t lddy, const float* dsum, int64_t ldds, float* dx, int64_t lddx,
+                          float* dweight, int accumulate, void* stream) {
+  RTB_CHECK_CTX(ctx);
+  NormBwdDesc n;
+  n.rows = rows; n.d = d; n.x = x; n.ldx = ldx; n.rstd = rstd; n.g = norm_weight;
+  n.dy = dy; n.lddy = lddy; n.dsum = dsum; n.ldds = ldds; n.dx = dx; n.lddx = lddx;
+  n.dg = dweight; n.accumulate = accumulate;
+  return rms_norm_backward(ctx, "rms_norm_backward", n, stream);
+}
+
+int rtb_rms_norm_backward_fp8(rtb_ctx* ctx, int64_t rows, int64_t d, const uint8_t* q,
+                              int64_t ldq, const uint8_t* scale, int64_t lds, const float* rstd,
+                              const float* norm_weight, const float* dy, int64_t lddy,
+                              const float* dsum, int64_t ldds, float* dx, int64_t lddx,
+                              float* dweight, int accumulate, void* stream) {
+  RTB_CHECK_CTX(ctx);
+  NormBwdDesc n;
+  n.rows = rows; n.d = d; n.q = q; n.ldq = ldq; n.scale = scale; n.lds = lds; n.rstd = rstd;
+  n.g = norm_weight; n.dy = dy; n.lddy = lddy; n.dsum = dsum; n.ldds = ldds; n.dx = dx;
+  n.lddx = lddx; n.dg = dweight; n.accumulate = accumulate;
+  return rms_norm_backward(ctx, "rms_norm_backward_fp8", n, stream);
+}
+
 // ---------------------------------------------------------------- 8-bit block-scaled tensors
 static int check_blocks(const char* who, int64_t rows, int64_t cols, int block_rows) {
   const std::string w = std::string(who) + ": ";
@@ -1276,6 +1360,73 @@ int rtb_matmul_backward_fp8(rtb_ctx* ctx, int64_t M, int64_t N, int64_t K, const
   if (st == RTB_OK) st = wgrad_run(ctx, w, s);
   ws_free(ws, s);
   return st;
+}
+
+// ---------------------------------------------------------------- 4-bit block-scaled tensors
+static int check_fp4(const char* who, int64_t rows, int64_t cols) {
+  const std::string w = std::string(who) + ": ";
+  if (rows < 0 || cols < 0) return set_error(RTB_E_INVALID, w + "negative dimension");
+  if (cols > kMaxExtent) return set_error(RTB_E_UNSUPPORTED, w + "too many columns");
+  return RTB_OK;
+}
+
+int rtb_fp4_quantize(rtb_ctx* ctx, int64_t rows, int64_t cols, const float* x, int64_t ldx,
+                     int transX, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds,
+                     void* stream) {
+  RTB_CHECK_CTX(ctx);
+  int st;
+  if ((st = check_fp4("fp4_quantize", rows, cols))) return st;
+  if (transX != 0 && transX != 1)
+    return set_error(RTB_E_INVALID, "fp4_quantize: transX must be 0 or 1");
+  if (rows == 0 || cols == 0) return RTB_OK;
+  if (!x || !q || !scale) return set_error(RTB_E_INVALID, "fp4_quantize: null pointer");
+  if (ldx < (transX ? rows : cols) || ldq < (cols + 1) / 2 || lds < (cols + 31) / 32)
+    return set_error(RTB_E_INVALID, "fp4_quantize: leading dimension below the row's length");
+  DeviceGuard g(ctx->device);
+  return launch_fp4_quantize(ctx, x, ldx, transX, rows, cols, q, ldq, scale, lds,
+                             pick_stream(ctx, stream));
+}
+
+int rtb_fp4_dequantize(rtb_ctx* ctx, int64_t rows, int64_t cols, const uint8_t* q, int64_t ldq,
+                       const uint8_t* scale, int64_t lds, float* y, int64_t ldy, void* stream) {
+  RTB_CHECK_CTX(ctx);
+  int st;
+  if ((st = check_fp4("fp4_dequantize", rows, cols))) return st;
+  if (rows == 0 || cols == 0) return RTB_OK;
+  if (!q || !scale || !y) return set_error(RTB_E_INVALID, "fp4_dequantize: null pointer");
+  if (ldy < cols || ldq < (cols + 1) / 2 || lds < (cols + 31) / 32)
+    return set_error(RTB_E_INVALID, "fp4_dequantize: leading dimension below the row's length");
+  DeviceGuard g(ctx->device);
+  return launch_fp4_dequantize(ctx, q, ldq, rows, cols, scale, lds, y, ldy,
+                               pick_stream(ctx, stream));
+}
+
+int rtb_fp4_matmul(rtb_ctx* ctx, int64_t M, int64_t N, int64_t K, const uint8_t* A, int64_t lda,
+                   const uint8_t* scale_a, int64_t ldsa, const uint8_t* B, int64_t ldb,
+                   const uint8_t* scale_b, int64_t ldsb, const float* bias, int act, float* C,
+                   int64_t ldc, void* stream) {
+  RTB_CHECK_CTX(ctx);
+  int st;
+  if (M < 0 || N < 0 || K < 0) return set_error(RTB_E_INVALID, "fp4_matmul: negative dimension");
+  if (K % 2) return set_error(RTB_E_INVALID, "fp4_matmul: K is odd (two elements lie in a byte)");
+  if ((st = check_act(act))) return st;
+  if (M > kMaxExtent || N > kMaxExtent || K > kMaxExtent)
+    return set_error(RTB_E_UNSUPPORTED, "fp4_matmul: dimension too large");
+  if (M == 0 || N == 0) return RTB_OK;
+  if (!C) return set_error(RTB_E_INVALID, "fp4_matmul: null C");
+  if (ldc < N) return set_error(RTB_E_INVALID, "fp4_matmul: ldc < N");
+  DeviceGuard g(ctx->device);
+  cudaStream_t s = pick_stream(ctx, stream);
+  if (K == 0) return launch_fill_rows(C, M, N, ldc, bias, act, s);
+  if (!A || !B || !scale_a || !scale_b) return set_error(RTB_E_INVALID, "fp4_matmul: null operand");
+  const int64_t kb = (K + 31) / 32;
+  if (lda < K / 2 || ldb < K / 2 || ldsa < kb || ldsb < kb)
+    return set_error(RTB_E_INVALID, "fp4_matmul: leading dimension below the row's length");
+  Fp4Desc d;
+  d.M = M; d.N = N; d.K = K; d.A = A; d.lda = lda; d.B = B; d.ldb = ldb;
+  d.sa = scale_a; d.ldsa = ldsa; d.sb = scale_b; d.ldsb = ldsb;
+  d.bias = bias; d.act = act; d.C = C; d.ldc = ldc;
+  return fp4_gemm_run(ctx, d, s);
 }
 
 // ---------------------------------------------------------------- small ops

@@ -223,7 +223,8 @@ int launch_layernorm_act(rtb_ctx* ctx, const float* X, int64_t ldx, float* Y, in
 
 // LayerNorm backward (rtb_norm_bwd.cu): x as fp32 (x != null) or as an 8-bit
 // checkpoint (q, scale); mean, rstd as the forward pass left them.  Any of dx,
-// dg, db may be null.
+// dg, db may be null.  mean null: the root-mean-square norm's backward pass (no
+// bias, no activation), which adds dsum to dx.
 struct NormBwdDesc {
   int64_t rows = 0, d = 0;
   const float* x = nullptr;
@@ -237,12 +238,28 @@ struct NormBwdDesc {
   int act = 0;
   const float* dy = nullptr;
   int64_t lddy = 0;
+  const float* dsum = nullptr;
+  int64_t ldds = 0;
   float* dx = nullptr;
   int64_t lddx = 0;
   float *dg = nullptr, *db = nullptr;
   int accumulate = 0;
 };
 int norm_backward_run(rtb_ctx* ctx, const NormBwdDesc& d, cudaStream_t s);
+
+// Root-mean-square norm (rtb_rms.cu): h = x + residual, y = h rstd w, as fp32 (y) or
+// as 8-bit blocks (q, scale); residual, w, sum (h's place) and rstd may be null.
+struct RmsDesc {
+  int64_t rows = 0, d = 0;
+  const float *x = nullptr, *residual = nullptr, *w = nullptr;
+  int64_t ldx = 0, ldr = 0;
+  float eps = 0.0f;
+  float *sum = nullptr, *y = nullptr, *rstd = nullptr;
+  int64_t ldsum = 0, ldy = 0;
+  uint8_t *q = nullptr, *scale = nullptr;
+  int64_t ldq = 0, lds = 0;
+};
+int rms_norm_run(rtb_ctx* ctx, const RmsDesc& d, cudaStream_t s);
 
 // 8-bit block-scaled tensors (rtb_fp8.cu).
 int launch_fp8_quantize(rtb_ctx* ctx, const float* x, int64_t ldx, int64_t rows, int64_t cols,
@@ -251,6 +268,28 @@ int launch_fp8_quantize(rtb_ctx* ctx, const float* x, int64_t ldx, int64_t rows,
 int launch_fp8_dequantize(rtb_ctx* ctx, const uint8_t* q, int64_t ldq, int64_t rows, int64_t cols,
                           const uint8_t* scale, int64_t lds, int block_rows, float* y, int64_t ldy,
                           cudaStream_t s);
+
+// 4-bit block-scaled tensors (rtb_fp4.cu): e2m1 codes, two in a byte, one e8m0 scale
+// for each 32 columns of a row.  trans: x is stored as its transpose.
+int launch_fp4_quantize(rtb_ctx* ctx, const float* x, int64_t ldx, int trans, int64_t rows,
+                        int64_t cols, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds,
+                        cudaStream_t s);
+int launch_fp4_dequantize(rtb_ctx* ctx, const uint8_t* q, int64_t ldq, int64_t rows, int64_t cols,
+                          const uint8_t* scale, int64_t lds, float* y, int64_t ldy, cudaStream_t s);
+// C [M, N] = act(A . B^T + bias): A [M, K], B [N, K] of K elements each (even), row
+// strides lda, ldb in bytes; the scales' rows are contiguous (ld_col 1).
+struct Fp4Desc {
+  int64_t M = 0, N = 0, K = 0;
+  const uint8_t *A = nullptr, *B = nullptr;
+  int64_t lda = 0, ldb = 0;
+  const uint8_t *sa = nullptr, *sb = nullptr;
+  int64_t ldsa = 0, ldsb = 0;
+  const float* bias = nullptr;
+  int act = 0;
+  float* C = nullptr;
+  int64_t ldc = 0;
+};
+int fp4_gemm_run(rtb_ctx* ctx, const Fp4Desc& d, cudaStream_t s);
 // dst[r][c] = c < cols ? src[r * rs + c * cs] : 0 for c < ldd (rs or cs is 1,
 // ldd % 16 == 0), of up to two matrices in one launch; a null dst is left out.
 struct PackDesc {

@@ -4,7 +4,10 @@
 //   dg = sum_rows dz u,  db = sum_rows dz
 //   dx = rstd (h - mean_j(h) - u mean_j(h u)),  h = dz g
 // x is fp32 or an 8-bit checkpoint (rtb_fp8.cuh); mean and rstd are the
-// forward pass's.  HBM-bound: x and dy are read and dx written once (12 bytes
+// forward pass's.
+// RMS (rtb_rms.cu's backward pass): no mean, no bias, no activation, and the
+// gradient that reaches x from elsewhere (the residual stream) is added:
+//   u = x rstd,  dx = rstd (h - u mean_j(h u)) + dsum,  h = dy g,  dg = sum_rows dy u.  HBM-bound: x and dy are read and dx written once (12 bytes
 // an element, 9 from a checkpoint).
 //
 // A row belongs to a group of threads that holds it in registers, rows strided
@@ -46,6 +49,8 @@ struct NormBwdParams {
   int act;
   const float* dy;
   int64_t lddy;
+  const float* dsum;  // RMS: added to dx; or null
+  int64_t ldds;
   float* dx;
   int64_t lddx;
   float* part;  // [CTA][2][d] partial dg, db; null when neither is wanted
@@ -109,7 +114,7 @@ __global__ void __launch_bounds__(kThreads) norm_bwd_kernel(const NormBwdParams 
   float* pb = pg ? pg + p.d : nullptr;  // (an index p.d + j would pass 32 bits)
   bool first = true;
   for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x, first = false) {
-    const float mean = p.mean[r], rstd = p.rstd[r];
+    const float mean = p.mean ? p.mean[r] : 0.0f, rstd = p.rstd[r];  // (RMS: no mean)
     const float* dyr = p.dy + r * p.lddy;
     auto at = [&](int j, float& u, float& dz, float& h) {
       float x;
@@ -138,12 +143,14 @@ __global__ void __launch_bounds__(kThreads) norm_bwd_kernel(const NormBwdParams 
     }
     if (!p.dx) continue;
     const float2 t = block_sum2(s1, s2, red);
-    const float m1 = t.x / p.d, m2 = t.y / p.d;
+    const float m1 = p.mean ? t.x / p.d : 0.0f, m2 = t.y / p.d;
     float* dxr = p.dx + r * p.lddx;
+    const float* dsr = p.dsum ? p.dsum + r * p.ldds : nullptr;
     for (int j = threadIdx.x; j < p.d; j += kThreads) {
       float u, dz, h;
       at(j, u, dz, h);
-      const float v = rstd * (h - m1 - u * m2);
+      float v = rstd * (h - m1 - u * m2);
+      if (dsr) v += dsr[j];
       dxr[j] = p.accumulate ? dxr[j] + v : v;
     }
   }
@@ -218,7 +225,7 @@ __device__ __forceinline__ void copy_row(uint32_t dst, const void* row, int byte
 template <int kBlock, bool VEC, bool SAVED>
 constexpr bool kRows = VEC || SAVED || kBlock > 512;  // rows through the ring
 
-template <int kBlock, int E, bool VEC, bool SAVED, bool ACT, bool FULL>
+template <int kBlock, int E, bool VEC, bool SAVED, bool ACT, bool FULL, bool RMS>
 __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
     norm_bwd_rows_kernel(const NormBwdParams p, const int T, const float inv_d, float* dg,
                          float* db) {
@@ -241,10 +248,10 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
   const int row_bytes = xbytes + ((yrow + (VEC ? 15 : 30)) & ~15);
   const uint32_t slot0 = smem_u32(ring4) + (uint32_t)(grp * kRing * row_bytes);
   constexpr bool kKeep = VEC && !ACT;  // the weight stays in registers
-  unsigned long long ag[P], ab[P], gw[kKeep ? P : 1];
+  unsigned long long ag[P], ab[RMS ? 1 : P], gw[kKeep ? P : 1];
 #pragma unroll
   for (int i = 0; i < P; ++i) {
-    ag[i] = ab[i] = 0ull;
+    ag[i] = ab[RMS ? 0 : i] = 0ull;
     if (kKeep) gw[i] = pack2(1.0f, 1.0f);
   }
   // the pair of a column vector's values that belongs to values 2 i, 2 i + 1
@@ -263,7 +270,7 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
   // row's address is one multiply-add
   const int rows = (int)p.rows, step = (int)gridDim.x * R;
   const int ldx = (int)p.ldx, ldq = (int)p.ldq, lds = (int)p.lds, lddy = (int)p.lddy,
-            lddx = (int)p.lddx;
+            lddx = (int)p.lddx, ldds = (int)p.ldds;
   auto xrow_at = [&](int r) {
     return SAVED ? reinterpret_cast<const char*>(p.q + (int64_t)r * ldq)
                  : reinterpret_cast<const char*>(p.x + (int64_t)r * ldx);
@@ -307,7 +314,7 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
   float mean = 0.0f, rstd = 0.0f;
   uint32_t sb[NS] = {};
   if (r < rows) {
-    mean = __ldg(p.mean + r);
+    if (!RMS) mean = __ldg(p.mean + r);
     rstd = __ldg(p.rstd + r);
     if (kAhead) scales(r, sb);
     if (SHARED) {
@@ -320,7 +327,7 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
   for (; r < rows; r += step, phase ^= 1) {
     // the next row's statistics and block scales
     const int rn = r + step < rows ? r + step : r;
-    const float mean_n = __ldg(p.mean + rn), rstd_n = __ldg(p.rstd + rn);
+    const float mean_n = RMS ? 0.0f : __ldg(p.mean + rn), rstd_n = __ldg(p.rstd + rn);
     uint32_t sb_n[NS] = {};
     if (kAhead) scales(rn, sb_n);
     else if (SAVED) scales(r, sb);
@@ -374,20 +381,43 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
         h[i] = pack2(g[2 * i], g[2 * i + 1]);
       }
     }
+    // (RMS: the registers that the bias's sums have otherwise; loaded here, so that
+    // the row's sums hide the latency)
+    unsigned long long ds[RMS ? P : 1];
+    if (RMS) {
+      const float* dsr = p.dsum + (int64_t)r * ldds + C * k0;
+#pragma unroll
+      for (int i = 0; i < P; ++i) ds[RMS ? i : 0] = 0ull;
+      if (p.dsum && p.dx) {
+#pragma unroll
+        for (int i = 0; i < G; i += VEC ? 1 : 2) {
+          if (VEC) {
+            if (32 * i < rem) {
+              const float4 f = __ldcs(reinterpret_cast<const float4*>(dsr) + 32 * i);
+              ds[RMS ? 2 * i : 0] = pack2(f.x, f.y);
+              ds[RMS ? 2 * i + 1 : 0] = pack2(f.z, f.w);
+            }
+          } else {
+            ds[RMS ? i / 2 : 0] = pack2(32 * i < rem ? __ldcs(dsr + 32 * i) : 0.0f,
+                                        32 * (i + 1) < rem ? __ldcs(dsr + 32 * (i + 1)) : 0.0f);
+          }
+        }
+      }
+    }
     unsigned long long t1 = 0ull, t2 = 0ull;
     const unsigned long long rs = pack2(rstd, rstd), nm = pack2(-mean, -mean);
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      u[i] = mul2(add2(u[i], nm), rs);
+      u[i] = RMS ? mul2(u[i], rs) : mul2(add2(u[i], nm), rs);
       const unsigned long long gv = kKeep ? gw[kKeep ? i : 0] : columns(p.g, i, 1.0f);
       if (ACT) {
         const float2 z = unpack2(fma2(u[i], gv, columns(p.b, i, 0.0f)));
         h[i] = mul2(h[i], act_slope2(z, p.act));
       }
       ag[i] = fma2(h[i], u[i], ag[i]);
-      ab[i] = add2(ab[i], h[i]);
+      if (!RMS) ab[RMS ? 0 : i] = add2(ab[RMS ? 0 : i], h[i]);
       h[i] = mul2(h[i], gv);
-      t1 = add2(t1, h[i]);
+      if (!RMS) t1 = add2(t1, h[i]);
       t2 = fma2(h[i], u[i], t2);
     }
     float s1 = unpack2(t1).x + unpack2(t1).y, s2 = unpack2(t2).x + unpack2(t2).y;
@@ -424,7 +454,9 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
       const unsigned long long m1 = pack2(-s1 * inv_d, -s1 * inv_d), m2 = pack2(-s2 * inv_d, -s2 * inv_d);
       float* dxr = p.dx + (int64_t)r * lddx + C * k0;
 #pragma unroll
-      for (int i = 0; i < P; ++i) u[i] = mul2(rs, fma2(u[i], m2, add2(h[i], m1)));
+      for (int i = 0; i < P; ++i)
+        u[i] = RMS ? fma2(rs, fma2(u[i], m2, h[i]), ds[RMS ? i : 0])
+                   : mul2(rs, fma2(u[i], m2, add2(h[i], m1)));
       if (SHARED && !p.dx) {
         // (only the sums were asked for)
       } else if (VEC) {
@@ -467,9 +499,9 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
       for (int i = 0; i < E; ++i) {
         if (32 * (i / C) >= rem) continue;
         const int j = C * (k0 + 32 * (i / C)) + i % C;
-        const float2 a = unpack2(ag[i / 2]), b = unpack2(ab[i / 2]);
+        const float2 a = unpack2(ag[i / 2]), b = unpack2(ab[RMS ? 0 : i / 2]);
         put(acc_s + j, i % 2 ? a.y : a.x, gi > 0);
-        put(acc_s + p.d + j, i % 2 ? b.y : b.x, gi > 0);
+        if (!RMS) put(acc_s + p.d + j, i % 2 ? b.y : b.x, gi > 0);
       }
     }
     __syncthreads();
@@ -478,10 +510,10 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
     if (p.part) {
       float* pr = p.part + (int64_t)blockIdx.x * 2 * p.d;
       pr[j] = acc_s[j];
-      pr[p.d + j] = acc_s[p.d + j];
+      if (!RMS) pr[p.d + j] = acc_s[p.d + j];
     } else {
       if (dg) put(dg + j, acc_s[j], p.accumulate);
-      if (db) put(db + j, acc_s[p.d + j], p.accumulate);
+      if (!RMS && db) put(db + j, acc_s[p.d + j], p.accumulate);
     }
   }
 }
@@ -491,7 +523,7 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
 // thread leave no room, in shared memory.
 constexpr int kWide = 1024;
 
-template <bool VEC, bool SAVED>
+template <bool VEC, bool SAVED, bool RMS>
 __global__ void __launch_bounds__(kWide, 1)
     norm_bwd_direct_kernel(const NormBwdParams p, float* dg, float* db) {
   constexpr int E = 16, G = VEC ? E / 4 : E;  // values, loads of x (and of dy) a thread
@@ -505,13 +537,13 @@ __global__ void __launch_bounds__(kWide, 1)
   const int units = VEC ? p.d >> 2 : p.d;
   const bool sums = p.part || dg || db;
   if (sums) {
-    for (int j = t; j < 2 * p.d; j += kWide) acc_s[j] = 0.0f;
+    for (int j = t; j < (RMS ? 1 : 2) * p.d; j += kWide) acc_s[j] = 0.0f;
     __syncthreads();
   }
   int phase = 0;
   for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x, phase ^= 1) {
     float u[E], h[E];  // x, then u; dy, then h
-    const float mean = __ldg(p.mean + r), rstd = __ldg(p.rstd + r);
+    const float mean = RMS ? 0.0f : __ldg(p.mean + r), rstd = __ldg(p.rstd + r);
     const float* dyr = p.dy + r * p.lddy;
 #pragma unroll
     for (int i = 0; i < G; ++i) {
@@ -570,7 +602,7 @@ __global__ void __launch_bounds__(kWide, 1)
       float4 sg, sb;
       if (add && VEC) {
         sg = reinterpret_cast<const float4*>(acc_s)[k];
-        sb = reinterpret_cast<const float4*>(acc_s + p.d)[k];
+        if (!RMS) sb = reinterpret_cast<const float4*>(acc_s + p.d)[k];
       }
 #pragma unroll
       for (int c = 0; c < C; ++c) {
@@ -580,10 +612,10 @@ __global__ void __launch_bounds__(kWide, 1)
         if (p.act != RTB_ACT_NONE) dz *= act_slope(fmaf(u[e], gv[c], bv[c]), p.act);
         if (add && VEC) {
           (&sg.x)[c] = fmaf(dz, u[e], (&sg.x)[c]);
-          (&sb.x)[c] += dz;
+          if (!RMS) (&sb.x)[c] += dz;
         } else if (add) {
           acc_s[k] = fmaf(dz, u[e], acc_s[k]);
-          acc_s[p.d + k] += dz;
+          if (!RMS) acc_s[p.d + k] += dz;
         }
         h[e] = dz * gv[c];
         s1 += h[e];
@@ -591,7 +623,7 @@ __global__ void __launch_bounds__(kWide, 1)
       }
       if (add && VEC) {
         reinterpret_cast<float4*>(acc_s)[k] = sg;
-        reinterpret_cast<float4*>(acc_s + p.d)[k] = sb;
+        if (!RMS) reinterpret_cast<float4*>(acc_s + p.d)[k] = sb;
       }
     }
     if (!p.dx) continue;
@@ -612,8 +644,9 @@ __global__ void __launch_bounds__(kWide, 1)
       s1 += red[phase][k][0];
       s2 += red[phase][k][1];
     }
-    const float m1 = s1 / p.d, m2 = s2 / p.d;
+    const float m1 = RMS ? 0.0f : s1 / p.d, m2 = s2 / p.d;
     float* dxr = p.dx + r * p.lddx;
+    const float* dsr = RMS && p.dsum ? p.dsum + r * p.ldds : nullptr;
 #pragma unroll
     for (int i = 0; i < G; ++i) {
       const int k = t + kWide * i;
@@ -621,6 +654,13 @@ __global__ void __launch_bounds__(kWide, 1)
       float v[C];
 #pragma unroll
       for (int c = 0; c < C; ++c) v[c] = rstd * (h[C * i + c] - m1 - u[C * i + c] * m2);
+      if (RMS && dsr) {
+        float e[C];
+        if (VEC) *reinterpret_cast<float4*>(e) = __ldcs(reinterpret_cast<const float4*>(dsr) + k);
+        else e[0] = __ldcs(dsr + k);
+#pragma unroll
+        for (int c = 0; c < C; ++c) v[c] += e[c];
+      }
       if (VEC) {
         float4* o = reinterpret_cast<float4*>(dxr) + k;
         float4 w = *reinterpret_cast<const float4*>(v);
@@ -640,10 +680,10 @@ __global__ void __launch_bounds__(kWide, 1)
     if (p.part) {
       float* pr = p.part + (int64_t)blockIdx.x * 2 * p.d;
       pr[j] = acc_s[j];
-      pr[p.d + j] = acc_s[p.d + j];
+      if (!RMS) pr[p.d + j] = acc_s[p.d + j];
     } else {
       if (dg) put(dg + j, acc_s[j], p.accumulate);
-      if (db) put(db + j, acc_s[p.d + j], p.accumulate);
+      if (!RMS && db) put(db + j, acc_s[p.d + j], p.accumulate);
     }
   }
 }
@@ -705,9 +745,9 @@ int launch_with_sums(rtb_ctx* ctx, NormBwdParams& p, int grid, float* dg, float*
   return e == cudaSuccess ? RTB_OK : cuda_status(e, "layer_norm_backward launch");
 }
 
-template <bool VEC, bool SAVED>
+template <bool VEC, bool SAVED, bool RMS>
 int launch_direct(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStream_t s) {
-  auto* k = norm_bwd_direct_kernel<VEC, SAVED>;
+  auto* k = norm_bwd_direct_kernel<VEC, SAVED, RMS>;
   const size_t smem = (dg || db) ? (size_t)2 * p.d * sizeof(float) : 0;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        2 * 16384 * (int)sizeof(float));
@@ -718,11 +758,11 @@ int launch_direct(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStre
   });
 }
 
-template <int kBlock, int E, bool VEC, bool SAVED, bool ACT, bool FULL>
+template <int kBlock, int E, bool VEC, bool SAVED, bool ACT, bool FULL, bool RMS>
 int launch_rows_as(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStream_t s) {
   constexpr int G = VEC ? E / 4 : E;
   constexpr int kPerSm = 1024 / kBlock;
-  auto* k = norm_bwd_rows_kernel<kBlock, E, VEC, SAVED, ACT, FULL>;
+  auto* k = norm_bwd_rows_kernel<kBlock, E, VEC, SAVED, ACT, FULL, RMS>;
   const int units = VEC ? p.d / 4 : p.d;
   const int T = (units + 32 * G - 1) / (32 * G) * 32, R = kBlock / T;
   constexpr int kPad = VEC ? 15 : 30;
@@ -747,16 +787,22 @@ int launch_rows_as(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStr
   });
 }
 
-template <int kBlock, int E, bool VEC, bool SAVED, bool ACT>
+template <int kBlock, int E, bool VEC, bool SAVED, bool ACT, bool RMS = false>
 int launch_rows(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStream_t s) {
   if (VEC && p.d % (32 * E) == 0)
-    return launch_rows_as<kBlock, E, VEC, SAVED, ACT, VEC>(ctx, p, dg, db, s);
-  return launch_rows_as<kBlock, E, VEC, SAVED, ACT, false>(ctx, p, dg, db, s);
+    return launch_rows_as<kBlock, E, VEC, SAVED, ACT, VEC, RMS>(ctx, p, dg, db, s);
+  return launch_rows_as<kBlock, E, VEC, SAVED, ACT, false, RMS>(ctx, p, dg, db, s);
 }
 
 template <bool VEC, bool SAVED>
 int launch_width(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStream_t s) {
   const bool act = p.act != RTB_ACT_NONE;
+  if (!p.mean) {  // RMS
+    if (p.d <= 128) return launch_rows<512, 4, VEC, SAVED, false, true>(ctx, p, dg, db, s);
+    if (p.d <= 4096) return launch_rows<512, 8, VEC, SAVED, false, true>(ctx, p, dg, db, s);
+    if (p.d <= 8192) return launch_rows<1024, 8, VEC, SAVED, false, true>(ctx, p, dg, db, s);
+    return launch_direct<VEC, SAVED, true>(ctx, p, dg, db, s);
+  }
   if (p.d <= 128)
     return act ? launch_rows<512, 4, VEC, SAVED, true>(ctx, p, dg, db, s)
                : launch_rows<512, 4, VEC, SAVED, false>(ctx, p, dg, db, s);
@@ -766,7 +812,7 @@ int launch_width(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStrea
   if (p.d <= 8192)
     return act ? launch_rows<1024, 8, VEC, SAVED, true>(ctx, p, dg, db, s)
                : launch_rows<1024, 8, VEC, SAVED, false>(ctx, p, dg, db, s);
-  return launch_direct<VEC, SAVED>(ctx, p, dg, db, s);
+  return launch_direct<VEC, SAVED, false>(ctx, p, dg, db, s);
 }
 
 }  // namespace
@@ -788,17 +834,20 @@ int norm_backward_run(rtb_ctx* ctx, const NormBwdDesc& d, cudaStream_t s) {
   p.act = d.act;
   p.dy = d.dy;
   p.lddy = d.lddy;
+  p.dsum = d.dsum;
+  p.ldds = d.ldds;
   p.dx = d.dx;
   p.lddx = d.lddx;
   p.accumulate = d.accumulate;
   // (the row kernels index rows and rows' addresses with 32-bit factors)
   constexpr int64_t kMax32 = INT32_MAX - (1 << 20);
   if (d.d <= 16384 && d.rows <= kMax32 && d.ldx <= kMax32 && d.ldq <= kMax32 && d.lds <= kMax32 &&
-      d.lddy <= kMax32 && d.lddx <= kMax32) {
+      d.lddy <= kMax32 && d.lddx <= kMax32 && d.ldds <= kMax32) {
     auto al = [](const void* q, uintptr_t n) { return (reinterpret_cast<uintptr_t>(q) % n) == 0; };
     const bool vec = d.d % 4 == 0 && al(d.dy, 16) && d.lddy % 4 == 0 &&
                      (!d.dx || (al(d.dx, 16) && d.lddx % 4 == 0)) && (!d.g || al(d.g, 16)) &&
                      (!d.b || al(d.b, 16)) &&
+                     (!d.dsum || (al(d.dsum, 16) && d.ldds % 4 == 0)) &&
                      (d.q ? al(d.q, 4) && d.ldq % 4 == 0 : al(d.x, 16) && d.ldx % 4 == 0);
     if (d.q) return vec ? launch_width<true, true>(ctx, p, d.dg, d.db, s)
                         : launch_width<false, true>(ctx, p, d.dg, d.db, s);
