@@ -1231,7 +1231,7 @@ int rtb_fp8_dequantize(rtb_ctx* ctx, int64_t rows, int64_t cols, const uint8_t* 
                                pick_stream(ctx, stream));
 }
 
-// [rows, K] e4m3 with K contiguous, as the tensor maps want it: the caller's
+// [rows, K] bytes with K contiguous, as the tensor maps want it: the caller's
 // matrix where its base and row stride are multiples of 16 bytes, else a copy
 // (src -> a place in the workspace, `need` bytes further on).
 static void fp8_operand(const uint8_t* src, int64_t rows, int64_t K, int64_t rs, int64_t cs,
@@ -1423,10 +1423,23 @@ int rtb_fp4_matmul(rtb_ctx* ctx, int64_t M, int64_t N, int64_t K, const uint8_t*
   if (lda < K / 2 || ldb < K / 2 || ldsa < kb || ldsb < kb)
     return set_error(RTB_E_INVALID, "fp4_matmul: leading dimension below the row's length");
   Fp4Desc d;
-  d.M = M; d.N = N; d.K = K; d.A = A; d.lda = lda; d.B = B; d.ldb = ldb;
-  d.sa = scale_a; d.ldsa = ldsa; d.sb = scale_b; d.ldsb = ldsb;
+  d.M = M; d.N = N; d.K = K; d.sa = scale_a; d.ldsa = ldsa; d.sb = scale_b; d.ldsb = ldsb;
   d.bias = bias; d.act = act; d.C = C; d.ldc = ldc;
-  return fp4_gemm_run(ctx, d, s);
+  PackDesc pa, pb;
+  size_t need = 0;
+  void* ws = nullptr;
+  fp8_operand(A, M, K / 2, lda, 1, &d.A, &d.lda, &pa, &need);
+  const size_t at_b = need;
+  fp8_operand(B, N, K / 2, ldb, 1, &d.B, &d.ldb, &pb, &need);
+  if (need) {
+    if ((st = ws_alloc(ctx, &ws, need, s))) return st;
+    if (!d.A) d.A = pa.dst = static_cast<uint8_t*>(ws);
+    if (!d.B) d.B = pb.dst = static_cast<uint8_t*>(ws) + at_b;
+    st = launch_pack_bytes(ctx, pa, pb, s);
+  }
+  if (st == RTB_OK) st = fp4_gemm_run(ctx, d, s);
+  ws_free(ws, s);
+  return st;
 }
 
 // ---------------------------------------------------------------- small ops

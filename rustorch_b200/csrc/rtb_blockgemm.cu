@@ -9,6 +9,8 @@
 //                       (kind::mxf8f6f4, see rtb_mxgemm.cu): a promotion every
 //                       1024 elements.  MODE 0 takes 1500 clocks a block, the
 //                       epilogue's chain of barrier, TMEM loads and adds.
+//   MODE 3  as MODE 2 with e2m1 operands and a scale for each 32 columns
+//                       (kind::mxf4): a stage's 128 bytes are 256 elements
 //
 // In the first two the MMAs of one 128-element block accumulate in TMEM and the
 // epilogue warps add the block's partial sum into fp32 registers on the CUDA
@@ -56,12 +58,14 @@ struct Cfg {
   static constexpr int kStageBytes = kXBytes + kPieces * kYPiece;
   // Narrow tiles, two CTAs on an SM: one's loads pass behind the other's start and
   // end (a token row by 8192 x 8192: 19.9 us with one CTA of eight stages, 18.8).
-  static constexpr int kPerSm = MODE == 2 && BN <= 32 ? 2 : 1;
-  static constexpr int kSf = kPerSm == 2 ? 8 : 16;     // MODE 2: blocks of a scale buffer, of two
+  static constexpr int kPerSm = MODE >= 2 && BN <= 32 ? 2 : 1;
+  // MODE 2, 3: stages of a scale buffer, of two; a stage's scales of one operand
+  static constexpr int kSf = (kPerSm == 2 ? 8 : 16) / (MODE == 3 ? 2 : 1);
+  static constexpr int kSfBytes = MODE == 3 ? 1024 : 512;
   static constexpr int kBudget = kPerSm == 2 ? kSmemHalf : kSmemMax;
   static constexpr int kSy = YVEC ? BN : 1;            // column scales of a block
   static constexpr int kScaleBytes =
-      MODE == 0 ? kScaleUnits * (128 + kSy) * 4 : (MODE == 2 ? 2 * kSf * 1024 : 0);
+      MODE == 0 ? kScaleUnits * (128 + kSy) * 4 : (MODE >= 2 ? 2 * kSf * 2 * kSfBytes : 0);
   static constexpr int kStagesRaw = (kBudget - kReserve - kScaleBytes) / kStageBytes;
   static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;
   static constexpr int kSmemBytes = kStages * kStageBytes + kScaleBytes + kReserve;
@@ -69,10 +73,11 @@ struct Cfg {
   // output's columns
   static_assert(kStages * kStageBytes >= 128 * (BN + 4) * 4 &&
                     kStages * kStageBytes >= BN * 132 * 4, "the ring holds the finished tile");
-  static constexpr int kPerUnit = MODE == 0 ? 1 : (MODE == 1 ? 2 : 8);  // stages between promotions
+  // stages between promotions
+  static constexpr int kPerUnit = MODE == 0 ? 1 : (MODE == 1 ? 2 : (kSf < 8 ? kSf : 8));
   static constexpr int kGrain = MODE == 1 ? 2 : 1;     // stages that parts are cut at
-  // MODE 2: two buffers of 4 + 4 scale columns behind the accumulators
-  static constexpr int kTmemNeed = 2 * BN + (MODE == 2 ? 16 : 0);
+  // MODE 2, 3: two buffers of 4 + 4 or 8 + 8 scale columns behind the accumulators
+  static constexpr int kTmemNeed = 2 * BN + (MODE == 2 ? 16 : MODE == 3 ? 32 : 0);
   static constexpr int kTmemCols =
       kTmemNeed <= 32 ? 32 : kTmemNeed <= 64 ? 64 : kTmemNeed <= 128 ? 128 : kTmemNeed <= 256 ? 256 : 512;
   static_assert(kStages >= 2, "two stages");
@@ -125,6 +130,35 @@ __device__ __forceinline__ void mx_stage1_e(uint32_t d, uint64_t a, uint64_t b, 
       : "memory");
 }
 
+// MODE 3: the stage's scale groups (two of each operand, 128 columns each), and four
+// MMAs of 64 contraction elements with the scales in bytes 0, 1 and 2, 3 of a group's
+// words.
+__device__ __forceinline__ void mx4_stage1_e(uint32_t d, uint64_t a, uint64_t b, uint32_t id0,
+                                             uint32_t id2, uint32_t sa, uint64_t cx, uint64_t cy,
+                                             uint32_t acc, uint64_t* empty) {
+  asm volatile(
+      "{\n\t.reg .pred p, t, e;\n\t.reg .b32 r, s1, s2, s3;\n\t"
+      ".reg .b64 a1, a2, a3, b1, b2, b3, x1, y1;\n\t"
+      "setp.ne.b32 p, %8, 0;\n\t"
+      "setp.eq.b32 t, 0, 0;\n\t"
+      "add.u32 s1, %5, 4;\n\tadd.u32 s2, %5, 8;\n\tadd.u32 s3, %5, 12;\n\t"
+      "add.s64 x1, %6, 32;\n\tadd.s64 y1, %7, 32;\n\t"
+      "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
+      "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
+      "elect.sync r|e, 0xffffffff;\n\t"
+      "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%5], %6;\n\t"
+      "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [s1], x1;\n\t"
+      "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [s2], %7;\n\t"
+      "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [s3], y1;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [s2], p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], a1, b1, %4, [%5], [s2], t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], a2, b2, %3, [s1], [s3], t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], a3, b3, %4, [s1], [s3], t;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%9];\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(id0), "r"(id2), "r"(sa), "l"(cx), "l"(cy), "r"(acc), "r"(smem_u32(empty))
+      : "memory");
+}
+
 // MODE 2: the scale bytes of blocks u .. u + n - 1 (n <= N) of row r; 2^0 for rows
 // past the operand.
 template <int N>
@@ -136,13 +170,22 @@ __device__ __forceinline__ void load_scale_bytes(const ScaleRef& s, int64_t r, i
 #pragma unroll
   for (int k = 0; k < N; ++k) raw[k] = in && k < n ? __ldg(p + (int64_t)k * s.ld_col) : 127u;
 }
+// MODE 3: ... the words j .. j + n - 1, two for each stage.
+template <int N>
+__device__ __forceinline__ void load_scale_words(const ScaleRef& s, int64_t r, int64_t rows, int j,
+                                                 int n, int bytes, int vec, uint32_t (&raw)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    raw[k] = r < rows && k < n ? fp4_scale_word(s, r, j + k, bytes, vec) : 0x7F7F7F7Fu;
+}
 // ... as words of the 512-byte groups that the tensor core takes (row l of a group:
 // the word at 16 (l % 32) + 4 (l / 32), its byte four times).
-template <int N>
+template <int MODE, int N>
 __device__ __forceinline__ void store_scale_words(const uint32_t (&raw)[N], uint8_t* group, int l) {
 #pragma unroll
   for (int k = 0; k < N; ++k)
-    *reinterpret_cast<uint32_t*>(group + 512 * k + 16 * (l & 31) + 4 * (l >> 5)) = raw[k] * 0x01010101u;
+    *reinterpret_cast<uint32_t*>(group + 512 * k + 16 * (l & 31) + 4 * (l >> 5)) =
+        MODE == 3 ? raw[k] : raw[k] * 0x01010101u;
 }
 
 // The scales of blocks u .. u + n - 1 of row r, decoded, to dst[0], dst[step],
@@ -204,11 +247,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<MODE, BN, YVEC>::kPerSm)
   uint64_t* empty = full + S;
   uint64_t* tfull = empty + S;
   uint64_t* tempty = tfull + 2;
-  uint64_t* sfull = tempty + 2;   // MODE 2: scale buffers
+  uint64_t* sfull = tempty + 2;   // MODE 2, 3: scale buffers
   uint64_t* sempty = sfull + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sempty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  uint8_t* sf = reinterpret_cast<uint8_t*>(sx);  // MODE 2: [2][X, Y][kSf][512]
+  uint8_t* sf = reinterpret_cast<uint8_t*>(sx);  // MODE 2, 3: [2][X, Y][kSf][kSfBytes]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -297,8 +340,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<MODE, BN, YVEC>::kPerSm)
             !(ok = wait(&full[s], (i / S) & 1, DEV_TIMEOUT_FULL)))
           break;
         if (j == 0 && !(ok = wait(&tempty[b], ((u >> 1) & 1) ^ 1, DEV_TIMEOUT_TMEM_EMPTY))) break;
-        const int c = i / C::kSf, k = i % C::kSf;  // MODE 2: scale buffer c & 1, its block k
-        if (MODE == 2 && k == 0 && !(ok = wait(&sfull[c & 1], (c >> 1) & 1, DEV_TIMEOUT_LOADED)))
+        const int c = i / C::kSf, k = i % C::kSf;  // MODE 2, 3: scale buffer c & 1, its stage k
+        if (MODE >= 2 && k == 0 && !(ok = wait(&sfull[c & 1], (c >> 1) & 1, DEV_TIMEOUT_LOADED)))
           break;
         tc_fence_after();
         if (lane == 0) next_full = mbar_test_wait(&full[(i + 1) % S], ((i + 1) / S) & 1);
@@ -320,11 +363,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<MODE, BN, YVEC>::kPerSm)
                        j > 0 || r > 0 || q < p.pieces - 1);
           umma_commit_e(&empty[s]);
         } else {
-          const uint32_t g = smem_u32(sf) + (uint32_t)((c & 1) * C::kSf * 1024 + 512 * k);
-          mx_stage1_e(d, umma_desc(xa, 16, 1024, kLayoutSW128), umma_desc(ya, 16, 1024, kLayoutSW128),
-                      ((uint32_t)(BN >> 3) << 17) | (1u << 23) | ((uint32_t)(kX >> 4) << 24),
-                      tmem + 2 * BN + 8u * (uint32_t)(i & 1), umma_desc(g, 128, 128, 0),
-                      umma_desc(g + C::kSf * 512, 128, 128, 0), j > 0, &empty[s]);
+          constexpr uint32_t kOperand = C::kSf * C::kSfBytes;  // Y's scales behind X's
+          const uint32_t g = smem_u32(sf) + (uint32_t)(c & 1) * 2 * kOperand + (uint32_t)(C::kSfBytes * k);
+          if (MODE == 3)
+            mx4_stage1_e(d, umma_desc(xa, 16, 1024, kLayoutSW128), umma_desc(ya, 16, 1024, kLayoutSW128),
+                         mx4_idesc(kX, BN, 0), mx4_idesc(kX, BN, 2), tmem + 2 * BN + 16u * (uint32_t)(i & 1),
+                         umma_desc(g, 128, 128, 0), umma_desc(g + kOperand, 128, 128, 0), j > 0, &empty[s]);
+          else
+            mx_stage1_e(d, umma_desc(xa, 16, 1024, kLayoutSW128), umma_desc(ya, 16, 1024, kLayoutSW128),
+                        ((uint32_t)(BN >> 3) << 17) | (1u << 23) | ((uint32_t)(kX >> 4) << 24),
+                        tmem + 2 * BN + 8u * (uint32_t)(i & 1), umma_desc(g, 128, 128, 0),
+                        umma_desc(g + kOperand, 128, 128, 0), j > 0, &empty[s]);
           if (k == C::kSf - 1) umma_commit_e(&sempty[c & 1]);
         }
       }
@@ -339,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<MODE, BN, YVEC>::kPerSm)
 #pragma unroll
     for (int j = 0; j < BN / 2; ++j) acc[j] = 0ull;
     bool ok = true;
-    // MODE 2: the scales of blocks kSf c .. into buffer c & 1
+    // MODE 2, 3: the scales of stages kSf c .. into buffer c & 1
     auto scale_words = [&](int c) {
       const int first = c * C::kSf;
       if (first >= nst) return;
@@ -351,21 +400,29 @@ __global__ void __launch_bounds__(kThreads, Cfg<MODE, BN, YVEC>::kPerSm)
         ok = __shfl_sync(0xffffffffu, got, 0) != 0;
       }
       const int n = nst - first < C::kSf ? nst - first : C::kSf;
-      uint8_t* g = sf + (c & 1) * C::kSf * 1024;
+      uint8_t* g = sf + (c & 1) * C::kSf * 2 * C::kSfBytes;
       // (both operands' loads before the first store: one latency, not two)
-      uint32_t rx[C::kSf], ry[C::kSf];
-      load_scale_bytes(p.scx, (int64_t)tx * kX + et, p.xrows, i0 + first, n, rx);
-      load_scale_bytes(p.scy, (int64_t)ty * BN + et, et < BN ? p.ycols : 0, i0 + first, n, ry);
-      store_scale_words(rx, g, et);
-      store_scale_words(ry, g + C::kSf * 512, et);
+      constexpr int kWords = C::kSf * C::kSfBytes / 512;
+      uint32_t rx[kWords], ry[kWords];
+      if (MODE == 3) {
+        load_scale_words(p.scx, (int64_t)tx * kX + et, p.xrows, 2 * (i0 + first), 2 * n, p.sc_bytes,
+                         p.sc_vec, rx);
+        load_scale_words(p.scy, (int64_t)ty * BN + et, et < BN ? p.ycols : 0, 2 * (i0 + first), 2 * n,
+                         p.sc_bytes, p.sc_vec, ry);
+      } else {
+        load_scale_bytes(p.scx, (int64_t)tx * kX + et, p.xrows, i0 + first, n, rx);
+        load_scale_bytes(p.scy, (int64_t)ty * BN + et, et < BN ? p.ycols : 0, i0 + first, n, ry);
+      }
+      store_scale_words<MODE>(rx, g, et);
+      store_scale_words<MODE>(ry, g + C::kSf * C::kSfBytes, et);
       fence_proxy_async_smem();  // the tensor core's copies read them
       mbar_arrive(&sfull[c & 1]);
     };
-    if (MODE == 2) scale_words(0);
+    if (MODE >= 2) scale_words(0);
     for (int u = 0; u < units; ++u) {
       const int b = u & 1;
       // the next buffer, while this one's blocks are multiplied
-      if (MODE == 2 && u * C::kPerUnit % C::kSf == 0) scale_words(u * C::kPerUnit / C::kSf + 1);
+      if (MODE >= 2 && u * C::kPerUnit % C::kSf == 0) scale_words(u * C::kPerUnit / C::kSf + 1);
       if (MODE == 0 && u % kScaleUnits == 0) {
         // the next blocks' scales, decoded, eight loads in flight a thread
         const int n = units - u < kScaleUnits ? units - u : kScaleUnits;
@@ -639,7 +696,7 @@ int fp8_gemm_run(rtb_ctx* ctx, const Fp8Desc& d, cudaStream_t s) {
   const uint8_t* Y = swap ? d.A : d.B;
   const bool pairs = !swap && use_pairs(ctx, p);
   if (pairs && !p.scx.is_f32 && !p.scy.is_f32)
-    return launch_mx(ctx, X, d.lda, Y, d.ldb, p, s);
+    return launch_mx(ctx, X, d.lda, Y, d.ldb, p, false, s);
   CUtensorMap tmX, tmY;
   if ((st = make_tmap_2d_bytes(&tmX, X, 1, (uint64_t)d.K, (uint64_t)p.xrows,
                                (uint64_t)(swap ? d.ldb : d.lda), 128, kX)))
@@ -658,6 +715,48 @@ int fp8_gemm_run(rtb_ctx* ctx, const Fp8Desc& d, cudaStream_t s) {
   if (bn == 32) return yvec ? launch<0, 32, true>(ctx, tmX, tmY, p, s) : launch<0, 32, false>(ctx, tmX, tmY, p, s);
   if (bn == 64) return yvec ? launch<0, 64, true>(ctx, tmX, tmY, p, s) : launch<0, 64, false>(ctx, tmX, tmY, p, s);
   return yvec ? launch<0, 128, true>(ctx, tmX, tmY, p, s) : launch<0, 128, false>(ctx, tmX, tmY, p, s);
+}
+
+int fp4_gemm_run(rtb_ctx* ctx, const Fp4Desc& d, cudaStream_t s) {
+  int st;
+  if ((st = check_extents(d.M, d.N, d.K))) return st;
+  const bool swap = d.M <= 64;  // few rows of A: as in fp8_gemm_run
+  BlockParams p{};
+  p.xrows = swap ? d.N : d.M;
+  p.ycols = swap ? d.M : d.N;
+  p.depth = (int)(d.K / 2);
+  p.out = d.C;
+  p.ldo = d.ldc;
+  p.swap = swap;
+  p.bias = d.bias;
+  p.act = d.act;
+  ScaleRef sa, sb;
+  sa.p = d.sa;
+  sa.ld_row = d.ldsa;
+  sb.p = d.sb;
+  sb.ld_row = d.ldsb;
+  p.scx = swap ? sb : sa;
+  p.scy = swap ? sa : sb;
+  p.sc_bytes = (int)((d.K + 31) / 32);
+  p.sc_vec = ((reinterpret_cast<uintptr_t>(d.sa) | reinterpret_cast<uintptr_t>(d.sb)) & 3u) == 0 &&
+             d.ldsa % 4 == 0 && d.ldsb % 4 == 0;
+  p.err = ctx->d_err;
+  p.timeout_ns = ctx->timeout_ns;
+  const int bn = swap ? (d.M <= 16 ? 16 : d.M <= 32 ? 32 : 64) : 128;
+  const uint8_t* X = swap ? d.B : d.A;
+  const uint8_t* Y = swap ? d.A : d.B;
+  const int64_t ldx = swap ? d.ldb : d.lda, ldy = swap ? d.lda : d.ldb;
+  if (!swap && use_pairs(ctx, p)) return launch_mx(ctx, X, ldx, Y, ldy, p, true, s);
+  CUtensorMap tmX, tmY;
+  if ((st = make_tmap_2d_bytes(&tmX, X, 1, (uint64_t)p.depth, (uint64_t)p.xrows, (uint64_t)ldx, 128, kX)))
+    return st;
+  if ((st = make_tmap_2d_bytes(&tmY, Y, 1, (uint64_t)p.depth, (uint64_t)p.ycols, (uint64_t)ldy, 128,
+                               (uint32_t)bn)))
+    return st;
+  if (bn == 16) return launch<3, 16, false>(ctx, tmX, tmY, p, s);
+  if (bn == 32) return launch<3, 32, false>(ctx, tmX, tmY, p, s);
+  if (bn == 64) return launch<3, 64, false>(ctx, tmX, tmY, p, s);
+  return launch<3, 128, false>(ctx, tmX, tmY, p, s);
 }
 
 int wgrad_run(rtb_ctx* ctx, const WgradDesc& d, cudaStream_t s) {

@@ -14,7 +14,7 @@ namespace rtb {
 
 struct BlockParams {
   int64_t xrows, ycols;  // output extents along X and Y
-  int depth;             // contraction length
+  int depth;             // contraction length (4-bit operands: bytes of a row)
   int stages_total;      // ceil(depth / kDepth)
   int tiles_x, tiles_y;
   float* out;            // row-major, leading dimension ldo
@@ -25,7 +25,8 @@ struct BlockParams {
   int accumulate;
   int pieces;            // MODE 1
   int64_t piece_rows;    // MODE 1: contraction rows between Y's pieces
-  ScaleRef scx, scy;     // MODE 0
+  ScaleRef scx, scy;
+  int sc_bytes, sc_vec;  // 4-bit operands: scales of a row, and whether their rows are 4-byte aligned
   // MODE 0, CTA pairs: the scales as fp32, [block][row], zero past the operand
   // (launch_scale_tables)
   const float *tabx, *taby;
@@ -78,9 +79,29 @@ __device__ __forceinline__ void tmem_wait_x16(uint32_t (&r)[16]) {
 // a quad can be loaded ahead without a check.
 inline int64_t table_blocks(int64_t units) { return (units + 3) / 4 * 4 + 4; }
 
+// 4-bit operands: word j of row r's scales, four blocks of 32 columns; 2^0 past the
+// row's last one.
+__device__ __forceinline__ uint32_t fp4_scale_word(const ScaleRef& s, int64_t r, int j, int bytes,
+                                                   int vec) {
+  const uint8_t* p = static_cast<const uint8_t*>(s.p) + r * s.ld_row + (int64_t)4 * j;
+  const int left = bytes - 4 * j;
+  if (vec && left >= 4) return __ldg(reinterpret_cast<const uint32_t*>(p));
+  uint32_t v = 0;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) v |= (b < left ? (uint32_t)__ldg(p + b) : 127u) << (8 * b);
+  return v;
+}
+// Instruction descriptor of kind::mxf4: e2m1 operands ([7,10), [10,12) = 1), K-major,
+// N >> 3 at [17,23), scales e8m0 [23], M >> 4 at [24,29); the scales' place in their
+// word, byte 0 or 2, at [4,6) (B) and [29,31) (A).
+constexpr __host__ __device__ uint32_t mx4_idesc(int m, int n, int byte) {
+  return ((uint32_t)byte << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) |
+         ((uint32_t)(m >> 4) << 24) | ((uint32_t)byte << 29);
+}
+
 // Products on CTA pairs (rtb_pairgemm.cu); yvec as in rtb_blockgemm.cu.
 int launch_mx(rtb_ctx* ctx, const uint8_t* X, int64_t ldx, const uint8_t* Y, int64_t ldy,
-              BlockParams& p, cudaStream_t s);  // e8m0 scales (rtb_mxgemm.cu)
+              BlockParams& p, bool fp4, cudaStream_t s);  // e8m0 scales (rtb_mxgemm.cu)
 int launch_pair(rtb_ctx* ctx, int mode, bool yvec, const CUtensorMap& tmX, const CUtensorMap& tmY,
                 BlockParams& p, cudaStream_t s);
 

@@ -1,9 +1,7 @@
-// Writing and restoring 4-bit block-scaled tensors (rtb_fp4.cuh), and a first form of
-// their product.
+// Writing and restoring 4-bit block-scaled tensors (rtb_fp4.cuh).
 //   save:    s = 2^ceil(log2(max|x| / 6)) over the block, q = e2m1(x / s)
 //   restore: x' = q * s
 // Both stream their operands once (4.53 bytes a value): HBM-bound.
-#include "rtb_act.cuh"
 #include "rtb_fp4.cuh"
 #include "rtb_internal.h"
 #include "rtb_ptx.cuh"
@@ -248,57 +246,6 @@ __global__ void __launch_bounds__(kThreads) fp4_dequantize_any_kernel(const uint
   }
 }
 
-// The product, 64 x 64 outputs a CTA, 32 contraction elements (one block) at a time:
-// exact products of codes, summed in fp32, a block's scales applied to its sum.
-__global__ void __launch_bounds__(kThreads) fp4_matmul_kernel(const Fp4Desc p) {
-  __shared__ float as[32][65], bs[32][65];
-  __shared__ float sa[64], sb[64];
-  griddep_wait();
-  griddep_launch_dependents();
-  const int64_t m0 = (int64_t)blockIdx.y * 64, n0 = (int64_t)blockIdx.x * 64;
-  const int tr = threadIdx.x >> 4, tc = threadIdx.x & 15;
-  float acc[4][4] = {};
-  const int64_t half = p.K / 2;
-  for (int64_t k0 = 0; k0 < p.K; k0 += 32) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < 64 * 16; i += kThreads) {
-      const int r = i >> 4, b = i & 15;
-      const int64_t at = k0 / 2 + b;
-      float v[8], u[8];
-      e2m1x8_to_float(m0 + r < p.M && at < half ? p.A[(m0 + r) * p.lda + at] : 0u, v);
-      e2m1x8_to_float(n0 + r < p.N && at < half ? p.B[(n0 + r) * p.ldb + at] : 0u, u);
-      as[2 * b][r] = v[0];
-      as[2 * b + 1][r] = v[1];
-      bs[2 * b][r] = u[0];
-      bs[2 * b + 1][r] = u[1];
-    }
-    if (threadIdx.x < 64) {
-      const int r = threadIdx.x;
-      sa[r] = m0 + r < p.M ? e8m0_to_float(p.sa[(m0 + r) * p.ldsa + k0 / 32]) : 0.0f;
-      sb[r] = n0 + r < p.N ? e8m0_to_float(p.sb[(n0 + r) * p.ldsb + k0 / 32]) : 0.0f;
-    }
-    __syncthreads();
-    float t[4][4] = {};
-    for (int k = 0; k < 32; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) t[i][j] = fmaf(as[k][tr + 16 * i], bs[k][tc + 16 * j], t[i][j]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] += t[i][j] * sa[tr + 16 * i] * sb[tc + 16 * j];
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + tr + 16 * i, n = n0 + tc + 16 * j;
-      if (m < p.M && n < p.N)
-        p.C[m * p.ldc + n] = activate(acc[i][j] + (p.bias ? p.bias[n] : 0.0f), p.act);
-    }
-}
-
 template <typename... KArgs, typename... Args>
 int run(const char* what, void (*k)(KArgs...), int grid, cudaStream_t s, Args... args) {
   clear_stale_cuda_error();
@@ -348,15 +295,6 @@ int launch_fp4_dequantize(rtb_ctx* ctx, const uint8_t* q, int64_t ldq, int64_t r
   return run("fp4_dequantize launch", fp4_dequantize_any_kernel,
              grid_for(ctx, (total + 8 * kBlocks - 1) / (8 * kBlocks), 8), s, q, ldq, total, (int)cols,
              cblocks, scale, lds, y, ldy);
-}
-
-int fp4_gemm_run(rtb_ctx* ctx, const Fp4Desc& d, cudaStream_t s) {
-  const int64_t gx = (d.N + 63) / 64, gy = (d.M + 63) / 64;
-  if (gy > 65535) return set_error(RTB_E_UNSUPPORTED, "fp4_matmul: too many rows");
-  clear_stale_cuda_error();
-  cudaError_t e = launch_pdl(fp4_matmul_kernel, dim3((unsigned)gx, (unsigned)gy), dim3(kThreads), 0, s, d);
-  if (e == cudaSuccess) e = cudaGetLastError();
-  return e == cudaSuccess ? RTB_OK : cuda_status(e, "fp4_matmul launch");
 }
 
 }  // namespace rtb

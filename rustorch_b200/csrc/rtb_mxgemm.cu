@@ -10,6 +10,10 @@
 // TMEM loads and adds, 1150 clocks against 512 of MMAs in rtb_pairgemm.cu, is out
 // of the way.
 //
+// The same for e2m1 operands with a scale for each 32 columns (FP4, kind::mxf4, 64
+// contraction elements an MMA): a stage's 128 bytes of a row are 256 elements with eight
+// scales, two groups of four for each 128 rows.
+//
 // Tile 256 x 256 with one accumulator or 256 x 224 with two (the scales need
 // columns of TMEM too), whichever takes less time in whole rounds of the pairs.
 // Roles (warps of each CTA): 0, 2, 3 TMA producers; 1 TMEM allocation, and in the
@@ -37,12 +41,15 @@ namespace {
 constexpr int kThreads = 384;
 constexpr int kTileX = 256;
 constexpr int kStages = 5;
-constexpr int kStageBytes = 16384 + 16384 + 2048;  // X, Y (half of the tile's rows), scales
+// X, Y (half of the tile's rows), scales
+constexpr int stage_bytes(bool fp4) { return 16384 + 16384 + (fp4 ? 3072 : 2048); }
 constexpr int kChunk = 128 * 16 * 4;               // a staged 128 x 16 fp32 piece of the output
 constexpr int kBufs = 3;                           // staging chunks of an epilogue half
-constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 2 * kBufs * kChunk + 512 + 1024;
-constexpr uint32_t kScaleCol = 448;                // TMEM: two buffers of 4 + 8 columns
-static_assert(kSmemBytes <= 232448, "shared memory");
+constexpr int smem_bytes(bool fp4) {
+  return 1024 + kStages * stage_bytes(fp4) + 2 * kBufs * kChunk + 512 + 1024;
+}
+constexpr uint32_t kScaleCol = 448;                // TMEM: two buffers of 4 + 8 columns (FP4: 8 + 16)
+static_assert(smem_bytes(true) <= 232448 && smem_bytes(false) <= 232448, "shared memory");
 
 // Instruction descriptor of kind::mxf8f6f4: scale ids 0 ([4,6) and [29,31)),
 // e4m3 operands, K-major, N >> 3 at [17,23), scales e8m0 [23], M >> 4 at [24,29).
@@ -79,6 +86,41 @@ __device__ __forceinline__ void mx_stage_e(uint32_t d, uint64_t a, uint64_t b, u
       "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
       "[%7], m;\n\t}" ::"r"(d),
       "l"(a), "l"(b), "r"(id), "r"(sa), "l"(sc), "r"(acc), "r"(smem_u32(empty))
+      : "memory");
+}
+
+// The same of FP4: six groups of 128 rows x 128 contraction elements (X's two, then
+// Y's two halves of the first 128 elements and of the second) into 24 columns, and MMAs
+// of 64 elements with the scales in bytes 0, 1 and 2, 3 of a group's words.
+__device__ __forceinline__ void mx4_stage_e(uint32_t d, uint64_t a, uint64_t b, uint32_t id0,
+                                            uint32_t id2, uint32_t sa, uint64_t sc, uint32_t acc,
+                                            uint64_t* empty) {
+  asm volatile(
+      "{\n\t.reg .pred p, t, e;\n\t.reg .b32 r, s1, s2, s3, s4, s5;\n\t.reg .b16 m;\n\t"
+      ".reg .b64 a1, a2, a3, b1, b2, b3, c1, c2, c3, c4, c5;\n\t"
+      "setp.ne.b32 p, %7, 0;\n\t"
+      "setp.eq.b32 t, 0, 0;\n\t"
+      "mov.b16 m, 3;\n\t"
+      "add.u32 s1, %5, 4;\n\tadd.u32 s2, %5, 8;\n\tadd.u32 s3, %5, 12;\n\t"
+      "add.u32 s4, %5, 16;\n\tadd.u32 s5, %5, 20;\n\t"
+      "add.s64 c1, %6, 32;\n\tadd.s64 c2, %6, 64;\n\tadd.s64 c3, %6, 96;\n\t"
+      "add.s64 c4, %6, 128;\n\tadd.s64 c5, %6, 160;\n\t"
+      "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
+      "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
+      "elect.sync r|e, 0xffffffff;\n\t"
+      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%5], %6;\n\t"
+      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [s1], c1;\n\t"
+      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [s2], c2;\n\t"
+      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [s3], c3;\n\t"
+      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [s4], c4;\n\t"
+      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [s5], c5;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [s2], p;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a1, b1, %4, [%5], [s2], t;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a2, b2, %3, [s1], [s4], t;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a3, b3, %4, [s1], [s4], t;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%8], m;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(id0), "r"(id2), "r"(sa), "l"(sc), "r"(acc), "r"(smem_u32(empty))
       : "memory");
 }
 
@@ -122,6 +164,43 @@ __global__ void __launch_bounds__(256) scale_groups_kernel(const ScaleGroups p) 
   }
 }
 
+// FP4: the groups of a stage's two halves of 128 elements, whose words are four scales
+// as they lie in a row: [xgroups][stage][2][128], then [y tiles][stage][2 halves][2
+// groups][128].  blockIdx.y: 32 words (16 stages).
+struct ScaleGroups4 {
+  ScaleRef x, y;
+  int64_t xrows, yrows;
+  int xgroups, tn, stages, bytes, vec;
+  uint32_t* out;
+};
+__global__ void __launch_bounds__(256) fp4_scale_groups_kernel(const ScaleGroups4 p) {
+  __shared__ uint32_t t[128][33];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int g = blockIdx.x, j0 = blockIdx.y * 32;
+  const bool isx = g < p.xgroups;
+  const int yg = g - p.xgroups, tile = yg >> 1, part = yg & 1;
+  const ScaleRef& s = isx ? p.x : p.y;
+  const int64_t first = isx ? (int64_t)g * 128 : (int64_t)tile * p.tn + part * 128;
+  const int64_t end = isx ? p.xrows : ((int64_t)(tile + 1) * p.tn < p.yrows ? (int64_t)(tile + 1) * p.tn : p.yrows);
+#pragma unroll 8
+  for (int i = w; i < 128; i += 8) {
+    const int64_t r = first + i;
+    t[i][lane] = r < end ? fp4_scale_word(s, r, j0 + lane, p.bytes, p.vec) : 0x7F7F7F7Fu;
+  }
+  __syncthreads();
+  // word q of a group is row q / 4 + 32 (q % 4)
+  const int64_t base = isx ? (int64_t)g * p.stages * 2
+                           : (int64_t)p.xgroups * p.stages * 2 + (int64_t)tile * p.stages * 4 + part;
+  const int step = isx ? 1 : 2;
+  for (int i = threadIdx.x; i < 32 * 128; i += 256) {
+    const int jj = i >> 7, q = i & 127;
+    if (j0 + jj < 2 * p.stages)
+      p.out[(base + (int64_t)(j0 + jj) * step) * 128 + q] = t[(q >> 2) + 32 * (q & 3)][jj];
+  }
+}
+
 // Tiles in bands of 8 X tiles, so that the 74 pairs' working set is about
 // square.
 __device__ __forceinline__ void mx_tile(const BlockParams& p, int t, int& tx, int& ty) {
@@ -134,17 +213,18 @@ __device__ __forceinline__ void mx_tile(const BlockParams& p, int t, int& tx, in
   ty = r / h;
 }
 
-template <int TN>
+template <int TN, bool FP4>
 __global__ void __launch_bounds__(kThreads, 1)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmY,
                    const __grid_constant__ CUtensorMap tmSx, const __grid_constant__ CUtensorMap tmSy,
                    const __grid_constant__ CUtensorMap tmC, const BlockParams p) {
   constexpr int S = kStages;
+  constexpr int kStageBytes = stage_bytes(FP4);
   constexpr int kHalf = TN / 2;  // columns of an epilogue half, Y rows of a CTA
   // two accumulators where the scales leave room for them; one is promoted half
   // as often, since its MMAs wait for the promotion
   constexpr int kAccBufs = 2 * TN <= (int)kScaleCol ? 2 : 1;
-  constexpr int kPerUnit = kAccBufs == 2 ? 8 : 16;  // blocks of 128 between promotions
+  constexpr int kPerUnit = kAccBufs == 2 ? 8 : 16;  // stages between promotions
   static_assert(TN % 32 == 0 && TN <= 256, "tile width");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -206,8 +286,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       // stage's four loads takes about 600 clocks, longer than its MMAs
       const int turn = warp ? warp - 1 : 0;
       int q = 0;
-      // X 128 rows, half of the Y rows and three scale groups, of both CTAs
-      const uint32_t bytes = 2u * (16384u + (uint32_t)kHalf * 128u + 3u * 512u);
+      // X 128 rows, half of the Y rows and three (FP4: six) scale groups, of both CTAs
+      const uint32_t bytes = 2u * (16384u + (uint32_t)kHalf * 128u + (FP4 ? 6u : 3u) * 512u);
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
@@ -229,8 +309,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
           tma_load_2d_pair(st, &tmX, bar, i * 128, x0);
           tma_load_2d_pair(st + 16384, &tmY, bar, i * 128, y0);
-          tma_load_2d_pair(st + 32768, &tmSx, bar, 0, (2 * tx + (int)rank) * nst + i);
-          tma_load_2d_pair(st + 32768 + 512, &tmSy, bar, 0, 2 * (ty * nst + i));
+          if (FP4) {
+            tma_load_2d_pair(st + 32768, &tmSx, bar, 0, 2 * ((2 * tx + (int)rank) * nst + i));
+            tma_load_2d_pair(st + 32768 + 1024, &tmSy, bar, 0, 4 * (ty * nst + i));
+          } else {
+            tma_load_2d_pair(st + 32768, &tmSx, bar, 0, (2 * tx + (int)rank) * nst + i);
+            tma_load_2d_pair(st + 32768 + 512, &tmSy, bar, 0, 2 * (ty * nst + i));
+          }
           if (++s == S) { s = 0; ph ^= 1; }
         }
       }
@@ -270,10 +355,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             // operands K-major in 128-byte swizzled rows; scale groups unswizzled,
             // 8-row groups 128 bytes apart
             const uint32_t xa = smem_u32(base + s * kStageBytes);
-            mx_stage_e(d, umma_desc(xa, 16, 1024, kLayoutSW128),
-                       umma_desc(xa + 16384, 16, 1024, kLayoutSW128), mx_idesc(TN),
-                       tmem + kScaleCol + 12u * (uint32_t)q, umma_desc(xa + 32768, 128, 128, 0), j > 0,
-                       &empty[s]);
+            if (FP4)
+              mx4_stage_e(d, umma_desc(xa, 16, 1024, kLayoutSW128),
+                          umma_desc(xa + 16384, 16, 1024, kLayoutSW128), mx4_idesc(kTileX, TN, 0),
+                          mx4_idesc(kTileX, TN, 2), tmem + kScaleCol + 24u * (uint32_t)q,
+                          umma_desc(xa + 32768, 128, 128, 0), j > 0, &empty[s]);
+            else
+              mx_stage_e(d, umma_desc(xa, 16, 1024, kLayoutSW128),
+                         umma_desc(xa + 16384, 16, 1024, kLayoutSW128), mx_idesc(TN),
+                         tmem + kScaleCol + 12u * (uint32_t)q, umma_desc(xa + 32768, 128, 128, 0), j > 0,
+                         &empty[s]);
             if (last) commit_pair_e(&tfull[b]);
             s = sn;
             ph = phn;
@@ -395,10 +486,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int TN>
+template <int TN, bool FP4>
 int launch(rtb_ctx* ctx, const uint8_t* X, int64_t ldx, const uint8_t* Y, int64_t ldy,
            BlockParams& p, cudaStream_t s) {
-  auto* k = mx_gemm_kernel<TN>;
+  constexpr int kSmemBytes = smem_bytes(FP4);
+  auto* k = mx_gemm_kernel<TN, FP4>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
   if (e != cudaSuccess) return cuda_status(e, "block-scaled gemm smem attribute");
   p.tiles_x = (int)((p.xrows + kTileX - 1) / kTileX);
@@ -424,26 +516,34 @@ int launch(rtb_ctx* ctx, const uint8_t* X, int64_t ldx, const uint8_t* Y, int64_
                                         (uint64_t)p.ldo, 16, 128, kTmapSwizzle64)))
     return st;
   // the scale groups: X's tiles of 256 rows have two, whole or not
-  ScaleGroups sg = {p.scx, p.scy, p.xrows, p.ycols, 2 * p.tiles_x, TN, p.stages_total, nullptr};
-  const int64_t groups = (int64_t)sg.xgroups + 2 * p.tiles_y;
-  const int64_t rows = groups * p.stages_total;
+  constexpr int kPer = FP4 ? 2 : 1;  // groups of 128 rows in a stage
+  const int xgroups = 2 * p.tiles_x;
+  const int64_t groups = (int64_t)xgroups + 2 * p.tiles_y;
+  const int64_t rows = groups * p.stages_total * kPer;
   if (rows > INT32_MAX / 2) return set_error(RTB_E_UNSUPPORTED, "block-scaled gemm: too many scales");
-  if ((st = ws_alloc(ctx, (void**)&sg.out, (size_t)rows * 512, s))) return st;
-  const float* fx = reinterpret_cast<const float*>(sg.out);
-  const int64_t xr = (int64_t)sg.xgroups * p.stages_total;
+  uint32_t* ws = nullptr;
+  if ((st = ws_alloc(ctx, (void**)&ws, (size_t)rows * 512, s))) return st;
+  const float* fx = reinterpret_cast<const float*>(ws);
+  const int64_t xr = (int64_t)xgroups * p.stages_total * kPer;
   CUtensorMap tmSx, tmSy;
-  st = make_tmap_2d_swz(&tmSx, fx, 128, (uint64_t)xr, 128, 128, 1, kTmapSwizzleNone);
+  st = make_tmap_2d_swz(&tmSx, fx, 128, (uint64_t)xr, 128, 128, kPer, kTmapSwizzleNone);
   if (st == RTB_OK)
-    st = make_tmap_2d_swz(&tmSy, fx + xr * 128, 128, (uint64_t)(rows - xr), 128, 128, 2,
+    st = make_tmap_2d_swz(&tmSy, fx + xr * 128, 128, (uint64_t)(rows - xr), 128, 128, 2 * kPer,
                           kTmapSwizzleNone);
   if (st != RTB_OK) {
-    ws_free(sg.out, s);
+    ws_free(ws, s);
     return st;
   }
   clear_stale_cuda_error();
-  e = launch_pdl(scale_groups_kernel,
-                 dim3((unsigned)groups, (unsigned)((p.stages_total + 31) / 32)), dim3(256), 0, s,
-                 (const ScaleGroups)sg);
+  const dim3 grid((unsigned)groups, (unsigned)((p.stages_total * kPer + 31) / 32));
+  if (FP4) {
+    const ScaleGroups4 sg = {p.scx, p.scy, p.xrows, p.ycols, xgroups, TN, p.stages_total, p.sc_bytes,
+                             p.sc_vec, ws};
+    e = launch_pdl(fp4_scale_groups_kernel, grid, dim3(256), 0, s, sg);
+  } else {
+    const ScaleGroups sg = {p.scx, p.scy, p.xrows, p.ycols, xgroups, TN, p.stages_total, ws};
+    e = launch_pdl(scale_groups_kernel, grid, dim3(256), 0, s, sg);
+  }
   const int64_t pairs = ctx->sm_count / 2 < tiles ? ctx->sm_count / 2 : tiles;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * pairs));
@@ -461,14 +561,14 @@ int launch(rtb_ctx* ctx, const uint8_t* X, int64_t ldx, const uint8_t* Y, int64_
   cfg.numAttrs = 2;
   if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, k, tmX, tmY, tmSx, tmSy, tmC, (const BlockParams)p);
   if (e == cudaSuccess) e = cudaGetLastError();
-  ws_free(sg.out, s);
+  ws_free(ws, s);
   return e == cudaSuccess ? RTB_OK : cuda_status(e, "block-scaled gemm launch");
 }
 
 }  // namespace
 
 int launch_mx(rtb_ctx* ctx, const uint8_t* X, int64_t ldx, const uint8_t* Y, int64_t ldy,
-              BlockParams& p, cudaStream_t s) {
+              BlockParams& p, bool fp4, cudaStream_t s) {
   // 256 columns move fewer bytes for a product, 224 have room for a second
   // accumulator, behind which a tile's epilogue (and the promotions) pass.  In
   // whole rounds of the pairs, from the measured times of a round: 0.37 us a
@@ -479,8 +579,10 @@ int launch_mx(rtb_ctx* ctx, const uint8_t* X, int64_t ldx, const uint8_t* Y, int
     const int64_t pairs = ctx->sm_count / 2;
     return (double)((tiles + pairs - 1) / pairs) * (0.37 * ((p.depth + 127) / 128) + tile_us);
   };
-  return cost(224, 4.0) < 0.95 * cost(256, 6.0) ? launch<224>(ctx, X, ldx, Y, ldy, p, s)
-                                                : launch<256>(ctx, X, ldx, Y, ldy, p, s);
+  const bool narrow = cost(224, 4.0) < 0.95 * cost(256, 6.0);
+  if (fp4)
+    return narrow ? launch<224, true>(ctx, X, ldx, Y, ldy, p, s) : launch<256, true>(ctx, X, ldx, Y, ldy, p, s);
+  return narrow ? launch<224, false>(ctx, X, ldx, Y, ldy, p, s) : launch<256, false>(ctx, X, ldx, Y, ldy, p, s);
 }
 
 }  // namespace rtb
