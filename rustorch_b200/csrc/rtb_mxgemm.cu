@@ -12,7 +12,12 @@
 //
 // The same for e2m1 operands with a scale for each 32 columns (FP4, kind::mxf4, 64
 // contraction elements an MMA): a stage's 128 bytes of a row are 256 elements with eight
-// scales, two groups of four for each 128 rows.
+// scales, two groups of four for each 128 rows.  Twice the scales in the same time: the
+// tensor core runs its copies between the MMAs and not beside them, six a stage then, 20
+// clocks each.  So four more warps read the groups out of shared memory and write them
+// into TMEM (tcgen05.st), a place for each stage of the ring: 8192 x 4096 x 8192 126 ->
+// 120 us.  (The same words straight from global memory into registers, a stage ahead: 171
+// us, each stage waiting for them; copies a stage ahead of their MMAs: 131.)
 //
 // Tile 256 x 256 with one accumulator or 256 x 224 with two (the scales need
 // columns of TMEM too), whichever takes less time in whole rounds of the pairs.
@@ -32,13 +37,20 @@
 // 2.1 PFLOP/s; 8192 x 8192 x 1024 in 97 and 105.  Outputs that TMA cannot store (N or
 // ldc off a multiple of 4) leave by scalar stores, 32 rows an instruction: 8192 x 4097
 // x 8192 429 us.
+//
+// FP4: 8192 x 4096 x 8192 in 120 us, 4.6 PFLOP/s (135 in a loop, the power cap); 8192 x
+// 4096 x 16384 in 224, 4.9.  A stage takes 0.46 us where its MMAs take 0.31 (the clock
+// at 1.65 GHz): the rest is its operands' way from L2, 35 KB an SM, 11 TB/s over all;
+// without the loads 0.34.  A ring of 4 stages: 131 us, of 6: no change.  Tiles 192 wide
+// with two accumulators: 145 us, and 4% faster where the contraction has 4 stages (2048
+// x 8192 x 1024 33.2 us, 31.8): not kept.
 #include "rtb_pair.cuh"
 
 namespace rtb {
 
 namespace {
 
-constexpr int kThreads = 384;
+constexpr int threads(bool fp4) { return fp4 ? 512 : 384; }
 constexpr int kTileX = 256;
 constexpr int kStages = 5;
 // X, Y (half of the tile's rows), scales
@@ -48,7 +60,8 @@ constexpr int kBufs = 3;                           // staging chunks of an epilo
 constexpr int smem_bytes(bool fp4) {
   return 1024 + kStages * stage_bytes(fp4) + 2 * kBufs * kChunk + 512 + 1024;
 }
-constexpr uint32_t kScaleCol = 448;                // TMEM: two buffers of 4 + 8 columns (FP4: 8 + 16)
+// TMEM: two buffers of 4 + 8 columns; FP4: 8 + 16 for each stage of the ring
+constexpr uint32_t scale_col(bool fp4) { return fp4 ? 512 - 24 * kStages : 448; }
 static_assert(smem_bytes(true) <= 232448 && smem_bytes(false) <= 232448, "shared memory");
 
 // Instruction descriptor of kind::mxf8f6f4: scale ids 0 ([4,6) and [29,31)),
@@ -89,38 +102,42 @@ __device__ __forceinline__ void mx_stage_e(uint32_t d, uint64_t a, uint64_t b, u
       : "memory");
 }
 
-// The same of FP4: six groups of 128 rows x 128 contraction elements (X's two, then
-// Y's two halves of the first 128 elements and of the second) into 24 columns, and MMAs
-// of 64 elements with the scales in bytes 0, 1 and 2, 3 of a group's words.
+// FP4: four MMAs of 64 elements with the scales in bytes 0, 1 and 2, 3 of their words;
+// X's words of the stage's two halves at columns sa and sa + 4, Y's at sa + 8 and sa + 16.
 __device__ __forceinline__ void mx4_stage_e(uint32_t d, uint64_t a, uint64_t b, uint32_t id0,
-                                            uint32_t id2, uint32_t sa, uint64_t sc, uint32_t acc,
-                                            uint64_t* empty) {
+                                            uint32_t id2, uint32_t sa, uint32_t acc, uint64_t* empty) {
   asm volatile(
-      "{\n\t.reg .pred p, t, e;\n\t.reg .b32 r, s1, s2, s3, s4, s5;\n\t.reg .b16 m;\n\t"
-      ".reg .b64 a1, a2, a3, b1, b2, b3, c1, c2, c3, c4, c5;\n\t"
-      "setp.ne.b32 p, %7, 0;\n\t"
+      "{\n\t.reg .pred p, t, e;\n\t.reg .b32 r, s1, s2, s4;\n\t.reg .b16 m;\n\t"
+      ".reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
       "setp.eq.b32 t, 0, 0;\n\t"
       "mov.b16 m, 3;\n\t"
-      "add.u32 s1, %5, 4;\n\tadd.u32 s2, %5, 8;\n\tadd.u32 s3, %5, 12;\n\t"
-      "add.u32 s4, %5, 16;\n\tadd.u32 s5, %5, 20;\n\t"
-      "add.s64 c1, %6, 32;\n\tadd.s64 c2, %6, 64;\n\tadd.s64 c3, %6, 96;\n\t"
-      "add.s64 c4, %6, 128;\n\tadd.s64 c5, %6, 160;\n\t"
+      "add.u32 s1, %5, 4;\n\tadd.u32 s2, %5, 8;\n\tadd.u32 s4, %5, 16;\n\t"
       "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
       "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
       "elect.sync r|e, 0xffffffff;\n\t"
-      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%5], %6;\n\t"
-      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [s1], c1;\n\t"
-      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [s2], c2;\n\t"
-      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [s3], c3;\n\t"
-      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [s4], c4;\n\t"
-      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [s5], c5;\n\t"
       "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [s2], p;\n\t"
       "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a1, b1, %4, [%5], [s2], t;\n\t"
       "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a2, b2, %3, [s1], [s4], t;\n\t"
       "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a3, b3, %4, [s1], [s4], t;\n\t"
       "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
-      "[%8], m;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(id0), "r"(id2), "r"(sa), "l"(sc), "r"(acc), "r"(smem_u32(empty))
+      "[%7], m;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(id0), "r"(id2), "r"(sa), "r"(acc), "r"(smem_u32(empty))
+      : "memory");
+}
+// 32 lanes x 24 columns of TMEM: lane l's six quads of words.
+__device__ __forceinline__ void tmem_st_quads(uint32_t taddr, const float4 (&v)[6]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+      "f"(v[0].x), "f"(v[0].y), "f"(v[0].z), "f"(v[0].w), "f"(v[1].x), "f"(v[1].y), "f"(v[1].z),
+      "f"(v[1].w)
+      : "memory");
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16};" ::"r"(taddr + 8),
+      "f"(v[2].x), "f"(v[2].y), "f"(v[2].z), "f"(v[2].w), "f"(v[3].x), "f"(v[3].y), "f"(v[3].z),
+      "f"(v[3].w), "f"(v[4].x), "f"(v[4].y), "f"(v[4].z), "f"(v[4].w), "f"(v[5].x), "f"(v[5].y),
+      "f"(v[5].z), "f"(v[5].w)
       : "memory");
 }
 
@@ -184,10 +201,25 @@ __global__ void __launch_bounds__(256) fp4_scale_groups_kernel(const ScaleGroups
   const ScaleRef& s = isx ? p.x : p.y;
   const int64_t first = isx ? (int64_t)g * 128 : (int64_t)tile * p.tn + part * 128;
   const int64_t end = isx ? p.xrows : ((int64_t)(tile + 1) * p.tn < p.yrows ? (int64_t)(tile + 1) * p.tn : p.yrows);
-#pragma unroll 8
-  for (int i = w; i < 128; i += 8) {
-    const int64_t r = first + i;
-    t[i][lane] = r < end ? fp4_scale_word(s, r, j0 + lane, p.bytes, p.vec) : 0x7F7F7F7Fu;
+  // (whole words first, all of a thread's loads in flight; the few others behind them)
+  const bool whole = p.vec && 4 * (j0 + lane) + 4 <= p.bytes;
+  uint32_t v[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const int64_t r = first + w + 8 * k;
+    v[k] = 0x7F7F7F7Fu;
+    if (whole && r < end)
+      v[k] = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(s.p) + r * s.ld_row) +
+                   j0 + lane);
+  }
+#pragma unroll
+  for (int k = 0; k < 16; ++k) t[w + 8 * k][lane] = v[k];
+  if (!whole && 4 * (j0 + lane) < p.bytes) {
+#pragma unroll 4
+    for (int k = 0; k < 16; ++k) {
+      const int64_t r = first + w + 8 * k;
+      if (r < end) t[w + 8 * k][lane] = fp4_scale_word(s, r, j0 + lane, p.bytes, 0);
+    }
   }
   __syncthreads();
   // word q of a group is row q / 4 + 32 (q % 4)
@@ -214,11 +246,13 @@ __device__ __forceinline__ void mx_tile(const BlockParams& p, int t, int& tx, in
 }
 
 template <int TN, bool FP4>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(threads(FP4), 1)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmY,
                    const __grid_constant__ CUtensorMap tmSx, const __grid_constant__ CUtensorMap tmSy,
                    const __grid_constant__ CUtensorMap tmC, const BlockParams p) {
   constexpr int S = kStages;
+  constexpr int kEpi = FP4 ? 8 : 4;  // the first epilogue warp
+  constexpr uint32_t kScaleCol = scale_col(FP4);
   constexpr int kStageBytes = stage_bytes(FP4);
   constexpr int kHalf = TN / 2;  // columns of an epilogue half, Y rows of a CTA
   // two accumulators where the scales leave room for them; one is promoted half
@@ -234,7 +268,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* empty = full + S;
   uint64_t* tfull = empty + S;
   uint64_t* tempty = tfull + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  uint64_t* sfull = tempty + 2;  // FP4: this CTA's scales
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sfull + S);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* bias_s = reinterpret_cast<float*>(staging + 2 * kBufs * kChunk + 512);  // [2][128]
 
@@ -242,8 +277,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t rank = cluster_rank();
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], FP4 ? 9 : 1);  // the loads, FP4: and four warps' scales of both CTAs
       mbar_init(&empty[s], 1);
+      mbar_init(&sfull[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
@@ -286,8 +322,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       // stage's four loads takes about 600 clocks, longer than its MMAs
       const int turn = warp ? warp - 1 : 0;
       int q = 0;
-      // X 128 rows, half of the Y rows and three (FP4: six) scale groups, of both CTAs
-      const uint32_t bytes = 2u * (16384u + (uint32_t)kHalf * 128u + (FP4 ? 6u : 3u) * 512u);
+      // X 128 rows, half of the Y rows and three scale groups, of both CTAs
+      const uint32_t bytes = 2u * (16384u + (uint32_t)kHalf * 128u + (FP4 ? 0u : 3u * 512u));
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
@@ -310,8 +346,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           tma_load_2d_pair(st, &tmX, bar, i * 128, x0);
           tma_load_2d_pair(st + 16384, &tmY, bar, i * 128, y0);
           if (FP4) {
-            tma_load_2d_pair(st + 32768, &tmSx, bar, 0, 2 * ((2 * tx + (int)rank) * nst + i));
-            tma_load_2d_pair(st + 32768 + 1024, &tmSy, bar, 0, 4 * (ty * nst + i));
+            mbar_arrive_expect_tx(&sfull[s], 6u * 512u);
+            uint8_t* sc = base + s * kStageBytes + 32768;
+            tma_load_2d(sc, &tmSx, &sfull[s], 0, 2 * ((2 * tx + (int)rank) * nst + i));
+            tma_load_2d(sc + 1024, &tmSy, &sfull[s], 0, 4 * (ty * nst + i));
           } else {
             tma_load_2d_pair(st + 32768, &tmSx, bar, 0, (2 * tx + (int)rank) * nst + i);
             tma_load_2d_pair(st + 32768 + 512, &tmSy, bar, 0, 2 * (ty * nst + i));
@@ -358,8 +396,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (FP4)
               mx4_stage_e(d, umma_desc(xa, 16, 1024, kLayoutSW128),
                           umma_desc(xa + 16384, 16, 1024, kLayoutSW128), mx4_idesc(kTileX, TN, 0),
-                          mx4_idesc(kTileX, TN, 2), tmem + kScaleCol + 24u * (uint32_t)q,
-                          umma_desc(xa + 32768, 128, 128, 0), j > 0, &empty[s]);
+                          mx4_idesc(kTileX, TN, 2), tmem + kScaleCol + 24u * (uint32_t)s, j > 0,
+                          &empty[s]);
             else
               mx_stage_e(d, umma_desc(xa, 16, 1024, kLayoutSW128),
                          umma_desc(xa + 16384, 16, 1024, kLayoutSW128), mx_idesc(TN),
@@ -372,11 +410,37 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
+  } else if (warp < kEpi) {
+    // FP4: a stage's scales from shared memory into lanes 32 (w % 4).. of their columns.
+    // The stage's loads were issued behind its release, so that the columns are free too.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    const uint32_t t_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + kScaleCol;
+    int s = 0;
+    uint32_t ph = 0;
+    int left = pair < tiles ? (tiles - pair + pairs - 1) / pairs * nst : 0;
+    for (; left > 0; --left) {
+      int got = 0;
+      if (lane == 0)
+        got = mbar_wait_bounded(&sfull[s], ph, abort_flag, p.err, DEV_TIMEOUT_LOADED, p.timeout_ns);
+      if (!__shfl_sync(0xffffffffu, got, 0)) break;
+      tc_fence_after();
+      const uint32_t at = smem_u32(base + s * kStageBytes) + 32768 + 16 * lane;
+      float4 v[6];
+#pragma unroll
+      for (int k = 0; k < 6; ++k) v[k] = lds128(at + 512 * k);
+      tmem_st_quads(t_lane + 24u * (uint32_t)s, v);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_pair(map_rank(smem_u32(&full[s]), 0));
+      if (++s == S) { s = 0; ph ^= 1; }
+    }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    if (FP4) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     const int row = 32 * (warp & 3) + lane;
-    const int half = (warp - 4) >> 2;
-    const int et = threadIdx.x - 128 - 128 * half;  // 0..127 within the half
+    const int half = (warp - kEpi) >> 2;
+    const int et = threadIdx.x - 32 * kEpi - 128 * half;  // 0..127 within the half
     const uint32_t t_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)(kHalf * half);
     const uint32_t tempty0[2] = {map_rank(smem_u32(&tempty[0]), 0), map_rank(smem_u32(&tempty[1]), 0)};
     uint8_t* stg0 = staging + half * kBufs * kChunk;
@@ -547,7 +611,7 @@ int launch(rtb_ctx* ctx, const uint8_t* X, int64_t ldx, const uint8_t* Y, int64_
   const int64_t pairs = ctx->sm_count / 2 < tiles ? ctx->sm_count / 2 : tiles;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * pairs));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads(FP4));
   cfg.dynamicSmemBytes = kSmemBytes;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
@@ -579,9 +643,8 @@ int launch_mx(rtb_ctx* ctx, const uint8_t* X, int64_t ldx, const uint8_t* Y, int
     const int64_t pairs = ctx->sm_count / 2;
     return (double)((tiles + pairs - 1) / pairs) * (0.37 * ((p.depth + 127) / 128) + tile_us);
   };
+  if (fp4) return launch<256, true>(ctx, X, ldx, Y, ldy, p, s);
   const bool narrow = cost(224, 4.0) < 0.95 * cost(256, 6.0);
-  if (fp4)
-    return narrow ? launch<224, true>(ctx, X, ldx, Y, ldy, p, s) : launch<256, true>(ctx, X, ldx, Y, ldy, p, s);
   return narrow ? launch<224, false>(ctx, X, ldx, Y, ldy, p, s) : launch<256, false>(ctx, X, ldx, Y, ldy, p, s);
 }
 
