@@ -1,7 +1,10 @@
 // Writing and restoring 4-bit block-scaled tensors (rtb_fp4.cuh).
 //   save:    s = 2^ceil(log2(max|x| / 6)) over the block, q = e2m1(x / s)
 //   restore: x' = q * s
-// Both stream their operands once (4.53 bytes a value): HBM-bound.
+// Both stream their operands once (4.53 bytes a value): HBM-bound.  8192 x 4096 saved in
+// 25.9 us (5.9 TB/s, 90% of a copy), as its transpose in 30.4, restored in 28.4; rows off
+// the 16-byte boundaries, 8192 x 4100, 41 and 30 us (a block a warp and byte stores: 126
+// and 84).
 #include "rtb_fp4.cuh"
 #include "rtb_internal.h"
 #include "rtb_ptx.cuh"
@@ -21,10 +24,24 @@ int grid_for(rtb_ctx* ctx, int64_t blocks, int per_sm) {
 
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
+// 32 bytes at once (a lane's eight columns), past L1: a value is used once.
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+  asm volatile("ld.global.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "l"(p)
+               : "memory");
+}
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]),
+               "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+
 // Aligned rows: eight columns a lane, 256 columns a warp and kChunks such chunks at a
 // time, whose loads are all in flight before the first maximum; four lanes share a
-// block.
-constexpr int kChunks = 2;
+// block.  WIDE: rows on 32-byte boundaries.
+constexpr int kChunks = 4;
+template <bool WIDE>
 __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const float* __restrict__ x, int64_t ldx,
                                                                 int64_t total, int cols, int chunks,
                                                                 uint8_t* q, int64_t ldq, uint8_t* scale,
@@ -35,22 +52,34 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const float* __r
   const int64_t step = (int64_t)gridDim.x * (kThreads / 32) * kChunks;
   for (int64_t w = ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kChunks; w < total;
        w += step) {
+    int64_t r = w / chunks;
+    int c = (int)(w - r * chunks) * 256 + 8 * lane;
     int64_t row[kChunks];
     int col[kChunks];
     float v[kChunks][8];
 #pragma unroll
     for (int n = 0; n < kChunks; ++n) {
-      row[n] = (w + n) / chunks;
-      col[n] = (int)((w + n) - row[n] * chunks) * 256 + 8 * lane;
-      if (w + n >= total) col[n] = cols;  // (past the last row)
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+      row[n] = r;
+      col[n] = w + n < total ? c : cols;  // (past the last row)
       if (col[n] < cols) {  // cols % 8 == 0
-        const float4* p = reinterpret_cast<const float4*>(x + row[n] * ldx + col[n]);
-        a = __ldcs(p);
-        b = __ldcs(p + 1);
+        const float* p = x + r * ldx + c;
+        if (WIDE) {
+          load8(p, v[n]);
+        } else {
+          const float4 a = __ldcs(reinterpret_cast<const float4*>(p));
+          const float4 b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+          v[n][0] = a.x; v[n][1] = a.y; v[n][2] = a.z; v[n][3] = a.w;
+          v[n][4] = b.x; v[n][5] = b.y; v[n][6] = b.z; v[n][7] = b.w;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[n][j] = 0.0f;
       }
-      v[n][0] = a.x; v[n][1] = a.y; v[n][2] = a.z; v[n][3] = a.w;
-      v[n][4] = b.x; v[n][5] = b.y; v[n][6] = b.z; v[n][7] = b.w;
+      c += 256;
+      if (c >= chunks * 256) {
+        c -= chunks * 256;
+        ++r;
+      }
     }
 #pragma unroll
     for (int n = 0; n < kChunks; ++n) {
@@ -69,44 +98,91 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const float* __r
   }
 }
 
-// Any rows: a warp a block, a column a lane, kBlocks blocks at a time.
-constexpr int kBlocks = 8;
+// A chunk's codes, four bytes a lane, to a row of any alignment: `n` bytes from q on.
+// The lanes' bytes are shifted to the words of memory; those at the ends go byte by byte.
+__device__ __forceinline__ void store_codes(uint8_t* q, uint32_t code, int n, int lane) {
+  const int off = (int)(reinterpret_cast<uintptr_t>(q) & 3u);
+  const uint32_t prev = __shfl_up_sync(0xffffffffu, code, 1);
+  const uint32_t word = off ? __funnelshift_l(prev, code, 8 * off) : code;
+  const int at = 4 * lane - off;  // the word's first byte
+  if (at >= 0 && at + 4 <= n) {
+    *reinterpret_cast<uint32_t*>(q + at) = word;
+  } else {
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      if (at + b >= 0 && at + b < n) q[at + b] = (uint8_t)(word >> (8 * b));
+  }
+  if (lane == 31) {
+    for (int b = 0; b < off; ++b)
+      if (128 - off + b < n) q[128 - off + b] = (uint8_t)(code >> (8 * (4 - off + b)));
+  }
+}
+// ... and from it: n bytes, 0 behind them.  (No word is read that holds none of them.)
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* q, int n, int lane) {
+  const int off = (int)(reinterpret_cast<uintptr_t>(q) & 3u);
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(q - off);
+  const int left = n - 4 * lane;  // bytes from this lane's first one on
+  if (left <= 0) return 0u;
+  const uint32_t lo = __ldg(w + lane);
+  const uint32_t hi = off + (left < 4 ? left : 4) > 4 ? __ldg(w + lane + 1) : 0u;
+  const uint32_t v = __funnelshift_r(lo, hi, 8 * off);
+  return left < 4 ? v & ((1u << (8 * left)) - 1u) : v;
+}
+
+// Any rows: chunks of 256 columns a warp, loaded a column a lane and turned through
+// shared memory, so that a lane has eight columns side by side as above.
+constexpr int kAny = 2;  // chunks at a time (4: 8192 x 4100 38 and 28 us, 4096 x 1001 7.8 and 6.4 for 7.8 and 5.5)
 __global__ void __launch_bounds__(kThreads) fp4_quantize_any_kernel(const float* __restrict__ x,
                                                                     int64_t ldx, int64_t total, int cols,
-                                                                    int cblocks, uint8_t* q, int64_t ldq,
+                                                                    int chunks, uint8_t* q, int64_t ldq,
                                                                     uint8_t* scale, int64_t lds) {
+  __shared__ __align__(16) float turn[kThreads / 32][256];
   griddep_wait();
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31;
-  const int64_t step = (int64_t)gridDim.x * (kThreads / 32) * kBlocks;
-  for (int64_t w = ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kBlocks; w < total;
-       w += step) {
-    int64_t r = w / cblocks;
-    int cb = (int)(w - r * cblocks);
-    int64_t row[kBlocks];
-    int block[kBlocks];
-    float v[kBlocks];
+  float* mine = turn[threadIdx.x >> 5];
+  const int64_t step = (int64_t)gridDim.x * (kThreads / 32) * kAny;
+  for (int64_t w = ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kAny; w < total; w += step) {
+    int64_t r = w / chunks;
+    int c = (int)(w - r * chunks) * 256;
+    int64_t row[kAny];
+    int col[kAny];
+    float v[kAny][8];
 #pragma unroll
-    for (int n = 0; n < kBlocks; ++n) {
+    for (int n = 0; n < kAny; ++n) {
       row[n] = r;
-      block[n] = cb;
-      const int left = cols - cb * kFp4Block;  // columns from the block's first one on
-      v[n] = w + n < total && lane < left ? __ldcs(x + r * ldx + cb * kFp4Block + lane) : 0.0f;
-      if (++cb == cblocks) {
-        cb = 0;
+      col[n] = c;
+      const float* p = x + r * ldx + c + lane;
+      const int left = w + n < total ? cols - c - lane : 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[n][j] = 32 * j < left ? __ldcs(p + 32 * j) : 0.0f;
+      c += 256;
+      if (c >= chunks * 256) {
+        c = 0;
         ++r;
       }
     }
 #pragma unroll
-    for (int n = 0; n < kBlocks; ++n) {
+    for (int n = 0; n < kAny; ++n) {
       if (w + n >= total) break;
-      const uint32_t sb = fp4_scale_byte(__reduce_max_sync(0xffffffffu, magnitude(v[n])));
-      const float next = __shfl_down_sync(0xffffffffu, v[n], 1);
-      const float two[8] = {v[n], next};
-      const uint32_t byte = sb == 255 ? 0u : e2m1x8(two, fp4_inverse(sb)) & 0xFFu;
-      if ((lane & 1) == 0 && lane < cols - block[n] * kFp4Block)
-        q[row[n] * ldq + block[n] * (kFp4Block / 2) + lane / 2] = (uint8_t)byte;
-      if (lane == 0) scale[row[n] * lds + block[n]] = (uint8_t)sb;
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mine[32 * j + lane] = v[n][j];
+      __syncwarp();
+      float e[8];
+      *reinterpret_cast<float4*>(e) = *reinterpret_cast<const float4*>(mine + 8 * lane);
+      *reinterpret_cast<float4*>(e + 4) = *reinterpret_cast<const float4*>(mine + 8 * lane + 4);
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, magnitude(e[j]));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const uint32_t sb = fp4_scale_byte(top);
+      const uint32_t eight = e2m1x8(e, fp4_inverse(sb));
+      const int left = cols - col[n];
+      store_codes(q + row[n] * ldq + col[n] / 2, sb == 255 ? 0u : eight, left < 256 ? (left + 1) / 2 : 128, lane);
+      if ((lane & 3) == 0 && 8 * lane < left)
+        scale[row[n] * lds + col[n] / kFp4Block + lane / 4] = (uint8_t)sb;
     }
   }
 }
@@ -114,9 +190,11 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_any_kernel(const float*
 // The transpose of a row-major matrix [cols, rows] (row stride ldx): a CTA takes 256
 // columns of 32 rows, warp w the w-th block of 32 columns, lane l the l-th row, so that
 // loads run along the stored rows and a block's maximum is one thread's.  The codes
-// pass through shared memory and leave along the result's rows, 128 bytes each.
+// pass through shared memory and leave along the result's rows, 128 bytes each.  Five
+// CTAs on an SM: 8192 x 4096 in 30.4 us; four 32.3, three 37.8, six, whose registers do
+// not hold the 32 values, 37.
 template <typename Word>  // how the result's rows are aligned
-__global__ void __launch_bounds__(kThreads) fp4_quantize_columns_kernel(const float* __restrict__ x,
+__global__ void __launch_bounds__(kThreads, 5) fp4_quantize_columns_kernel(const float* __restrict__ x,
                                                                         int64_t ldx, int64_t rows, int64_t cols,
                                                                         int64_t row_tiles, int64_t tiles,
                                                                         uint8_t* q, int64_t ldq, uint8_t* scale,
@@ -168,80 +246,101 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_columns_kernel(const fl
   }
 }
 
-// Aligned rows: eight columns a thread, four such groups at a time (their loads in
-// flight together).
+// Aligned rows, the same way: kChunks chunks of 256 columns a warp.
+template <bool WIDE>
 __global__ void __launch_bounds__(kThreads) fp4_dequantize_kernel(const uint8_t* __restrict__ q, int64_t ldq,
-                                                                  int64_t rows, int cols,
+                                                                  int64_t total, int cols, int chunks,
                                                                   const uint8_t* __restrict__ scale, int64_t lds,
                                                                   float* y, int64_t ldy) {
   griddep_wait();
   griddep_launch_dependents();
-  const int groups = cols / 8;
-  const int64_t total = rows * groups, step = (int64_t)gridDim.x * kThreads;
-  for (int64_t i0 = (int64_t)blockIdx.x * kThreads + threadIdx.x; i0 < total; i0 += 4 * step) {
-    uint32_t eight[4], sb[4];
-    int64_t at[4];
+  const int lane = threadIdx.x & 31;
+  const int64_t step = (int64_t)gridDim.x * (kThreads / 32) * kChunks;
+  for (int64_t w = ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kChunks; w < total;
+       w += step) {
+    int64_t r = w / chunks;
+    int c = (int)(w - r * chunks) * 256 + 8 * lane;
+    float* out[kChunks];
+    uint32_t eight[kChunks], sb[kChunks];
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const int64_t i = i0 + n * step;
+    for (int n = 0; n < kChunks; ++n) {
+      out[n] = nullptr;
       eight[n] = sb[n] = 0;
-      at[n] = -1;
-      if (i < total) {
-        const int64_t r = i / groups;
-        const int c = (int)(i - r * groups) * 8;
-        at[n] = r * ldy + c;
+      if (w + n < total && c < cols) {  // cols % 8 == 0
+        out[n] = y + r * ldy + c;
         sb[n] = __ldg(scale + r * lds + c / kFp4Block);
         eight[n] = __ldcs(reinterpret_cast<const uint32_t*>(q + r * ldq + c / 2));
       }
-    }
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      if (at[n] < 0) break;
-      const float s = e8m0_to_float(sb[n]);
-      float v[8];
-      e2m1x8_to_float(eight[n], v);
-      float4* o = reinterpret_cast<float4*>(y + at[n]);
-      __stcs(o, make_float4(v[0] * s, v[1] * s, v[2] * s, v[3] * s));
-      __stcs(o + 1, make_float4(v[4] * s, v[5] * s, v[6] * s, v[7] * s));
-    }
-  }
-}
-
-// Any rows: a warp a block, a column a lane, kBlocks blocks at a time.
-__global__ void __launch_bounds__(kThreads) fp4_dequantize_any_kernel(const uint8_t* __restrict__ q, int64_t ldq,
-                                                                      int64_t total, int cols, int cblocks,
-                                                                      const uint8_t* __restrict__ scale,
-                                                                      int64_t lds, float* y, int64_t ldy) {
-  griddep_wait();
-  griddep_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int64_t step = (int64_t)gridDim.x * (kThreads / 32) * kBlocks;
-  for (int64_t w = ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kBlocks; w < total;
-       w += step) {
-    int64_t r = w / cblocks;
-    int cb = (int)(w - r * cblocks);
-    uint32_t code[kBlocks], sb[kBlocks];
-    float* out[kBlocks];
-#pragma unroll
-    for (int n = 0; n < kBlocks; ++n) {
-      out[n] = nullptr;
-      code[n] = sb[n] = 0;
-      if (w + n < total && lane < cols - cb * kFp4Block) {
-        const int64_t c = (int64_t)cb * kFp4Block + lane;
-        out[n] = y + r * ldy + c;
-        sb[n] = __ldg(scale + r * lds + cb);
-        code[n] = __ldcs(q + r * ldq + c / 2);
-      }
-      if (++cb == cblocks) {
-        cb = 0;
+      c += 256;
+      if (c >= chunks * 256) {
+        c -= chunks * 256;
         ++r;
       }
     }
 #pragma unroll
-    for (int n = 0; n < kBlocks; ++n) {
+    for (int n = 0; n < kChunks; ++n) {
+      if (!out[n]) continue;
+      const float s = e8m0_to_float(sb[n]);
       float v[8];
-      e2m1x8_to_float(code[n] >> (lane & 1 ? 4 : 0), v);
-      if (out[n]) __stcs(out[n], v[0] * e8m0_to_float(sb[n]));
+      e2m1x8_to_float(eight[n], v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= s;
+      if (WIDE) {
+        store8(out[n], v);
+      } else {
+        float4* o = reinterpret_cast<float4*>(out[n]);
+        __stcs(o, make_float4(v[0], v[1], v[2], v[3]));
+        __stcs(o + 1, make_float4(v[4], v[5], v[6], v[7]));
+      }
+    }
+  }
+}
+
+// Any rows: chunks of 256 columns a warp, turned through shared memory.
+__global__ void __launch_bounds__(kThreads) fp4_dequantize_any_kernel(const uint8_t* __restrict__ q, int64_t ldq,
+                                                                      int64_t total, int cols, int chunks,
+                                                                      const uint8_t* __restrict__ scale,
+                                                                      int64_t lds, float* y, int64_t ldy) {
+  __shared__ __align__(16) float turn[kThreads / 32][256];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  float* mine = turn[threadIdx.x >> 5];
+  const int64_t step = (int64_t)gridDim.x * (kThreads / 32) * kAny;
+  for (int64_t w = ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kAny; w < total; w += step) {
+    int64_t r = w / chunks;
+    int c = (int)(w - r * chunks) * 256;
+    int64_t row[kAny];
+    int col[kAny];
+    uint32_t eight[kAny], sb[kAny];
+#pragma unroll
+    for (int n = 0; n < kAny; ++n) {
+      row[n] = r;
+      col[n] = c;
+      const int left = w + n < total ? cols - c : 0;
+      eight[n] = load_codes(q + r * ldq + c / 2, left < 256 ? (left + 1) / 2 : 128, lane);
+      sb[n] = 8 * lane < left ? __ldg(scale + r * lds + c / kFp4Block + lane / 4) : 0u;
+      c += 256;
+      if (c >= chunks * 256) {
+        c = 0;
+        ++r;
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < kAny; ++n) {
+      if (w + n >= total) break;
+      const float s = e8m0_to_float(sb[n]);
+      float v[8];
+      e2m1x8_to_float(eight[n], v);
+      __syncwarp();
+      *reinterpret_cast<float4*>(mine + 8 * lane) = make_float4(v[0] * s, v[1] * s, v[2] * s, v[3] * s);
+      *reinterpret_cast<float4*>(mine + 8 * lane + 4) = make_float4(v[4] * s, v[5] * s, v[6] * s, v[7] * s);
+      __syncwarp();
+      float* out = y + row[n] * ldy + col[n] + lane;
+      const int left = cols - col[n] - lane;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (32 * j < left) __stcs(out + 32 * j, mine[32 * j + lane]);
     }
   }
 }
@@ -272,29 +371,31 @@ int launch_fp4_quantize(rtb_ctx* ctx, const float* x, int64_t ldx, int trans, in
     return run(what, fp4_quantize_columns_kernel<uint8_t>, grid, s, x, ldx, rows, cols, row_tiles, tiles,
                q, ldq, scale, lds);
   }
+  const int chunks = (int)((cols + 255) / 256);
+  const int64_t total = rows * chunks;
   if (cols % 8 == 0 && ldx % 4 == 0 && aligned(x, 16) && ldq % 4 == 0 && aligned(q, 4)) {
-    const int chunks = (int)((cols + 255) / 256);
-    const int64_t total = rows * chunks;
-    return run(what, fp4_quantize_kernel, grid_for(ctx, (total + 8 * kChunks - 1) / (8 * kChunks), 8), s, x,
-               ldx, total, (int)cols, chunks, q, ldq, scale, lds);
+    const bool wide = aligned(x, 32) && ldx % 8 == 0;
+    return run(what, wide ? fp4_quantize_kernel<true> : fp4_quantize_kernel<false>,
+               grid_for(ctx, (total + 8 * kChunks - 1) / (8 * kChunks), 8), s, x, ldx, total, (int)cols, chunks,
+               q, ldq, scale, lds);
   }
-  const int cblocks = (int)((cols + kFp4Block - 1) / kFp4Block);
-  const int64_t total = rows * cblocks;
-  return run(what, fp4_quantize_any_kernel, grid_for(ctx, (total + 8 * kBlocks - 1) / (8 * kBlocks), 8), s,
-             x, ldx, total, (int)cols, cblocks, q, ldq, scale, lds);
+  return run(what, fp4_quantize_any_kernel, grid_for(ctx, (total + 8 * kAny - 1) / (8 * kAny), 8), s, x, ldx,
+             total, (int)cols, chunks, q, ldq, scale, lds);
 }
 
 int launch_fp4_dequantize(rtb_ctx* ctx, const uint8_t* q, int64_t ldq, int64_t rows, int64_t cols,
                           const uint8_t* scale, int64_t lds, float* y, int64_t ldy, cudaStream_t s) {
-  if (cols % 8 == 0 && ldy % 4 == 0 && aligned(y, 16) && ldq % 4 == 0 && aligned(q, 4))
-    return run("fp4_dequantize launch", fp4_dequantize_kernel,
-               grid_for(ctx, (rows * (cols / 8) + kThreads - 1) / kThreads, 8), s, q, ldq, rows, (int)cols,
+  const int chunks = (int)((cols + 255) / 256);
+  const int64_t total = rows * chunks;
+  if (cols % 8 == 0 && ldy % 4 == 0 && aligned(y, 16) && ldq % 4 == 0 && aligned(q, 4)) {
+    const bool wide = aligned(y, 32) && ldy % 8 == 0;
+    return run("fp4_dequantize launch", wide ? fp4_dequantize_kernel<true> : fp4_dequantize_kernel<false>,
+               grid_for(ctx, (total + 8 * kChunks - 1) / (8 * kChunks), 8), s, q, ldq, total, (int)cols, chunks,
                scale, lds, y, ldy);
-  const int cblocks = (int)((cols + kFp4Block - 1) / kFp4Block);
-  const int64_t total = rows * cblocks;
+  }
   return run("fp4_dequantize launch", fp4_dequantize_any_kernel,
-             grid_for(ctx, (total + 8 * kBlocks - 1) / (8 * kBlocks), 8), s, q, ldq, total, (int)cols,
-             cblocks, scale, lds, y, ldy);
+             grid_for(ctx, (total + 8 * kAny - 1) / (8 * kAny), 8), s, q, ldq, total, (int)cols, chunks, scale,
+             lds, y, ldy);
 }
 
 }  // namespace rtb
