@@ -1425,6 +1425,10 @@ int rtb_fp4_matmul(rtb_ctx* ctx, int64_t M, int64_t N, int64_t K, const uint8_t*
   Fp4Desc d;
   d.M = M; d.N = N; d.K = K; d.sa = scale_a; d.ldsa = ldsa; d.sb = scale_b; d.ldsb = ldsb;
   d.bias = bias; d.act = act; d.C = C; d.ldc = ldc;
+  if (M <= kFp4RowsMax) {
+    d.A = A; d.lda = lda; d.B = B; d.ldb = ldb;
+    return fp4_rows_run(ctx, d, s);
+  }
   PackDesc pa, pb;
   size_t need = 0;
   void* ws = nullptr;

@@ -76,8 +76,9 @@ struct Cfg {
   // stages between promotions
   static constexpr int kPerUnit = MODE == 0 ? 1 : (MODE == 1 ? 2 : (kSf < 8 ? kSf : 8));
   static constexpr int kGrain = MODE == 1 ? 2 : 1;     // stages that parts are cut at
-  // MODE 2, 3: two buffers of 4 + 4 or 8 + 8 scale columns behind the accumulators
-  static constexpr int kTmemNeed = 2 * BN + (MODE == 2 ? 16 : MODE == 3 ? 32 : 0);
+  // behind the accumulators: two stages of 4 + 4 scale columns (MODE 2), two buffers of
+  // kSf stages of 8 + 8 (MODE 3)
+  static constexpr int kTmemNeed = 2 * BN + (MODE == 2 ? 16 : MODE == 3 ? 2 * kSf * 16 : 0);
   static constexpr int kTmemCols =
       kTmemNeed <= 32 ? 32 : kTmemNeed <= 64 ? 64 : kTmemNeed <= 128 ? 128 : kTmemNeed <= 256 ? 256 : 512;
   static_assert(kStages >= 2, "two stages");
@@ -130,32 +131,36 @@ __device__ __forceinline__ void mx_stage1_e(uint32_t d, uint64_t a, uint64_t b, 
       : "memory");
 }
 
-// MODE 3: the stage's scale groups (two of each operand, 128 columns each), and four
-// MMAs of 64 contraction elements with the scales in bytes 0, 1 and 2, 3 of a group's
-// words.
+// MODE 3: a stage's four MMAs of 64 contraction elements, with the scales in bytes 0, 1
+// and 2, 3 of their words (X's of the stage's two halves at columns sa and sa + 4, Y's at
+// sa + 8 and sa + 12), and its release.
 __device__ __forceinline__ void mx4_stage1_e(uint32_t d, uint64_t a, uint64_t b, uint32_t id0,
-                                             uint32_t id2, uint32_t sa, uint64_t cx, uint64_t cy,
-                                             uint32_t acc, uint64_t* empty) {
+                                             uint32_t id2, uint32_t sa, uint32_t acc, uint64_t* empty) {
   asm volatile(
       "{\n\t.reg .pred p, t, e;\n\t.reg .b32 r, s1, s2, s3;\n\t"
-      ".reg .b64 a1, a2, a3, b1, b2, b3, x1, y1;\n\t"
-      "setp.ne.b32 p, %8, 0;\n\t"
+      ".reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
       "setp.eq.b32 t, 0, 0;\n\t"
       "add.u32 s1, %5, 4;\n\tadd.u32 s2, %5, 8;\n\tadd.u32 s3, %5, 12;\n\t"
-      "add.s64 x1, %6, 32;\n\tadd.s64 y1, %7, 32;\n\t"
       "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
       "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
       "elect.sync r|e, 0xffffffff;\n\t"
-      "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%5], %6;\n\t"
-      "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [s1], x1;\n\t"
-      "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [s2], %7;\n\t"
-      "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [s3], y1;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [s2], p;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], a1, b1, %4, [%5], [s2], t;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], a2, b2, %3, [s1], [s3], t;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], a3, b3, %4, [s1], [s3], t;\n\t"
-      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%9];\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(id0), "r"(id2), "r"(sa), "l"(cx), "l"(cy), "r"(acc), "r"(smem_u32(empty))
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%7];\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(id0), "r"(id2), "r"(sa), "r"(acc), "r"(smem_u32(empty))
+      : "memory");
+}
+// 32 lanes x 16 columns of TMEM: lane l's four quads of words.
+__device__ __forceinline__ void tmem_st_quads(uint32_t taddr, const float4 (&v)[4]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16};" ::"r"(taddr),
+      "f"(v[0].x), "f"(v[0].y), "f"(v[0].z), "f"(v[0].w), "f"(v[1].x), "f"(v[1].y), "f"(v[1].z),
+      "f"(v[1].w), "f"(v[2].x), "f"(v[2].y), "f"(v[2].z), "f"(v[2].w), "f"(v[3].x), "f"(v[3].y),
+      "f"(v[3].z), "f"(v[3].w)
       : "memory");
 }
 
@@ -174,6 +179,19 @@ __device__ __forceinline__ void load_scale_bytes(const ScaleRef& s, int64_t r, i
 template <int N>
 __device__ __forceinline__ void load_scale_words(const ScaleRef& s, int64_t r, int64_t rows, int j,
                                                  int n, int bytes, int vec, uint32_t (&raw)[N]) {
+  // Whole pairs of words, without a branch, so that all loads are in flight.  (A row
+  // past the operand takes another's scales: its codes are 0, its outputs not stored.)
+  if (vec == 2 && n == N && 4 * (j + N) <= bytes) {
+    const uint2* p = reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(s.p) +
+                                                    (r < rows ? r : 0) * s.ld_row + (int64_t)4 * j);
+#pragma unroll
+    for (int k = 0; k < N; k += 2) {
+      const uint2 two = __ldg(p + k / 2);
+      raw[k] = two.x;
+      raw[k + 1] = two.y;
+    }
+    return;
+  }
 #pragma unroll
   for (int k = 0; k < N; ++k)
     raw[k] = r < rows && k < n ? fp4_scale_word(s, r, j + k, bytes, vec) : 0x7F7F7F7Fu;
@@ -227,6 +245,65 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
                : "r"(addr)
                : "memory");
   return v;
+}
+
+// The finished tile's rows out of shared memory: this CTA's share of them, the sum over
+// the P parts in rank order, bias, activation, the stores.  I quads of all parts at a
+// time: a load out of another CTA takes longer than the whole of the work on it.
+template <int P, int I, int BN>
+__device__ __forceinline__ void finish_rows(const BlockParams& p, uint32_t tb, int rank, int tx, int ty) {
+  const int trows = p.swap ? BN : kX, tcols = p.swap ? kX : BN;
+  const int pitch = tcols + 4, quads = tcols / 4, share = trows / P;
+  const int64_t m0 = p.swap ? (int64_t)ty * BN : (int64_t)tx * kX;
+  const int64_t n0 = p.swap ? (int64_t)tx * kX : (int64_t)ty * BN;
+  const int64_t M = p.swap ? p.ycols : p.xrows, N = p.swap ? p.xrows : p.ycols;
+  const int total = share * quads;
+  for (int e0 = threadIdx.x; e0 < total; e0 += I * kThreads) {
+    float4 w[I][P];
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      const int e = e0 + i * kThreads;
+      if (e < total) {
+        const uint32_t at = tb + (uint32_t)((rank * share + e / quads) * pitch + e % quads * 4) * 4;
+#pragma unroll
+        for (int q = 0; q < P; ++q) w[i][q] = P == 1 ? lds128(at) : ld_cluster(map_rank(at, (uint32_t)q));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      const int e = e0 + i * kThreads;
+      if (e >= total) break;
+      const int64_t m = m0 + rank * share + e / quads, n = n0 + e % quads * 4;
+      if (m >= M || n >= N) continue;
+      float4 x = w[i][0];
+#pragma unroll
+      for (int q = 1; q < P; ++q) {
+        x.x += w[i][q].x; x.y += w[i][q].y; x.z += w[i][q].z; x.w += w[i][q].w;
+      }
+      float* o = p.out + m * p.ldo + n;
+      if (p.vec_ok && n + 4 <= N) {
+        if (p.bias) {
+          const float4 b4 = __ldg(reinterpret_cast<const float4*>(p.bias + n));
+          x.x += b4.x; x.y += b4.y; x.z += b4.z; x.w += b4.w;
+        }
+        if (p.accumulate) {
+          const float4 q = *reinterpret_cast<const float4*>(o);
+          x.x += q.x; x.y += q.y; x.z += q.z; x.w += q.w;
+        }
+        *reinterpret_cast<float4*>(o) = activate4(x, p.act);
+      } else {
+        const float ve[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (n + j >= N) break;
+          float v = ve[j];
+          if (p.bias) v += __ldg(p.bias + n + j);
+          if (p.accumulate) v += o[j];
+          o[j] = activate(v, p.act);
+        }
+      }
+    }
+  }
 }
 
 // YVEC (MODE 0): a scale for every Y column (block_rows 1); otherwise the
@@ -298,6 +375,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<MODE, BN, YVEC>::kPerSm)
       // three producers take the stages in turn: one thread's wait and issue
       // takes longer than a stage's MMAs
       const uint32_t tx_bytes = kXBytes + (MODE == 1 ? p.pieces : 1) * C::kYPiece;
+#pragma unroll 1
       for (int i = i0 + (warp ? warp - 5 : 0); i < i1; i += 3) {
         const int s = (i - i0) % S;
         if (!mbar_wait_bounded(&empty[s], (((i - i0) / S) & 1) ^ 1, abort_flag, p.err,
@@ -328,23 +406,31 @@ __global__ void __launch_bounds__(kThreads, Cfg<MODE, BN, YVEC>::kPerSm)
       if (lane == 0) got = mbar_wait_bounded(bar, parity, abort_flag, p.err, code, p.timeout_ns);
       return __shfl_sync(0xffffffffu, got, 0) != 0;
     };
-    // (lane 0) the next stage's operands were found ready before this stage's
-    // MMAs: a wait costs 200 clocks even when its barrier is complete
-    int next_full = 0;
+    // Stages found ready ahead: a wait or a test costs 200 clocks even when its barrier
+    // is complete, so lane l tests the l-th stage from here and one test serves them all.
+    int ready = 0;
+#pragma unroll 1
     for (int u = 0, i = 0; u < units && ok; ++u) {
       const int b = u & 1;
       const uint32_t d = tmem + (uint32_t)(b * BN);
+#pragma unroll 1
       for (int j = 0; j < C::kPerUnit && i < nst; ++j, ++i) {
         const int s = i % S;
-        if (!__shfl_sync(0xffffffffu, next_full, 0) &&
-            !(ok = wait(&full[s], (i / S) & 1, DEV_TIMEOUT_FULL)))
-          break;
+        if (ready == 0) {
+          const int il = i + lane;
+          const int got = lane < S && il < nst ? mbar_test_wait(&full[il % S], (il / S) & 1) : 0;
+          ready = __ffs(~__ballot_sync(0xffffffffu, got)) - 1;
+          __syncwarp();
+          if (ready == 0 && !(ok = wait(&full[s], (i / S) & 1, DEV_TIMEOUT_FULL))) break;
+          if (ready > 0) --ready;
+        } else {
+          --ready;
+        }
         if (j == 0 && !(ok = wait(&tempty[b], ((u >> 1) & 1) ^ 1, DEV_TIMEOUT_TMEM_EMPTY))) break;
         const int c = i / C::kSf, k = i % C::kSf;  // MODE 2, 3: scale buffer c & 1, its stage k
         if (MODE >= 2 && k == 0 && !(ok = wait(&sfull[c & 1], (c >> 1) & 1, DEV_TIMEOUT_LOADED)))
           break;
         tc_fence_after();
-        if (lane == 0) next_full = mbar_test_wait(&full[(i + 1) % S], ((i + 1) / S) & 1);
         const uint32_t xa = smem_u32(base + s * C::kStageBytes), ya = xa + kXBytes;
         if (MODE == 0) {
 #pragma unroll
@@ -367,8 +453,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<MODE, BN, YVEC>::kPerSm)
           const uint32_t g = smem_u32(sf) + (uint32_t)(c & 1) * 2 * kOperand + (uint32_t)(C::kSfBytes * k);
           if (MODE == 3)
             mx4_stage1_e(d, umma_desc(xa, 16, 1024, kLayoutSW128), umma_desc(ya, 16, 1024, kLayoutSW128),
-                         mx4_idesc(kX, BN, 0), mx4_idesc(kX, BN, 2), tmem + 2 * BN + 16u * (uint32_t)(i & 1),
-                         umma_desc(g, 128, 128, 0), umma_desc(g + kOperand, 128, 128, 0), j > 0, &empty[s]);
+                         mx4_idesc(kX, BN, 0), mx4_idesc(kX, BN, 2),
+                         tmem + 2 * BN + 16u * (uint32_t)((c & 1) * C::kSf + k), j > 0, &empty[s]);
           else
             mx_stage1_e(d, umma_desc(xa, 16, 1024, kLayoutSW128), umma_desc(ya, 16, 1024, kLayoutSW128),
                         ((uint32_t)(BN >> 3) << 17) | (1u << 23) | ((uint32_t)(kX >> 4) << 24),
@@ -407,18 +493,41 @@ __global__ void __launch_bounds__(kThreads, Cfg<MODE, BN, YVEC>::kPerSm)
       if (MODE == 3) {
         load_scale_words(p.scx, (int64_t)tx * kX + et, p.xrows, 2 * (i0 + first), 2 * n, p.sc_bytes,
                          p.sc_vec, rx);
-        load_scale_words(p.scy, (int64_t)ty * BN + et, et < BN ? p.ycols : 0, 2 * (i0 + first), 2 * n,
-                         p.sc_bytes, p.sc_vec, ry);
+        load_scale_words(p.scy, (int64_t)ty * BN + et % BN, p.ycols, 2 * (i0 + first), 2 * n, p.sc_bytes,
+                         p.sc_vec, ry);
       } else {
         load_scale_bytes(p.scx, (int64_t)tx * kX + et, p.xrows, i0 + first, n, rx);
         load_scale_bytes(p.scy, (int64_t)ty * BN + et, et < BN ? p.ycols : 0, i0 + first, n, ry);
       }
       store_scale_words<MODE>(rx, g, et);
       store_scale_words<MODE>(ry, g + C::kSf * C::kSfBytes, et);
-      fence_proxy_async_smem();  // the tensor core's copies read them
+      if (MODE == 3) {
+        // From there into TMEM, every warp its lanes: the tensor core's own copies run
+        // between the MMAs and made a stage 0.43 us long (0.XX us so).  (A buffer of
+        // shared memory is written again two buffers later, behind the barrier of the
+        // one between, which every reader of this one has passed.)
+        named_bar_sync(1, 128);
+        tc_fence_after();
+        const uint32_t from = smem_u32(g) + 16 * lane;
+#pragma unroll
+        for (int k = 0; k < C::kSf; ++k) {
+          float4 v[4];
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            v[q] = lds128(from + C::kSfBytes * k + 512 * q);
+            v[2 + q] = lds128(from + C::kSfBytes * (C::kSf + k) + 512 * q);
+          }
+          tmem_st_quads(t_lane + 2 * BN + 16 * ((c & 1) * C::kSf + k), v);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+      } else {
+        fence_proxy_async_smem();  // the tensor core's copies read them
+      }
       mbar_arrive(&sfull[c & 1]);
     };
     if (MODE >= 2) scale_words(0);
+#pragma unroll 1
     for (int u = 0; u < units; ++u) {
       const int b = u & 1;
       // the next buffer, while this one's blocks are multiplied
@@ -495,71 +604,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<MODE, BN, YVEC>::kPerSm)
   // Each CTA of the cluster adds its share of the rows over all parts, in rank
   // order, and writes them.
   {
-    const int trows = p.swap ? BN : kX, tcols = p.swap ? kX : BN;
-    const int pitch = tcols + 4, quads = tcols / 4, share = trows / parts;
-    const int64_t m0 = p.swap ? (int64_t)ty * BN : (int64_t)tx * kX;
-    const int64_t n0 = p.swap ? (int64_t)tx * kX : (int64_t)ty * BN;
-    const int64_t M = p.swap ? p.ycols : p.xrows, N = p.swap ? p.xrows : p.ycols;
     const uint32_t tb = smem_u32(base);
-    // four quads at a time: a load out of another CTA takes longer than the
-    // whole of the work on it
-    const int total = share * quads;
-    for (int e0 = threadIdx.x; e0 < total; e0 += 4 * kThreads) {
-      float4 v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int e = e0 + i * kThreads;
-        if (e < total) {
-          const uint32_t at =
-              tb + (uint32_t)((rank * share + e / quads) * pitch + e % quads * 4) * 4;
-          v[i] = parts == 1 ? lds128(at) : ld_cluster(map_rank(at, 0));
-        }
-      }
-      for (int q = 1; q < parts; ++q) {
-        float4 w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int e = e0 + i * kThreads;
-          if (e < total)
-            w[i] = ld_cluster(map_rank(
-                tb + (uint32_t)((rank * share + e / quads) * pitch + e % quads * 4) * 4, (uint32_t)q));
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[i].x += w[i].x; v[i].y += w[i].y; v[i].z += w[i].z; v[i].w += w[i].w;
-        }
-      }
-#pragma unroll 1
-      for (int i = 0; i < 4; ++i) {
-        const int e = e0 + i * kThreads;
-        if (e >= total) break;
-        const int64_t m = m0 + rank * share + e / quads, n = n0 + e % quads * 4;
-        if (m >= M || n >= N) continue;
-        float4 x = i == 0 ? v[0] : i == 1 ? v[1] : i == 2 ? v[2] : v[3];
-        float* o = p.out + m * p.ldo + n;
-        if (p.vec_ok && n + 4 <= N) {
-          if (p.bias) {
-            const float4 b4 = __ldg(reinterpret_cast<const float4*>(p.bias + n));
-            x.x += b4.x; x.y += b4.y; x.z += b4.z; x.w += b4.w;
-          }
-          if (p.accumulate) {
-            const float4 q = *reinterpret_cast<const float4*>(o);
-            x.x += q.x; x.y += q.y; x.z += q.z; x.w += q.w;
-          }
-          *reinterpret_cast<float4*>(o) = activate4(x, p.act);
-        } else {
-          const float ve[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (n + j >= N) break;
-            float w = ve[j];
-            if (p.bias) w += __ldg(p.bias + n + j);
-            if (p.accumulate) w += o[j];
-            o[j] = activate(w, p.act);
-          }
-        }
-      }
-    }
+    if (parts == 1) finish_rows<1, 4, BN>(p, tb, rank, tx, ty);
+    else if (parts == 2) finish_rows<2, 4, BN>(p, tb, rank, tx, ty);
+    else if (parts == 4) finish_rows<4, 2, BN>(p, tb, rank, tx, ty);
+    else finish_rows<8, 1, BN>(p, tb, rank, tx, ty);
   }
 
   // ------------------------------------------------------------ teardown
@@ -738,8 +787,9 @@ int fp4_gemm_run(rtb_ctx* ctx, const Fp4Desc& d, cudaStream_t s) {
   p.scx = swap ? sb : sa;
   p.scy = swap ? sa : sb;
   p.sc_bytes = (int)((d.K + 31) / 32);
-  p.sc_vec = ((reinterpret_cast<uintptr_t>(d.sa) | reinterpret_cast<uintptr_t>(d.sb)) & 3u) == 0 &&
-             d.ldsa % 4 == 0 && d.ldsb % 4 == 0;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(d.sa) | reinterpret_cast<uintptr_t>(d.sb) |
+                       (uintptr_t)d.ldsa | (uintptr_t)d.ldsb;
+  p.sc_vec = at % 8 == 0 ? 2 : at % 4 == 0 ? 1 : 0;
   p.err = ctx->d_err;
   p.timeout_ns = ctx->timeout_ns;
   const int bn = swap ? (d.M <= 16 ? 16 : d.M <= 32 ? 32 : 64) : 128;

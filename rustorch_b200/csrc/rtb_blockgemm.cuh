@@ -26,7 +26,8 @@ struct BlockParams {
   int pieces;            // MODE 1
   int64_t piece_rows;    // MODE 1: contraction rows between Y's pieces
   ScaleRef scx, scy;
-  int sc_bytes, sc_vec;  // 4-bit operands: scales of a row, and whether their rows are 4-byte aligned
+  // 4-bit operands: scales of a row; whether their rows are 4-byte (1) or 8-byte (2) aligned
+  int sc_bytes, sc_vec;
   // MODE 0, CTA pairs: the scales as fp32, [block][row], zero past the operand
   // (launch_scale_tables)
   const float *tabx, *taby;
