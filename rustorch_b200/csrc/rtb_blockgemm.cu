@@ -58,14 +58,18 @@ struct Cfg {
   static constexpr int kStageBytes = kXBytes + kPieces * kYPiece;
   // Narrow tiles, two CTAs on an SM: one's loads pass behind the other's start and
   // end (a token row by 8192 x 8192: 19.9 us with one CTA of eight stages, 18.8).
-  static constexpr int kPerSm = MODE >= 2 && BN <= 32 ? 2 : 1;
-  // MODE 2, 3: stages of a scale buffer, of two; a stage's scales of one operand
-  static constexpr int kSf = (kPerSm == 2 ? 8 : 16) / (MODE == 3 ? 2 : 1);
+  // MODE 3: two (YVEC) only where tiles would wait for an SM; else the whole ring for one
+  // that shares its tile's contraction with others (64 x 28672 x 8192, 224 tiles, 32.0 us
+  // with two, 39.4 with one; 48 x 8192 x 8192, 64 tiles, 12.4 and 11.7).
+  static constexpr int kPerSm = (MODE == 2 && BN <= 32) || (MODE == 3 && YVEC) ? 2 : 1;
+  // MODE 2, 3: stages of a scale buffer, of two (MODE 3: in TMEM, one in shared memory);
+  // a stage's scales of one operand
+  static constexpr int kSf = MODE == 3 ? 4 : kPerSm == 2 ? 8 : 16;
   static constexpr int kSfBytes = MODE == 3 ? 1024 : 512;
   static constexpr int kBudget = kPerSm == 2 ? kSmemHalf : kSmemMax;
   static constexpr int kSy = YVEC ? BN : 1;            // column scales of a block
   static constexpr int kScaleBytes =
-      MODE == 0 ? kScaleUnits * (128 + kSy) * 4 : (MODE >= 2 ? 2 * kSf * 2 * kSfBytes : 0);
+      MODE == 0 ? kScaleUnits * (128 + kSy) * 4 : (MODE >= 2 ? (MODE == 2 ? 2 : 1) * kSf * 2 * kSfBytes : 0);
   static constexpr int kStagesRaw = (kBudget - kReserve - kScaleBytes) / kStageBytes;
   static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;
   static constexpr int kSmemBytes = kStages * kStageBytes + kScaleBytes + kReserve;
@@ -181,12 +185,12 @@ __device__ __forceinline__ void load_scale_words(const ScaleRef& s, int64_t r, i
                                                  int n, int bytes, int vec, uint32_t (&raw)[N]) {
   // Whole pairs of words, without a branch, so that all loads are in flight.  (A row
   // past the operand takes another's scales: its codes are 0, its outputs not stored.)
-  if (vec == 2 && n == N && 4 * (j + N) <= bytes) {
+  if (vec == 2 && 4 * (j + n) <= bytes) {
     const uint2* p = reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(s.p) +
                                                     (r < rows ? r : 0) * s.ld_row + (int64_t)4 * j);
 #pragma unroll
     for (int k = 0; k < N; k += 2) {
-      const uint2 two = __ldg(p + k / 2);
+      const uint2 two = k < n ? __ldg(p + k / 2) : make_uint2(0u, 0u);
       raw[k] = two.x;
       raw[k + 1] = two.y;
     }
@@ -247,24 +251,38 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
   return v;
 }
 
+// sigmoid and tanh of a quad.  (One copy of their code: inlined for every quad of a
+// thread they are most of the kernel's, and a short call waits for it to be fetched.)
+__device__ __noinline__ float4 curved4(float4 v, int act) { return activate4(v, act); }
+__device__ __forceinline__ float4 finish4(float4 v, int act) {
+  if (act == RTB_ACT_NONE) return v;
+  if (act == RTB_ACT_RELU)
+    return make_float4(fmaxf(v.x, 0.0f), fmaxf(v.y, 0.0f), fmaxf(v.z, 0.0f), fmaxf(v.w, 0.0f));
+  return curved4(v, act);
+}
+
 // The finished tile's rows out of shared memory: this CTA's share of them, the sum over
 // the P parts in rank order, bias, activation, the stores.  I quads of all parts at a
 // time: a load out of another CTA takes longer than the whole of the work on it.
+// Of a thread's quads, all in the same columns, the bias is `b4`.
 template <int P, int I, int BN>
-__device__ __forceinline__ void finish_rows(const BlockParams& p, uint32_t tb, int rank, int tx, int ty) {
+__device__ __forceinline__ void finish_rows(const BlockParams& p, uint32_t tb, int rank, int tx, int ty,
+                                            float4 b4) {
   const int trows = p.swap ? BN : kX, tcols = p.swap ? kX : BN;
-  const int pitch = tcols + 4, quads = tcols / 4, share = trows / P;
+  const int pitch = tcols + 4, share = trows / P;
+  const int shift = p.swap ? 5 : BN == 128 ? 5 : BN == 64 ? 4 : BN == 32 ? 3 : 2;  // quads of a row
+  const int mask = (1 << shift) - 1;
   const int64_t m0 = p.swap ? (int64_t)ty * BN : (int64_t)tx * kX;
   const int64_t n0 = p.swap ? (int64_t)tx * kX : (int64_t)ty * BN;
   const int64_t M = p.swap ? p.ycols : p.xrows, N = p.swap ? p.xrows : p.ycols;
-  const int total = share * quads;
+  const int total = share << shift;
   for (int e0 = threadIdx.x; e0 < total; e0 += I * kThreads) {
     float4 w[I][P];
 #pragma unroll
     for (int i = 0; i < I; ++i) {
       const int e = e0 + i * kThreads;
       if (e < total) {
-        const uint32_t at = tb + (uint32_t)((rank * share + e / quads) * pitch + e % quads * 4) * 4;
+        const uint32_t at = tb + (uint32_t)((rank * share + (e >> shift)) * pitch + (e & mask) * 4) * 4;
 #pragma unroll
         for (int q = 0; q < P; ++q) w[i][q] = P == 1 ? lds128(at) : ld_cluster(map_rank(at, (uint32_t)q));
       }
@@ -273,7 +291,7 @@ __device__ __forceinline__ void finish_rows(const BlockParams& p, uint32_t tb, i
     for (int i = 0; i < I; ++i) {
       const int e = e0 + i * kThreads;
       if (e >= total) break;
-      const int64_t m = m0 + rank * share + e / quads, n = n0 + e % quads * 4;
+      const int64_t m = m0 + rank * share + (e >> shift), n = n0 + (e & mask) * 4;
       if (m >= M || n >= N) continue;
       float4 x = w[i][0];
 #pragma unroll
@@ -281,33 +299,34 @@ __device__ __forceinline__ void finish_rows(const BlockParams& p, uint32_t tb, i
         x.x += w[i][q].x; x.y += w[i][q].y; x.z += w[i][q].z; x.w += w[i][q].w;
       }
       float* o = p.out + m * p.ldo + n;
+      if (p.bias) {
+        x.x += b4.x; x.y += b4.y; x.z += b4.z; x.w += b4.w;
+      }
       if (p.vec_ok && n + 4 <= N) {
-        if (p.bias) {
-          const float4 b4 = __ldg(reinterpret_cast<const float4*>(p.bias + n));
-          x.x += b4.x; x.y += b4.y; x.z += b4.z; x.w += b4.w;
-        }
         if (p.accumulate) {
           const float4 q = *reinterpret_cast<const float4*>(o);
           x.x += q.x; x.y += q.y; x.z += q.z; x.w += q.w;
         }
-        *reinterpret_cast<float4*>(o) = activate4(x, p.act);
+        *reinterpret_cast<float4*>(o) = finish4(x, p.act);
       } else {
-        const float ve[4] = {x.x, x.y, x.z, x.w};
+        const int left = N - n < 4 ? (int)(N - n) : 4;
+        float ve[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (n + j >= N) break;
-          float v = ve[j];
-          if (p.bias) v += __ldg(p.bias + n + j);
-          if (p.accumulate) v += o[j];
-          o[j] = activate(v, p.act);
+          if (j < left && p.accumulate) ve[j] += o[j];
         }
+        const float4 y = finish4(make_float4(ve[0], ve[1], ve[2], ve[3]), p.act);
+        o[0] = y.x;
+        if (left > 1) o[1] = y.y;
+        if (left > 2) o[2] = y.z;
+        if (left > 3) o[3] = y.w;
       }
     }
   }
 }
 
 // YVEC (MODE 0): a scale for every Y column (block_rows 1); otherwise the
-// tile's columns lie in one 128-row block and share one.
+// tile's columns lie in one 128-row block and share one.  MODE 3: two CTAs on an SM.
 template <int MODE, int BN, bool YVEC>
 __global__ void __launch_bounds__(kThreads, Cfg<MODE, BN, YVEC>::kPerSm)
     block_gemm_kernel(const __grid_constant__ CUtensorMap tmX,
@@ -328,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<MODE, BN, YVEC>::kPerSm)
   uint64_t* sempty = sfull + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sempty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  uint8_t* sf = reinterpret_cast<uint8_t*>(sx);  // MODE 2, 3: [2][X, Y][kSf][kSfBytes]
+  uint8_t* sf = reinterpret_cast<uint8_t*>(sx);  // MODE 2: [2][X, Y][kSf][kSfBytes]; 3: once
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -486,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<MODE, BN, YVEC>::kPerSm)
         ok = __shfl_sync(0xffffffffu, got, 0) != 0;
       }
       const int n = nst - first < C::kSf ? nst - first : C::kSf;
-      uint8_t* g = sf + (c & 1) * C::kSf * 2 * C::kSfBytes;
+      uint8_t* g = sf + (MODE == 2 ? (c & 1) * C::kSf * 2 * C::kSfBytes : 0);
       // (both operands' loads before the first store: one latency, not two)
       constexpr int kWords = C::kSf * C::kSfBytes / 512;
       uint32_t rx[kWords], ry[kWords];
@@ -499,18 +518,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<MODE, BN, YVEC>::kPerSm)
         load_scale_bytes(p.scx, (int64_t)tx * kX + et, p.xrows, i0 + first, n, rx);
         load_scale_bytes(p.scy, (int64_t)ty * BN + et, et < BN ? p.ycols : 0, i0 + first, n, ry);
       }
+      if (MODE == 3) named_bar_sync(1, 128);  // the buffer before is in TMEM
       store_scale_words<MODE>(rx, g, et);
       store_scale_words<MODE>(ry, g + C::kSf * C::kSfBytes, et);
       if (MODE == 3) {
         // From there into TMEM, every warp its lanes: the tensor core's own copies run
-        // between the MMAs and made a stage 0.43 us long (0.XX us so).  (A buffer of
-        // shared memory is written again two buffers later, behind the barrier of the
-        // one between, which every reader of this one has passed.)
+        // between the MMAs, 16 x 8192 x 8192 12.0 us so and 10.9 without.
         named_bar_sync(1, 128);
         tc_fence_after();
         const uint32_t from = smem_u32(g) + 16 * lane;
 #pragma unroll
         for (int k = 0; k < C::kSf; ++k) {
+          if (k >= n) break;
           float4 v[4];
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
@@ -595,6 +614,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<MODE, BN, YVEC>::kPerSm)
     }
   }
 
+  // (loaded here: its latency passes behind the barrier)
+  float4 bias = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (p.bias) {
+    const int tcols = p.swap ? kX : BN;
+    const int64_t n = (int64_t)(p.swap ? tx : ty) * tcols + (threadIdx.x * 4) % tcols;
+    const int64_t N = p.swap ? p.xrows : p.ycols;
+    if (n < N) bias.x = __ldg(p.bias + n);
+    if (n + 1 < N) bias.y = __ldg(p.bias + n + 1);
+    if (n + 2 < N) bias.z = __ldg(p.bias + n + 2);
+    if (n + 3 < N) bias.w = __ldg(p.bias + n + 3);
+  }
   __syncwarp();
   tc_fence_before();
   if (parts > 1) cluster_sync();
@@ -605,10 +635,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<MODE, BN, YVEC>::kPerSm)
   // order, and writes them.
   {
     const uint32_t tb = smem_u32(base);
-    if (parts == 1) finish_rows<1, 4, BN>(p, tb, rank, tx, ty);
-    else if (parts == 2) finish_rows<2, 4, BN>(p, tb, rank, tx, ty);
-    else if (parts == 4) finish_rows<4, 2, BN>(p, tb, rank, tx, ty);
-    else finish_rows<8, 1, BN>(p, tb, rank, tx, ty);
+    if (parts == 1) finish_rows<1, 4, BN>(p, tb, rank, tx, ty, bias);
+    else if (parts == 2) finish_rows<2, 4, BN>(p, tb, rank, tx, ty, bias);
+    else if (parts == 4) finish_rows<4, 2, BN>(p, tb, rank, tx, ty, bias);
+    else finish_rows<8, 1, BN>(p, tb, rank, tx, ty, bias);
   }
 
   // ------------------------------------------------------------ teardown
@@ -679,8 +709,7 @@ int launch(rtb_ctx* ctx, const CUtensorMap& tmX, const CUtensorMap& tmY, BlockPa
   const int64_t tiles = (int64_t)p.tiles_x * p.tiles_y;
   if (tiles > INT32_MAX / 8) return set_error(RTB_E_UNSUPPORTED, "block gemm: too many tiles");
   p.parts = pick_parts<MODE, BN, YVEC>(ctx, tiles, (p.stages_total + C::kGrain - 1) / C::kGrain);
-  p.vec_ok = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 && p.ldo % 4 == 0 &&
-             (!p.bias || (reinterpret_cast<uintptr_t>(p.bias) & 15u) == 0);
+  p.vec_ok = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 && p.ldo % 4 == 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * p.parts));
   cfg.blockDim = dim3(kThreads);
@@ -792,7 +821,8 @@ int fp4_gemm_run(rtb_ctx* ctx, const Fp4Desc& d, cudaStream_t s) {
   p.sc_vec = at % 8 == 0 ? 2 : at % 4 == 0 ? 1 : 0;
   p.err = ctx->d_err;
   p.timeout_ns = ctx->timeout_ns;
-  const int bn = swap ? (d.M <= 16 ? 16 : d.M <= 32 ? 32 : 64) : 128;
+  const int64_t tiles = ((p.xrows + 127) / 128) * ((p.ycols + 127) / 128);
+  const int bn = swap ? (d.M <= 16 ? 16 : d.M <= 32 ? 32 : 64) : tiles * 3 <= ctx->sm_count ? 64 : 128;
   const uint8_t* X = swap ? d.B : d.A;
   const uint8_t* Y = swap ? d.A : d.B;
   const int64_t ldx = swap ? d.ldb : d.lda, ldy = swap ? d.lda : d.ldb;
@@ -803,9 +833,10 @@ int fp4_gemm_run(rtb_ctx* ctx, const Fp4Desc& d, cudaStream_t s) {
   if ((st = make_tmap_2d_bytes(&tmY, Y, 1, (uint64_t)p.depth, (uint64_t)p.ycols, (uint64_t)ldy, 128,
                                (uint32_t)bn)))
     return st;
-  if (bn == 16) return launch<3, 16, false>(ctx, tmX, tmY, p, s);
-  if (bn == 32) return launch<3, 32, false>(ctx, tmX, tmY, p, s);
-  if (bn == 64) return launch<3, 64, false>(ctx, tmX, tmY, p, s);
+  const bool two = (p.xrows + 127) / 128 * ((p.ycols + bn - 1) / bn) > ctx->sm_count;
+  if (bn == 16) return two ? launch<3, 16, true>(ctx, tmX, tmY, p, s) : launch<3, 16, false>(ctx, tmX, tmY, p, s);
+  if (bn == 32) return two ? launch<3, 32, true>(ctx, tmX, tmY, p, s) : launch<3, 32, false>(ctx, tmX, tmY, p, s);
+  if (bn == 64) return two ? launch<3, 64, true>(ctx, tmX, tmY, p, s) : launch<3, 64, false>(ctx, tmX, tmY, p, s);
   return launch<3, 128, false>(ctx, tmX, tmY, p, s);
 }
 

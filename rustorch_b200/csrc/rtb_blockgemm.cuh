@@ -34,7 +34,7 @@ struct BlockParams {
   int64_t pitchx, pitchy;
   int c_tma;             // CTA pairs: rows of the output leave through TMA stores
   int parts;             // CTAs that share a tile (a cluster)
-  int vec_ok;            // 16-byte aligned output rows and bias
+  int vec_ok;            // 16-byte aligned output rows
   int* err;
   unsigned long long timeout_ns;
 };

@@ -1,20 +1,21 @@
 // The 4-bit product for few rows of A (a generation step's tokens): a stream over the
 // weight on the CUDA cores,
 //   C[m,n] = act( sum_b 2^(sa[m,b] + sb[n,b] - 254) sum_{k in b} qa[m,k] qb[n,k] + bias[n] )
-// over blocks b of 32 elements.  Twice a code's value is a whole number of at most 12,
-// so a block's sum is exact in integers: four products an instruction (dp4a).  A code
-// becomes a byte by table lookup: PRMT's selector takes a code's three magnitude bits as
-// they lie, and a selector with the sign bit set gives 0 where the table's bytes are
-// positive; so the tables 16 + v and 16 - v, the latter asked with the signs turned,
-// together give 16 + value, and the 16 times the sum of the row's values is taken off
-// the block's sum, where it starts.  Then one conversion, one multiply-add by the two
-// scales: fp32 sees exact block sums.
+// over blocks b of 32 elements.  A code's value is a half-precision number as it
+// stands, so two codes become one register by one conversion (a PRMT lookup of bytes for
+// integer dot products takes 4.7 clocks a warp and eight codes, this 2.5), and the
+// products are packed half-precision multiply-adds that are exact: a chain of eight
+// products is a multiple of 1/4 of at most 288, eleven bits.  A block's four chains are
+// added in fp32, exactly too, then one multiply-add by the two scales: fp32 rounds once
+// for each block.
 //
 // A warp takes four weight rows, a lane a block (16 bytes) of each at a time, so that A
-// out of shared memory serves four; with few rows several warps share a contraction,
-// their sums added in a fixed order.
+// out of shared memory serves four; with few weight rows several warps share a
+// contraction, their sums added in a fixed order.  A CTA keeps A for all of its rows.
 //
-// Measured: XX
+// Measured (in a graph): a row by 4096 x 4096 in 4.1 us, by 8192 x 8192 in 9.2 out of L2
+// and 11.5 from memory (3.1 TB/s); by 1000 x 1000, rows of 500 bytes, 3.4.  Bound by the
+// conversions and products, 2.5 of the 4.4 clocks that a warp takes for eight codes.
 #include "rtb_act.cuh"
 #include "rtb_fp4.cuh"
 #include "rtb_internal.h"
@@ -27,25 +28,29 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kRows = 4;      // weight rows of a warp
-// Blocks of A in shared memory at a time (40 KB, 80 for eight rows).
-constexpr int chunk(int rows) { return rows == 1 ? 1024 : rows == 2 ? 512 : 256; }
+// Blocks of A in shared memory at a time (68 KB).
+constexpr int chunk(int rows) { return 1024 / rows; }
 
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
-  uint32_t d;
-  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
-  return d;
+// Eight codes -> four pairs of half-precision values, exactly.
+__device__ __forceinline__ void codes_to_halves(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
 }
-// Eight codes -> bytes of 16 + twice the value, the first four and the last four.
-__device__ __forceinline__ void codes_to_bytes(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  const uint32_t x = w ^ 0x88888888u;
-  lo = prmt(0x13121110u, 0x1C181614u, w) | prmt(0x0D0E0F10u, 0x04080A0Cu, x);
-  hi = prmt(0x13121110u, 0x1C181614u, w >> 16) | prmt(0x0D0E0F10u, 0x04080A0Cu, x >> 16);
+__device__ __forceinline__ void fma_halves(uint32_t& d, uint32_t a, uint32_t b) {
+  asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(d) : "r"(a), "r"(b));
 }
-// c + the dot product of four unsigned and four signed bytes
-__device__ __forceinline__ int dot4(uint32_t u, uint32_t s, int c) {
-  int d;
-  asm("dp4a.u32.s32 %0, %1, %2, %3;" : "=r"(d) : "r"(u), "r"(s), "r"(c));
-  return d;
+__device__ __forceinline__ float sum_of_halves(uint32_t h) {
+  float lo, hi;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}"
+      : "=f"(lo), "=f"(hi)
+      : "r"(h));
+  return lo + hi;
 }
 
 // The 16 bytes of block b of a row of `half` bytes, 0 behind the row.  VEC: the row is on
@@ -67,6 +72,7 @@ __device__ __forceinline__ uint4 load_block(const uint8_t* row, int b, int half)
 struct RowsParams {
   int64_t N;
   int M, half, blocks, split;  // split: warps that share a contraction
+  int64_t groups;              // of weight rows
   const uint8_t *A, *B, *sa, *sb;
   int64_t lda, ldb, ldsa, ldsb;
   const float* bias;
@@ -75,151 +81,167 @@ struct RowsParams {
   int64_t ldc;
 };
 
-// MT: rows of A in the registers (M of them exist).  Shared memory: A's bytes
-// [MT][2 halves][kChunk][16], then [MT][kChunk] pairs of what a block's sum starts from
-// and half of half of its scale.
+// MT: rows of A in the registers (M of them exist).  Shared memory: A's halves
+// [MT][4 words][kChunk][16 bytes], then [MT][kChunk] scales.
 template <int MT, bool VEC>
-__global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const RowsParams p) {
+__global__ void __launch_bounds__(kThreads, 2) fp4_rows_kernel(const RowsParams p) {
   constexpr int kChunk = chunk(MT);
   extern __shared__ uint4 a_s[];
-  int2* start_s = reinterpret_cast<int2*>(a_s + MT * 2 * kChunk);
+  float* scale_s = reinterpret_cast<float*>(a_s + MT * 4 * kChunk);
   __shared__ float red[kWarps][kRows * MT];
   griddep_wait();
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int split = p.split, part = warp % split;
-  const int64_t n0 = ((int64_t)blockIdx.x * (kWarps / split) + warp / split) * kRows;
-  float acc[kRows * MT];
+  const int split = p.split, part = warp % split, per = kWarps / split;  // per: groups of a CTA
+  for (int64_t g0 = (int64_t)blockIdx.x * per; g0 < p.groups; g0 += (int64_t)gridDim.x * per) {
+    const int64_t n0 = (g0 + warp / split) * kRows;
+    float acc[kRows * MT];
 #pragma unroll
-  for (int i = 0; i < kRows * MT; ++i) acc[i] = 0.0f;
-  uint4 w[kRows];
-  uint32_t sb[kRows];
-  auto load = [&](int b) {
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      w[r] = make_uint4(0u, 0u, 0u, 0u);
-      sb[r] = 127u;
-      if (b < p.blocks && n0 + r < p.N) {
-        w[r] = load_block<VEC>(p.B + (n0 + r) * p.ldb, b, p.half);
-        sb[r] = __ldg(p.sb + (n0 + r) * p.ldsb + b);
-      }
-    }
-  };
-  int b = 32 * part + lane;
-  load(b);  // on its way while A is laid out
-  for (int c0 = 0; c0 < p.blocks; c0 += kChunk) {
-    const int cn = p.blocks - c0 < kChunk ? p.blocks - c0 : kChunk;
-    if (c0) __syncthreads();  // the chunk before has been read
-    for (int i = threadIdx.x; i < MT * cn; i += kThreads) {
-      const int m = i / cn, k = i - m * cn;
-      uint4 q = make_uint4(0u, 0u, 0u, 0u);
-      uint32_t s = 127u;
-      if (m < p.M) {
-        q = load_block<false>(p.A + m * p.lda, c0 + k, p.half);
-        s = __ldg(p.sa + m * p.ldsa + c0 + k);
-        const int left = p.half - 16 * (c0 + k);  // bytes behind the row are none of its own
-        if (left < 16) {
-          uint32_t* e = &q.x;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            e[j] = left >= 4 * j + 4 ? e[j] : left <= 4 * j ? 0u : e[j] & ((1u << (8 * (left - 4 * j))) - 1u);
-        }
-      }
-      uint32_t v[8];
-      codes_to_bytes(q.x, v[0], v[1]);
-      codes_to_bytes(q.y, v[2], v[3]);
-      codes_to_bytes(q.z, v[4], v[5]);
-      codes_to_bytes(q.w, v[6], v[7]);
-      int sum = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[j] = __vsub4(v[j], 0x10101010u);
-        sum = __dp4a((int)v[j], 0x01010101, sum);
-      }
-      a_s[(2 * m) * kChunk + k] = make_uint4(v[0], v[1], v[2], v[3]);
-      a_s[(2 * m + 1) * kChunk + k] = make_uint4(v[4], v[5], v[6], v[7]);
-      start_s[m * kChunk + k] = make_int2(-16 * sum, __float_as_int(0.25f * e8m0_to_float(s)));
-    }
-    __syncthreads();
-    while (b < c0 + cn) {
-      uint32_t u[kRows][8];
-      float fb[kRows];
+    for (int i = 0; i < kRows * MT; ++i) acc[i] = 0.0f;
+    uint4 w[kRows];
+    uint32_t sb[kRows];
+    auto load = [&](int b) {
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
-        codes_to_bytes(w[r].x, u[r][0], u[r][1]);
-        codes_to_bytes(w[r].y, u[r][2], u[r][3]);
-        codes_to_bytes(w[r].z, u[r][4], u[r][5]);
-        codes_to_bytes(w[r].w, u[r][6], u[r][7]);
-        fb[r] = e8m0_to_float(sb[r]);
+        w[r] = make_uint4(0u, 0u, 0u, 0u);
+        sb[r] = 127u;
+        if (b < p.blocks && n0 + r < p.N) {
+          w[r] = load_block<VEC>(p.B + (n0 + r) * p.ldb, b, p.half);
+          sb[r] = __ldg(p.sb + (n0 + r) * p.ldsb + b);
+        }
       }
-      const int k = b - c0;
-      b += 32 * split;
-      load(b);  // the next block's, while this one's are multiplied
+    };
+    int b = 32 * part + lane;
+    load(b);  // on its way while A is laid out
+    for (int c0 = 0; c0 < p.blocks; c0 += kChunk) {
+      const int cn = p.blocks - c0 < kChunk ? p.blocks - c0 : kChunk;
+      // (A that fits stays for all of the CTA's groups)
+      if (p.blocks > kChunk || g0 == (int64_t)blockIdx.x * per) {
+        if (p.blocks > kChunk) __syncthreads();  // the chunk before has been read
+        for (int i = threadIdx.x; i < MT * cn; i += kThreads) {
+          const int m = i / cn, k = i - m * cn;
+          uint4 q = make_uint4(0u, 0u, 0u, 0u);
+          uint32_t s = 127u;
+          if (m < p.M) {
+            q = load_block<false>(p.A + m * p.lda, c0 + k, p.half);
+            s = __ldg(p.sa + m * p.ldsa + c0 + k);
+            const int left = p.half - 16 * (c0 + k);  // bytes behind the row are none of its own
+            if (left < 16) {
+              uint32_t* e = &q.x;
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const uint4 x = a_s[(2 * m) * kChunk + k], y = a_s[(2 * m + 1) * kChunk + k];
-        const int2 st = start_s[m * kChunk + k];
-        const float fa = __int_as_float(st.y);
+              for (int j = 0; j < 4; ++j)
+                e[j] = left >= 4 * j + 4 ? e[j] : left <= 4 * j ? 0u : e[j] & ((1u << (8 * (left - 4 * j))) - 1u);
+            }
+          }
+          const uint32_t e[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t h[4];
+            codes_to_halves(e[j], h);
+            a_s[(4 * m + j) * kChunk + k] = make_uint4(h[0], h[1], h[2], h[3]);
+          }
+          scale_s[m * kChunk + k] = e8m0_to_float(s);
+        }
+        __syncthreads();
+      }
+      while (b < c0 + cn) {
+        const int k = b - c0;
+        uint4 u[kRows];
+        float fb[kRows];
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
-          int d = st.x;
-          d = dot4(u[r][0], x.x, d);
-          d = dot4(u[r][1], x.y, d);
-          d = dot4(u[r][2], x.z, d);
-          d = dot4(u[r][3], x.w, d);
-          d = dot4(u[r][4], y.x, d);
-          d = dot4(u[r][5], y.y, d);
-          d = dot4(u[r][6], y.z, d);
-          d = dot4(u[r][7], y.w, d);
-          acc[r * MT + m] = fmaf((float)d, fa * fb[r], acc[r * MT + m]);
+          u[r] = w[r];
+          fb[r] = e8m0_to_float(sb[r]);
+        }
+        b += 32 * split;
+        load(b);  // the next block's, while this one's are multiplied
+        uint32_t d[kRows * MT][2];  // two chains: words 0 and 1, 2 and 3
+#pragma unroll
+        for (int i = 0; i < kRows * MT; ++i) d[i][0] = d[i][1] = 0u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint4 x[MT];
+#pragma unroll
+          for (int m = 0; m < MT; ++m) x[m] = a_s[(4 * m + j) * kChunk + k];
+#pragma unroll
+          for (int r = 0; r < kRows; ++r) {
+            uint32_t h[4];
+            codes_to_halves(j == 0 ? u[r].x : j == 1 ? u[r].y : j == 2 ? u[r].z : u[r].w, h);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              fma_halves(d[r * MT + m][j / 2], h[0], x[m].x);
+              fma_halves(d[r * MT + m][j / 2], h[1], x[m].y);
+              fma_halves(d[r * MT + m][j / 2], h[2], x[m].z);
+              fma_halves(d[r * MT + m][j / 2], h[3], x[m].w);
+            }
+          }
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const float fa = scale_s[m * kChunk + k];
+#pragma unroll
+          for (int r = 0; r < kRows; ++r)
+            acc[r * MT + m] = fmaf(sum_of_halves(d[r * MT + m][0]) + sum_of_halves(d[r * MT + m][1]),
+                                   fa * fb[r], acc[r * MT + m]);
         }
       }
     }
-  }
-  // The lanes' sums: halves of the values change places until each lane has one, then
-  // the rest of the lanes that share it.
-  int index = 0;
+    // The lanes' sums: halves of the values change places until each lane has one, then
+    // the rest of the lanes that share it.
+    int index = 0;
 #pragma unroll
-  for (int step = 0; step < 5; ++step) {
-    const int o = 16 >> step, n = (kRows * MT) >> (step + 1);  // a constant each
-    if (n > 0) {
-      const bool upper = lane & o;
-      index = 2 * index + upper;
+    for (int step = 0; step < 5; ++step) {
+      const int o = 16 >> step, n = (kRows * MT) >> (step + 1);  // a constant each
+      if (n > 0) {
+        const bool upper = lane & o;
+        index = 2 * index + upper;
 #pragma unroll
-      for (int i = 0; i < n; ++i) {
-        const float send = upper ? acc[i] : acc[i + n], keep = upper ? acc[i + n] : acc[i];
-        acc[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        for (int i = 0; i < n; ++i) {
+          const float send = upper ? acc[i] : acc[i + n], keep = upper ? acc[i + n] : acc[i];
+          acc[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+      } else {
+        acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], o);
       }
-    } else {
-      acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], o);
     }
-  }
-  if ((lane & (32 / (kRows * MT) - 1)) == 0) red[warp][index] = acc[0];
-  __syncthreads();
-  for (int i = threadIdx.x; i < kWarps / split * kRows * MT; i += kThreads) {
-    const int g = i / (kRows * MT), v = i % (kRows * MT), m = v % MT;
-    const int64_t n = ((int64_t)blockIdx.x * (kWarps / split) + g) * kRows + v / MT;
-    if (m >= p.M || n >= p.N) continue;
-    float sum = red[g * split][v];
-    for (int k = 1; k < split; ++k) sum += red[g * split + k][v];
-    p.C[m * p.ldc + n] = activate(sum + (p.bias ? __ldg(p.bias + n) : 0.0f), p.act);
+    const bool mine = (lane & (32 / (kRows * MT) - 1)) == 0;
+    const int m = index % MT;
+    if (split == 1) {
+      const int64_t n = n0 + index / MT;
+      if (mine && m < p.M && n < p.N)
+        p.C[m * p.ldc + n] = activate(acc[0] + (p.bias ? __ldg(p.bias + n) : 0.0f), p.act);
+      continue;
+    }
+    if (mine) red[warp][index] = acc[0];
+    __syncthreads();
+    for (int i = threadIdx.x; i < per * kRows * MT; i += kThreads) {
+      const int g = i / (kRows * MT), v = i % (kRows * MT), mm = v % MT;
+      const int64_t n = (g0 + g) * kRows + v / MT;
+      if (mm >= p.M || n >= p.N) continue;
+      float sum = red[g * split][v];
+      for (int k = 1; k < split; ++k) sum += red[g * split + k][v];
+      p.C[mm * p.ldc + n] = activate(sum + (p.bias ? __ldg(p.bias + n) : 0.0f), p.act);
+    }
+    __syncthreads();  // red[] is free
   }
 }
 
 template <int MT, bool VEC>
 int launch(rtb_ctx* ctx, RowsParams& p, cudaStream_t s) {
   auto* k = fp4_rows_kernel<MT, VEC>;
-  constexpr int kSmem = MT * chunk(MT) * 40;
-  if (kSmem > 48 * 1024) {
+  constexpr int kSmem = MT * chunk(MT) * 68;
+  {
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return cuda_status(e, "fp4_matmul smem attribute");
   }
-  const int64_t groups = (p.N + kRows - 1) / kRows;
-  // warps that share a contraction: until 16 warps an SM have work, each a block a lane
+  p.groups = (p.N + kRows - 1) / kRows;
+  // Two CTAs on an SM at once; warps that share a contraction while that many have work
+  // and each lane a block.
+  const int64_t warps = (int64_t)2 * ctx->sm_count * kWarps;
   p.split = 1;
-  while (p.split < kWarps && groups * p.split < (int64_t)16 * ctx->sm_count && p.split * 64 <= p.blocks)
-    p.split *= 2;
-  const int64_t per = kWarps / p.split, grid = (groups + per - 1) / per;
+  while (p.split < kWarps && p.groups * p.split * 2 <= warps && p.split * 64 <= p.blocks) p.split *= 2;
+  const int64_t per = kWarps / p.split, need = (p.groups + per - 1) / per;
+  const int64_t grid = need < 2 * ctx->sm_count ? need : 2 * ctx->sm_count;
   clear_stale_cuda_error();
   cudaError_t e = launch_pdl(k, dim3((unsigned)grid), dim3(kThreads), (size_t)kSmem, s, (const RowsParams)p);
   if (e == cudaSuccess) e = cudaGetLastError();
@@ -249,8 +271,7 @@ int fp4_rows_run(rtb_ctx* ctx, const Fp4Desc& d, cudaStream_t s) {
   const bool vec = (reinterpret_cast<uintptr_t>(d.B) & 15u) == 0 && d.ldb % 16 == 0;
   if (d.M == 1) return vec ? launch<1, true>(ctx, p, s) : launch<1, false>(ctx, p, s);
   if (d.M == 2) return vec ? launch<2, true>(ctx, p, s) : launch<2, false>(ctx, p, s);
-  if (d.M <= 4) return vec ? launch<4, true>(ctx, p, s) : launch<4, false>(ctx, p, s);
-  return vec ? launch<8, true>(ctx, p, s) : launch<8, false>(ctx, p, s);
+  return vec ? launch<4, true>(ctx, p, s) : launch<4, false>(ctx, p, s);
 }
 
 }  // namespace rtb

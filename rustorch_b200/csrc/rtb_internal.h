@@ -290,8 +290,8 @@ struct Fp4Desc {
   int64_t ldc = 0;
 };
 int fp4_gemm_run(rtb_ctx* ctx, const Fp4Desc& d, cudaStream_t s);  // 16-byte aligned bases and rows
-// Few rows of A, any alignment (rtb_fp4_rows.cu).
-constexpr int64_t kFp4RowsMax = 8;
+// Few rows of A on the CUDA cores, any alignment (rtb_fp4_rows.cu).
+constexpr int64_t kFp4RowsMax = 4;
 int fp4_rows_run(rtb_ctx* ctx, const Fp4Desc& d, cudaStream_t s);
 // dst[r][c] = c < cols ? src[r * rs + c * cs] : 0 for c < ldd (rs or cs is 1,
 // ldd % 16 == 0), of up to two matrices in one launch; a null dst is left out.
