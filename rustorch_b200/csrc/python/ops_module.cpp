@@ -535,26 +535,43 @@ PyObject* rms_norm_backward(PyObject* const* a) {
   return pack({wrap(dx), wrap(dw)});
 }
 
-// A 4-bit tensor's bytes as rows (its last dimension counts them).
-Rows codes(const Tensor& t, const char* who) {
-  if (!(t.is_cuda() && t.scalar_type() == ScalarType::Float4_e2m1fn_x2))
-    refuse(std::string(who) + " expects float4_e2m1fn_x2 CUDA tensors");
-  if (t.dim() == 0) refuse(std::string(who) + ": a 4-bit tensor needs a last dimension");
-  return rows_of(t.view(ScalarType::Byte), t.size(-1));
-}
 // The rows that a tensor's leading dimensions count (a last dimension of 0 has some too).
 int64_t leading(const Tensor& t) {
   int64_t n = 1;
   for (int64_t i = 0; i + 1 < t.dim(); ++i) n *= t.size(i);
   return n;
 }
-Rows scales4(const Tensor& s, int64_t rows, int64_t cols, const char* who) {
+// A tensor of one-byte elements as rows of d contiguous bytes that do not overlap; trans:
+// as the rows of its transpose.  No view is made where it lies so already.
+Rows byte_rows(const Tensor& t, bool trans) {
+  if (t.dim() == 2) {
+    const int64_t rows = t.size(trans ? 1 : 0), d = t.size(trans ? 0 : 1);
+    const int64_t rs = t.stride(trans ? 1 : 0), cs = t.stride(trans ? 0 : 1);
+    if ((d <= 1 || cs == 1) && (rows <= 1 || rs >= d)) {
+      Rows r;
+      r.hold = t;
+      r.rows = rows;
+      r.ld = rs > d ? rs : d;
+      return r;
+    }
+  }
+  const Tensor bytes = t.view(ScalarType::Byte);
+  return rows_of(trans ? bytes.t() : bytes, t.size(trans ? 0 : -1));
+}
+// A 4-bit tensor's codes (its last dimension, or its first, counts bytes).
+Rows codes(const Tensor& t, bool trans, const char* who) {
+  if (!(t.is_cuda() && t.scalar_type() == ScalarType::Float4_e2m1fn_x2))
+    refuse(std::string(who) + " expects float4_e2m1fn_x2 CUDA tensors");
+  if (t.dim() == 0) refuse(std::string(who) + ": a 4-bit tensor needs a last dimension");
+  return byte_rows(t, trans);
+}
+Rows scales4(const Tensor& s, bool trans, int64_t rows, int64_t cols, const char* who) {
   if (!(s.is_cuda() && s.scalar_type() == ScalarType::Float8_e8m0fnu))
     refuse(std::string(who) + ": scales are float8_e8m0fnu CUDA tensors");
   const int64_t cb = (cols + 31) / 32;
-  if (s.dim() < 1 || s.size(-1) != cb || leading(s) != rows)
+  if (s.dim() < 1 || s.size(trans ? 0 : -1) != cb || (trans ? s.size(1) : leading(s)) != rows)
     refuse(std::string(who) + ": scales must be [rows, ceil(cols / 32)]");
-  return rows_of(s.view(ScalarType::Byte), cb);
+  return byte_rows(s, trans);
 }
 
 PyObject* fp4_quantize(PyObject* const* a) {
@@ -595,11 +612,11 @@ PyObject* fp4_dequantize(PyObject* const* a) {
   const Tensor* out = optional(a[3], "out");
   need_f32(out);
   same_device(q, {&scale, out});
-  const Rows qr = codes(q, who);
+  const Rows qr = codes(q, false, who);
   if (cols == -1) cols = 2 * q.size(-1);
   if (cols < 0 || (cols + 1) / 2 != q.size(-1))
     refuse("fp4_dequantize: q holds two columns in each byte of its last dimension");
-  const Rows sr = scales4(scale, leading(q), cols, who);
+  const Rows sr = scales4(scale, false, leading(q), cols, who);
   c10::SmallVector<int64_t, 6> shape(q.sizes().begin(), q.sizes().end());
   shape.back() = cols;
   if (out && (out->sizes() != at::IntArrayRef(shape) || !out->is_contiguous()))
@@ -629,8 +646,8 @@ PyObject* fp4_matmul(PyObject* const* a) {
   if (A.dim() != 2 || B.dim() != 2 || Bs.dim() != 2) refuse("Matmul only supports 2D");
   const int64_t M = A.size(0), K = 2 * A.size(1), N = B.size(1);
   if (2 * B.size(0) != K) refuse("Matmul dimension mismatch");
-  const Rows ar = codes(A, who), br = codes(B.t(), who);
-  const Rows sa = scales4(As, M, K, who), sb = scales4(Bs.t(), N, K, who);
+  const Rows ar = codes(A, false, who), br = codes(B, true, who);
+  const Rows sa = scales4(As, false, M, K, who), sb = scales4(Bs, true, N, K, who);
   const Vec bv = vec(bias, N, "fp4_matmul: bias must have N elements");
   if (out && (out->dim() != 2 || out->size(0) != M || out->size(1) != N ||
               (N > 1 && out->stride(1) != 1) || (M > 1 && out->stride(0) < N)))
