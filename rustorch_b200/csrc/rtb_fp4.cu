@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_any_kernel(const float*
 // pass through shared memory and leave along the result's rows, 128 bytes each.  Five
 // CTAs on an SM: 8192 x 4096 in 30.4 us; four 32.3, three 37.8, six, whose registers do
 // not hold the 32 values, 37.
-template <typename Word>  // how the result's rows are aligned
+template <bool VEC>  // the result's rows are on 16-byte boundaries
 __global__ void __launch_bounds__(kThreads, 5) fp4_quantize_columns_kernel(const float* __restrict__ x,
                                                                         int64_t ldx, int64_t rows, int64_t cols,
                                                                         int64_t row_tiles, int64_t tiles,
@@ -228,17 +228,25 @@ __global__ void __launch_bounds__(kThreads, 5) fp4_quantize_columns_kernel(const
     *reinterpret_cast<uint4*>(&codes[lane][16 * w]) = make_uint4(word[0], word[1], word[2], word[3]);
     bytes[lane][w] = (uint8_t)sb;
     __syncthreads();
-    constexpr int kWords = 128 / sizeof(Word);
     const int64_t qcols = (cols + 1) / 2, scols = (cols + kFp4Block - 1) / kFp4Block;
-    for (int i = threadIdx.x; i < 32 * kWords; i += kThreads) {
-      const int r = i / kWords, k = i % kWords;
-      const int64_t at = c0 / 2 + k * (int)sizeof(Word);
-      if (r0 + r >= rows) break;
-      uint8_t* o = q + (r0 + r) * ldq + at;
-      if (at + (int)sizeof(Word) <= qcols) {
-        *reinterpret_cast<Word*>(o) = *reinterpret_cast<const Word*>(&codes[r][k * sizeof(Word)]);
-      } else {
-        for (int b = 0; b < (int)sizeof(Word) && at + b < qcols; ++b) o[b] = codes[r][k * sizeof(Word) + b];
+    if (VEC) {
+      const int r = threadIdx.x >> 3, k = threadIdx.x & 7;
+      const int64_t at = c0 / 2 + 16 * k;
+      if (r0 + r < rows) {
+        uint8_t* o = q + (r0 + r) * ldq + at;
+        if (at + 16 <= qcols) {
+          *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(&codes[r][16 * k]);
+        } else {
+          for (int b = 0; b < 16 && at + b < qcols; ++b) o[b] = codes[r][16 * k + b];
+        }
+      }
+    } else {
+      const int n = qcols - c0 / 2 < 128 ? (int)(qcols - c0 / 2) : 128;  // bytes of a row here
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        const int r = w + 8 * i;
+        if (r0 + r >= rows) break;
+        store_codes(q + (r0 + r) * ldq + c0 / 2, *reinterpret_cast<const uint32_t*>(&codes[r][4 * lane]), n, lane);
       }
     }
     const int r = threadIdx.x >> 3, k = threadIdx.x & 7;
@@ -362,14 +370,9 @@ int launch_fp4_quantize(rtb_ctx* ctx, const float* x, int64_t ldx, int trans, in
   if (trans) {
     const int64_t row_tiles = (rows + 31) / 32, tiles = row_tiles * ((cols + 255) / 256);
     const int grid = grid_for(ctx, tiles, 32);
-    if (aligned(q, 16) && ldq % 16 == 0)
-      return run(what, fp4_quantize_columns_kernel<uint4>, grid, s, x, ldx, rows, cols, row_tiles, tiles,
-                 q, ldq, scale, lds);
-    if (aligned(q, 4) && ldq % 4 == 0)
-      return run(what, fp4_quantize_columns_kernel<uint32_t>, grid, s, x, ldx, rows, cols, row_tiles, tiles,
-                 q, ldq, scale, lds);
-    return run(what, fp4_quantize_columns_kernel<uint8_t>, grid, s, x, ldx, rows, cols, row_tiles, tiles,
-               q, ldq, scale, lds);
+    const bool vec = aligned(q, 16) && ldq % 16 == 0;
+    return run(what, vec ? fp4_quantize_columns_kernel<true> : fp4_quantize_columns_kernel<false>, grid, s, x, ldx,
+               rows, cols, row_tiles, tiles, q, ldq, scale, lds);
   }
   const int chunks = (int)((cols + 255) / 256);
   const int64_t total = rows * chunks;

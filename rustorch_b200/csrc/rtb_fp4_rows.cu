@@ -28,8 +28,12 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kRows = 4;      // weight rows of a warp
-// Blocks of A in shared memory at a time (68 KB).
-constexpr int chunk(int rows) { return 1024 / rows; }
+// Blocks of a weight row that a warp takes at a time.  Rows on 16-byte boundaries: one a
+// lane.  Else a lane loads the 16 aligned bytes in which its block begins, the rest are
+// the next lane's, and the last lane is there for its neighbour only.
+constexpr int lanes(bool vec) { return vec ? 32 : 31; }
+// Blocks of A in shared memory at a time (68 KB): whole turns of a warp.
+constexpr int chunk(int rows, bool vec) { return 1024 / rows / 32 * lanes(vec); }
 
 // Eight codes -> four pairs of half-precision values, exactly.
 __device__ __forceinline__ void codes_to_halves(uint32_t w, uint32_t (&h)[4]) {
@@ -53,12 +57,10 @@ __device__ __forceinline__ float sum_of_halves(uint32_t h) {
   return lo + hi;
 }
 
-// The 16 bytes of block b of a row of `half` bytes, 0 behind the row.  VEC: the row is on
-// a 16-byte boundary.  Else aligned words, each read only where one of its bytes exists.
-template <bool VEC>
+// The 16 bytes of block b of a row of `half` bytes at any address, by aligned words, each
+// read only where one of its bytes exists.
 __device__ __forceinline__ uint4 load_block(const uint8_t* row, int b, int half) {
   const uint8_t* p = row + (int64_t)16 * b;
-  if (VEC) return __ldg(reinterpret_cast<const uint4*>(p));  // (a row's last block: its own 16 bytes)
   const int off = (int)(reinterpret_cast<uintptr_t>(p) & 3u);
   const uint32_t* w = reinterpret_cast<const uint32_t*>(p - off);
   const int left = half - 16 * b;
@@ -67,6 +69,21 @@ __device__ __forceinline__ uint4 load_block(const uint8_t* row, int b, int half)
   for (int i = 0; i < 5; ++i) v[i] = 4 * i - off < left && (i < 4 || off) ? __ldg(w + i) : 0u;
   return make_uint4(__funnelshift_r(v[0], v[1], 8 * off), __funnelshift_r(v[1], v[2], 8 * off),
                     __funnelshift_r(v[2], v[3], 8 * off), __funnelshift_r(v[3], v[4], 8 * off));
+}
+// The 16 bytes that begin `off` (0..15, the same in all lanes) behind this lane's 16,
+// which the next lane's follow.
+__device__ __forceinline__ uint4 behind(uint4 w, int off) {
+  if (off == 0) return w;
+  uint32_t v[8] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[4 + i] = __shfl_down_sync(0xffffffffu, v[i], 1);
+#pragma unroll
+  for (int i = 0; i < 6; ++i) v[i] = off & 8 ? v[i + 2] : v[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) v[i] = off & 4 ? v[i + 1] : v[i];
+  const int s = 8 * (off & 3);
+  return make_uint4(__funnelshift_r(v[0], v[1], s), __funnelshift_r(v[1], v[2], s),
+                    __funnelshift_r(v[2], v[3], s), __funnelshift_r(v[3], v[4], s));
 }
 
 struct RowsParams {
@@ -85,7 +102,7 @@ struct RowsParams {
 // [MT][4 words][kChunk][16 bytes], then [MT][kChunk] scales.
 template <int MT, bool VEC>
 __global__ void __launch_bounds__(kThreads, 2) fp4_rows_kernel(const RowsParams p) {
-  constexpr int kChunk = chunk(MT);
+  constexpr int kChunk = chunk(MT, VEC), kLanes = lanes(VEC);
   extern __shared__ uint4 a_s[];
   float* scale_s = reinterpret_cast<float*>(a_s + MT * 4 * kChunk);
   __shared__ float red[kWarps][kRows * MT];
@@ -105,13 +122,19 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_rows_kernel(const RowsParams 
       for (int r = 0; r < kRows; ++r) {
         w[r] = make_uint4(0u, 0u, 0u, 0u);
         sb[r] = 127u;
-        if (b < p.blocks && n0 + r < p.N) {
-          w[r] = load_block<VEC>(p.B + (n0 + r) * p.ldb, b, p.half);
-          sb[r] = __ldg(p.sb + (n0 + r) * p.ldsb + b);
+        if (n0 + r < p.N) {
+          const uint8_t* row = p.B + (n0 + r) * p.ldb;
+          if (VEC) {
+            if (b < p.blocks) w[r] = __ldg(reinterpret_cast<const uint4*>(row) + b);
+          } else {  // the 16 bytes of memory in which the block begins
+            const uintptr_t at = (reinterpret_cast<uintptr_t>(row) + (int64_t)16 * b) & ~uintptr_t(15);
+            if (at < reinterpret_cast<uintptr_t>(row) + p.half) w[r] = __ldg(reinterpret_cast<const uint4*>(at));
+          }
+          if (b < p.blocks) sb[r] = __ldg(p.sb + (n0 + r) * p.ldsb + b);
         }
       }
     };
-    int b = 32 * part + lane;
+    int b = kLanes * part + lane;
     load(b);  // on its way while A is laid out
     for (int c0 = 0; c0 < p.blocks; c0 += kChunk) {
       const int cn = p.blocks - c0 < kChunk ? p.blocks - c0 : kChunk;
@@ -123,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_rows_kernel(const RowsParams 
           uint4 q = make_uint4(0u, 0u, 0u, 0u);
           uint32_t s = 127u;
           if (m < p.M) {
-            q = load_block<false>(p.A + m * p.lda, c0 + k, p.half);
+            q = load_block(p.A + m * p.lda, c0 + k, p.half);
             s = __ldg(p.sa + m * p.ldsa + c0 + k);
             const int left = p.half - 16 * (c0 + k);  // bytes behind the row are none of its own
             if (left < 16) {
@@ -144,16 +167,17 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_rows_kernel(const RowsParams 
         }
         __syncthreads();
       }
-      while (b < c0 + cn) {
-        const int k = b - c0;
+      while (b - lane < c0 + cn) {  // (a warp's lanes stay together)
+        const bool mine = lane < kLanes && b < c0 + cn;
+        const int k = mine ? b - c0 : 0;
         uint4 u[kRows];
         float fb[kRows];
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
-          u[r] = w[r];
+          u[r] = VEC ? w[r] : behind(w[r], (int)((reinterpret_cast<uintptr_t>(p.B) + (n0 + r) * p.ldb) & 15));
           fb[r] = e8m0_to_float(sb[r]);
         }
-        b += 32 * split;
+        b += kLanes * split;
         load(b);  // the next block's, while this one's are multiplied
         uint32_t d[kRows * MT][2];  // two chains: words 0 and 1, 2 and 3
 #pragma unroll
@@ -181,8 +205,9 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_rows_kernel(const RowsParams 
           const float fa = scale_s[m * kChunk + k];
 #pragma unroll
           for (int r = 0; r < kRows; ++r)
-            acc[r * MT + m] = fmaf(sum_of_halves(d[r * MT + m][0]) + sum_of_halves(d[r * MT + m][1]),
-                                   fa * fb[r], acc[r * MT + m]);
+            if (mine)
+              acc[r * MT + m] = fmaf(sum_of_halves(d[r * MT + m][0]) + sum_of_halves(d[r * MT + m][1]),
+                                     fa * fb[r], acc[r * MT + m]);
         }
       }
     }
@@ -229,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_rows_kernel(const RowsParams 
 template <int MT, bool VEC>
 int launch(rtb_ctx* ctx, RowsParams& p, cudaStream_t s) {
   auto* k = fp4_rows_kernel<MT, VEC>;
-  constexpr int kSmem = MT * chunk(MT) * 68;
+  constexpr int kSmem = MT * chunk(MT, VEC) * 68;
   {
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return cuda_status(e, "fp4_matmul smem attribute");
@@ -239,7 +264,8 @@ int launch(rtb_ctx* ctx, RowsParams& p, cudaStream_t s) {
   // and each lane a block.
   const int64_t warps = (int64_t)2 * ctx->sm_count * kWarps;
   p.split = 1;
-  while (p.split < kWarps && p.groups * p.split * 2 <= warps && p.split * 64 <= p.blocks) p.split *= 2;
+  while (p.split < kWarps && p.groups * p.split * 2 <= warps && p.split * 2 * lanes(VEC) <= p.blocks)
+    p.split *= 2;
   const int64_t per = kWarps / p.split, need = (p.groups + per - 1) / per;
   const int64_t grid = need < 2 * ctx->sm_count ? need : 2 * ctx->sm_count;
   clear_stale_cuda_error();

@@ -5,11 +5,17 @@
 // backward pass (rtb_norm_bwd.cu).  HBM-bound: x and the residual are read once, h
 // and y written once.
 //
-// A row of up to 16384 columns lives in the registers of a group of 32..256
+// A row of up to 16384 columns lives in the registers of a group of 32..512
 // threads: warp w of the group holds the 128-column blocks w, w + W, ..., so that
 // an 8-bit block's maximum is one warp's.  The sum of squares is fp32 in a thread
-// (at most 64 terms) and double from there on.  Wider rows take a CTA each and two
-// passes, the second out of L2.
+// (at most 32 terms) and double from there on.  1024 threads of 64 registers share an
+// SM: that many rows in flight hide a row's chain of loads, sum and stores (16 values a
+// thread of 512 and not 32 of 256, 4095 x 8191: 92 us, 96; 32 of 512 and not 64 of 256,
+// 2047 x 16383: 97 us, 142).  Wider rows take a CTA each and two passes, the second out
+// of L2.
+//
+// Measured: 8192 x 4096 with a residual 88 us (6.1 TB/s, 93% of a copy), with the 8-bit
+// output 71 (6.2 TB/s); 16384 x 2048 87 us, 2048 x 16384 94 and 88.
 #include "rtb_fp8.cuh"
 #include "rtb_internal.h"
 #include "rtb_ptx.cuh"
@@ -103,10 +109,12 @@ __device__ __forceinline__ void finish4(const RmsParams& p, int64_t m, int c0, i
   if (lane == 0) p.scale[m * p.lds + c0 / kFp8Block] = (uint8_t)sb;
 }
 
+constexpr int cta(int T) { return T > kThreads ? T : kThreads; }
+
 // T threads a row, NB blocks of 128 columns a warp.
 template <int T, int NB, bool VEC, bool FP8>
-__global__ void __launch_bounds__(kThreads) rms_rows_kernel(const RmsParams p) {
-  constexpr int R = kThreads / T;  // rows a CTA works on
+__global__ void __launch_bounds__(cta(T), T == 512 ? 2 : 4) rms_rows_kernel(const RmsParams p) {
+  constexpr int R = cta(T) / T;  // rows a CTA works on
   constexpr int W = T / 32;        // warps a row
   __shared__ double red[2][R][W];  // two buffers, so that one barrier a row is enough
   griddep_wait();
@@ -202,19 +210,19 @@ __global__ void __launch_bounds__(kThreads) rms_wide_kernel(const RmsParams p) {
   }
 }
 
-int launch(rtb_ctx* ctx, void (*k)(const RmsParams), int64_t ctas, const RmsParams& p,
+int launch(rtb_ctx* ctx, void (*k)(const RmsParams), int64_t ctas, int threads, const RmsParams& p,
            cudaStream_t s) {
   const int64_t cap = (int64_t)ctx->sm_count * 8;
   clear_stale_cuda_error();
-  cudaError_t e = launch_pdl(k, dim3((unsigned)(ctas < cap ? ctas : cap)), dim3(kThreads), 0, s, p);
+  cudaError_t e = launch_pdl(k, dim3((unsigned)(ctas < cap ? ctas : cap)), dim3((unsigned)threads), 0, s, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? RTB_OK : cuda_status(e, "rms_norm launch");
 }
 
 template <int T, int NB, bool VEC, bool FP8>
 int rows_as(rtb_ctx* ctx, const RmsParams& p, cudaStream_t s) {
-  constexpr int R = kThreads / T;
-  return launch(ctx, rms_rows_kernel<T, NB, VEC, FP8>, (p.rows + R - 1) / R, p, s);
+  constexpr int R = cta(T) / T;
+  return launch(ctx, rms_rows_kernel<T, NB, VEC, FP8>, (p.rows + R - 1) / R, cta(T), p, s);
 }
 
 template <bool VEC, bool FP8>
@@ -226,9 +234,9 @@ int run(rtb_ctx* ctx, const RmsParams& p, cudaStream_t s) {
   if (blocks <= 8) return rows_as<64, 4, VEC, FP8>(ctx, p, s);
   if (blocks <= 16) return rows_as<128, 4, VEC, FP8>(ctx, p, s);
   if (blocks <= 32) return rows_as<256, 4, VEC, FP8>(ctx, p, s);
-  if (blocks <= 64) return rows_as<256, 8, VEC, FP8>(ctx, p, s);
-  if (blocks <= 128) return rows_as<256, 16, VEC, FP8>(ctx, p, s);
-  return launch(ctx, rms_wide_kernel<VEC, FP8>, p.rows, p, s);
+  if (blocks <= 64) return rows_as<512, 4, VEC, FP8>(ctx, p, s);
+  if (blocks <= 128) return rows_as<512, 8, VEC, FP8>(ctx, p, s);
+  return launch(ctx, rms_wide_kernel<VEC, FP8>, p.rows, kThreads, p, s);
 }
 
 }  // namespace
