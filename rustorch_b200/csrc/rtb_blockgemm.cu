@@ -179,15 +179,14 @@ __device__ __forceinline__ void load_scale_bytes(const ScaleRef& s, int64_t r, i
 #pragma unroll
   for (int k = 0; k < N; ++k) raw[k] = in && k < n ? __ldg(p + (int64_t)k * s.ld_col) : 127u;
 }
-// MODE 3: ... the words j .. j + n - 1, two for each stage.
+// MODE 3: ... the words j .. j + n - 1, two for each stage.  (A row past the operand takes
+// another's scales: its codes are 0, its outputs not stored.)
 template <int N>
 __device__ __forceinline__ void load_scale_words(const ScaleRef& s, int64_t r, int64_t rows, int j,
                                                  int n, int bytes, int vec, uint32_t (&raw)[N]) {
-  // Whole pairs of words, without a branch, so that all loads are in flight.  (A row
-  // past the operand takes another's scales: its codes are 0, its outputs not stored.)
-  if (vec == 2 && 4 * (j + n) <= bytes) {
-    const uint2* p = reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(s.p) +
-                                                    (r < rows ? r : 0) * s.ld_row + (int64_t)4 * j);
+  const uint8_t* row = static_cast<const uint8_t*>(s.p) + (r < rows ? r : 0) * s.ld_row;
+  if (vec && 4 * (j + n) <= bytes) {  // whole pairs of words
+    const uint2* p = reinterpret_cast<const uint2*>(row + (int64_t)4 * j);
 #pragma unroll
     for (int k = 0; k < N; k += 2) {
       const uint2 two = k < n ? __ldg(p + k / 2) : make_uint2(0u, 0u);
@@ -196,9 +195,11 @@ __device__ __forceinline__ void load_scale_words(const ScaleRef& s, int64_t r, i
     }
     return;
   }
+  ScaleWord v[N];
 #pragma unroll
-  for (int k = 0; k < N; ++k)
-    raw[k] = r < rows && k < n ? fp4_scale_word(s, r, j + k, bytes, vec) : 0x7F7F7F7Fu;
+  for (int k = 0; k < N; ++k) v[k] = fp4_load_scales(row, j + k, bytes);
+#pragma unroll
+  for (int k = 0; k < N; ++k) raw[k] = fp4_scale_word(v[k], row, j + k, bytes);
 }
 // ... as words of the 512-byte groups that the tensor core takes (row l of a group:
 // the word at 16 (l % 32) + 4 (l / 32), its byte four times).
@@ -818,7 +819,7 @@ int fp4_gemm_run(rtb_ctx* ctx, const Fp4Desc& d, cudaStream_t s) {
   p.sc_bytes = (int)((d.K + 31) / 32);
   const uintptr_t at = reinterpret_cast<uintptr_t>(d.sa) | reinterpret_cast<uintptr_t>(d.sb) |
                        (uintptr_t)d.ldsa | (uintptr_t)d.ldsb;
-  p.sc_vec = at % 8 == 0 ? 2 : at % 4 == 0 ? 1 : 0;
+  p.sc_vec = at % 8 == 0;
   p.err = ctx->d_err;
   p.timeout_ns = ctx->timeout_ns;
   const int64_t tiles = ((p.xrows + 127) / 128) * ((p.ycols + 127) / 128);

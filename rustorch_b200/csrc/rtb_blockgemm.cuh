@@ -26,8 +26,7 @@ struct BlockParams {
   int pieces;            // MODE 1
   int64_t piece_rows;    // MODE 1: contraction rows between Y's pieces
   ScaleRef scx, scy;
-  // 4-bit operands: scales of a row; whether their rows are 4-byte (1) or 8-byte (2) aligned
-  int sc_bytes, sc_vec;
+  int sc_bytes, sc_vec;  // 4-bit operands: scales of a row, and whether their rows are 8-byte aligned
   // MODE 0, CTA pairs: the scales as fp32, [block][row], zero past the operand
   // (launch_scale_tables)
   const float *tabx, *taby;
@@ -80,17 +79,27 @@ __device__ __forceinline__ void tmem_wait_x16(uint32_t (&r)[16]) {
 // a quad can be loaded ahead without a check.
 inline int64_t table_blocks(int64_t units) { return (units + 3) / 4 * 4 + 4; }
 
-// 4-bit operands: word j of row r's scales, four blocks of 32 columns; 2^0 past the
-// row's last one.
-__device__ __forceinline__ uint32_t fp4_scale_word(const ScaleRef& s, int64_t r, int j, int bytes,
-                                                   int vec) {
-  const uint8_t* p = static_cast<const uint8_t*>(s.p) + r * s.ld_row + (int64_t)4 * j;
-  const int left = bytes - 4 * j;
-  if (vec && left >= 4) return __ldg(reinterpret_cast<const uint32_t*>(p));
-  uint32_t v = 0;
-#pragma unroll
-  for (int b = 0; b < 4; ++b) v |= (b < left ? (uint32_t)__ldg(p + b) : 127u) << (8 * b);
+// 4-bit operands: four scales, for blocks of 32 columns each, from byte 4 j on of a row of
+// `bytes` that begins anywhere: aligned words of memory, `lo` and `hi`.  A word that
+// holds none of the row's bytes is not read but the row's first one in its place, without
+// a branch, so that many are in flight at once.
+struct ScaleWord {
+  uint32_t lo, hi;
+};
+__device__ __forceinline__ ScaleWord fp4_load_scales(const uint8_t* row, int j, int bytes) {
+  const int off = (int)(reinterpret_cast<uintptr_t>(row) & 3u);
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(row - off);
+  ScaleWord v;
+  v.lo = __ldg(w + (4 * j < bytes ? j : 0));
+  v.hi = __ldg(w + (4 * j + 4 - off < bytes && off ? j + 1 : 0));
   return v;
+}
+// ... their four bytes; 2^0 past the row's last.
+__device__ __forceinline__ uint32_t fp4_scale_word(const ScaleWord& v, const uint8_t* row, int j, int bytes) {
+  const uint32_t word = __funnelshift_r(v.lo, v.hi, 8 * (uint32_t)(reinterpret_cast<uintptr_t>(row) & 3u));
+  const int n = bytes - 4 * j;
+  const uint32_t mask = n >= 4 ? 0xFFFFFFFFu : n > 0 ? (1u << (8 * n)) - 1u : 0u;
+  return (word & mask) | (0x7F7F7F7Fu & ~mask);
 }
 // Instruction descriptor of kind::mxf4: e2m1 operands ([7,10), [10,12) = 1), K-major,
 // N >> 3 at [17,23), scales e8m0 [23], M >> 4 at [24,29); the scales' place in their

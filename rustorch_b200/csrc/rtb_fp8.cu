@@ -266,23 +266,35 @@ __global__ void __launch_bounds__(kThreads) pack_bytes_kernel(const PackSide a, 
   griddep_launch_dependents();
   const PackSide& p = blockIdx.y ? b : a;
   if (p.cs == 1) {
-    const int64_t words = p.ldd / 4, total = p.rows * words;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total;
-         i += (int64_t)gridDim.x * kThreads) {
-      const int64_t r = i / words, c = (i - r * words) * 4;
-      const uint8_t* sp = p.src + r * p.rs + c;
-      const int64_t n = p.cols - c;  // bytes of the word that exist
-      uint32_t v = 0;
-      if (n > 0) {
-        const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(sp) & 3);
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(sp - off);
-        const uint32_t lo = __ldg(w);
-        // the second word only where one of the wanted bytes lies in it
-        const uint32_t hi = off + (n < 4 ? (uint32_t)n : 4u) > 4u ? __ldg(w + 1) : 0u;
-        v = __funnelshift_r(lo, hi, 8 * off);
-        if (n < 4) v &= (1u << (8 * n)) - 1u;
+    // a warp takes 128 words of a row, so that a division serves four of a lane's
+    const int lane = threadIdx.x & 31;
+    const int64_t words = p.ldd / 4, chunks = (words + 127) / 128, total = p.rows * chunks;
+    for (int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < total;
+         i += (int64_t)gridDim.x * (kThreads / 32)) {
+      const int64_t r = total <= UINT32_MAX ? (int64_t)((uint32_t)i / (uint32_t)chunks) : i / chunks;
+      const int64_t k0 = (i - r * chunks) * 128 + lane;
+      const uint8_t* row = p.src + r * p.rs;
+      uint32_t v[4];
+      // (a word that holds none of the row's bytes is not read but the row's first one in
+      // its place, without a branch: all loads are in flight)
+      const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(row) & 3);
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(row - off);
+      uint32_t lo[4], hi[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t k = k0 + 32 * j;
+        lo[j] = __ldg(w + (4 * k < p.cols ? k : 0));
+        hi[j] = __ldg(w + (4 * k + 4 - (int64_t)off < p.cols && off ? k + 1 : 0));
       }
-      *reinterpret_cast<uint32_t*>(p.dst + r * p.ldd + c) = v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t n = p.cols - 4 * (k0 + 32 * j);  // bytes of the word that exist
+        v[j] = __funnelshift_r(lo[j], hi[j], 8 * off);
+        if (n < 4) v[j] = n > 0 ? v[j] & ((1u << (8 * n)) - 1u) : 0u;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (k0 + 32 * j < words) *reinterpret_cast<uint32_t*>(p.dst + r * p.ldd + (k0 + 32 * j) * 4) = v[j];
     }
     return;
   }
@@ -450,7 +462,7 @@ int launch_pack_bytes(rtb_ctx* ctx, const PackDesc& a, const PackDesc& b, cudaSt
   for (const PackDesc* p : d) {
     if (!p->dst) continue;
     side[n++] = {p->src, p->rows, p->cols, p->rs, p->cs, p->dst, p->ldd};
-    const int64_t ctas = p->cs == 1 ? (p->rows * (p->ldd / 4) + kThreads - 1) / kThreads
+    const int64_t ctas = p->cs == 1 ? (p->rows * ((p->ldd / 4 + 127) / 128) + kThreads / 32 - 1) / (kThreads / 32)
                                     : (p->rows + 63) / 64 * ((p->ldd + 63) / 64);
     most = ctas > most ? ctas : most;
   }

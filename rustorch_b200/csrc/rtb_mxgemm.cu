@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(256) scale_groups_kernel(const ScaleGroups p) 
 struct ScaleGroups4 {
   ScaleRef x, y;
   int64_t xrows, yrows;
-  int xgroups, tn, stages, bytes, vec;
+  int xgroups, tn, stages, bytes, words;  // words: rows of whole words on 4-byte boundaries
   uint32_t* out;
 };
 __global__ void __launch_bounds__(256) fp4_scale_groups_kernel(const ScaleGroups4 p) {
@@ -201,25 +201,24 @@ __global__ void __launch_bounds__(256) fp4_scale_groups_kernel(const ScaleGroups
   const ScaleRef& s = isx ? p.x : p.y;
   const int64_t first = isx ? (int64_t)g * 128 : (int64_t)tile * p.tn + part * 128;
   const int64_t end = isx ? p.xrows : ((int64_t)(tile + 1) * p.tn < p.yrows ? (int64_t)(tile + 1) * p.tn : p.yrows);
-  // (whole words first, all of a thread's loads in flight; the few others behind them)
-  const bool whole = p.vec && 4 * (j0 + lane) + 4 <= p.bytes;
-  uint32_t v[16];
-#pragma unroll
-  for (int k = 0; k < 16; ++k) {
+  auto row_of = [&](int k) {  // (a row past the tile: the operand's first)
     const int64_t r = first + w + 8 * k;
-    v[k] = 0x7F7F7F7Fu;
-    if (whole && r < end)
-      v[k] = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(s.p) + r * s.ld_row) +
-                   j0 + lane);
-  }
+    return static_cast<const uint8_t*>(s.p) + (r < end ? r : 0) * s.ld_row;
+  };
+  if (p.words) {  // rows of whole words on 4-byte boundaries
+    const bool in = 4 * (j0 + lane) < p.bytes;
+    uint32_t v[16];
 #pragma unroll
-  for (int k = 0; k < 16; ++k) t[w + 8 * k][lane] = v[k];
-  if (!whole && 4 * (j0 + lane) < p.bytes) {
-#pragma unroll 4
-    for (int k = 0; k < 16; ++k) {
-      const int64_t r = first + w + 8 * k;
-      if (r < end) t[w + 8 * k][lane] = fp4_scale_word(s, r, j0 + lane, p.bytes, 0);
-    }
+    for (int k = 0; k < 16; ++k) v[k] = __ldg(reinterpret_cast<const uint32_t*>(row_of(k)) + (in ? j0 + lane : 0));
+#pragma unroll
+    for (int k = 0; k < 16; ++k) t[w + 8 * k][lane] = in && first + w + 8 * k < end ? v[k] : 0x7F7F7F7Fu;
+  } else {
+    ScaleWord v[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = fp4_load_scales(row_of(k), j0 + lane, p.bytes);
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      t[w + 8 * k][lane] = first + w + 8 * k < end ? fp4_scale_word(v[k], row_of(k), j0 + lane, p.bytes) : 0x7F7F7F7Fu;
   }
   __syncthreads();
   // word q of a group is row q / 4 + 32 (q % 4)
@@ -626,8 +625,10 @@ int launch(rtb_ctx* ctx, const uint8_t* X, int64_t ldx, const uint8_t* Y, int64_
   clear_stale_cuda_error();
   const dim3 grid((unsigned)groups, (unsigned)((p.stages_total * kPer + 31) / 32));
   if (FP4) {
+    const bool words = ((reinterpret_cast<uintptr_t>(p.scx.p) | reinterpret_cast<uintptr_t>(p.scy.p) |
+                           (uintptr_t)p.scx.ld_row | (uintptr_t)p.scy.ld_row | (uintptr_t)p.sc_bytes) & 3u) == 0;
     const ScaleGroups4 sg = {p.scx, p.scy, p.xrows, p.ycols, xgroups, TN, p.stages_total, p.sc_bytes,
-                             p.sc_vec, ws};
+                             words, ws};
     e = launch_pdl(fp4_scale_groups_kernel, grid, dim3(256), 0, s, sg);
   } else {
     const ScaleGroups sg = {p.scx, p.scy, p.xrows, p.ycols, xgroups, TN, p.stages_total, ws};
