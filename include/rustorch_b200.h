@@ -299,8 +299,9 @@ int rtb_rms_norm_fwd(rtb_ctx* ctx, int64_t rows, int64_t d, const float* x, int6
                      const float* residual, int64_t ldr, const float* norm_weight, float eps,
                      float* sum, int64_t ldsum, float* y, int64_t ldy, float* rstd, void* stream);
 /* The same with y as 8-bit blocks of 128 columns (q [rows, d] e4m3, scale [rows,
- * ceil(d / 128)] e8m0: what rtb_fp8_quantize with block_rows = 1 makes of y), the
- * left operand of rtb_fp8_matmul. */
+ * ceil(d / 128)] e8m0, as rtb_fp8_quantize writes them with block_rows = 1), the left
+ * operand of rtb_fp8_matmul.  y is not rounded to fp32 in between: where it lies so near
+ * to the middle of two codes that fp32 would not tell, it goes to the nearer one. */
 int rtb_rms_norm_fp8(rtb_ctx* ctx, int64_t rows, int64_t d, const float* x, int64_t ldx,
                      const float* residual, int64_t ldr, const float* norm_weight, float eps,
                      float* sum, int64_t ldsum, uint8_t* q, int64_t ldq, uint8_t* scale,
@@ -408,7 +409,15 @@ int rtb_fp4_dequantize(rtb_ctx* ctx, int64_t rows, int64_t cols, const uint8_t* 
  * B [N,K] (nn::Linear's weight) as rtb_fp4_quantize writes them, K elements to a row
  * (even: two lie in a byte; a quantised row of odd length counts its zero), lda and ldb
  * in bytes; scale_a [M, ceil(K / 32)], scale_b [N, ceil(K / 32)].  bias [N] or NULL;
- * act: any RTB_ACT_*.  K = 0 gives act(bias) or zeros. */
+ * act: any RTB_ACT_*.
+ * Accuracy, relative to S = sum over k of |deq(A) deq(B)|: the products of codes are
+ * exact.  On the tensor cores they are summed 64 at a time in the accumulator, where an
+ * addition truncates (at most 2^-21 of the sum so far), and the sums are added up in
+ * fp32 after every 1024 elements, 4096 for products of many tiles; measured at most 2.5e-8
+ * S on any codes with scales of a few powers of two.  For up to four rows of A
+ * the sum of a block of 32 is exact and rounded to fp32 with the two scales; which of the
+ * two ways is taken goes by the sizes and the weight's alignment alone.  Scales whose
+ * product leaves fp32's range are outside of this.  K = 0 gives act(bias) or zeros. */
 int rtb_fp4_matmul(rtb_ctx* ctx, int64_t M, int64_t N, int64_t K, const uint8_t* A, int64_t lda,
                    const uint8_t* scale_a, int64_t ldsa, const uint8_t* B, int64_t ldb,
                    const uint8_t* scale_b, int64_t ldsb, const float* bias, int act, float* C,

@@ -385,9 +385,9 @@ def rms_norm_fwd(x, norm_weight=None, eps: float = 1e-5, residual=None, out=None
 
 
 def rms_norm_fp8(x, norm_weight=None, eps: float = 1e-5, residual=None, out_sum=None):
-    """(q, scale, sum, rstd): rms_norm_fwd with its y as fp8_quantize(y) holds it
+    """(q, scale, sum, rstd): rms_norm_fwd with its y in fp8_quantize's format
     (float8_e4m3fn values, a power-of-two scale for each 128 columns), fp8_matmul's
-    left operand, in one pass."""
+    left operand, in one pass and with one rounding of y, to 8 bits."""
     return (_ops_module or _load_ops()).rms_norm_fp8(x, norm_weight, eps, residual, out_sum)
 
 

@@ -35,6 +35,7 @@ struct RmsParams {
   int64_t ldr;
   const float* w;  // null: 1
   float eps;
+  double inv_d;
   float* h;        // null: not wanted
   int64_t ldh;
   float* y;        // fp32 output
@@ -77,17 +78,50 @@ __device__ __forceinline__ void store4(float* row, int c0, int d, int lane, cons
   }
 }
 
+// The row's statistic, rounded, and what the rounding left.
+struct Rstd {
+  float hi, lo;
+};
+__device__ __forceinline__ Rstd rstd_of(double total, double inv_d, float eps) {
+  const double r = rsqrt(fma(total, inv_d, (double)eps));
+  const float hi = (float)r;
+  return {hi, (float)(r - (double)hi)};
+}
+// h rstd w in fp32 as the next rounding wants it: where the product is no fp32 number,
+// the one of its two neighbours with an odd last bit, which is never half way between two
+// codes.
+__device__ __forceinline__ float product_to_odd(float h, Rstd r, float w) {
+  const float u = h * r.hi, ue = fmaf(h, r.lo, fmaf(h, r.hi, -u));
+  const float y = u * w, ye = fmaf(ue, w, fmaf(u, w, -y));
+  const float s = y + ye, rest = ye - (s - y);
+  const uint32_t bits = __float_as_uint(s);
+  if ((bits & 1u) || !(fabsf(rest) > 0.0f) || s == 0.0f) return s;  // (NaN: s is no number)
+  return __uint_as_float((rest > 0.0f) == (s > 0.0f) ? bits + 1 : bits - 1);
+}
+
 // y of a block's four columns, and its way out.
 template <bool VEC, bool FP8>
-__device__ __forceinline__ void finish4(const RmsParams& p, int64_t m, int c0, int lane, float rstd,
+__device__ __forceinline__ void finish4(const RmsParams& p, int64_t m, int c0, int lane, Rstd rstd,
                                         const float (&h)[4]) {
   float y[4], w[4] = {1.0f, 1.0f, 1.0f, 1.0f};
   if (p.w) load4<VEC>(p.w, c0, p.d, lane, w);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) y[j] = h[j] * rstd * w[j];
+  for (int j = 0; j < 4; ++j) y[j] = h[j] * rstd.hi * w[j];
   if (!FP8) {
     store4<VEC>(p.y + m * p.ldy, c0, p.d, lane, y);
     return;
+  }
+  // A value is to be rounded once, to 8 bits, and y has been three times, by 3 units of its
+  // last place at most.  That changes a code only within as much of the middle of two codes
+  // (or, the block's scale, of 448 times a power of two), numbers of five bits, whose last
+  // 19 are zero: these few (1 in 60000) are multiplied again with twice the digits.
+  constexpr uint32_t kNear = 8u << 13;
+  auto off = [&](int j) { return (__float_as_uint(y[j]) << 13) + (kNear >> 1); };
+  if (min(min(off(0), off(1)), min(off(2), off(3))) < kNear) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (off(j) < kNear && y[j] != 0.0f && fabsf(y[j]) <= 3.402823466e38f)
+        y[j] = product_to_odd(h[j], rstd, w[j]);
   }
   // (magnitudes compare as their bits do)
   uint32_t top = 0;
@@ -150,8 +184,8 @@ __global__ void __launch_bounds__(cta(T), T == 512 ? 2 : 4) rms_rows_kernel(cons
 #pragma unroll
       for (int k = 0; k < W; ++k) total += red[phase][grp][k];
     }
-    const float rstd = (float)(1.0 / sqrt(total / p.d + (double)p.eps));
-    if (p.rstd && lane == 0 && w == 0) p.rstd[m] = rstd;
+    const Rstd rstd = rstd_of(total, p.inv_d, p.eps);
+    if (p.rstd && lane == 0 && w == 0) p.rstd[m] = rstd.hi;
     if (p.h) {
 #pragma unroll
       for (int i = 0; i < NB; ++i)
@@ -199,8 +233,8 @@ __global__ void __launch_bounds__(kThreads) rms_wide_kernel(const RmsParams p) {
     double total = 0.0;
 #pragma unroll
     for (int k = 0; k < W; ++k) total += red[k];
-    const float rstd = (float)(1.0 / sqrt(total / p.d + (double)p.eps));
-    if (p.rstd && threadIdx.x == 0) p.rstd[m] = rstd;
+    const Rstd rstd = rstd_of(total, p.inv_d, p.eps);
+    if (p.rstd && threadIdx.x == 0) p.rstd[m] = rstd.hi;
     for (int b = w; b < blocks; b += W) {
       float h[4];
       if (p.h) load4<VEC>(p.h + m * p.ldh, 128 * b, p.d, lane, h);
@@ -251,6 +285,7 @@ int rms_norm_run(rtb_ctx* ctx, const RmsDesc& d, cudaStream_t s) {
   p.ldr = d.ldr;
   p.w = d.w;
   p.eps = d.eps;
+  p.inv_d = 1.0 / (double)p.d;
   p.h = d.sum;
   p.ldh = d.ldsum;
   p.y = d.y;

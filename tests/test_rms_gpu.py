@@ -64,16 +64,52 @@ def test_forward(gpu, rows, d, with_res):
 @pytest.mark.parametrize("rows,d", SHAPES)
 @pytest.mark.parametrize("with_res", [False, True])
 def test_forward_fp8(gpu, rows, d, with_res):
-    """The 8-bit output is what fp8_quantize makes of the fp32 one, to the bit."""
+    """The 8-bit output is the float64 one rounded once: off by half of a code's step at
+    most, and by what rstd is (34 U); the scale is the smallest power of two that holds
+    the block within 448."""
     x, res, w = make(rows, d, 2)
     res = res if with_res else None
     y, h, rstd = gpu.rms_norm_fwd(x, w, EPS, residual=res)
     q, s, h8, r8 = gpu.rms_norm_fp8(x, w, EPS, residual=res)
     assert q.dtype == E4M3 and s.dtype == E8M0 and tuple(s.shape) == (rows, -(-d // 128))
     assert torch.equal(h8, h) and torch.equal(r8, rstd)
-    wq, ws = gpu.fp8_quantize(y)
-    same_codes(q, wq)
-    assert torch.equal(s.view(torch.uint8), ws.view(torch.uint8))
+    check_codes(q, s, forward64(h, w)[0], 36 * U)
+
+
+def check_codes(q, s, y, off):
+    d = y.shape[1]
+    wide = torch.nn.functional.pad(y.abs(), (0, -d % 128)).view(y.shape[0], -1, 128).amax(2)
+    scale = torch.pow(2.0, s.view(torch.uint8).double() - 127)
+    assert bool((wide <= 448 * scale * (1 + off)).all())
+    assert bool(((wide > 224 * scale * (1 - off)) | (wide == 0) & (scale == 1)).all())
+    scale = scale.repeat_interleave(128, 1)[:, :d]
+    v = y / scale
+    step = torch.pow(2.0, torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -6))) - 3)
+    assert bool(((q.double() - v).abs() <= step / 2 + off * v.abs()).all())
+
+
+@pytest.mark.parametrize("rows,d", [(60, 64), (40, 77), (30, 128), (50, 300), (20, 1001), (10, 2048), (9, 4097), (5, 8192),
+                                    (3, 16384), (2, 20001), (2, 20004)])
+def test_forward_fp8_between_two_codes(gpu, rows, d):
+    """Values within an fp32 rounding of the middle of two codes, where the nearer one
+    shows only behind fp32's last place: whole numbers, so that the sum of squares is
+    exact, and weights that put each value there."""
+    g = torch.Generator().manual_seed(41)
+    for row in range(rows):
+        h = torch.randint(1, 100, (1, d), generator=g).double() * (2 * torch.randint(0, 2, (1, d), generator=g) - 1)
+        rstd = (h.square().sum() / d + float(torch.tensor(EPS))) ** -0.5
+        k = torch.randint(-6, 8, (1, d), generator=g).double()
+        middle = (1 + (2 * torch.randint(0, 6, (1, d), generator=g) + 1) / 16) * torch.pow(2.0, k)
+        middle[:, ::128] = 232  # the block's largest: its scale is 1
+        w = (middle / (h * rstd)).float()
+        y = h * rstd * w.double()
+        q, s, _, _ = gpu.rms_norm_fp8(h.float().cuda(), w[0].cuda(), EPS)
+        assert bool((s.view(torch.uint8) == 127).all())
+        step = torch.pow(2.0, k - 3)
+        step[:, ::128] = 16
+        up, down = middle + step / 2, middle - step / 2
+        assert bool((y != middle).all())
+        assert torch.equal(q.double().cpu(), torch.where(y.abs() > middle, up, down) * torch.sign(y))
 
 
 def reference(x, rstd, w, dy, ds):
