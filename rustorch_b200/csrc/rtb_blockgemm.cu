@@ -24,9 +24,9 @@
 // part of the contraction, and adds the parts out of one another's shared
 // memory in rank order (no workspace, no counters, the same bits every time).
 // Roles (warp index): 0, 6, 7 TMA producers, 1 TMEM allocator + MMA issuer, 2..5
-// epilogue (TMEM lanes 32 (w % 4)..; MODE 2: they also lay out the scales).  The
-// accumulator is double buffered in TMEM, so the promotion of one block overlaps the MMAs of the next.  The
-// finished tile goes through shared memory (the idle load ring), so that its
+// epilogue (TMEM lanes 32 (w % 4)..; MODE 2: they also lay out the scales, MODE 3: write
+// them into TMEM).  The accumulator is double buffered in TMEM, so the promotion of one
+// block overlaps the MMAs of the next.  The finished tile goes through shared memory (the idle load ring), so that its
 // stores run along the output's rows and bias, activation and the sum of the
 // parts are one short loop.  Every wait is bounded: after a timeout a role goes
 // on without waiting (no thread leaves early, so that barriers still meet), the
@@ -57,7 +57,8 @@ struct Cfg {
   static constexpr int kYPiece = BN * 128;             // one Y piece of a stage (BN x 128 B)
   static constexpr int kStageBytes = kXBytes + kPieces * kYPiece;
   // Narrow tiles, two CTAs on an SM: one's loads pass behind the other's start and
-  // end (a token row by 8192 x 8192: 19.9 us with one CTA of eight stages, 18.8).
+  // end (a token row by 8192 x 8192: 19.9 us with one CTA of eight stages, 18.8; since then
+  // 16.4).
   // MODE 3: two (YVEC) only where tiles would wait for an SM; else the whole ring for one
   // that shares its tile's contraction with others (64 x 28672 x 8192, 224 tiles, 32.0 us
   // with two, 39.4 with one; 48 x 8192 x 8192, 64 tiles, 12.4 and 11.7).
@@ -682,9 +683,10 @@ int max_clusters(const rtb_ctx* ctx, int parts) {
 // CTAs that share a tile: a power of two up to 8 with at least two blocks of the
 // contraction each, such that all clusters run at once (16 tiles of 8 CTAs, one on
 // an SM, take a second round for the last one: 128 x 2048 x 4096 22.8 us, 12.4 with
-// four; 512 x 512 x 4096 23.0, 12.4).  With two CTAs on an SM (the query counts one)
-// and eight blocks for each a few clusters may follow: a token row by 4096 x
-// 4096 10.7 us with eight, 10.0 with four; 32 x 4096 x 14336 18.6, 20.8.
+// four; 512 x 512 x 4096 23.0, 12.4; since then 10.9 and 10.7).  With two CTAs on an SM
+// (the query counts one) and eight blocks for each a few clusters may follow: a token row
+// by 4096 x 4096 10.7 us with eight, 10.0 with four; 32 x 4096 x 14336 18.6, 20.8 (since
+// then 8.8 and 17.4).
 template <int MODE, int BN, bool YVEC>
 int pick_parts(const rtb_ctx* ctx, int64_t tiles, int64_t units) {
   constexpr int kPerSm = Cfg<MODE, BN, YVEC>::kPerSm;
@@ -732,8 +734,8 @@ int launch(rtb_ctx* ctx, const CUtensorMap& tmX, const CUtensorMap& tmY, BlockPa
 }
 
 // CTA pairs where their 256 x 256 tiles occupy more than half of the SMs.
-// Measured, one CTA a tile against pairs: 512 x 4096 x 4096 (32 tiles) 23.1 us,
-// 24.9; 1024 x 2048 x 1024 (32) 13.8, 14.7; 1024 x 4096 x 4096 (64) 44.3, 26.0;
+// Measured, one CTA a tile against pairs: 512 x 4096 x 4096 (32 tiles) 23.1 us (since then
+// 19.5), 24.9; 1024 x 2048 x 1024 (32) 13.8 (10.4), 14.7; 1024 x 4096 x 4096 (64) 44.3, 26.0;
 // 2048 x 2048 x 512 (64) 23.2, 14.0; weight gradients with 32 and 64 tiles, 4096
 // rows, 72 us, 85, and 130, 92.
 bool use_pairs(const rtb_ctx* ctx, const BlockParams& p) {
@@ -754,7 +756,7 @@ int fp8_gemm_run(rtb_ctx* ctx, const Fp8Desc& d, cudaStream_t s) {
   if ((st = check_extents(d.M, d.N, d.K))) return st;
   // Few rows of A: the weight's rows fill the 128-row tile and A is the narrow
   // side (C^T = B . A^T), so that at most 15 rows of 16, 31 of 64 are padding and
-  // not 64 of 128 (16 x 8192 x 8192: 19.3 us in a loop, 3.5 TB/s of the weight).
+  // not 64 of 128 (16 x 8192 x 8192: 17.4 us, 3.9 TB/s of the weight).
   const bool swap = d.M <= 64;
   BlockParams p{};
   p.xrows = swap ? d.N : d.M;

@@ -13,9 +13,10 @@
 // out of shared memory serves four; with few weight rows several warps share a
 // contraction, their sums added in a fixed order.  A CTA keeps A for all of its rows.
 //
-// Measured (in a graph): a row by 4096 x 4096 in 4.1 us, by 8192 x 8192 in 9.2 out of L2
-// and 11.5 from memory (3.1 TB/s); by 1000 x 1000, rows of 500 bytes, 3.4.  Bound by the
-// conversions and products, 2.5 of the 4.4 clocks that a warp takes for eight codes.
+// Measured (in a graph): a row by 4096 x 4096 in 4.1 us out of L2 and 5.2 from memory (two
+// rows 5.8, four 7.3); by 1000 x 1000, rows of 500 bytes, 3.4.  Bound by the conversions and
+// products, 2.5 of the 4.4 clocks that a warp takes for eight codes, and a short call by its
+// start and end.
 #include "rtb_act.cuh"
 #include "rtb_fp4.cuh"
 #include "rtb_internal.h"

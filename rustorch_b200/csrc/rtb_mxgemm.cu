@@ -23,7 +23,7 @@
 // columns of TMEM too), whichever takes less time in whole rounds of the pairs.
 // Roles (warps of each CTA): 0, 2, 3 TMA producers; 1 TMEM allocation, and in the
 // pair's first CTA the issue for both; 4..11 epilogue (lanes 32 (w % 4).., one
-// half of the columns).
+// half of the columns).  FP4: 4..7 the scales, 8..15 epilogue; 256 x 256 only.
 //
 // Scales: a kernel before lays them out once per call as 512-byte groups of 128
 // rows for each block (row r: the 32-bit word at 16 (r % 32) + 4 (r / 32), its
@@ -34,16 +34,16 @@
 // for their loads and fences.)
 //
 // Measured: 8192 x 4096 x 8192 in 212 us alone, 262 to 273 in a loop (the power cap),
-// 2.1 PFLOP/s; 8192 x 8192 x 1024 in 97 and 105.  Outputs that TMA cannot store (N or
-// ldc off a multiple of 4) leave by scalar stores, 32 rows an instruction: 8192 x 4097
-// x 8192 429 us.
+// 2.1 PFLOP/s; 8192 x 8192 x 1024 in 92 and 101.  Outputs that TMA cannot store (N or
+// ldc off a multiple of 4) leave by scalar stores, two rows an instruction: 8192 x 4097
+// x 8192 261 us alone, 302 in a loop.
 //
-// FP4: 8192 x 4096 x 8192 in 120 us, 4.6 PFLOP/s (135 in a loop, the power cap); 8192 x
-// 4096 x 16384 in 224, 4.9.  A stage takes 0.46 us where its MMAs take 0.31 (the clock
-// at 1.65 GHz): the rest is its operands' way from L2, 35 KB an SM, 11 TB/s over all;
-// without the loads 0.34.  A ring of 4 stages: 131 us, of 6: no change.  Tiles 192 wide
-// with two accumulators: 145 us, and 4% faster where the contraction has 4 stages (2048
-// x 8192 x 1024 33.2 us, 31.8): not kept.
+// FP4: 8192 x 4096 x 8192 in 112 to 116 us, 4.8 PFLOP/s (134 to 140 in a loop, the power
+// cap); 8192 x 4096 x 16384 in 213, 5.2; 8192 x 4097 x 8192 in 176.  A stage takes 0.46 us
+// where its MMAs take 0.31 (the clock at 1.65 GHz): the rest is its operands' way from L2,
+// 35 KB an SM, 11 TB/s over all; without the loads 0.34.  A ring of 4 stages: 131 us where
+// 5 took 120, of 6: no change.  Tiles 192 wide with two accumulators: 145 us, and 4% faster
+// where the contraction has 4 stages (2048 x 8192 x 1024 33.2 us, 31.8): not kept.
 #include "rtb_pair.cuh"
 
 namespace rtb {

@@ -14,8 +14,9 @@
 // 2047 x 16383: 97 us, 142).  Wider rows take a CTA each and two passes, the second out
 // of L2.
 //
-// Measured: 8192 x 4096 with a residual 88 us (6.1 TB/s, 93% of a copy), with the 8-bit
-// output 71 (6.2 TB/s); 16384 x 2048 87 us, 2048 x 16384 94 and 88.
+// Measured: 8192 x 4096 with a residual 89 us (6.0 TB/s, 92% of a copy), with the 8-bit
+// output 71 (6.2 TB/s); 16384 x 2048 90 and 72 us, 2048 x 16384 93 and 90, 8192 x 4097 101
+// and 103.
 #include "rtb_fp8.cuh"
 #include "rtb_internal.h"
 #include "rtb_ptx.cuh"
