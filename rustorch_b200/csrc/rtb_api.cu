@@ -1426,9 +1426,10 @@ int rtb_fp4_matmul(rtb_ctx* ctx, int64_t M, int64_t N, int64_t K, const uint8_t*
   d.M = M; d.N = N; d.K = K; d.sa = scale_a; d.ldsa = ldsa; d.sb = scale_b; d.ldsb = ldsb;
   d.bias = bias; d.act = act; d.C = C; d.ldc = ldc;
   // Few rows: on the CUDA cores where the weight is small, or would have to be copied for
-  // the tensor cores' loads.  Measured (in a graph; these, then the tensor cores): 1 x
-  // 4096 x 4096 4.1 us, 6.0; 2 rows 5.1, 6.0; 4 rows 7.2, 6.0; 1 x 8192 x 8192 9.2, 9.5; 1 x
-  // 28672 x 8192 36.6, 26.0; 4 x 1000 x 1000 (unaligned rows) 4.0, 7.5.
+  // the tensor cores' loads.  Measured (in a graph, from memory; these, then the tensor
+  // cores): 1 x 4096 x 4096 4.4 us, 6.1; 2 rows 5.3, 6.1; 4 rows 7.6, 6.2; 1 x 8192 x 4096
+  // 6.3, 7.6; 1 x 8192 x 8192 10.4, 10.2; 1 x 28672 x 8192 34.0, 25.4; 4 x 2048 x 2048 3.4,
+  // 4.7; out of L2 4 x 1000 x 1000 (unaligned rows) 4.0, 7.5.
   if (M <= kFp4RowsMax &&
       (!aligned16(B) || ldb % 16 != 0 || N <= (int64_t(1) << 25) / (M * K))) {
     d.A = A; d.lda = lda; d.B = B; d.ldb = ldb;

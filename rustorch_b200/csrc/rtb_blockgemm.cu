@@ -57,12 +57,12 @@ struct Cfg {
   static constexpr int kYPiece = BN * 128;             // one Y piece of a stage (BN x 128 B)
   static constexpr int kStageBytes = kXBytes + kPieces * kYPiece;
   // Narrow tiles, two CTAs on an SM: one's loads pass behind the other's start and
-  // end (a token row by 8192 x 8192: 19.9 us with one CTA of eight stages, 18.8; since then
-  // 16.4).
-  // MODE 3: two (YVEC) only where tiles would wait for an SM; else the whole ring for one
-  // that shares its tile's contraction with others (64 x 28672 x 8192, 224 tiles, 32.0 us
-  // with two, 39.4 with one; 48 x 8192 x 8192, 64 tiles, 12.4 and 11.7).
-  static constexpr int kPerSm = (MODE == 2 && BN <= 32) || (MODE == 3 && YVEC) ? 2 : 1;
+  // end (a token row by 8192 x 8192 in 8 bits: 19.9 us with one CTA of eight stages, 18.8).
+  // MODE 3, 64 columns: two (YVEC) only where tiles would wait for an SM; else the whole
+  // ring for one that shares its tile's contraction with others (64 x 28672 x 8192, 224
+  // tiles, 32.0 us with two, 39.4 with one; 48 x 8192 x 8192, 64 tiles, 14.2 and 12.9; but 16
+  // x 4096 x 4096 6.3 and 6.7).
+  static constexpr int kPerSm = (MODE >= 2 && BN <= 32) || (MODE == 3 && YVEC) ? 2 : 1;
   // MODE 2, 3: stages of a scale buffer, of two (MODE 3: in TMEM, one in shared memory);
   // a stage's scales of one operand
   static constexpr int kSf = MODE == 3 ? 4 : kPerSm == 2 ? 8 : 16;
@@ -378,8 +378,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<MODE, BN, YVEC>::kPerSm)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  griddep_wait();
-  griddep_launch_dependents();
 
   // the cluster's tile, and this CTA's part of the contraction
   const int parts = p.parts, rank = (int)blockIdx.x % parts, tile = (int)blockIdx.x / parts;
@@ -390,6 +388,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<MODE, BN, YVEC>::kPerSm)
   const int i1 = i1g < p.stages_total ? i1g : p.stages_total;
   const int nst = i1 - i0;
   const int units = (nst + C::kPerUnit - 1) / C::kPerUnit;
+  // The first of the weight into L2, while the kernel before ends (a hint, which reads
+  // nothing: the weight may still be written.  Four stages: a token by
+  // 8192 x 8192 in 4 bits 11.7 -> 11.1 us, 1 x 4096 x 4096 in 8 bits 8.7 -> 7.7; two 11.1
+  // and 7.9, eight 11.6 and 7.9, all of them 12.3 and 8.0).
+  if (MODE >= 2 && lane == 0 && (warp == 0 || warp >= 6))
+    for (int i = i0 + (warp ? warp - 5 : 0); i < i1 && i < i0 + 4; i += 3) {
+      if (p.swap) tma_prefetch_2d(&tmX, i * 128, tx * kX);
+      else tma_prefetch_2d(&tmY, i * 128, ty * BN);
+    }
+  griddep_wait();
+  griddep_launch_dependents();
 
   if (warp == 0 || warp >= 6) {
     if (lane == 0) {
@@ -683,10 +692,10 @@ int max_clusters(const rtb_ctx* ctx, int parts) {
 // CTAs that share a tile: a power of two up to 8 with at least two blocks of the
 // contraction each, such that all clusters run at once (16 tiles of 8 CTAs, one on
 // an SM, take a second round for the last one: 128 x 2048 x 4096 22.8 us, 12.4 with
-// four; 512 x 512 x 4096 23.0, 12.4; since then 10.9 and 10.7).  With two CTAs on an SM
+// four; 512 x 512 x 4096 23.0, 12.4; both under 11 since).  With two CTAs on an SM
 // (the query counts one) and eight blocks for each a few clusters may follow: a token row
 // by 4096 x 4096 10.7 us with eight, 10.0 with four; 32 x 4096 x 14336 18.6, 20.8 (since
-// then 8.8 and 17.4).
+// then 7.6 and 17).
 template <int MODE, int BN, bool YVEC>
 int pick_parts(const rtb_ctx* ctx, int64_t tiles, int64_t units) {
   constexpr int kPerSm = Cfg<MODE, BN, YVEC>::kPerSm;
@@ -756,7 +765,7 @@ int fp8_gemm_run(rtb_ctx* ctx, const Fp8Desc& d, cudaStream_t s) {
   if ((st = check_extents(d.M, d.N, d.K))) return st;
   // Few rows of A: the weight's rows fill the 128-row tile and A is the narrow
   // side (C^T = B . A^T), so that at most 15 rows of 16, 31 of 64 are padding and
-  // not 64 of 128 (16 x 8192 x 8192: 17.4 us, 3.9 TB/s of the weight).
+  // not 64 of 128 (16 x 8192 x 8192: 16.4 us, 4.1 TB/s of the weight).
   const bool swap = d.M <= 64;
   BlockParams p{};
   p.xrows = swap ? d.N : d.M;
@@ -837,8 +846,8 @@ int fp4_gemm_run(rtb_ctx* ctx, const Fp4Desc& d, cudaStream_t s) {
                                (uint32_t)bn)))
     return st;
   const bool two = (p.xrows + 127) / 128 * ((p.ycols + bn - 1) / bn) > ctx->sm_count;
-  if (bn == 16) return two ? launch<3, 16, true>(ctx, tmX, tmY, p, s) : launch<3, 16, false>(ctx, tmX, tmY, p, s);
-  if (bn == 32) return two ? launch<3, 32, true>(ctx, tmX, tmY, p, s) : launch<3, 32, false>(ctx, tmX, tmY, p, s);
+  if (bn == 16) return launch<3, 16, false>(ctx, tmX, tmY, p, s);
+  if (bn == 32) return launch<3, 32, false>(ctx, tmX, tmY, p, s);
   if (bn == 64) return two ? launch<3, 64, true>(ctx, tmX, tmY, p, s) : launch<3, 64, false>(ctx, tmX, tmY, p, s);
   return launch<3, 128, false>(ctx, tmX, tmY, p, s);
 }

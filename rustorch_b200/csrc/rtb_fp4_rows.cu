@@ -13,8 +13,8 @@
 // out of shared memory serves four; with few weight rows several warps share a
 // contraction, their sums added in a fixed order.  A CTA keeps A for all of its rows.
 //
-// Measured (in a graph): a row by 4096 x 4096 in 4.1 us out of L2 and 5.2 from memory (two
-// rows 5.8, four 7.3); by 1000 x 1000, rows of 500 bytes, 3.4.  Bound by the conversions and
+// Measured (in a graph): a row by 4096 x 4096 in 4.1 us out of L2 and 4.4 from memory (two
+// rows 5.3, four by 2048 x 2048 3.4); by 1000 x 1000, rows of 500 bytes, 3.8.  Bound by the conversions and
 // products, 2.5 of the 4.4 clocks that a warp takes for eight codes, and a short call by its
 // start and end.
 #include "rtb_act.cuh"
@@ -87,6 +87,10 @@ __device__ __forceinline__ uint4 behind(uint4 w, int off) {
                     __funnelshift_r(v[2], v[3], s), __funnelshift_r(v[3], v[4], s));
 }
 
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+}
+
 struct RowsParams {
   int64_t N;
   int M, half, blocks, split;  // split: warps that share a contraction
@@ -107,10 +111,22 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_rows_kernel(const RowsParams 
   extern __shared__ uint4 a_s[];
   float* scale_s = reinterpret_cast<float*>(a_s + MT * 4 * kChunk);
   __shared__ float red[kWarps][kRows * MT];
-  griddep_wait();
-  griddep_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int split = p.split, part = warp % split, per = kWarps / split;  // per: groups of a CTA
+  // The first of the weight into L2, while the kernel before ends (a hint, which reads
+  // nothing: the weight may still be written; a row by 4096 x 4096 5.2 -> 4.4 us).
+  {
+    const int64_t n0 = ((int64_t)blockIdx.x * per + warp / split) * kRows;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int64_t at = (int64_t)16 * (kLanes * (part + k * split) + lane);
+        if (n0 + r < p.N && at < p.half) prefetch_l2(p.B + (n0 + r) * p.ldb + at);
+      }
+  }
+  griddep_wait();
+  griddep_launch_dependents();
   for (int64_t g0 = (int64_t)blockIdx.x * per; g0 < p.groups; g0 += (int64_t)gridDim.x * per) {
     const int64_t n0 = (g0 + warp / split) * kRows;
     float acc[kRows * MT];
