@@ -456,3 +456,22 @@ def test_refusals(gpu):
     both = torch.zeros_like(x)
     with pytest.raises(gpu.RtbError, match="one place"):
         gpu.rms_norm_fwd(x, w, residual=res, out=both, out_sum=both)
+
+
+@pytest.mark.parametrize("d", [4, 100, 301, 512, 1001, 1024, 4096, 4097, 8192, 8191])
+def test_backward_of_one_cta_and_more(gpu, d):
+    """Row counts on both sides of what one CTA takes alone, with and without the
+    reduced gradient, added to what is there."""
+    for rows in (1, 2, 3, 4, 5, 8, 9, 16, 17, 32, 33):
+        x, dy, w = make(rows, d, 51)
+        rstd = forward64(x, None)[1].float()
+        want, bound = reference(x, rstd, w, dy, x)
+        got = gpu.rms_norm_backward(x, rstd, dy, w, grad_sum=x)
+        check(got, want, bound)
+        only = gpu.rms_norm_backward(x, rstd, dy, w, grad_sum=x, need_weight=False)
+        assert only[1] is None and torch.equal(only[0], got[0])
+        only = gpu.rms_norm_backward(x, rstd, dy, w, need_x=False)
+        assert only[0] is None and torch.equal(only[1], got[1])
+        out = torch.ones(d, device="cuda")
+        gpu.rms_norm_backward(x, rstd, dy, w, need_x=False, out_weight=out, accumulate=True)
+        assert torch.equal(out, 1 + got[1])
