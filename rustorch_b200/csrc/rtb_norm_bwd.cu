@@ -23,10 +23,10 @@
 //
 // Measured: 8192 x 4096 75 us (5.4 TB/s of the 12 bytes an element, 82% of a copy),
 // 16384 x 2048 from a checkpoint 67 us (4.5 TB/s of 9 bytes: the instructions of
-// the row's fixed part count as much), 2048 x 16384 108 us, 8192 x 4097 130 us;
+// the row's fixed part count as much), 2048 x 16384 102 us, 8192 x 4097 130 us;
 // 8192 x 4096 with sigmoid 99 us, with tanh 101.  RMS, 8192 x 4096: 73 us, with dsum 90
-// (6.0 TB/s), from a checkpoint 79 and 92; 16384 x 2048 from one 71; 2048 x 16384 with dsum
-// 119, 8192 x 4097 170; 1531 x 1001 from a checkpoint 11.4.
+// (6.0 TB/s), from a checkpoint 79 and 83; 16384 x 2048 from one 71; 2048 x 16384 with dsum
+// 112, 8192 x 4097 153; 1531 x 1001 from a checkpoint 11.4.
 #include "rtb_act.cuh"
 #include "rtb_f32x2.cuh"
 #include "rtb_fp8.cuh"
@@ -166,6 +166,9 @@ __device__ __forceinline__ void put(float* out, float v, int accumulate) {
 
 constexpr int kRing = 3;  // stages of the row ring: 96 KB for 512 threads of 8 values
 
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+}
 __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -330,6 +333,9 @@ __global__ void __launch_bounds__(kBlock, 1024 / kBlock)
   for (; r < rows; r += step, phase ^= 1) {
     // the next row's statistics and block scales
     const int rn = r + step < rows ? r + step : r;
+    // (its dsum, which no ring takes, into L2 at least: 8192 x 4097 170 -> 153 us, from a
+    // checkpoint x 4096 90 -> 83; rows without a ring, 65536 x 301, 64.5 -> 70.7)
+    if (RING && RMS && p.dsum && p.dx && 32 * t < p.d) prefetch_l2(p.dsum + (int64_t)rn * ldds + 32 * t);
     const float mean_n = RMS ? 0.0f : __ldg(p.mean + rn), rstd_n = __ldg(p.rstd + rn);
     uint32_t sb_n[NS] = {};
     if (kAhead) scales(rn, sb_n);
@@ -548,6 +554,18 @@ __global__ void __launch_bounds__(kWide, 1)
     float u[E], h[E];  // x, then u; dy, then h
     const float mean = RMS ? 0.0f : __ldg(p.mean + r), rstd = __ldg(p.rstd + r);
     const float* dyr = p.dy + r * p.lddy;
+    // The next row into L2 (2048 x 16384 110 -> 102 us, RMS with dsum from a checkpoint 128 ->
+    // 107).  fp32 rows off the 16-byte boundaries, whose single loads are many, do not gain
+    // (2048 x 16383 163 -> 170) but by dsum, which is loaded last (229 -> 204).
+    const int64_t rn = r + gridDim.x;
+    if (rn < p.rows && 32 * t < p.d) {
+      if (VEC || SAVED) {
+        prefetch_l2(p.dy + rn * p.lddy + 32 * t);
+        if (!SAVED) prefetch_l2(p.x + rn * p.ldx + 32 * t);
+        else if (128 * t < p.d) prefetch_l2(p.q + rn * p.ldq + 128 * t);
+      }
+      if (RMS && p.dsum && p.dx) prefetch_l2(p.dsum + rn * p.ldds + 32 * t);
+    }
 #pragma unroll
     for (int i = 0; i < G; ++i) {
       const int k = t + kWide * i;
