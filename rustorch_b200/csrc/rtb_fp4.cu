@@ -2,9 +2,9 @@
 //   save:    s = 2^ceil(log2(max|x| / 6)) over the block, q = e2m1(x / s)
 //   restore: x' = q * s
 // Both stream their operands once (4.53 bytes a value): HBM-bound.  8192 x 4096 saved in
-// 25.9 us (5.9 TB/s, 90% of a copy), as its transpose in 30.4, restored in 28.4; rows off
-// the 16-byte boundaries, 8192 x 4100, 41 and 30 us (a block a warp and byte stores: 126
-// and 84).
+// 24.8 us (6.1 TB/s, 94% of a copy), as its transpose in 29.5, restored in 28.4; rows off
+// the 16-byte boundaries, 8192 x 4100, 36.5, 36.7 and 35 us (a block a warp and byte stores:
+// 126 and 84; words shifted between the lanes 40 and, transposed, 47).
 #include "rtb_fp4.cuh"
 #include "rtb_internal.h"
 #include "rtb_ptx.cuh"
@@ -98,26 +98,19 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const float* __r
   }
 }
 
-// A chunk's codes, four bytes a lane, to a row of any alignment: `n` bytes from q on.
-// The lanes' bytes are shifted to the words of memory; those at the ends go byte by byte.
-__device__ __forceinline__ void store_codes(uint8_t* q, uint32_t code, int n, int lane) {
-  const int off = (int)(reinterpret_cast<uintptr_t>(q) & 3u);
-  const uint32_t prev = __shfl_up_sync(0xffffffffu, code, 1);
-  const uint32_t word = off ? __funnelshift_l(prev, code, 8 * off) : code;
-  const int at = 4 * lane - off;  // the word's first byte
-  if (at >= 0 && at + 4 <= n) {
-    *reinterpret_cast<uint32_t*>(q + at) = word;
-  } else {
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-      if (at + b >= 0 && at + b < n) q[at + b] = (uint8_t)(word >> (8 * b));
-  }
-  if (lane == 31) {
-    for (int b = 0; b < off; ++b)
-      if (128 - off + b < n) q[128 - off + b] = (uint8_t)(code >> (8 * (4 - off + b)));
-  }
+// n (at most 128) bytes in shared memory, on a 4-byte boundary and with four readable ones
+// behind the 128, to a row of any alignment by a warp: whole words of memory, and the bytes
+// at the two ends by lanes of their own.
+__device__ __forceinline__ void store_bytes(uint8_t* q, const uint8_t* from, int n, int lane) {
+  const int head = (int)(-reinterpret_cast<uintptr_t>(q) & 3u);  // bytes before the first whole word
+  const int words = n > head ? (n - head) >> 2 : 0;
+  const uint32_t* in = reinterpret_cast<const uint32_t*>(from);
+  if (lane < words)
+    *reinterpret_cast<uint32_t*>(q + head + 4 * lane) = __funnelshift_r(in[lane], in[lane + 1], 8 * head);
+  const int k = lane < 4 ? lane : head + 4 * words + lane - 4;
+  if (lane < 8 && k < (lane < 4 && head < n ? head : n)) q[k] = from[k];
 }
-// ... and from it: n bytes, 0 behind them.  (No word is read that holds none of them.)
+// A chunk's codes, four bytes a lane, from a row of any alignment: n bytes, 0 behind them.  (No word is read that holds none of them.)
 __device__ __forceinline__ uint32_t load_codes(const uint8_t* q, int n, int lane) {
   const int off = (int)(reinterpret_cast<uintptr_t>(q) & 3u);
   const uint32_t* w = reinterpret_cast<const uint32_t*>(q - off);
@@ -131,7 +124,7 @@ __device__ __forceinline__ uint32_t load_codes(const uint8_t* q, int n, int lane
 
 // Any rows: chunks of 256 columns a warp, loaded a column a lane and turned through
 // shared memory, so that a lane has eight columns side by side as above.
-constexpr int kAny = 2;  // chunks at a time (4: 8192 x 4100 38 and 28 us, 4096 x 1001 7.8 and 6.4 for 7.8 and 5.5)
+constexpr int kAny = 2;  // chunks at a time (4: 8192 x 4100 38 and 35 us for 36.5 and 35, 4096 x 1001 7.3 and 7.0 for 6.5 and 6.2)
 __global__ void __launch_bounds__(kThreads) fp4_quantize_any_kernel(const float* __restrict__ x,
                                                                     int64_t ldx, int64_t total, int cols,
                                                                     int chunks, uint8_t* q, int64_t ldq,
@@ -180,7 +173,11 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_any_kernel(const float*
       const uint32_t sb = fp4_scale_byte(top);
       const uint32_t eight = e2m1x8(e, fp4_inverse(sb));
       const int left = cols - col[n];
-      store_codes(q + row[n] * ldq + col[n] / 2, sb == 255 ? 0u : eight, left < 256 ? (left + 1) / 2 : 128, lane);
+      __syncwarp();  // the values have been read
+      *reinterpret_cast<uint32_t*>(mine + lane) = sb == 255 ? 0u : eight;
+      __syncwarp();
+      store_bytes(q + row[n] * ldq + col[n] / 2, reinterpret_cast<const uint8_t*>(mine),
+                  left < 256 ? (left + 1) / 2 : 128, lane);
       if ((lane & 3) == 0 && 8 * lane < left)
         scale[row[n] * lds + col[n] / kFp4Block + lane / 4] = (uint8_t)sb;
     }
@@ -191,7 +188,7 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_any_kernel(const float*
 // columns of 32 rows, warp w the w-th block of 32 columns, lane l the l-th row, so that
 // loads run along the stored rows and a block's maximum is one thread's.  The codes
 // pass through shared memory and leave along the result's rows, 128 bytes each.  Five
-// CTAs on an SM: 8192 x 4096 in 30.4 us; four 32.3, three 37.8, six, whose registers do
+// CTAs on an SM: 8192 x 4096 in 29.5 us; four 32.3, three 37.8, six, whose registers do
 // not hold the 32 values, 37.
 template <bool VEC>  // the result's rows are on 16-byte boundaries
 __global__ void __launch_bounds__(kThreads, 5) fp4_quantize_columns_kernel(const float* __restrict__ x,
@@ -242,11 +239,11 @@ __global__ void __launch_bounds__(kThreads, 5) fp4_quantize_columns_kernel(const
       }
     } else {
       const int n = qcols - c0 / 2 < 128 ? (int)(qcols - c0 / 2) : 128;  // bytes of a row here
-#pragma unroll 1
+#pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int r = w + 8 * i;
         if (r0 + r >= rows) break;
-        store_codes(q + (r0 + r) * ldq + c0 / 2, *reinterpret_cast<const uint32_t*>(&codes[r][4 * lane]), n, lane);
+        store_bytes(q + (r0 + r) * ldq + c0 / 2, codes[r], n, lane);
       }
     }
     const int r = threadIdx.x >> 3, k = threadIdx.x & 7;
