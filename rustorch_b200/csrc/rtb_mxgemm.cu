@@ -54,7 +54,7 @@ constexpr int threads(bool fp4) { return fp4 ? 512 : 384; }
 constexpr int kTileX = 256;
 constexpr int kStages = 5;
 // X, Y (half of the tile's rows), scales
-constexpr int stage_bytes(bool fp4) { return 16384 + 16384 + (fp4 ? 3072 : 2048); }
+constexpr int stage_bytes(bool fp4) { return 16384 + 16384 + (fp4 ? 6 * 512 : 2048); }
 constexpr int kChunk = 128 * 16 * 4;               // a staged 128 x 16 fp32 piece of the output
 constexpr int kBufs = 3;                           // staging chunks of an epilogue half
 constexpr int smem_bytes(bool fp4) {
