@@ -294,14 +294,16 @@ int rtb_layer_norm_backward_fp8(rtb_ctx* ctx, int64_t rows, int64_t d, const uin
  * not wanted) is what the backward pass reads, together with h.  y and sum may each
  * be x or residual (in place, with the same leading dimension), but not the same
  * place.  d >= 1.  h is rounded to fp32 once and enters the sum of squares and y as
- * rounded. */
+ * rounded; the squares and their sum are double, so that no finite row leaves the range
+ * (rstd itself is infinite where it is no fp32 number: a row under 3e-39 with eps 0). */
 int rtb_rms_norm_fwd(rtb_ctx* ctx, int64_t rows, int64_t d, const float* x, int64_t ldx,
                      const float* residual, int64_t ldr, const float* norm_weight, float eps,
                      float* sum, int64_t ldsum, float* y, int64_t ldy, float* rstd, void* stream);
 /* The same with y as 8-bit blocks of 128 columns (q [rows, d] e4m3, scale [rows,
  * ceil(d / 128)] e8m0, as rtb_fp8_quantize writes them with block_rows = 1), the left
  * operand of rtb_fp8_matmul.  y is not rounded to fp32 in between: where it lies so near
- * to the middle of two codes that fp32 would not tell, it goes to the nearer one. */
+ * to the middle of two codes that fp32 would not tell, it goes to the nearer one (of
+ * magnitudes from 2^-120 to fp32's largest). */
 int rtb_rms_norm_fp8(rtb_ctx* ctx, int64_t rows, int64_t d, const float* x, int64_t ldx,
                      const float* residual, int64_t ldr, const float* norm_weight, float eps,
                      float* sum, int64_t ldsum, uint8_t* q, int64_t ldq, uint8_t* scale,

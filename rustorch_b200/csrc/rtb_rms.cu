@@ -7,16 +7,18 @@
 //
 // A row of up to 16384 columns lives in the registers of a group of 32..512
 // threads: warp w of the group holds the 128-column blocks w, w + W, ..., so that
-// an 8-bit block's maximum is one warp's.  The sum of squares is fp32 in a thread
-// (at most 32 terms) and double from there on.  1024 threads of 64 registers share an
-// SM: that many rows in flight hide a row's chain of loads, sum and stores (16 values a
-// thread of 512 and not 32 of 256, 4095 x 8191: 92 us, 96; 32 of 512 and not 64 of 256,
-// 2047 x 16383: 97 us, 142).  Wider rows take a CTA each and two passes, the second out
-// of L2.
+// an 8-bit block's maximum is one warp's.  Squares and their sum are double: fp32 ones
+// leave its range from magnitudes of 2e19 on (and under 1e-23), and are off by more than
+// the middle of two 8-bit codes forgives (up to 1e-7 of rstd; the conversions cost 0 to 8%,
+// 65536 x 512 with the 8-bit output 41.2 -> 44.5 us).  1024 threads of 64 registers share an
+// SM: that many rows in flight hide a row's chain of loads, sum and stores (with fp32
+// squares, 16 values a thread of 512 and not 32 of 256, 4095 x 8191: 92 us, 96; 32 of 512
+// and not 64 of 256, 2047 x 16383: 97 us, 142).  Wider rows take a CTA each and two passes,
+// the second out of L2.
 //
 // Measured: 8192 x 4096 with a residual 89 us (6.0 TB/s, 92% of a copy), with the 8-bit
-// output 71 (6.2 TB/s); 16384 x 2048 90 and 72 us, 2048 x 16384 93 and 90, 8192 x 4097 101
-// and 103.
+// output 71 (6.2 TB/s); 16384 x 2048 88 and 71 us, 2048 x 16384 92 and 90, 8192 x 4097 103
+// and 107.
 #include "rtb_fp8.cuh"
 #include "rtb_internal.h"
 #include "rtb_ptx.cuh"
@@ -79,18 +81,23 @@ __device__ __forceinline__ void store4(float* row, int c0, int d, int lane, cons
   }
 }
 
-// The row's statistic, rounded, and what the rounding left.
+// The row's statistic, rounded, and its factors: rstd = scale (hi + lo), scale a power of
+// two and hi in [1, 2) but at the ends of fp32's range.  A row's values times scale are of
+// the order of 1, so that y is exact to its last place where rstd itself, of a row beyond
+// 8e37 or under 3e-39, is no normal number of fp32.
 struct Rstd {
-  float hi, lo;
+  float value, scale, hi, lo;
 };
 __device__ __forceinline__ Rstd rstd_of(double total, double inv_d, float eps) {
   const double r = rsqrt(fma(total, inv_d, (double)eps));
-  const float hi = (float)r;
-  return {hi, (float)(r - (double)hi)};
+  const int e = min(max((__double2hiint(r) >> 20 & 0x7FF) - 1023, -126), 127);
+  const double unit = r * __hiloint2double((1023 - e) << 20, 0);
+  const float hi = (float)unit;
+  return {(float)r, __int_as_float((e + 127) << 23), hi, (float)(unit - (double)hi)};
 }
-// h rstd w in fp32 as the next rounding wants it: where the product is no fp32 number,
-// the one of its two neighbours with an odd last bit, which is never half way between two
-// codes.
+// h (r.hi + r.lo) w in fp32 as the next rounding wants it: where the product is no fp32
+// number, the one of its two neighbours with an odd last bit, which is never half way
+// between two codes.
 __device__ __forceinline__ float product_to_odd(float h, Rstd r, float w) {
   const float u = h * r.hi, ue = fmaf(h, r.lo, fmaf(h, r.hi, -u));
   const float y = u * w, ye = fmaf(ue, w, fmaf(u, w, -y));
@@ -100,7 +107,7 @@ __device__ __forceinline__ float product_to_odd(float h, Rstd r, float w) {
   return __uint_as_float((rest > 0.0f) == (s > 0.0f) ? bits + 1 : bits - 1);
 }
 
-// y of a block's four columns, and its way out.
+// y of a block's four columns, from h times the row's scale, and its way out.
 template <bool VEC, bool FP8>
 __device__ __forceinline__ void finish4(const RmsParams& p, int64_t m, int c0, int lane, Rstd rstd,
                                         const float (&h)[4]) {
@@ -172,12 +179,12 @@ __global__ void __launch_bounds__(cta(T), T == 512 ? 2 : 4) rms_rows_kernel(cons
 #pragma unroll
         for (int j = 0; j < 4; ++j) h[i][j] += r[i][j];
     }
-    float ss = 0.0f;
+    double ss = 0.0;
 #pragma unroll
     for (int i = 0; i < NB; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) ss = fmaf(h[i][j], h[i][j], ss);
-    double total = warp_sum((double)ss);
+      for (int j = 0; j < 4; ++j) ss = fma((double)h[i][j], (double)h[i][j], ss);
+    double total = warp_sum(ss);
     if (W > 1) {
       if (lane == 0) red[phase][grp][w] = total;
       named_bar_sync(1 + grp, T);
@@ -186,12 +193,16 @@ __global__ void __launch_bounds__(cta(T), T == 512 ? 2 : 4) rms_rows_kernel(cons
       for (int k = 0; k < W; ++k) total += red[phase][grp][k];
     }
     const Rstd rstd = rstd_of(total, p.inv_d, p.eps);
-    if (p.rstd && lane == 0 && w == 0) p.rstd[m] = rstd.hi;
+    if (p.rstd && lane == 0 && w == 0) p.rstd[m] = rstd.value;
     if (p.h) {
 #pragma unroll
       for (int i = 0; i < NB; ++i)
         store4<VEC>(p.h + m * p.ldh, 128 * (w + W * i), p.d, lane, h[i]);
     }
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[i][j] *= rstd.scale;
 #pragma unroll
     for (int i = 0; i < NB; ++i)
       if (128 * (w + W * i) < p.d) finish4<VEC, FP8>(p, m, 128 * (w + W * i), lane, rstd, h[i]);
@@ -235,11 +246,13 @@ __global__ void __launch_bounds__(kThreads) rms_wide_kernel(const RmsParams p) {
 #pragma unroll
     for (int k = 0; k < W; ++k) total += red[k];
     const Rstd rstd = rstd_of(total, p.inv_d, p.eps);
-    if (p.rstd && threadIdx.x == 0) p.rstd[m] = rstd.hi;
+    if (p.rstd && threadIdx.x == 0) p.rstd[m] = rstd.value;
     for (int b = w; b < blocks; b += W) {
       float h[4];
       if (p.h) load4<VEC>(p.h + m * p.ldh, 128 * b, p.d, lane, h);
       else input(128 * b, h);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[j] *= rstd.scale;
       finish4<VEC, FP8>(p, m, 128 * b, lane, rstd, h);
     }
   }
