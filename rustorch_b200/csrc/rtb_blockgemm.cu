@@ -265,8 +265,10 @@ __device__ __forceinline__ float4 finish4(float4 v, int act) {
 
 // The finished tile's rows out of shared memory: this CTA's share of them, the sum over
 // the P parts in rank order, bias, activation, the stores.  I quads of all parts at a
-// time: a load out of another CTA takes longer than the whole of the work on it.
-// Of a thread's quads, all in the same columns, the bias is `b4`.
+// time: a load out of another CTA takes longer than the whole of the work on it.  A quad
+// of padding is not loaded at all: every value that is loaded is used, so that all loads
+// have returned when this CTA arrives at the cluster's last barrier, behind which the
+// others' shared memory goes.  Of a thread's quads, all in the same columns, the bias is `b4`.
 template <int P, int I, int BN>
 __device__ __forceinline__ void finish_rows(const BlockParams& p, uint32_t tb, int rank, int tx, int ty,
                                             float4 b4) {
@@ -280,21 +282,26 @@ __device__ __forceinline__ void finish_rows(const BlockParams& p, uint32_t tb, i
   const int total = share << shift;
   for (int e0 = threadIdx.x; e0 < total; e0 += I * kThreads) {
     float4 w[I][P];
+    auto at = [&](int i, int64_t& m, int64_t& n) {  // a quad that lies in the output
+      const int e = e0 + i * kThreads;
+      m = m0 + rank * share + (e >> shift);
+      n = n0 + (e & mask) * 4;
+      return e < total && m < M && n < N;
+    };
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-      const int e = e0 + i * kThreads;
-      if (e < total) {
-        const uint32_t at = tb + (uint32_t)((rank * share + (e >> shift)) * pitch + (e & mask) * 4) * 4;
+      int64_t m, n;
+      if (at(i, m, n)) {
+        const int e = e0 + i * kThreads;
+        const uint32_t from = tb + (uint32_t)((rank * share + (e >> shift)) * pitch + (e & mask) * 4) * 4;
 #pragma unroll
-        for (int q = 0; q < P; ++q) w[i][q] = P == 1 ? lds128(at) : ld_cluster(map_rank(at, (uint32_t)q));
+        for (int q = 0; q < P; ++q) w[i][q] = P == 1 ? lds128(from) : ld_cluster(map_rank(from, (uint32_t)q));
       }
     }
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-      const int e = e0 + i * kThreads;
-      if (e >= total) break;
-      const int64_t m = m0 + rank * share + (e >> shift), n = n0 + (e & mask) * 4;
-      if (m >= M || n >= N) continue;
+      int64_t m, n;
+      if (!at(i, m, n)) continue;
       float4 x = w[i][0];
 #pragma unroll
       for (int q = 1; q < P; ++q) {
