@@ -419,8 +419,9 @@ int rtb_fp4_dequantize(rtb_ctx* ctx, int64_t rows, int64_t cols, const uint8_t* 
  * normal operands, and at most 1.9e-6 S on positive ones with a long tail (exp(3 N(0,1)),
  * 16384 long).  For up to four rows of A
  * the sum of a block of 32 is exact and rounded to fp32 with the two scales; which of the
- * two ways is taken goes by the sizes and the weight's alignment alone.  Scales whose
- * product leaves fp32's range are outside of this.  K = 0 gives act(bias) or zeros. */
+ * two ways is taken goes by the sizes and the weight's alignment alone.  The product of two
+ * scales may leave fp32's range where that of a block's sum and both does not.  K = 0 gives
+ * act(bias) or zeros. */
 int rtb_fp4_matmul(rtb_ctx* ctx, int64_t M, int64_t N, int64_t K, const uint8_t* A, int64_t lda,
                    const uint8_t* scale_a, int64_t ldsa, const uint8_t* B, int64_t ldb,
                    const uint8_t* scale_b, int64_t ldsb, const float* bias, int act, float* C,

@@ -6,8 +6,8 @@
 // integer dot products takes 4.7 clocks a warp and eight codes, this 2.5), and the
 // products are packed half-precision multiply-adds that are exact: a chain of eight
 // products is a multiple of 1/4 of at most 288, eleven bits.  A block's four chains are
-// added in fp32, exactly too, then one multiply-add by the two scales: fp32 rounds once
-// for each block.
+// added in fp32, exactly too, then multiplied by the smaller scale (exactly) and by the
+// larger in a multiply-add: fp32 rounds once for each block.
 //
 // A warp takes four weight rows, a lane a block (16 bytes) of each at a time, so that A
 // out of shared memory serves four; with few weight rows several warps share a
@@ -49,6 +49,12 @@ __device__ __forceinline__ void codes_to_halves(uint32_t w, uint32_t (&h)[4]) {
 }
 __device__ __forceinline__ void fma_halves(uint32_t& d, uint32_t a, uint32_t b) {
   asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(d) : "r"(a), "r"(b));
+}
+// The smaller of two scales and the larger; NaN where one of them is.
+__device__ __forceinline__ float2 ordered(float a, float b) {
+  float2 f;
+  asm("min.NaN.f32 %0, %2, %3;\n\tmax.NaN.f32 %1, %2, %3;" : "=f"(f.x), "=f"(f.y) : "f"(a), "f"(b));
+  return f;
 }
 __device__ __forceinline__ float sum_of_halves(uint32_t h) {
   float lo, hi;
@@ -221,10 +227,13 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_rows_kernel(const RowsParams 
         for (int m = 0; m < MT; ++m) {
           const float fa = scale_s[m * kChunk + k];
 #pragma unroll
-          for (int r = 0; r < kRows; ++r)
-            if (mine)
-              acc[r * MT + m] = fmaf(sum_of_halves(d[r * MT + m][0]) + sum_of_halves(d[r * MT + m][1]),
-                                     fa * fb[r], acc[r * MT + m]);
+          for (int r = 0; r < kRows; ++r) {
+            // (the smaller scale first: exact, and finite where the product of the sum and
+            // both is, which the product of the two need not be)
+            const float2 f = ordered(fa, fb[r]);
+            const float sum = sum_of_halves(d[r * MT + m][0]) + sum_of_halves(d[r * MT + m][1]);
+            if (mine) acc[r * MT + m] = fmaf(sum * f.x, f.y, acc[r * MT + m]);
+          }
         }
       }
     }
