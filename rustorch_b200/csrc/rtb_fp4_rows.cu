@@ -14,11 +14,14 @@
 // contraction, their sums added in a fixed order.  A CTA keeps A for all of its rows.
 //
 // Measured (in a graph): a row by 4096 x 4096 in 4.1 us out of L2 and 4.4 from memory (two
-// rows 5.3, four by 2048 x 2048 3.4); by 1000 x 1000, rows of 500 bytes, 3.8.  Bound by the conversions and
+// rows 5.3, four by 2048 x 2048 3.4); by 1000 x 1000, rows of 500 bytes, 3.7.  Bound by the conversions and
 // products, 2.5 of the 4.4 clocks that a warp takes for eight codes, and a short call by its
 // start and end.
+#include <type_traits>
+
 #include "rtb_act.cuh"
 #include "rtb_fp4.cuh"
+#include "rtb_fp4_load.cuh"
 #include "rtb_internal.h"
 #include "rtb_ptx.cuh"
 
@@ -64,19 +67,6 @@ __device__ __forceinline__ float sum_of_halves(uint32_t h) {
   return lo + hi;
 }
 
-// The 16 bytes of block b of a row of `half` bytes at any address, by aligned words, each
-// read only where one of its bytes exists.
-__device__ __forceinline__ uint4 load_block(const uint8_t* row, int b, int half) {
-  const uint8_t* p = row + (int64_t)16 * b;
-  const int off = (int)(reinterpret_cast<uintptr_t>(p) & 3u);
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(p - off);
-  const int left = half - 16 * b;
-  uint32_t v[5];
-#pragma unroll
-  for (int i = 0; i < 5; ++i) v[i] = 4 * i - off < left && (i < 4 || off) ? __ldg(w + i) : 0u;
-  return make_uint4(__funnelshift_r(v[0], v[1], 8 * off), __funnelshift_r(v[1], v[2], 8 * off),
-                    __funnelshift_r(v[2], v[3], 8 * off), __funnelshift_r(v[3], v[4], 8 * off));
-}
 // The 16 bytes that begin `off` (0..15, the same in all lanes) behind this lane's 16,
 // which the next lane's follow.
 __device__ __forceinline__ uint4 behind(uint4 w, int off) {
@@ -105,13 +95,78 @@ struct RowsParams {
   int64_t lda, ldb, ldsa, ldsb;
   const float* bias;
   int act;
+  int16_t front, back;         // ENDS: weight rows in front of the first and behind the N-th
   float* C;
   int64_t ldc;
 };
+static_assert(sizeof(RowsParams) <= 128, "more: other registers, a row by 4096 x 4096 4.4 -> 4.8 us");
+
+// A block of a row of A, 0 where the row has ended.  (The large kernel has these lines in
+// its loop: with this call it takes other registers, a row by 4096 x 4096 4.4 -> 4.6 us.)
+__device__ __forceinline__ uint4 load_a(const RowsParams& p, int m, int b) {
+  uint4 q = load_block(p.A + m * p.lda, b, p.half);
+  const int left = p.half - 16 * b;  // bytes behind the row are none of its own
+  if (left < 16) {
+    uint32_t* e = &q.x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      e[j] = left >= 4 * j + 4 ? e[j] : left <= 4 * j ? 0u : e[j] & ((1u << (8 * (left - 4 * j))) - 1u);
+  }
+  return q;
+}
+
+// The weight's ends: the first and last rows, whose 16-byte loads would reach over the
+// matrix, by words, a row at a time for the whole CTA.  (One CTA more for them: a row by
+// 1000 x 1000 3.7 us as before, by 28672 x 8190 49.3 -> 47.7.  Both kinds of loads in one
+// loop cost every row, 28672 x 8190 64 us.)
+template <int MT>
+__device__ __forceinline__ void end_rows(const RowsParams& p, float (*red)[kRows * MT]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll 1
+  for (int e = 0; e < p.front + p.back; ++e) {
+    const int64_t n = e < p.front ? e - p.front : p.N + e - p.front;
+    float acc[MT] = {};
+#pragma unroll 1
+    for (int b = threadIdx.x; b < p.blocks; b += kThreads) {
+      const uint4 q = load_block(p.B + n * p.ldb, b, p.half);
+      const float fb = e8m0_to_float(__ldg(p.sb + n * p.ldsb + b));
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        if (m >= p.M) break;
+        const uint4 x = load_a(p, m, b);
+        const float2 f = ordered(e8m0_to_float(__ldg(p.sa + m * p.ldsa + b)), fb);
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t hq[4], hx[4], d = 0u;
+          codes_to_halves(j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w, hq);
+          codes_to_halves(j == 0 ? x.x : j == 1 ? x.y : j == 2 ? x.z : x.w, hx);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) fma_halves(d, hq[k], hx[k]);
+          sum += sum_of_halves(d);
+        }
+        acc[m] = fmaf(sum * f.x, f.y, acc[m]);
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      for (int o = 16; o > 0; o >>= 1) acc[m] += __shfl_xor_sync(0xffffffffu, acc[m], o);
+      if (lane == 0) red[warp][m] = acc[m];
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < p.M) {
+      float sum = 0.0f;
+      for (int k = 0; k < kWarps; ++k) sum += red[k][threadIdx.x];
+      p.C[threadIdx.x * p.ldc + n] = activate(sum + (p.bias ? __ldg(p.bias + n) : 0.0f), p.act);
+    }
+    __syncthreads();  // red[] is free
+  }
+}
 
 // MT: rows of A in the registers (M of them exist).  Shared memory: A's halves
 // [MT][4 words][kChunk][16 bytes], then [MT][kChunk] scales.
-template <int MT, bool VEC>
+// ENDS: a CTA more, for the weight's ends.
+template <int MT, bool VEC, bool ENDS>
 __global__ void __launch_bounds__(kThreads, 2) fp4_rows_kernel(const RowsParams p) {
   constexpr int kChunk = chunk(MT, VEC), kLanes = lanes(VEC);
   extern __shared__ uint4 a_s[];
@@ -133,7 +188,12 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_rows_kernel(const RowsParams 
   }
   griddep_wait();
   griddep_launch_dependents();
-  for (int64_t g0 = (int64_t)blockIdx.x * per; g0 < p.groups; g0 += (int64_t)gridDim.x * per) {
+  const unsigned ctas = gridDim.x - ENDS;
+  if (ENDS && blockIdx.x == ctas) {
+    end_rows<MT>(p, red);
+    return;
+  }
+  for (int64_t g0 = (int64_t)blockIdx.x * per; g0 < p.groups; g0 += (int64_t)ctas * per) {
     const int64_t n0 = (g0 + warp / split) * kRows;
     float acc[kRows * MT];
 #pragma unroll
@@ -149,9 +209,8 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_rows_kernel(const RowsParams 
           const uint8_t* row = p.B + (n0 + r) * p.ldb;
           if (VEC) {
             if (b < p.blocks) w[r] = __ldg(reinterpret_cast<const uint4*>(row) + b);
-          } else {  // the 16 bytes of memory in which the block begins
-            const uintptr_t at = (reinterpret_cast<uintptr_t>(row) + (int64_t)16 * b) & ~uintptr_t(15);
-            if (at < reinterpret_cast<uintptr_t>(row) + p.half) w[r] = __ldg(reinterpret_cast<const uint4*>(at));
+          } else {
+            w[r] = load_chunk(row, b, p.half);
           }
           if (b < p.blocks) sb[r] = __ldg(p.sb + (n0 + r) * p.ldsb + b);
         }
@@ -277,9 +336,9 @@ __global__ void __launch_bounds__(kThreads, 2) fp4_rows_kernel(const RowsParams 
   }
 }
 
-template <int MT, bool VEC>
+template <int MT, bool VEC, bool ENDS>
 int launch(rtb_ctx* ctx, RowsParams& p, cudaStream_t s) {
-  auto* k = fp4_rows_kernel<MT, VEC>;
+  auto* k = fp4_rows_kernel<MT, VEC, ENDS>;
   constexpr int kSmem = MT * chunk(MT, VEC) * 68;
   {
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
@@ -293,9 +352,10 @@ int launch(rtb_ctx* ctx, RowsParams& p, cudaStream_t s) {
   while (p.split < kWarps && p.groups * p.split * 2 <= warps && p.split * 2 * lanes(VEC) <= p.blocks)
     p.split *= 2;
   const int64_t per = kWarps / p.split, need = (p.groups + per - 1) / per;
-  const int64_t grid = need < 2 * ctx->sm_count ? need : 2 * ctx->sm_count;
+  const int64_t most = 2 * ctx->sm_count - ENDS;
+  const int64_t ctas = need < most ? need : most;
   clear_stale_cuda_error();
-  cudaError_t e = launch_pdl(k, dim3((unsigned)grid), dim3(kThreads), (size_t)kSmem, s, (const RowsParams)p);
+  cudaError_t e = launch_pdl(k, dim3((unsigned)(ctas + ENDS)), dim3(kThreads), (size_t)kSmem, s, (const RowsParams)p);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? RTB_OK : cuda_status(e, "fp4_matmul launch");
 }
@@ -304,26 +364,36 @@ int launch(rtb_ctx* ctx, RowsParams& p, cudaStream_t s) {
 
 int fp4_rows_run(rtb_ctx* ctx, const Fp4Desc& d, cudaStream_t s) {
   RowsParams p{};
-  p.N = d.N;
   p.M = (int)d.M;
   p.half = (int)(d.K / 2);
   p.blocks = (int)((d.K + 31) / 32);
+  int front, back;
+  end_rows_of(d.B, d.N, d.ldb, p.half, &front, &back);
+  p.front = (int16_t)front;
+  p.back = (int16_t)back;
+  p.N = d.N - front - back;
   p.A = d.A;
   p.lda = d.lda;
-  p.B = d.B;
+  p.B = d.B + front * d.ldb;
   p.ldb = d.ldb;
   p.sa = d.sa;
   p.ldsa = d.ldsa;
-  p.sb = d.sb;
+  p.sb = d.sb + front * d.ldsb;
   p.ldsb = d.ldsb;
-  p.bias = d.bias;
+  p.bias = d.bias ? d.bias + front : nullptr;
   p.act = d.act;
-  p.C = d.C;
+  p.C = d.C + front;
   p.ldc = d.ldc;
   const bool vec = (reinterpret_cast<uintptr_t>(d.B) & 15u) == 0 && d.ldb % 16 == 0;
-  if (d.M == 1) return vec ? launch<1, true>(ctx, p, s) : launch<1, false>(ctx, p, s);
-  if (d.M == 2) return vec ? launch<2, true>(ctx, p, s) : launch<2, false>(ctx, p, s);
-  return vec ? launch<4, true>(ctx, p, s) : launch<4, false>(ctx, p, s);
+  const bool ends = front + back > 0;
+  auto as = [&](auto mt) {
+    constexpr int MT = decltype(mt)::value;
+    if (vec) return ends ? launch<MT, true, true>(ctx, p, s) : launch<MT, true, false>(ctx, p, s);
+    return ends ? launch<MT, false, true>(ctx, p, s) : launch<MT, false, false>(ctx, p, s);
+  };
+  if (d.M == 1) return as(std::integral_constant<int, 1>());
+  if (d.M == 2) return as(std::integral_constant<int, 2>());
+  return as(std::integral_constant<int, 4>());
 }
 
 }  // namespace rtb
