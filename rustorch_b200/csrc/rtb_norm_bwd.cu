@@ -108,13 +108,13 @@ __device__ __forceinline__ float2 block_sum2(float a, float b, float (*red)[2]) 
 }
 
 // Any width and alignment: three passes over the row's columns, the second and
-// third out of L1/L2.
-__global__ void __launch_bounds__(kThreads) norm_bwd_kernel(const NormBwdParams p) {
+// third out of L1/L2.  bias: the sums for db are wanted too.
+__global__ void __launch_bounds__(kThreads) norm_bwd_kernel(const NormBwdParams p, const int bias) {
   __shared__ float red[kThreads / 32][2];
   griddep_wait();
   griddep_launch_dependents();
   float* pg = p.part ? p.part + (int64_t)blockIdx.x * 2 * p.d : nullptr;
-  float* pb = pg ? pg + p.d : nullptr;  // (an index p.d + j would pass 32 bits)
+  float* pb = pg && bias ? pg + p.d : nullptr;  // (an index p.d + j would pass 32 bits)
   bool first = true;
   for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x, first = false) {
     const float mean = p.mean ? p.mean[r] : 0.0f, rstd = p.rstd[r];  // (RMS: no mean)
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kThreads) norm_bwd_kernel(const NormBwdParams 
       s2 = fmaf(h, u, s2);
       if (pg) {
         pg[j] = first ? dz * u : fmaf(dz, u, pg[j]);
-        pb[j] = first ? dz : pb[j] + dz;
+        if (pb) pb[j] = first ? dz : pb[j] + dz;
       }
     }
     if (!p.dx) continue;
@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(kWide, 1)
   constexpr int C = E / G;                    // columns of a load
   constexpr int W = kWide / 32;
   __shared__ float red[2][W][2];
-  extern __shared__ float acc_s[];  // [2][d]: the CTA's running sums
+  extern __shared__ float acc_s[];  // [2][d] (RMS [d]): the CTA's running sums
   griddep_wait();
   griddep_launch_dependents();
   const int t = threadIdx.x;
@@ -769,7 +769,7 @@ int launch_with_sums(rtb_ctx* ctx, NormBwdParams& p, int grid, float* dg, float*
 template <bool VEC, bool SAVED, bool RMS>
 int launch_direct(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStream_t s) {
   auto* k = norm_bwd_direct_kernel<VEC, SAVED, RMS>;
-  const size_t smem = (dg || db) ? (size_t)2 * p.d * sizeof(float) : 0;
+  const size_t smem = (dg || db) ? (size_t)(RMS ? 1 : 2) * p.d * sizeof(float) : 0;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        2 * 16384 * (int)sizeof(float));
   if (e != cudaSuccess) return cuda_status(e, "layer_norm_backward smem attribute");
@@ -795,7 +795,7 @@ int launch_rows_as(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStr
   constexpr int kPad = VEC ? 15 : 30;
   const int row_bytes = (((SAVED ? p.d : 4 * p.d) + kPad) & ~15) + ((4 * p.d + kPad) & ~15);
   int smem = kRows<kBlock, VEC, SAVED> ? R * kRing * row_bytes : 0;
-  if (smem < 8 * p.d) smem = 8 * p.d;  // the CTA's sums
+  if (smem < (RMS ? 4 : 8) * p.d) smem = (RMS ? 4 : 8) * p.d;  // the CTA's sums
   // The limit belongs to the kernel and not to the launch, and another thread may
   // be between its own two: so it is one number, that of the widest launch.  Groups
   // of T threads hold at most E values a thread, R d <= kBlock E, and R is at most
@@ -890,9 +890,9 @@ int norm_backward_run(rtb_ctx* ctx, const NormBwdDesc& d, cudaStream_t s) {
     p.part = part;
   }
   clear_stale_cuda_error();
-  cudaError_t e = launch_pdl(norm_bwd_kernel, dim3((unsigned)grid), dim3(kThreads), 0, s, p);
+  cudaError_t e = launch_pdl(norm_bwd_kernel, dim3((unsigned)grid), dim3(kThreads), 0, s, p, (int)(d.db != nullptr));
   if (e == cudaSuccess && part)
-    e = launch_pdl(norm_bwd_reduce_kernel, dim3((unsigned)((d.d + 31) / 32), 2), dim3(kReduceThreads), 0,
+    e = launch_pdl(norm_bwd_reduce_kernel, dim3((unsigned)((d.d + 31) / 32), d.db ? 2 : 1), dim3(kReduceThreads), 0,
                    s, (const float*)part, grid, (int)d.d, d.dg, d.db, d.accumulate);
   if (e == cudaSuccess) e = cudaGetLastError();
   ws_free(part, s);
