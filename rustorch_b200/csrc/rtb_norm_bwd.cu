@@ -745,6 +745,11 @@ __global__ void __launch_bounds__(kReduceThreads) norm_bwd_reduce_kernel(const f
   }
 }
 
+// What an error is reported as, by the entry point (RMS: no mean).
+int failed(const NormBwdParams& p, cudaError_t e) {
+  return cuda_status(e, p.mean ? "layer_norm_backward launch" : "rms_norm_backward launch");
+}
+
 // The sums' way out: a partial row for each CTA and the second kernel, or the
 // only CTA's own stores.
 template <typename Launch>
@@ -763,7 +768,7 @@ int launch_with_sums(rtb_ctx* ctx, NormBwdParams& p, int grid, float* dg, float*
                    s, (const float*)part, grid, p.d, dg, db, p.accumulate);
   if (e == cudaSuccess) e = cudaGetLastError();
   ws_free(part, s);
-  return e == cudaSuccess ? RTB_OK : cuda_status(e, "layer_norm_backward launch");
+  return e == cudaSuccess ? RTB_OK : failed(p, e);
 }
 
 template <bool VEC, bool SAVED, bool RMS>
@@ -772,7 +777,7 @@ int launch_direct(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStre
   const size_t smem = (dg || db) ? (size_t)(RMS ? 1 : 2) * p.d * sizeof(float) : 0;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        2 * 16384 * (int)sizeof(float));
-  if (e != cudaSuccess) return cuda_status(e, "layer_norm_backward smem attribute");
+  if (e != cudaSuccess) return failed(p, e);
   const int grid = (int)(p.rows < ctx->sm_count ? p.rows : ctx->sm_count);
   return launch_with_sums(ctx, p, grid, dg, db, s, [&] {
     return launch_pdl(k, dim3((unsigned)grid), dim3(kWide), smem, s, (const NormBwdParams)p, dg, db);
@@ -805,7 +810,7 @@ int launch_rows_as(rtb_ctx* ctx, NormBwdParams& p, float* dg, float* db, cudaStr
   constexpr int kMost = kRows<kBlock, VEC, SAVED> && kRingMax > kSumsMax ? kRingMax : kSumsMax;
   static_assert(kMost + 1024 <= 232448, "shared memory");
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
-  if (e != cudaSuccess) return cuda_status(e, "layer_norm_backward smem attribute");
+  if (e != cudaSuccess) return failed(p, e);
   const int64_t need = (p.rows + R - 1) / R, cap = (int64_t)ctx->sm_count * kPerSm;
   const int grid = RMS && dg && need <= kAlone ? 1 : (int)(need < cap ? need : cap);
   return launch_with_sums(ctx, p, grid, dg, db, s, [&] {
@@ -896,7 +901,7 @@ int norm_backward_run(rtb_ctx* ctx, const NormBwdDesc& d, cudaStream_t s) {
                    s, (const float*)part, grid, (int)d.d, d.dg, d.db, d.accumulate);
   if (e == cudaSuccess) e = cudaGetLastError();
   ws_free(part, s);
-  return e == cudaSuccess ? RTB_OK : cuda_status(e, "layer_norm_backward launch");
+  return e == cudaSuccess ? RTB_OK : failed(p, e);
 }
 
 }  // namespace rtb
