@@ -314,7 +314,7 @@ int rtb_rms_norm_fp8(rtb_ctx* ctx, int64_t rows, int64_t d, const float* x, int6
  *   dx      = rstd * (g - u * mean(g * u)) + dsum     when dx != NULL
  *   dweight = sum over rows of dy * u                 when dweight != NULL
  * dx is the gradient of both the forward pass's x and its residual; it may be dy's or
- * dsum's place.  accumulate != 0 adds into dx and dweight.  The sums are fp32 in an
+ * dsum's place (with the same leading dimension).  accumulate != 0 adds into dx and dweight.  The sums are fp32 in an
  * order that depends on the sizes, the alignment and the device alone. */
 int rtb_rms_norm_backward(rtb_ctx* ctx, int64_t rows, int64_t d, const float* x, int64_t ldx,
                           const float* rstd, const float* norm_weight, const float* dy,

@@ -1108,6 +1108,12 @@ int rtb_layer_norm_backward_fp8(rtb_ctx* ctx, int64_t rows, int64_t d, const uin
 }
 
 // ---------------------------------------------------------------- root-mean-square norm
+// An output in an input's place whose rows lie elsewhere: a row would be written over
+// another one that is still to be read.
+static bool turned(int64_t rows, const float* out, int64_t ldo, const float* in, int64_t ldi) {
+  return out && out == in && rows > 1 && ldo != ldi;
+}
+
 static int rms_norm(rtb_ctx* ctx, const char* who, const RmsDesc& d, void* stream) {
   const std::string w = std::string(who) + ": ";
   if (d.rows < 0 || d.d < 0) return set_error(RTB_E_INVALID, w + "negative dimension");
@@ -1119,6 +1125,9 @@ static int rms_norm(rtb_ctx* ctx, const char* who, const RmsDesc& d, void* strea
       (d.y ? d.ldy < d.d : d.ldq < d.d || d.lds < (d.d + 127) / 128))
     return set_error(RTB_E_INVALID, w + "leading dimension below the row's length");
   if (d.sum && d.sum == d.y) return set_error(RTB_E_INVALID, w + "one place for two outputs");
+  if (turned(d.rows, d.y, d.ldy, d.x, d.ldx) || turned(d.rows, d.y, d.ldy, d.residual, d.ldr) ||
+      turned(d.rows, d.sum, d.ldsum, d.x, d.ldx) || turned(d.rows, d.sum, d.ldsum, d.residual, d.ldr))
+    return set_error(RTB_E_INVALID, w + "in place with another leading dimension");
   DeviceGuard g(ctx->device);
   return rms_norm_run(ctx, d, pick_stream(ctx, stream));
 }
@@ -1163,6 +1172,8 @@ static int rms_norm_backward(rtb_ctx* ctx, const char* who, const NormBwdDesc& n
   if ((n.x && n.ldx < n.d) || (n.q && (n.ldq < n.d || n.lds < (n.d + 127) / 128)) ||
       n.lddy < n.d || (n.dsum && n.ldds < n.d) || (n.dx && n.lddx < n.d))
     return set_error(RTB_E_INVALID, w + "leading dimension below the row's length");
+  if (turned(n.rows, n.dx, n.lddx, n.dy, n.lddy) || turned(n.rows, n.dx, n.lddx, n.dsum, n.ldds))
+    return set_error(RTB_E_INVALID, w + "in place with another leading dimension");
   return norm_backward_run(ctx, n, s);
 }
 
