@@ -752,7 +752,7 @@ int launch(rtb_ctx* ctx, const CUtensorMap& tmX, const CUtensorMap& tmY, BlockPa
 // CTA pairs where their 256 x 256 tiles occupy more than half of the SMs.
 // Measured, one CTA a tile against pairs: 512 x 4096 x 4096 (32 tiles) 23.1 us (since then
 // 19.5), 24.9; 1024 x 2048 x 1024 (32) 13.8 (10.4), 14.7; 1024 x 4096 x 4096 (64) 44.3, 26.0;
-// 2048 x 2048 x 512 (64) 23.2, 14.0; weight gradients with 32 and 64 tiles, 4096
+// 2048 x 2048 x 512 (64) 23.2, 14.0 (4 bits: fp4_gemm_run); weight gradients with 32 and 64 tiles, 4096
 // rows, 72 us, 85, and 130, 92.
 bool use_pairs(const rtb_ctx* ctx, const BlockParams& p) {
   const int64_t tiles = ((p.xrows + 255) / 256) * ((p.ycols + 255) / 256);
@@ -841,6 +841,14 @@ int fp4_gemm_run(rtb_ctx* ctx, const Fp4Desc& d, cudaStream_t s) {
   p.err = ctx->d_err;
   p.timeout_ns = ctx->timeout_ns;
   const int64_t tiles = ((p.xrows + 127) / 128) * ((p.ycols + 127) / 128);
+  // Tiles of 64 columns where those of 128 would take a third of the SMs at most, so that
+  // clusters share them.  Measured, 64 columns and 128: 128 x 1024 x 4096 (8 tiles of 128)
+  // 6.5 us, 7.6; 333 x 1000 x 1000 (24) 7.9, 9.1; 256 x 2048 x 4096 (32) 8.5, 8.9; 384 x 2048 x
+  // 4096 (48) 11.2, 10.1; 512 x 2048 x 4096 (64) 11.3, 10.3; x 8192 18.1, 14.1; 512 x 4096 x
+  // 4096 (128) 16.3, 13.4 (short contractions gain a little longer: 512 x 2048 x 1024 6.3,
+  // 7.5; 512 x 4096 x 1024 7.4, 7.8).  One CTA a tile and pairs (use_pairs): 512 x 4608 x 4096
+  // (36 tiles of 256 x 256) 13.6, 17.7; 1024 x 2560 x 4096 (40) 25.5, 17.2; 2048 x 2048 x 2048
+  // (64) 18.3, 14.5.
   const int bn = swap ? (d.M <= 16 ? 16 : d.M <= 32 ? 32 : 64) : tiles * 3 <= ctx->sm_count ? 64 : 128;
   const uint8_t* X = swap ? d.B : d.A;
   const uint8_t* Y = swap ? d.A : d.B;

@@ -19,14 +19,15 @@
 // a row of a [CTA][2][d] workspace, and the CTAs' rows are added by a second
 // kernel.  No atomics: the order depends on the sizes, the alignment (which kernel)
 // and the device (how many CTAs) alone.  A single CTA writes
-// its sums itself.  Rows beyond 16384 columns take a CTA each and three passes.
+// its sums itself.  Rows beyond 16384 columns take a CTA each and two passes.
 //
 // Measured: 8192 x 4096 75 us (5.4 TB/s of the 12 bytes an element, 82% of a copy),
 // 16384 x 2048 from a checkpoint 67 us (4.5 TB/s of 9 bytes: the instructions of
 // the row's fixed part count as much), 2048 x 16384 102 us, 8192 x 4097 130 us;
 // 8192 x 4096 with sigmoid 99 us, with tanh 101.  RMS, 8192 x 4096: 73 us, with dsum 90
-// (6.0 TB/s), from a checkpoint 79 and 83; 16384 x 2048 from one 71; 2048 x 16384 with dsum
-// 112, 8192 x 4097 153; 1531 x 1001 from a checkpoint 11.4.
+// (6.0 TB/s), from a checkpoint 74 and 83; 16384 x 2048 from one 68; 2048 x 16384 with dsum
+// 112, 8192 x 4097 154; 1531 x 1001 from a checkpoint 12.5; 600 x 40000, the kernel of any
+// width, with dsum 579.
 #include "rtb_act.cuh"
 #include "rtb_f32x2.cuh"
 #include "rtb_fp8.cuh"
@@ -107,8 +108,8 @@ __device__ __forceinline__ float2 block_sum2(float a, float b, float (*red)[2]) 
   return make_float2(a, b);
 }
 
-// Any width and alignment: three passes over the row's columns, the second and
-// third out of L1/L2.  bias: the sums for db are wanted too.
+// Any width and alignment: two passes over the row's columns, the second out of L1 or
+// L2.  bias: the sums for db are wanted too.
 __global__ void __launch_bounds__(kThreads) norm_bwd_kernel(const NormBwdParams p, const int bias) {
   __shared__ float red[kThreads / 32][2];
   griddep_wait();
