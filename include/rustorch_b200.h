@@ -416,8 +416,8 @@ int rtb_fp4_dequantize(rtb_ctx* ctx, int64_t rows, int64_t cols, const uint8_t* 
  * exact.  On the tensor cores they are summed 64 at a time in the accumulator, where an
  * addition truncates (at most 2^-21 of the sum so far), and the sums are added up in
  * fp32 after every 1024 elements, 4096 for products of many tiles; measured exact on
- * normal operands, and at most 1.9e-6 S on positive ones with a long tail (exp(3 N(0,1)),
- * 16384 long).  For up to four rows of A
+ * normal operands, and where a row's scales lie up to 2^30 apart at most 1.2e-6 S, 3.2e-6 S
+ * for products of many tiles.  For up to four rows of A
  * the sum of a block of 32 is exact and rounded to fp32 with the two scales; which of the
  * two ways is taken goes by the sizes and the weight's alignment alone.  The product of two
  * scales may leave fp32's range where that of a block's sum and both does not.  K = 0 gives
